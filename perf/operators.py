@@ -1,0 +1,471 @@
+"""Operators of the paged 8-bit cache (``kvquant.PagedKVCache``), each in its plain form and as the package's own call.
+
+A row (sequence) of the cache is cut into blocks of 64 tokens.  A full block lies in a page, 8 bits a value, with one scale per kv-head for its keys
+and one for its values; the newest tokens, fewer than 64, stay in 16 bits in the row's tail.  Of a block's values x (what is not finite counts
+as 0) with a = max |x| the scale s is the smallest number of 8 significant bits that is not below a / top (top: 127 for int8, 448 for e4m3),
+2^-100 at least; the codes are x / s to the nearest, ties to even.
+
+* store:   tokens are appended to rows, full blocks go into pages, and the cache is read back as dense keys and values;
+* attend:  queries of the newest tokens over the cache, with any of a tanh cap, a bias by distance, a window, a prefix, document starts;
+* pages:   rows are forked or reordered and continued, pools of pages compacted.
+"""
+from __future__ import annotations
+
+import math
+import os
+import sys
+
+import torch
+
+own = False
+sys.path.insert(1, os.path.join(os.getcwd(), "odm-kv_amd"))
+
+D = 128
+BLOCK = 64
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+CODES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+TOP = {"int8": 127.0, "e4m3": 448.0}
+HEADS = ((32, 8), (28, 4), (16, 2), (24, 8), (8, 8))               # query and kv heads: groups of 4, 7, 8, 3 and 1
+
+
+# ------------------------------------------------------------------------------------------------ the cases
+def _case(kind, name=None, *, tokens, batch=1, queries=1, q_heads=32, kv_heads=8, layers=1, dtype="fp16", codes="int8", ragged=False, cap=0.0,
+          bias=False, window=0, prefix=0, documents=0):
+    c = dict(kind=kind, tokens=tokens, batch=batch, queries=queries, q_heads=q_heads, kv_heads=kv_heads, layers=layers, dtype=dtype, codes=codes,
+             ragged=ragged, cap=cap, bias=bias, window=window, prefix=prefix, documents=documents)
+    return c if name is None else dict(c, name=name)
+
+
+def listed():
+    return [
+        # a chat turn's first steps: one short row, where latency is everything
+        _case("attend", "step_500", tokens=500),
+        # one token over a 32k-token context
+        _case("attend", "step_32k", tokens=32768, dtype="bf16"),
+        # a serving batch, rows of their own lengths
+        _case("attend", "step_batch", tokens=8192, batch=16, ragged=True, codes="e4m3"),
+        # the longest context, capped scores and a bias by distance, 28 query heads over 4
+        _case("attend", "step_131k_capped", tokens=131071, q_heads=28, kv_heads=4, dtype="bf16", cap=50.0, bias=True),
+        # a question about a 32k-token prompt: a block of 29 tokens
+        _case("attend", "question_32k", tokens=32768, queries=29, dtype="bf16"),
+        # a chunk of a long prompt over what is cached of it, capped scores inside a window
+        _case("attend", "chunk_window", tokens=12000, queries=2048, dtype="bf16", cap=30.0, window=4096),
+        # a prompt of packed documents, none of which sees another
+        _case("attend", "documents", tokens=4096, queries=4096, documents=7),
+        # a batch of prompts whose first tokens (an image's, a system text's) see one another
+        _case("attend", "prefixes", tokens=777, batch=4, queries=777, prefix=256, codes="e4m3", dtype="bf16", ragged=True),
+        # a 32k-token prompt is stored in the place of a finished one and read back
+        _case("store", "store_32k", tokens=32768),
+        # prompts of ragged lengths, padded to the longest
+        _case("store", "store_ragged", tokens=3001, batch=5, ragged=True, dtype="bf16", codes="e4m3"),
+        # a step of beam search over 8k-token prompts: the survivors are copied, every copy takes a token
+        _case("beams", "beams_8k", tokens=8191, batch=16, layers=4),
+        # a pool half of whose pages are free is compacted
+        _case("compact", "compact_pool", tokens=16384, batch=16, layers=2, dtype="bf16"),
+    ]
+
+
+def draw(rng):
+    def size(lo, hi):
+        t = int(lo * (hi / lo) ** rng.random())
+        return t | 1 if rng.random() < 0.7 else t
+
+    kind = rng.choice(("attend", "attend", "attend", "attend", "store", "beams", "compact"))
+    q, kv = rng.choice(HEADS)
+    c = dict(q_heads=q, kv_heads=kv, dtype=rng.choice(("fp16", "bf16")), codes=rng.choice(("int8", "int8", "e4m3")))
+    if kind == "store":
+        batch = rng.choice((1, 1, 2, 5))
+        return _case(kind, tokens=size(100, 32768 / batch), batch=batch, ragged=batch > 1 and rng.random() < 0.6, **c)
+    if kind == "beams":
+        batch = rng.choice((2, 4, 8, 16))
+        return _case(kind, tokens=size(64, 8192), batch=batch, layers=rng.choice((1, 2, 4)), **dict(c, codes="int8"))
+    if kind == "compact":
+        batch = rng.choice((3, 8, 16))
+        return _case(kind, tokens=size(500, 16384), batch=batch, layers=rng.choice((1, 2)), **dict(c, codes="int8"))
+    c.update(cap=rng.choice((0.0, 0.0, 20.0, 50.0)), bias=rng.random() < 0.3)
+    if rng.random() < 0.5:                                           # steps: one token a row, or a few
+        batch = rng.choice((1, 1, 3, 16))
+        tokens = size(65, 131072 / batch)
+        return _case("attend", tokens=tokens, batch=batch, queries=rng.choice((1, 1, 1, 2, 5)), ragged=batch > 1 and rng.random() < 0.7,
+                     window=rng.choice((0, 0, 0, 1000)), **c)
+    batch = rng.choice((1, 1, 2, 4))
+    queries = size(6, 2048 / batch)
+    tokens = queries + (0 if rng.random() < 0.3 else size(1, 12000 / batch))
+    return _case("attend", tokens=tokens, batch=batch, queries=queries, ragged=batch > 1 and rng.random() < 0.5, window=rng.choice((0, 0, 0, 300)),
+                 prefix=rng.choice((0, 0, tokens // 3)), documents=rng.choice((0, 0, 3)), **c)
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def _lengths(case, seed):
+    """Tokens of every row; a ragged batch's first row is the longest."""
+    n, least = case["tokens"], max(case["queries"] if case["kind"] == "attend" else 1, 1)
+    if not case["ragged"]:
+        return [n] * case["batch"]
+    g = torch.Generator().manual_seed(seed)
+    return [n] + [max(least, int(n * (0.3 + 0.7 * float(torch.rand(1, generator=g))))) for _ in range(case["batch"] - 1)]
+
+
+def _rows(case, gen, tokens):
+    """Keys and values [layers, batch, kv_heads, tokens, D]: keys with a few wide channels, values with a spread from token to token."""
+    shape = (case["layers"], case["batch"], case["kv_heads"], tokens, D)
+    k, v = (torch.randn(shape, generator=gen, device="cuda", dtype=torch.float32) for _ in range(2))
+    k[..., :4] *= 5.0
+    v *= 0.5 + torch.rand(shape[:-1], generator=gen, device="cuda").unsqueeze(-1)
+    return k.to(DTYPES[case["dtype"]]), v.to(DTYPES[case["dtype"]])
+
+
+def _mask_inputs(case, seed, lengths):
+    """Prefix lengths [batch] and the first visible position of every query [batch, queries], or None."""
+    L, prefix, starts = case["queries"], None, None
+    if case["prefix"]:
+        prefix = torch.tensor([min(case["prefix"], n) for n in lengths], dtype=torch.int32, device="cuda")
+    if case["documents"]:
+        g = torch.Generator().manual_seed(seed + 1)
+        rows = []
+        for n in lengths:
+            cuts = torch.cat([torch.zeros(1, dtype=torch.int64), torch.randint(1, max(n, 2), (case["documents"] - 1,), generator=g).sort().values])
+            at = torch.arange(n - L, n)
+            rows.append(cuts[torch.searchsorted(cuts, at, right=True) - 1])
+        starts = torch.stack(rows).to(torch.int32).cuda()
+    return prefix, starts
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    lengths = _lengths(case, seed)
+    kind, B, H, n = case["kind"], case["batch"], case["kv_heads"], case["tokens"]
+    state = dict(case=case, lengths=lengths)
+    if kind == "beams":
+        B = 2 * B                                                    # every beam's survivor and its copy
+        lengths = state["lengths"] = [n - 7 * (b % 10) if n > 100 else n for b in range(B)]
+        survivors = torch.randperm(B, generator=torch.Generator().manual_seed(seed))[:B // 2].sort().values
+        parents = torch.tensor([b if bool((survivors == b).any()) else int(survivors[b % (B // 2)]) for b in range(B)])
+        state["parents"] = parents.cuda()
+        state["counts"] = (parents != torch.arange(B)).to(torch.int32).cuda()      # the copies go on, what they come from stays for the next step
+        case = dict(case, batch=B)
+    k, v = _rows(case, gen, n)
+    if kind == "attend":
+        q = 2.0 * torch.randn(B, case["q_heads"], case["queries"], D, generator=gen, device="cuda")
+        state["q"] = q.to(DTYPES[case["dtype"]])
+        state["slopes"] = (torch.arange(1, case["q_heads"] + 1, device="cuda") * (-8.0 / case["q_heads"])).exp2().float() if case["bias"] else None
+        state["prefix"], state["starts"] = _mask_inputs(case, seed, lengths)
+    if kind == "store":
+        state["k"], state["v"] = k, v
+        state["counts"] = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    if kind == "beams":
+        k1, v1 = _rows(case, gen, 1)
+        state["k1"], state["v1"] = k1, v1
+    pages = _pages_of(case, lengths)
+    if own:
+        from kvquant import PagedKVCache
+        cache = state["cache"] = PagedKVCache(B, H, n + 1, layers=case["layers"], pages=pages, kind=case["codes"], dtype=DTYPES[case["dtype"]])
+        if kind != "store":
+            cache.extend(lengths)
+            for layer in range(case["layers"]):
+                cache.write(layer, k[layer], v[layer])
+        if kind == "compact":
+            cache.free(list(range(0, B, 2)))
+    else:
+        plain = state["plain"] = _plain_empty(case, B, n + 1, pages)
+        if kind != "store":
+            _plain_fill(plain, k, v, torch.tensor(lengths, device="cuda"))
+        if kind == "compact":
+            _plain_free(plain, range(0, B, 2))
+    if kind == "compact":
+        state["live"] = sum(m // BLOCK for m in lengths[1::2])
+    return state
+
+
+def _pages_of(case, lengths):
+    full = sum(m // BLOCK for m in lengths)
+    return max(1, full + (len(lengths) if case["kind"] == "beams" else 0))
+
+
+# ------------------------------------------------------------------------------------------------ the plain forms
+def _plain_empty(case, B, max_tokens, pages):
+    layers, H, blocks = case["layers"], case["kv_heads"], (max_tokens + BLOCK - 1) // BLOCK
+    z = lambda *shape, t: torch.zeros(shape, dtype=t, device="cuda")  # noqa: E731
+    codes, dtype = CODES[case["codes"]], DTYPES[case["dtype"]]
+    return dict(k_codes=z(layers, pages, H, BLOCK, D, t=codes), v_codes=z(layers, pages, H, D, BLOCK, t=codes),
+                k_scale=z(layers, pages, H, t=torch.float32), v_scale=z(layers, pages, H, t=torch.float32),
+                k_tail=z(layers, B, H, BLOCK, D, t=dtype), v_tail=z(layers, B, H, D, BLOCK, t=dtype),
+                table=z(B, blocks, t=torch.int32), length=z(B, t=torch.int32), slot=torch.arange(B, dtype=torch.int32, device="cuda"),
+                refs=z(pages, t=torch.int32), top=TOP[case["codes"]])
+
+
+def _plain_quantise(x, top, codes):
+    """x [..., BLOCK, D] -> codes and scales [...]."""
+    x = x.float()
+    a = x.abs().amax(dim=(-1, -2))
+    bits = (a / torch.full_like(a, top)).view(torch.int32)           # (a quotient by a number is a product with its reciprocal)
+    s = ((bits + 0xFFFF) & -0x10000).view(torch.float32)             # up to 8 significant bits
+    s = torch.where(a > 0, s.clamp(min=2.0 ** -100), torch.zeros_like(s))
+    y = x / torch.where(s > 0, s, torch.ones_like(s))[..., None, None]
+    return (y.round() if codes == torch.int8 else y).to(codes), s
+
+
+def _plain_fill(p, k, v, lengths):
+    """Rows that hold nothing take their first `lengths` of tokens [layers, B, H, T, D]."""
+    layers, B, H, T, _ = k.shape
+    blocks = (T + BLOCK - 1) // BLOCK
+    k, v = (torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0) for x in (k, v))
+    k, v = (torch.nn.functional.pad(x, (0, 0, 0, blocks * BLOCK - T)).view(layers, B, H, blocks, BLOCK, D) for x in (k, v))
+    full = lengths // BLOCK
+    taken = torch.arange(blocks, device="cuda") < full[:, None]      # [B, blocks]
+    free = torch.sort((p["refs"] > 0).int(), stable=True).indices    # the lowest free pages first
+    page = free[(torch.cumsum(taken.reshape(-1).int(), 0) - 1).clamp(min=0)].view(B, blocks)
+    b, j = taken.nonzero(as_tuple=True)
+    ids = page[b, j]
+    p["table"][b, j] = ids.int()
+    p["refs"][ids] = 1
+    codes = p["k_codes"].dtype
+    for x, name in ((k, "k"), (v, "v")):
+        c, s = _plain_quantise(x[:, b, :, j].transpose(0, 1), p["top"], codes)     # [layers, n, H, BLOCK, D]
+        c = c if name == "k" else c.transpose(-1, -2)
+        p[name + "_codes"].view(torch.int8)[:, ids] = c.contiguous().view(torch.int8)
+        p[name + "_scale"][:, ids] = s
+        tail = x[:, torch.arange(B, device="cuda"), :, full.clamp(max=blocks - 1)].transpose(0, 1)    # [layers, B, H, BLOCK, D]
+        tail = torch.where((torch.arange(BLOCK, device="cuda") < (lengths % BLOCK)[:, None])[None, :, None, :, None], tail, torch.zeros_like(tail))
+        p[name + "_tail"].copy_(tail if name == "k" else tail.transpose(-1, -2))
+    p["length"].copy_(lengths.int())
+
+
+def _plain_free(p, rows):
+    rows = torch.tensor(list(rows), device="cuda")
+    held = torch.arange(p["table"].shape[1], device="cuda") < (p["length"][rows] // BLOCK)[:, None]
+    p["refs"].index_add_(0, p["table"][p["slot"][rows].long()][held].long(), torch.full((int(held.sum()),), -1, dtype=torch.int32, device="cuda"))
+    p["length"][rows] = 0
+
+
+def _plain_dense(p, layer, T):
+    """Keys and values [B, H, T, D] in 32 bits, what lies behind a row's length 0."""
+    B, blocks = p["length"].shape[0], (T + BLOCK - 1) // BLOCK
+    slot, length = p["slot"].long(), p["length"]
+    table = p["table"][slot][:, :blocks].long()
+    at = torch.arange(blocks, device="cuda")
+    full, open_ = (at < (length // BLOCK)[:, None]), (at == (length // BLOCK)[:, None])
+    table = torch.where(full, table, torch.zeros_like(table))
+    held = (torch.arange(blocks * BLOCK, device="cuda") < length[:, None]).view(B, blocks, 1, BLOCK, 1)
+    out = []
+    for name in ("k", "v"):
+        c = p[name + "_codes"][layer].view(torch.int8)[table].view(p[name + "_codes"].dtype).float() * p[name + "_scale"][layer][table][..., None, None]
+        tail = p[name + "_tail"][layer][slot].float()[:, None].expand_as(c)
+        x = torch.where(open_[:, :, None, None, None], tail, c)
+        x = x if name == "k" else x.transpose(-1, -2)
+        x = torch.where(held, x, torch.zeros_like(x))
+        out.append(x.transpose(1, 2).reshape(B, -1, blocks * BLOCK, D)[:, :, :T])
+    return out
+
+
+def _visible(case, T, length, prefix, starts, dtype):
+    """[B, queries, T] truth values, and |i - j| of `dtype`."""
+    L = case["queries"]
+    i = length.long()[:, None] - L + torch.arange(L, device="cuda")  # [B, L]
+    j = torch.arange(T, device="cuda")
+    lo = torch.zeros_like(i) if starts is None else starts.long()
+    if case["window"]:
+        lo = torch.maximum(lo, i - case["window"] + 1)
+    hi = i + 1 if prefix is None else torch.maximum(i + 1, prefix.long()[:, None])
+    hi = torch.minimum(hi, length.long()[:, None])
+    return (j >= lo[..., None]) & (j < hi[..., None]), (i[..., None] - j).abs().to(dtype)
+
+
+def _softmax_times(x, seen, values):
+    """softmax over the seen places of x [..., T] times values, and the log of its sum; a row that sees nothing: 0 and -inf."""
+    x = x.masked_fill(~seen, -math.inf)
+    top = x.amax(dim=-1, keepdim=True)
+    top = torch.where(top > -math.inf, top, torch.zeros_like(top))
+    e = (x - top).exp()
+    total = e.sum(dim=-1, keepdim=True)
+    out = torch.matmul(e, values) / torch.where(total > 0, total, torch.ones_like(total))
+    return out, total.log() + top
+
+
+def _plain_attend(s):
+    case, p = s["case"], s["plain"]
+    B, H, L, G = case["batch"], case["kv_heads"], case["queries"], case["q_heads"] // case["kv_heads"]
+    k, v = _plain_dense(p, 0, case["tokens"])
+    q = s["q"].float().view(B, H, G * L, D)
+    x = torch.matmul(q, k.transpose(-1, -2).contiguous()) * D ** -0.5
+    seen, distance = _visible(case, case["tokens"], p["length"], s["prefix"], s["starts"], torch.float32)
+    if case["cap"]:
+        x = case["cap"] * torch.tanh(x / case["cap"])
+    x = x.view(B, H, G, L, -1)
+    if case["bias"]:
+        x = x - s["slopes"].view(1, H, G, 1, 1) * distance[:, None, None]
+    out, lse = _softmax_times(x, seen[:, None, None], v.unsqueeze(2))
+    return out.view(B, H * G, L, D).transpose(1, 2).contiguous().to(s["q"].dtype), lse.view(B, H * G, L)
+
+
+def _plain_store(s):
+    case, p = s["case"], s["plain"]
+    _plain_free(p, range(case["batch"]))
+    _plain_fill(p, s["k"], s["v"], s["counts"])
+    k, v = _plain_dense(p, 0, case["tokens"])
+    return k.to(s["k"].dtype), v.to(s["k"].dtype)
+
+
+def _plain_beams(s):
+    p, parents = s["plain"], s["parents"]
+    B = parents.shape[0]
+    rows, slot, length = torch.arange(B, device="cuda"), p["slot"].long(), p["length"].long()
+    at = torch.arange(p["table"].shape[1], device="cuda")
+    # a row whose parent has not kept its own place, or is not its first child, takes a place that nobody uses any more, lowest first
+    kept = torch.zeros(B, dtype=torch.bool, device="cuda").scatter_(0, parents, True)
+    first = torch.full((B,), B, device="cuda").scatter_reduce_(0, parents, rows, "amin")
+    first = torch.where(parents[rows] == rows, rows, first)          # by parent: the row that takes over its place
+    over = first[parents] == rows
+    unused = torch.sort(torch.where(kept, torch.full_like(slot, B), slot)).values
+    source = slot[parents]
+    target = torch.where(over, source, unused[(torch.cumsum((~over).int(), 0) - 1).clamp(min=0)])
+    dropped = (at < (length // BLOCK)[:, None]) & ~kept[:, None]
+    p["refs"].index_add_(0, p["table"][slot][dropped].long(), torch.full((int(dropped.sum()),), -1, dtype=torch.int32, device="cuda"))
+    shared = (at < (length[parents] // BLOCK)[:, None]) & ~over[:, None]
+    p["refs"].index_add_(0, p["table"][source][shared].long(), torch.ones(int(shared.sum()), dtype=torch.int32, device="cuda"))
+    for name, dim in (("table", 0), ("k_tail", 1), ("v_tail", 1)):
+        p[name].index_copy_(dim, target[~over], p[name].index_select(dim, source[~over]))
+    slot, length = target, length[parents]
+    p["slot"].copy_(slot)
+    # one token a row that goes on
+    goes_on = s["counts"] > 0
+    place, to = (length % BLOCK)[goes_on], slot[goes_on]
+    p["k_tail"][:, to, :, place] = s["k1"][:, goes_on, :, 0].transpose(0, 1)
+    p["v_tail"][:, to, :, :, place] = s["v1"][:, goes_on, :, 0].transpose(0, 1)
+    done = goes_on & (length % BLOCK == BLOCK - 1)
+    free = torch.sort((p["refs"] > 0).int(), stable=True).indices
+    ids = free[(torch.cumsum(done.int(), 0) - 1).clamp(min=0)][done]
+    p["table"][slot[done], length[done] // BLOCK] = ids.int()
+    p["refs"][ids] = 1
+    for name in ("k", "v"):
+        x = p[name + "_tail"][:, slot[done]]
+        c, sc = _plain_quantise(x, p["top"], p["k_codes"].dtype)
+        p[name + "_codes"][:, ids], p[name + "_scale"][:, ids] = c, sc
+    p["length"].copy_(length + s["counts"])
+    return [p[n] for n in ("slot", "length", "table", "refs", "k_codes", "v_codes", "k_scale", "v_scale", "k_tail", "v_tail")]
+
+
+def _plain_compact(s):
+    p = s["plain"]
+    live = (p["refs"] > 0).nonzero().view(-1)
+    to = torch.cumsum((p["refs"] > 0).int(), 0) - 1
+    held = torch.zeros_like(p["table"], dtype=torch.bool)
+    held[p["slot"].long()] = torch.arange(p["table"].shape[1], device="cuda") < (p["length"] // BLOCK)[:, None]
+    table = torch.where(held, to[p["table"].long()].int(), torch.zeros_like(p["table"]))
+    return [table, p["refs"][live]] + [p[n][:, live] for n in ("k_codes", "v_codes", "k_scale", "v_scale")]
+
+
+def run(state):
+    case, kind = state["case"], state["case"]["kind"]
+    if not own:
+        return {"attend": _plain_attend, "store": _plain_store, "beams": _plain_beams, "compact": _plain_compact}[kind](state)
+    cache = state["cache"]
+    if kind == "attend":
+        return cache.attend(0, state["q"], softcap=case["cap"] or None, slopes=state["slopes"], window=case["window"] or None, prefix=state["prefix"],
+                            starts=state["starts"], return_lse=True)
+    if kind == "store":
+        cache.free()
+        cache.extend(state["counts"], bound=case["tokens"])
+        cache.write(0, state["k"][0], state["v"][0])
+        return cache.read(0, case["tokens"])
+    if kind == "beams":
+        cache.reorder(state["parents"])
+        cache.extend(state["counts"], bound=1)
+        for layer in range(case["layers"]):
+            cache.write(layer, state["k1"][layer], state["v1"][layer])
+        return [cache.slot, cache.length, cache.table, cache.refs, cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail]
+    new = cache.compacted(pages=state["live"])
+    return [new.table, new.refs, new.k_codes, new.v_codes, new.k_scale, new.v_scale]
+
+
+# ------------------------------------------------------------------------------------------------ what a pass cannot do without
+def work(case):
+    lengths = _lengths(case, 0)
+    H, G, L = case["kv_heads"], case["q_heads"] // case["kv_heads"], case["queries"]
+    page = 2 * BLOCK * D + 8                                         # codes and scales of a block and head
+    if case["kind"] == "store":                                      # stored: 16 bits in, 8 out; read back the other way
+        return dict(bytes=sum(lengths) * H * D * 12 + 2 * case["batch"] * H * page // 8, flops=sum(lengths) * H * D * 6)
+    if case["kind"] == "beams":                                      # tails of the copies, a token a row, the blocks that it completes
+        B = 2 * case["batch"]
+        full = sum((case["tokens"] - 7 * (b % 10) if case["tokens"] > 100 else case["tokens"]) % BLOCK == BLOCK - 1 for b in range(B)) // 2
+        return dict(bytes=case["layers"] * H * (B // 2 * (2 * 4 * BLOCK * D + 8 * D) + full * page), flops=0)
+    if case["kind"] == "compact":
+        return dict(bytes=2 * case["layers"] * H * page * sum(m // BLOCK for m in lengths[1::2]), flops=0)
+    pairs = tokens = 0
+    for n in lengths:                                                # pairs of a query and a token that it sees (documents: of equal length)
+        window, span = case["window"] or n, n // max(case["documents"], 1)
+        first = n - L
+        low = max(0, first - window + 1) if not case["documents"] else max(0, first - span)
+        tokens += n - low
+        for i in range(first, n):
+            seen = min(i + 1, window)
+            seen = min(seen, i % span + 1) if case["documents"] else seen
+            pairs += seen + max(0, min(case["prefix"], n) - i - 1)
+    return dict(bytes=tokens * H * 2 * D + case["batch"] * case["q_heads"] * L * (4 * D + 4), flops=4 * D * H * G * pairs)
+
+
+# ------------------------------------------------------------------------------------------------ the definition in 64 bits
+def _power_of_two(e):
+    """2^e in 64 bits (torch.ldexp goes through a power that is an ulp off here and there on the GPU)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def _exact_scale(a, top):
+    """The smallest number of 8 significant bits that is not below a / top."""
+    a = a.double()
+    m, e = torch.frexp(a / top)
+    s = torch.ceil(m * 256.0) * _power_of_two(e - 8)
+    return torch.where(a > 0, s.clamp(min=2.0 ** -100), torch.zeros_like(s))
+
+
+def _exact_values(x, kind):
+    """What the cache holds of blocks x [..., BLOCK, D] in 64 bits: codes times scales."""
+    x = x.double()
+    s = _exact_scale(x.abs().amax(dim=(-1, -2), keepdim=True), TOP[kind])
+    y = x / torch.where(s > 0, s, torch.ones_like(s))
+    if kind == "e4m3":                                               # steps of 2^(e - 3) from 2^e to 2^(e + 1), of 2^-9 below 2^-6
+        step = _power_of_two(torch.frexp(y.abs().clamp(min=2.0 ** -6)).exponent - 4)
+        return (y / step).round() * step * s
+    return y.round() * s
+
+
+def _exact_rows(x, lengths, kind):
+    """x [B, H, T, D] as the cache holds it, 0 behind a row's length."""
+    out = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    for b, n in enumerate(lengths):
+        full = n // BLOCK * BLOCK
+        out[b, :, full:n] = x[b, :, full:n].double()
+        if full:
+            out[b, :, :full] = _exact_values(x[b, :, :full].reshape(x.shape[1], -1, BLOCK, D), kind).view(x.shape[1], full, D)
+    return out
+
+
+def exact(case, seed):
+    if case["kind"] in ("beams", "compact"):
+        return None                                                  # copies and whole numbers
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    lengths = _lengths(case, seed)
+    k, v = _rows(case, gen, case["tokens"])
+    ek, ev = (_exact_rows(x[0], lengths, case["codes"]) for x in (k, v))
+    if case["kind"] == "store":
+        return ek, ev
+    B, H, L, G = case["batch"], case["kv_heads"], case["queries"], case["q_heads"] // case["kv_heads"]
+    q = 2.0 * torch.randn(B, case["q_heads"], L, D, generator=gen, device="cuda")
+    q = q.to(DTYPES[case["dtype"]]).double()
+    prefix, starts = _mask_inputs(case, seed, lengths)
+    length = torch.tensor(lengths, device="cuda")
+    out = torch.zeros(B, L, H * G, D, dtype=torch.float64, device="cuda")
+    lse = torch.zeros(B, H * G, L, dtype=torch.float64, device="cuda")
+    for b in range(B):
+        row = lambda t: None if t is None else t[b:b + 1]  # noqa: E731
+        seen, distance = _visible(case, case["tokens"], length[b:b + 1], row(prefix), row(starts), torch.float64)
+        for h in range(H * G):
+            x = (q[b, h] @ ek[b, h // G].T) / math.sqrt(D)
+            if case["cap"]:
+                x = case["cap"] * torch.tanh(x / case["cap"])
+            if case["bias"]:
+                x = x - 2.0 ** (-8.0 * (h + 1) / case["q_heads"]) * distance[0]
+            x = torch.where(seen[0], x, torch.full_like(x, -math.inf))
+            lse[b, h] = torch.logsumexp(x, dim=-1)
+            weights = torch.where(seen[0], torch.exp(x - torch.where(lse[b, h] > -math.inf, lse[b, h], torch.zeros_like(lse[b, h]))[:, None]), torch.zeros_like(x))
+            out[b, :, h] = weights @ ev[b, h // G]
+    return out, lse

@@ -140,8 +140,9 @@ def prepare(case, seed):
         lengths = state["lengths"] = [n - 7 * (b % 10) if n > 100 else n for b in range(B)]
         survivors = torch.randperm(B, generator=torch.Generator().manual_seed(seed))[:B // 2].sort().values
         parents = torch.tensor([b if bool((survivors == b).any()) else int(survivors[b % (B // 2)]) for b in range(B)])
-        state["parents"] = parents.cuda()
-        state["counts"] = (parents != torch.arange(B)).to(torch.int32).cuda()      # the copies go on, what they come from stays for the next step
+        counts = (parents != torch.arange(B)).to(torch.int32)        # the copies go on, what they come from stays for the next step
+        state["parents"], state["counts"] = parents.cuda(), counts.cuda()
+        state["parents_list"], state["counts_list"] = parents.tolist(), counts.tolist()
         case = dict(case, batch=B)
     k, v = _rows(case, gen, n)
     if kind == "attend":
@@ -177,8 +178,10 @@ def prepare(case, seed):
 
 
 def _pages_of(case, lengths):
-    full = sum(m // BLOCK for m in lengths)
-    return max(1, full + (len(lengths) if case["kind"] == "beams" else 0))
+    """Pages of the pool: what the rows fill, and for rows that go on or come again what they may take besides."""
+    if case["kind"] == "store":
+        return len(lengths) * ((case["tokens"] + BLOCK - 1) // BLOCK)
+    return max(1, sum(m // BLOCK for m in lengths) + (2 * len(lengths) if case["kind"] == "beams" else 0))
 
 
 # ------------------------------------------------------------------------------------------------ the plain forms
@@ -368,8 +371,8 @@ def run(state):
         cache.write(0, state["k"][0], state["v"][0])
         return cache.read(0, case["tokens"])
     if kind == "beams":
-        cache.reorder(state["parents"])
-        cache.extend(state["counts"], bound=1)
+        cache.reorder(state["parents_list"])
+        cache.extend(state["counts_list"])
         for layer in range(case["layers"]):
             cache.write(layer, state["k1"][layer], state["v1"][layer])
         return [cache.slot, cache.length, cache.table, cache.refs, cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail]

@@ -604,6 +604,95 @@ int odmkv_decode_attn_static(const void* q, int q_dtype, int B, int Hq, float sc
                              const float* codebooks_host, const float* inv_scales,
                              void* out, int out_dtype, float* lse, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged 8-bit cache: every token at 8 bits, a scale for each block of 64 tokens and kv-head, rows (sequences) of a batch that
+ * grow, fork, shrink and share pages.  No counterpart in the reference.
+ *
+ * Tokens [64 j, 64 j + 64) of a row are its block j.  A full block lies in a page and is never written again; the newest
+ * tokens, fewer than 64, stay in 16 bits in the row's tail, so that what the cache holds does not depend on how the tokens
+ * arrived.  A value that is not finite is stored as 0.  Of a block's values x of one kv-head (keys and values apart), with
+ * a = max |x|, the scale s is the smallest number of 8 significant bits that is not below a / top (top: 127 for int8, 448 for
+ * e4m3) and at least 2^-100 (0 where a is 0); a code is x / s to the nearest, ties to even, and stands for code * s.
+ *
+ * The bookkeeping (lengths, tables, counts of a page's holders) lies on the device and is shared by all layers: no call reads
+ * anything back, and calls that are captured into a graph go on from where the rows are at each replay.  A call that cannot be
+ * carried out (too few pages, a row longer than its table) changes nothing but status[2], which it sets to 1; callers that
+ * know the lengths see to it before the call.  All calls on a cache are ordered by the caller (one stream, or events).
+ */
+#define ODMKV_INT8 0
+#define ODMKV_E4M3 1
+#define ODMKV_PAGES_MAX_ROWS 1024
+
+typedef struct odmkv_pages {
+    int32_t layers, rows, Hkv, pages, blocks;    /* blocks: places of a table row, so at most blocks * 64 + 63 tokens a row */
+    int32_t dtype;                               /* ODMKV_F16 / ODMKV_BF16: the tails, new tokens, queries */
+    int32_t kind;                                /* ODMKV_INT8 / ODMKV_E4M3 */
+    uint8_t* kcodes;                             /* device [layers, pages, Hkv, 64, 128] */
+    uint8_t* vcodes;                             /* device [layers, pages, Hkv, 128, 64]: values dim by dim */
+    float* kscale;                               /* device [layers, pages, Hkv] */
+    float* vscale;
+    uint16_t* ktail;                             /* device [layers, rows, Hkv, 64, 128], by slot */
+    uint16_t* vtail;                             /* device [layers, rows, Hkv, 128, 64], by slot */
+    int32_t* table;                              /* device [rows, blocks], by slot: the page of a full block */
+    int32_t* length;                             /* device [rows] tokens of a row */
+    int32_t* start;                              /* device [rows] length before the last odmkv_pages_extend */
+    int32_t* slot;                               /* device [rows] where a row's table and tail lie */
+    int32_t* refs;                               /* device [pages] how many rows hold a page */
+    int32_t* status;                             /* device [4]: free pages, a page below which none is free, refused, live pages */
+} odmkv_pages_t;
+
+/* An empty cache: lengths 0, row b in slot b, all pages free, table and tails cleared. */
+int odmkv_pages_init(const odmkv_pages_t* p, void* stream);
+/* Every row grows by its count of tokens: device int32 [rows], or NULL: `count` for all.  Blocks that become full get the
+ * lowest free pages, row after row.  max_count: no count is larger (a larger or negative one refuses the call). */
+int odmkv_pages_extend(const odmkv_pages_t* p, const int32_t* counts, int count, int max_count, void* stream);
+/* The tokens that the last extend made room for, of one layer (once a layer and extend): K, V [rows, Hkv, T, 128] of the
+ * cache's dtype with element strides (multiples of 8, 16-byte aligned), row b's tokens at t < its count; T at least max_count. */
+int odmkv_pages_write(const odmkv_pages_t* p, int layer, const void* K, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t,
+                      const void* V, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, int T, void* stream);
+/* Dense keys and values of one layer, [rows, Hkv, T, 128] contiguous of out_dtype (any), 0 behind a row's length. */
+int odmkv_pages_read(const odmkv_pages_t* p, int layer, void* K, void* V, int out_dtype, int T, void* stream);
+/* Row b becomes a copy of row parents[b] (device int64 [rows], all at once): full blocks are shared, tails copied.  A row
+ * that stays, or else the first copy of one that does not, keeps its place.  A parent out of range refuses the call. */
+size_t odmkv_pages_reorder_workspace_bytes(int rows);
+int odmkv_pages_reorder(const odmkv_pages_t* p, const int64_t* parents, void* workspace, size_t workspace_bytes, void* stream);
+/* The rows of `to` (another batch over the same pages: same codes, scales, refs, status; its own table, tails, length, start,
+ * slot, rows; its rows hold nothing yet) become copies of rows parents[b] of p (device int64 [to->rows]).  p's rows stay. */
+int odmkv_pages_select(const odmkv_pages_t* p, const odmkv_pages_t* to, const int64_t* parents, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* Rows shrink to a length (device int32 [rows], or NULL: `length` for all; a longer one leaves the row): pages that nobody
+ * holds any more are free; a full block that is cut becomes the tail, as the values that it stands for.  row_mask: host
+ * uint32 [32], bit b of word b / 32 set for the rows meant, or NULL: all. */
+int odmkv_pages_truncate(const odmkv_pages_t* p, const int32_t* lengths, int length, const uint32_t* row_mask, void* stream);
+/* `to` (pages of its own, at least as many as p has in use; blocks of its own, at least what p's rows need; the rest as p's)
+ * becomes what p is, its pages in use one behind the other in their order.  workspace: 4 bytes a page of p. */
+size_t odmkv_pages_compact_workspace_bytes(int pages);
+int odmkv_pages_compact(const odmkv_pages_t* p, const odmkv_pages_t* to, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of the newest tokens' queries over the cache: query l of row b's n (counts[b], or L) stands at position
+ * i = length - n + l and sees the tokens lo <= j < hi,
+ *   lo = max(0, start of l, i - window + 1 if window > 0),  hi = min(max(i + 1, prefix), length):
+ *   x_j = scaling * q . k_j;  cap > 0: x_j = cap * tanh(x_j / cap);  slopes: x_j -= slope * |i - j|;
+ *   out = sum_j softmax(x)_j v_j,  lse = log sum_j exp(x_j);  a query that sees nothing: 0 and -inf.
+ * q [rows, Hq, L, 128] of the cache's dtype with element strides (multiples of 8, 16-byte aligned), row b's queries at l < n;
+ * out [rows, L, Hq, 128] of that dtype and lse fp32 [rows, Hq, L] contiguous; what belongs to l >= n is left as it was. */
+typedef struct odmkv_attend {
+    const odmkv_pages_t* pages;
+    const void* q; int64_t q_stride_b, q_stride_h, q_stride_l;
+    void* out;
+    float* lse;                                  /* or NULL */
+    const int32_t* counts;                       /* device [rows], or NULL: L each */
+    const float* slopes;                         /* device [Hq], or NULL */
+    const int32_t* prefix;                       /* device [rows], or NULL */
+    const int32_t* starts; int64_t start_stride_b, start_stride_l;     /* device, or NULL */
+    void* workspace; size_t workspace_bytes;
+    int32_t layer, L, Hq, window;
+    int32_t max_length;                          /* about how long the longest row is: how the work is cut, not what is seen */
+    float scaling, cap;                          /* cap 0: none */
+} odmkv_attend_t;
+size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length);
+int odmkv_pages_attend(const odmkv_attend_t* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -81,6 +81,21 @@ class Prompt(C.Structure):
                 + [("eps", C.c_float)])
 
 
+class Pages(C.Structure):
+    """struct odmkv_pages of include/odmkv.h."""
+    _fields_ = ([(n, C.c_int32) for n in ("layers", "rows", "Hkv", "pages", "blocks", "dtype", "kind")]
+                + [(n, C.c_void_p) for n in ("kcodes", "vcodes", "kscale", "vscale", "ktail", "vtail", "table", "length", "start", "slot",
+                                             "refs", "status")])
+
+
+class Attend(C.Structure):
+    """struct odmkv_attend of include/odmkv.h."""
+    _fields_ = ([("pages", C.POINTER(Pages)), ("q", C.c_void_p)] + [(n, C.c_int64) for n in ("q_stride_b", "q_stride_h", "q_stride_l")]
+                + [(n, C.c_void_p) for n in ("out", "lse", "counts", "slopes", "prefix", "starts")]
+                + [("start_stride_b", C.c_int64), ("start_stride_l", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+                + [(n, C.c_int32) for n in ("layer", "L", "Hq", "window", "max_length")] + [("scaling", C.c_float), ("cap", C.c_float)])
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -161,6 +176,18 @@ def _load() -> C.CDLL:
         "odmkv_exact_tail": (C.c_int, [C.POINTER(Packed), i32, vp, vp, vp]),
         "odmkv_flush_score": (C.c_int, [vp, vp, i32, i32, i32, vp, f32, f32, i32, vp, vp, vp, vp]),
         "odmkv_flush_rank": (C.c_int, [vp, vp, i32, i32, i32, vp, vp, vp]),
+        "odmkv_pages_init": (C.c_int, [C.POINTER(Pages), vp]),
+        "odmkv_pages_extend": (C.c_int, [C.POINTER(Pages), vp, i32, i32, vp]),
+        "odmkv_pages_write": (C.c_int, [C.POINTER(Pages), i32, vp, i64, i64, i64, vp, i64, i64, i64, i32, vp]),
+        "odmkv_pages_read": (C.c_int, [C.POINTER(Pages), i32, vp, vp, i32, i32, vp]),
+        "odmkv_pages_reorder_workspace_bytes": (sz, [i32]),
+        "odmkv_pages_reorder": (C.c_int, [C.POINTER(Pages), vp, vp, sz, vp]),
+        "odmkv_pages_select": (C.c_int, [C.POINTER(Pages), C.POINTER(Pages), vp, vp, sz, vp]),
+        "odmkv_pages_truncate": (C.c_int, [C.POINTER(Pages), vp, i32, vp, vp]),
+        "odmkv_pages_compact_workspace_bytes": (sz, [i32]),
+        "odmkv_pages_compact": (C.c_int, [C.POINTER(Pages), C.POINTER(Pages), vp, sz, vp]),
+        "odmkv_pages_attend_workspace_bytes": (sz, [C.POINTER(Pages), i32, i32, i32]),
+        "odmkv_pages_attend": (C.c_int, [C.POINTER(Attend), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -181,7 +208,9 @@ EXPORTS = ("odmkv_version", "odmkv_last_error", "odmkv_score_workspace_bytes", "
            "odmkv_dequantize_rows", "odmkv_quantize_rows_packed", "odmkv_dequantize_rows_packed",
            "odmkv_round_trip_workspace_bytes", "odmkv_round_trip_rows", "odmkv_lloyd_max", "odmkv_dequant", "odmkv_dequant_from", "odmkv_append_exact", "odmkv_append_exact_rows", "odmkv_drop_exact_tail", "odmkv_truncate",
            "odmkv_worklist_cut", "odmkv_decode_workspace_bytes", "odmkv_rotation_operands", "odmkv_decode_attn", "odmkv_decode_attn_static",
-           "odmkv_decode_step", "odmkv_decode_block_workspace_bytes", "odmkv_decode_block", "odmkv_block_merge", "odmkv_exact_tail", "odmkv_flush_score", "odmkv_flush_rank")
+           "odmkv_decode_step", "odmkv_decode_block_workspace_bytes", "odmkv_decode_block", "odmkv_block_merge", "odmkv_exact_tail", "odmkv_flush_score", "odmkv_flush_rank",
+           "odmkv_pages_init", "odmkv_pages_extend", "odmkv_pages_write", "odmkv_pages_read", "odmkv_pages_reorder_workspace_bytes", "odmkv_pages_reorder", "odmkv_pages_select",
+           "odmkv_pages_truncate", "odmkv_pages_compact_workspace_bytes", "odmkv_pages_compact", "odmkv_pages_attend_workspace_bytes", "odmkv_pages_attend")
 
 
 def check(rc: int) -> None:

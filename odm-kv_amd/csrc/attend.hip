@@ -5,6 +5,10 @@
 #include <algorithm>
 #include "pages.h"
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
 struct AttendArgs {
     odmkv_pages_t p;
     const uint16_t* q;
@@ -18,7 +22,13 @@ struct AttendArgs {
     int64_t sb, sl;
     int layer, L, Hq, G, window;
     float scaling, cap;
+    int splits;          // workgroups that share a row and kv-head's blocks
+    float* part_out;     // [rows, Hkv, splits, G L, 128]
+    float* part_lse;     // [rows, Hkv, splits, G L], base 2
 };
+
+#define LOG2E 1.4426950408889634f
+#define LN2 0.6931471805599453f
 
 // what query l of a row of `len` tokens, `n` of whose newest have queries, stands at and sees
 struct Sight { int pos, lo, hi; };
@@ -31,6 +41,361 @@ __device__ static inline Sight sight_of(const AttendArgs& a, int row, int len, i
     if (a.prefix) s.hi = max(s.hi, a.prefix[row]);
     s.hi = s.pos < 0 ? 0 : min(s.hi, len);
     return s;
+}
+
+// tanh: by its series where 1 - e loses digits, else by e = exp(-2 |t|)
+__device__ static inline float tanh_of(float t) {
+    const float a = fabsf(t), b = t * t;
+    float f = __fmaf_rn(b, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    f = __fmaf_rn(b, f, -17.0f / 315.0f);
+    f = __fmaf_rn(b, f, 2.0f / 15.0f);
+    f = __fmaf_rn(b, f, -1.0f / 3.0f);
+    const float e = __builtin_amdgcn_exp2f(-2.0f * LOG2E * a);
+    const float far = __builtin_copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), t);
+    return a < 0.3f ? __fmaf_rn(t * b, f, t) : far;
+}
+
+// eight codes as fp16, all of them exactly.  int8: c + 128 is the low byte of the fp16 number 1024 + (c + 128)
+template <int KIND>
+__device__ static inline f16x8 codes_f16(uint32_t w0, uint32_t w1) {
+    f16x2 h[4];
+    if constexpr (KIND == ODMKV_E4M3) {
+        h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false);
+        h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true);
+        h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false);
+        h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
+    } else {
+        const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+        w0 ^= 0x80808080u;
+        w1 ^= 0x80808080u;
+        h[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u)) + off;
+        h[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u)) + off;
+        h[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u)) + off;
+        h[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)) + off;
+    }
+    return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+}
+
+// 16-bit numbers on the fp16 matrix cores: times a power of two that takes the largest of them (its bits: `top`) to 64 .. 128.  Nothing that counts
+// is lost: what falls out of fp16's range is 2^-31 of the largest and less.
+struct Power { float up, down; };
+template <int DT>
+__device__ static inline Power power_for(uint32_t top) {
+    const float t = Elem<DT>::to_f32((uint16_t)top);
+    const int e = min(max((int)(__float_as_uint(t) >> 23) - 127, -100), 127);
+    return {__uint_as_float((uint32_t)(127 + 6 - e) << 23), __uint_as_float((uint32_t)(127 - 6 + e) << 23)};
+}
+template <int DT>
+__device__ static inline f16x8 scaled_f16(const uint4& v, float up) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    f16x8 h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[2 * i] = (_Float16)(Elem<DT>::to_f32((uint16_t)(w[i] & 0xffffu)) * up);
+        h[2 * i + 1] = (_Float16)(Elem<DT>::to_f32((uint16_t)(w[i] >> 16)) * up);
+    }
+    return h;
+}
+__device__ static inline uint32_t abs_max8(const uint4& v) {
+    return max(max(abs_max_pair(v.x), abs_max_pair(v.y)), max(abs_max_pair(v.z), abs_max_pair(v.w)));
+}
+
+// over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a query
+template <typename F>
+__device__ static inline float column_fold(float v, F f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ static inline float column_max(float v) { return column_fold(v, [](float x, float y) { return fmaxf(x, y); }); }
+__device__ static inline float column_sum(float v) { return column_fold(v, [](float x, float y) { return x + y; }); }
+__device__ static inline uint32_t larger_bits(uint32_t v, bool whole_wave) {
+    const auto f = [](float x, float y) { return __uint_as_float(max(__float_as_uint(x), __float_as_uint(y))); };
+    return __float_as_uint(whole_wave ? wave_fold(__uint_as_float(v), f) : column_fold(__uint_as_float(v), f));
+}
+__device__ static inline int wave_min_int(int v) {
+    return __float_as_int(wave_fold(__int_as_float(v), [](float x, float y) { return __int_as_float(min(__float_as_int(x), __float_as_int(y))); }));
+}
+
+// ---- up to sixteen queries of a kv-head -----------------------------------------------------------
+// A step of one token (G query heads share a kv-head's keys), or of a few.  The queries are the sixteen columns of the matrix instructions: keys times
+// queries (rows: 16 tokens), then values times weights (rows: 16 dims, contraction: 32 tokens).  Which token a row of the first product is, is free:
+// row 4 j + r of product tb is token 16 j + 4 tb + r, so that a lane ends with the weights of the sixteen tokens whose values of a dim it reads as
+// one piece of 16 bytes; and lane (n, j) takes dims 32 j .. 32 j + 31 of its token, 32 bytes that lie together.  No weight changes lanes.
+//
+// Codes are exact in fp16, queries as they are (bf16: times a power of two each), products and sums fp32; a block's scale joins the scores and, for values,
+// the weights: weights are rounded to fp16 (half a step, 2^-12 to 2^-11 of themselves) times 2^7 s / (largest s of the wavefront's blocks).
+//
+// A wavefront takes every fourth block of its workgroup's share, its pages and scales looked up 64 at a time, the next block's keys and values requested
+// as soon as this one's are used.  Bound by memory (256 bytes a token and head); the arithmetic of a block is about a third of the time its bytes take.
+#define NARROW 16
+#define NARROW_WAVES 4
+#define RISE 8.0f            // how far scores may pass the reference (base 2) before the sums are brought to a new one
+
+template <int DT, int KIND, bool PLAIN>
+__global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(AttendArgs a) {
+    const odmkv_pages_t& p = a.p;
+    __shared__ __align__(16) float acc_of[NARROW_WAVES][NARROW][HD + 4];
+    __shared__ float ref_of[NARROW_WAVES][NARROW], sum_of[NARROW_WAVES][NARROW];
+    const int split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits, row = pair / p.Hkv, h = pair % p.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, j = lane >> 4;
+    const int R = a.G * a.L, len = p.length[row], count = a.counts ? min(max(a.counts[row], 0), a.L) : a.L, slot = p.slot[row];
+    const int l = n / a.G, hq = h * a.G + n - l * a.G;
+    const bool valid = n < R && l < count;
+    Sight s = {0, 0, 0};
+    if (valid) s = sight_of(a, row, len, count, l);
+    const bool sees = valid && s.lo < s.hi;
+    const int first = wave_min_int(sees ? s.lo : 0x7fffffff) / BLOCK_TOKENS;
+    const int last = (-wave_min_int(sees ? -s.hi : 0) + BLOCK_TOKENS - 1) / BLOCK_TOKENS;        // one past the last block that is seen
+    // blocks from lo_max on and up to hi_min are seen by every query
+    const int lo_max = valid && !sees ? 0x7fffffff : s.lo;
+    const int open_from = -wave_min_int(valid ? -lo_max : 0), open_to = wave_min_int(valid ? s.hi : 0x7fffffff);
+    const int blocks = max(last - first, 0), share = (blocks + a.splits - 1) / a.splits;
+    const int b0 = first + split * share, mine = min(share, blocks - split * share);             // may be negative: nothing to do
+    const int full = len / BLOCK_TOKENS;
+
+    f16x8 q[4];
+    float qdown = 1.0f;
+    {
+        uint4 raw[4];
+        const uint16_t* src = a.q + row * a.qb + hq * a.qh + l * a.ql + 32 * j;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) raw[kk] = valid ? *reinterpret_cast<const uint4*>(src + 8 * kk) : make_uint4(0, 0, 0, 0);
+        if constexpr (DT == ODMKV_BF16) {
+            const uint32_t top = larger_bits(max(max(abs_max8(raw[0]), abs_max8(raw[1])), max(abs_max8(raw[2]), abs_max8(raw[3]))), false);
+            const Power pw = power_for<DT>(top);
+            qdown = pw.down;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) q[kk] = scaled_f16<DT>(raw[kk], pw.up);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) q[kk] = __builtin_bit_cast(f16x8, raw[kk]);
+        }
+    }
+    const float slope = !PLAIN && a.slopes && valid ? a.slopes[hq] * LOG2E : 0.0f;
+    const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const float qs = a.scaling * qdown * (PLAIN ? LOG2E : 1.0f);
+
+    float ref = -INFINITY, sum = 0.0f, vref = 0.0f;
+    f32x4 acc[8];
+#pragma unroll
+    for (int m = 0; m < 8; ++m) acc[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // raw products of a block to weights: x [tb][r] is token 64 block + 16 j + 4 tb + r.  Back come the weights as operands, times f.
+    const auto weigh = [&](const f32x4* dot, int block, float ks, float f, f16x8* w) {
+        float x[16];
+        const float c = ks * qs;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = dot[i >> 2][i & 3] * c;
+        const int t0 = block * BLOCK_TOKENS + 16 * j;
+        if constexpr (!PLAIN) {
+            if (inv_cap > 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = a.cap * tanh_of(x[i] * inv_cap);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = __fmaf_rn(x[i], LOG2E, -slope * fabsf((float)(s.pos - t0 - i)));
+        }
+        if (block * BLOCK_TOKENS < open_from || block * BLOCK_TOKENS + BLOCK_TOKENS > open_to) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = t0 + i >= s.lo && t0 + i < s.hi ? x[i] : -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+        if (__any(top > ref + RISE)) {
+            const float to = fmaxf(ref, column_max(top)), by = to > -INFINITY ? to : 0.0f, old = __builtin_amdgcn_exp2f(ref - by);
+            ref = to;
+            sum *= old;
+#pragma unroll
+            for (int m = 0; m < 8; ++m) acc[m] *= old;
+        }
+        const float by = ref > -INFINITY ? ref : 0.0f;
+        float z0 = 0.0f, z1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            x[i] = __builtin_amdgcn_exp2f(x[i] - by);
+            x[i + 1] = __builtin_amdgcn_exp2f(x[i + 1] - by);
+            z0 += x[i];
+            z1 += x[i + 1];
+        }
+        sum += z0 + z1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (_Float16)(x[i] * f);
+    };
+    const auto values_up_to = [&](float v) {                    // the sums' values are in units of vref from here on
+        if (v <= vref) return;
+        const float old = vref / v;
+#pragma unroll
+        for (int m = 0; m < 8; ++m) acc[m] *= old;
+        vref = v;
+    };
+
+    const int codes = min(mine, full - b0);                     // of the blocks of this workgroup those that lie in pages
+    const size_t kat = (size_t)(16 * (n >> 2) + (n & 3)) * HD + 32 * j, vat = (size_t)n * BLOCK_TOKENS + 16 * j;
+#pragma unroll 1
+    for (int g0 = wave; g0 < codes; g0 += 64 * NARROW_WAVES) {  // 64 blocks of this wavefront at a time
+        const int at = g0 + NARROW_WAVES * lane, todo = min((codes - g0 + NARROW_WAVES - 1) / NARROW_WAVES, 64);
+        const int page_of = at < codes ? p.table[(size_t)slot * p.blocks + b0 + at] : 0;
+        const float ks_of = at < codes ? p.kscale[scale_at(p, a.layer, page_of, h)] : 0.0f;
+        const float vs_of = at < codes ? p.vscale[scale_at(p, a.layer, page_of, h)] : 0.0f;
+        uint4 k[8], v[8];
+        const auto request_keys = [&](int i) {
+            const uint8_t* src = p.kcodes + page_at(p, a.layer, __builtin_amdgcn_readlane(page_of, i), h) + kat;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) k[c] = *reinterpret_cast<const uint4*>(src + (c >> 1) * 4 * HD + (c & 1) * 16);
+        };
+        const auto request_values = [&](int i) {
+            const uint8_t* src = p.vcodes + page_at(p, a.layer, __builtin_amdgcn_readlane(page_of, i), h) + vat;
+#pragma unroll
+            for (int m = 0; m < 8; ++m) v[m] = *reinterpret_cast<const uint4*>(src + m * 16 * BLOCK_TOKENS);
+        };
+        request_keys(0);
+        request_values(0);
+        values_up_to(wave_max(vs_of));
+        const float f_of = vref > 0.0f ? 128.0f * (vs_of / vref) : 0.0f;
+#pragma unroll 1
+        for (int i = 0; i < todo; ++i) {
+            f32x4 dot[4];
+#pragma unroll
+            for (int tb = 0; tb < 4; ++tb) {
+                dot[tb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    const uint4& c = k[2 * tb + (kk >> 1)];
+                    dot[tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk & 1 ? codes_f16<KIND>(c.z, c.w) : codes_f16<KIND>(c.x, c.y), q[kk], dot[tb], 0, 0, 0);
+                }
+            }
+            if (i + 1 < todo) request_keys(i + 1);
+            f16x8 w[2];
+            weigh(dot, b0 + g0 + NARROW_WAVES * i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_of), i)),
+                  __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f_of), i)), w);
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16<KIND>(v[m].x, v[m].y), w[0], acc[m], 0, 0, 0);
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16<KIND>(v[m].z, v[m].w), w[1], acc[m], 0, 0, 0);
+            }
+            if (i + 1 < todo) request_values(i + 1);
+        }
+    }
+    // the open block, by the wavefront whose turn it is
+    if (mine > 0 && b0 + mine > full && (mine - 1) % NARROW_WAVES == wave) {
+        const uint16_t* kt = p.ktail + tail_at(p, a.layer, slot, h) + kat;
+        const uint16_t* vt = p.vtail + tail_at(p, a.layer, slot, h) + vat;
+        uint4 k[16];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            k[c] = *reinterpret_cast<const uint4*>(kt + (c >> 2) * 4 * HD + (c & 3) * 8);
+            top = max(top, abs_max8(k[c]));
+        }
+        Power pw = power_for<DT>(larger_bits(top, true));
+        f32x4 dot[4];
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb) {
+            dot[tb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) dot[tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(k[4 * tb + kk], pw.up), q[kk], dot[tb], 0, 0, 0);
+        }
+        const float kdown = pw.down;
+        top = 0;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            k[c] = *reinterpret_cast<const uint4*>(vt + (c >> 1) * 16 * BLOCK_TOKENS + (c & 1) * 8);
+            top = max(top, abs_max8(k[c]));
+        }
+        top = larger_bits(top, true);
+        pw = power_for<DT>(top);
+        if (top > 0) values_up_to(pw.down);
+        f16x8 w[2];
+        weigh(dot, full, kdown, top > 0 ? 128.0f * (pw.down / vref) : 0.0f, w);
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(k[2 * m], pw.up), w[0], acc[m], 0, 0, 0);
+            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(k[2 * m + 1], pw.up), w[1], acc[m], 0, 0, 0);
+        }
+    }
+
+    sum = column_sum(sum);
+    const float unit = vref * (1.0f / 128.0f);
+#pragma unroll
+    for (int m = 0; m < 8; ++m) *reinterpret_cast<f32x4*>(&acc_of[wave][n][16 * m + 4 * j]) = acc[m] * unit;
+    if (j == 0) {
+        ref_of[wave][n] = ref;
+        sum_of[wave][n] = sum;
+    }
+    __syncthreads();
+    // a thread takes eight dims of a query
+    const int r = tid >> 4, d = (tid & 15) * 8, rl = r / a.G, rh = h * a.G + r - rl * a.G;
+    if (r >= R || rl >= count) return;
+    float to = ref_of[0][r], total = 0.0f, o[8];
+#pragma unroll
+    for (int w = 1; w < NARROW_WAVES; ++w) to = fmaxf(to, ref_of[w][r]);
+    const float by = to > -INFINITY ? to : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NARROW_WAVES; ++w) {
+        const float f = __builtin_amdgcn_exp2f(ref_of[w][r] - by);
+        // (a query that is not a number has a sum that is not, and a reference that may be anything)
+        total += sum_of[w][r] == 0.0f ? 0.0f : sum_of[w][r] * f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = __fmaf_rn(acc_of[w][r][d + e], f, o[e]);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = total == 0.0f ? 0.0f : o[e] * inv;
+    const float lse2 = total == 0.0f ? -INFINITY : to + __builtin_amdgcn_logf(total);
+    if (a.splits > 1) {
+        const size_t unit_at = ((size_t)pair * a.splits + split) * R + r;
+        f32x4* dst = reinterpret_cast<f32x4*>(a.part_out + unit_at * HD + d);
+        dst[0] = f32x4{o[0], o[1], o[2], o[3]};
+        dst[1] = f32x4{o[4], o[5], o[6], o[7]};
+        if (d == 0) a.part_lse[unit_at] = lse2;
+        return;
+    }
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = (uint32_t)to_16<DT>(o[2 * e]) | (uint32_t)to_16<DT>(o[2 * e + 1]) << 16;
+    *reinterpret_cast<uint4*>(a.out + (((size_t)row * a.L + rl) * a.Hq + rh) * HD + d) = make_uint4(b[0], b[1], b[2], b[3]);
+    if (a.lse && d == 0) a.lse[((size_t)row * a.Hq + rh) * a.L + rl] = lse2 * LN2;
+}
+
+// The shares of a row and kv-head's blocks, put together: a workgroup a query, its four wavefronts every fourth share, a lane two dims.
+template <int DT>
+__global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
+    const odmkv_pages_t& p = a.p;
+    const int R = a.G * a.L, r = blockIdx.x, h = blockIdx.y, row = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int l = r / a.G, hq = h * a.G + r - l * a.G;
+    if (l >= (a.counts ? min(max(a.counts[row], 0), a.L) : a.L)) return;
+    __shared__ float part[4][HD], top_of[4], sum_of[4];
+    const size_t at = ((size_t)row * p.Hkv + h) * a.splits * R + r;
+    float top = -INFINITY;
+    for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, a.part_lse[at + (size_t)i * R]);
+    top = wave_max(top);
+    const float by = top > -INFINITY ? top : 0.0f;
+    float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll 4
+    for (int i = wave; i < a.splits; i += 4) {
+        const float lse = a.part_lse[at + (size_t)i * R];
+        const float2 v = *reinterpret_cast<const float2*>(a.part_out + (at + (size_t)i * R) * HD + 2 * lane);
+        const float w = __builtin_amdgcn_exp2f(lse - by);
+        sum += w;
+        o0 = __fmaf_rn(w, v.x, o0);
+        o1 = __fmaf_rn(w, v.y, o1);
+    }
+    part[wave][2 * lane] = o0;
+    part[wave][2 * lane + 1] = o1;
+    if (lane == 0) sum_of[wave] = sum;
+    __syncthreads();
+    if (tid >= 64) return;
+    sum = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    o0 = ((part[0][2 * lane] + part[1][2 * lane]) + (part[2][2 * lane] + part[3][2 * lane])) * inv;
+    o1 = ((part[0][2 * lane + 1] + part[1][2 * lane + 1]) + (part[2][2 * lane + 1] + part[3][2 * lane + 1])) * inv;
+    *reinterpret_cast<uint32_t*>(a.out + (((size_t)row * a.L + l) * a.Hq + hq) * HD + 2 * lane) = (uint32_t)to_16<DT>(o0) | (uint32_t)to_16<DT>(o1) << 16;
+    if (a.lse && lane == 0) a.lse[((size_t)row * a.Hq + hq) * a.L + l] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
 // the simplest form: a workgroup a query, a thread a token and then a thread a dim
@@ -93,8 +458,31 @@ __global__ __launch_bounds__(128) void attend_simple_kernel(AttendArgs a) {
     if (a.lse && tid == 0) a.lse[((size_t)row * a.Hq + hq) * a.L + l] = none ? -INFINITY : m + logf(sum);
 }
 
+// Workgroups for a row and kv-head: two a compute unit in all, each with a block a wavefront at least.
+static int splits_of(const odmkv_pages_t& p, int max_length) {
+    const int blocks = max_length / BLOCK_TOKENS + 1, pairs = p.rows * p.Hkv;
+    return std::max(1, std::min((2 * compute_units() + pairs - 1) / pairs, blocks / NARROW_WAVES));
+}
+
 extern "C" size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length) {
-    (void)p; (void)Hq; (void)L; (void)max_length;
+    if (!p || p->Hkv <= 0 || p->rows <= 0 || Hq <= 0 || L <= 0 || max_length < 0) return 0;
+    const int R = Hq / p->Hkv * L;
+    if (R > NARROW) return 0;
+    const int splits = splits_of(*p, max_length);
+    return splits > 1 ? align_up((size_t)p->rows * p->Hkv * splits * R * (HD + 1) * sizeof(float), 256) : 0;
+}
+
+template <int DT, int KIND>
+static void launch_narrow(const AttendArgs& a, bool plain, hipStream_t st) {
+    const dim3 grid((unsigned)(a.p.rows * a.p.Hkv * a.splits)), block(NARROW_WAVES * 64);
+    if (plain) hipLaunchKernelGGL((attend_narrow_kernel<DT, KIND, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((attend_narrow_kernel<DT, KIND, false>), grid, block, 0, st, a);
+}
+static int launch_merge(const AttendArgs& a, hipStream_t st) {
+    const dim3 grid(a.G * a.L, a.p.Hkv, a.p.rows);
+    if (a.p.dtype == ODMKV_F16) hipLaunchKernelGGL(attend_merge_kernel<ODMKV_F16>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(attend_merge_kernel<ODMKV_BF16>, grid, dim3(256), 0, st, a);
+    ODMKV_CHECK_LAUNCH("attend_merge_kernel");
     return 0;
 }
 
@@ -113,8 +501,26 @@ extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
     ODMKV_CHECK_ARG(d->q && d->out, "pages_attend: null pointer");
     ODMKV_CHECK_ARG((((uintptr_t)d->q | (uintptr_t)d->out) & 15) == 0 && ((d->q_stride_b | d->q_stride_h | d->q_stride_l) & 7) == 0,
                     "pages_attend: rows must be 16-byte aligned");
-    const AttendArgs a = {p, (const uint16_t*)d->q, d->q_stride_b, d->q_stride_h, d->q_stride_l, (uint16_t*)d->out, d->lse, d->counts, d->slopes,
-                          d->prefix, d->starts, d->start_stride_b, d->start_stride_l, d->layer, d->L, d->Hq, d->Hq / p.Hkv, d->window, d->scaling, d->cap};
+    AttendArgs a = {p, (const uint16_t*)d->q, d->q_stride_b, d->q_stride_h, d->q_stride_l, (uint16_t*)d->out, d->lse, d->counts, d->slopes,
+                    d->prefix, d->starts, d->start_stride_b, d->start_stride_l, d->layer, d->L, d->Hq, d->Hq / p.Hkv, d->window, d->scaling, d->cap,
+                    1, nullptr, nullptr};
+    const size_t need = odmkv_pages_attend_workspace_bytes(&p, d->Hq, d->L, d->max_length);
+    if (need > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)) {
+        odmkv_set_error("pages_attend: workspace too small");
+        return ODMKV_ENOSPACE;
+    }
+    if (a.G * a.L <= NARROW) {
+        a.splits = splits_of(p, d->max_length);
+        a.part_out = (float*)d->workspace;
+        a.part_lse = a.part_out + (size_t)p.rows * p.Hkv * a.splits * a.G * a.L * HD;
+        const bool plain = a.cap == 0.0f && !a.slopes;
+        if (p.dtype == ODMKV_F16 && p.kind == ODMKV_INT8) launch_narrow<ODMKV_F16, ODMKV_INT8>(a, plain, (hipStream_t)stream);
+        else if (p.dtype == ODMKV_F16) launch_narrow<ODMKV_F16, ODMKV_E4M3>(a, plain, (hipStream_t)stream);
+        else if (p.kind == ODMKV_INT8) launch_narrow<ODMKV_BF16, ODMKV_INT8>(a, plain, (hipStream_t)stream);
+        else launch_narrow<ODMKV_BF16, ODMKV_E4M3>(a, plain, (hipStream_t)stream);
+        ODMKV_CHECK_LAUNCH("attend_narrow_kernel");
+        return a.splits > 1 ? launch_merge(a, (hipStream_t)stream) : 0;
+    }
     const dim3 grid(d->L, d->Hq, p.rows);
     hipStream_t st = (hipStream_t)stream;
     if (p.dtype == ODMKV_F16 && p.kind == ODMKV_INT8) hipLaunchKernelGGL((attend_simple_kernel<ODMKV_F16, ODMKV_INT8>), grid, dim3(128), 0, st, a);

@@ -83,4 +83,8 @@ def attend(q, k, v, *, scaling=None, cap=None, slopes=None, window=None, prefix=
     size = torch.where(seen, size, torch.zeros_like(size)).amax(dim=-1) if m else peak
     dx = 140 * e32 * size + 16 * e32 * (peak + (cap or 0.0) + 8)
     tol = (2 * dx + e16 + 2 * m * e32)[..., None] * mass
+    # weights below fp16's normal numbers are off by 2^-25 at most, half a step, where the sums' unit makes the largest value 127 to 128 and a weight
+    # of one (or more, never less: the sum is at least that) 2^7: a token adds 2^-25 * 2^-7 of the largest value
+    if m:
+        tol = tol + 1.01 * m * 2.0 ** -32 * v.abs().amax(dim=(1, 2))[:, None, None]
     return out.transpose(0, 1), lse, tol.transpose(0, 1), dx + (m + 8) * e32

@@ -398,90 +398,321 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
     if (a.lse && lane == 0) a.lse[((size_t)row * a.Hq + hq) * a.L + l] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// the simplest form: a workgroup a query, a thread a token and then a thread a dim
-template <int DT, int KIND>
-__global__ __launch_bounds__(128) void attend_simple_kernel(AttendArgs a) {
+// ---- many queries of a kv-head --------------------------------------------------------------------
+// A wavefront holds 32 queries (the columns of v_mfma_f32_32x32x16_f16), a workgroup 32 WAVES of them, token by token with the G heads of a
+// token together, so that a workgroup's tokens lie together and blocks that none of them sees are passed over.  A block of 64 tokens is turned into fp16 once a workgroup
+// and lies in LDS, the next block's codes are on their way in registers; rows of the first product are tokens as they lie, and row r of a half
+// wavefront's sixteen (8 (r / 4) + 4 half + r % 4) decides the order in which values lie in LDS: what a lane holds of the weights is
+// then its operand of the second product.  16-byte pieces of a row are moved by the row's number (xor), so that no two of eight rows meet in a bank.
+#define WIDE_WAVES 8
+#define WIDE_LDS (2 * (BLOCK_TOKENS * HD * 2 * 2))
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT, int KIND, bool PLAIN, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a) {
     const odmkv_pages_t& p = a.p;
-    const int row = blockIdx.z, hq = blockIdx.y, l = blockIdx.x, tid = threadIdx.x, h = hq / a.G;
-    const int len = p.length[row], n = a.counts ? min(max(a.counts[row], 0), a.L) : a.L, slot = p.slot[row];
-    if (l >= n) return;
-    const Sight s = sight_of(a, row, len, n, l);
-    __shared__ float q[HD], w[128], red[4];
-    q[tid] = Elem<DT>::to_f32(a.q[row * a.qb + hq * a.qh + l * a.ql + tid]);
-    __syncthreads();
-    const float slope = a.slopes ? a.slopes[hq] : 0.0f;
-    float m = -INFINITY, sum = 0.0f, acc = 0.0f;
-    for (int base = s.lo / 64 * 64; base < s.hi; base += 64) {
-        const bool full = base / 64 < len / 64;
-        const int page = full ? p.table[(size_t)slot * p.blocks + base / 64] : 0;
-        const size_t at = page_at(p, a.layer, page, h), tat = tail_at(p, a.layer, slot, h);
-        const float sk = full ? p.kscale[scale_at(p, a.layer, page, h)] : 1.0f, sv = full ? p.vscale[scale_at(p, a.layer, page, h)] : 1.0f;
-        float x = -INFINITY;
-        if (tid < 64 && base + tid >= s.lo && base + tid < s.hi) {
-            float dot = 0.0f;
-            for (int d = 0; d < HD; d += 4) {
-                float k[4];
-                if (full) values4<KIND>(*reinterpret_cast<const uint32_t*>(p.kcodes + at + tid * HD + d), k);
-                else for (int e = 0; e < 4; ++e) k[e] = Elem<DT>::to_f32(p.ktail[tat + tid * HD + d + e]);
-                for (int e = 0; e < 4; ++e) dot = __fmaf_rn(q[d + e], k[e], dot);
-            }
-            x = dot * sk * a.scaling;
-            if (a.cap > 0.0f) x = a.cap * tanhf(x / a.cap);
-            x -= slope * fabsf((float)(s.pos - base - tid));
-        }
-        if (tid < 64) {
-            const float top = wave_max(x);
-            if (tid == 0) red[0] = top;
-        }
-        __syncthreads();
-        const float mn = fmaxf(m, red[0]), by = mn > -INFINITY ? mn : 0.0f, old = expf(m - by);
-        const float e = x > -INFINITY || x != x ? expf(x - by) : 0.0f;
-        if (tid < 64) {
-            w[tid] = e;
-            const float z = wave_sum(e);
-            if (tid == 0) red[1] = z;
-        }
-        __syncthreads();
-        sum = sum * old + red[1];
-        acc *= old;
-        m = mn;
-        for (int t = 0; t < 64; t += 4) {
-            float v[4];
-            if (full) values4<KIND>(*reinterpret_cast<const uint32_t*>(p.vcodes + at + tid * 64 + t), v);
-            else for (int e2 = 0; e2 < 4; ++e2) v[e2] = Elem<DT>::to_f32(p.vtail[tat + tid * 64 + t + e2]);
-            for (int e2 = 0; e2 < 4; ++e2) acc = __fmaf_rn(w[t + e2] * sv, v[e2], acc);
-        }
-        __syncthreads();
+    extern __shared__ __align__(16) uint8_t lds[];              // [2][keys 64 x 256 bytes, values 128 x 128 bytes]
+    __shared__ int range[2][WAVES];
+    __shared__ uint32_t tops[2][WAVES];
+    constexpr int THREADS = WAVES * 64, BUFFER = BLOCK_TOKENS * HD * 4, VALUES = BLOCK_TOKENS * HD * 2;
+    const int pairs = p.rows * p.Hkv, R = a.G * a.L, tiles = (R + 32 * WAVES - 1) / (32 * WAVES);
+    // heads vary fastest (a die of the chip then keeps few heads' pages in its L2), the longest rows of blocks come first
+    const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs, split = rest % a.splits, tile = tiles - 1 - rest / a.splits;
+    const int row = pair / p.Hkv, h = pair % p.Hkv, tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int len = p.length[row], count = a.counts ? min(max(a.counts[row], 0), a.L) : a.L, slot = p.slot[row];
+    const int r0 = tile * 32 * WAVES + 32 * wave, r = r0 + col, l = r / a.G, hq = h * a.G + r - l * a.G;
+    const bool valid = r < R && l < count;
+    Sight s = {0, 0, 0};
+    if (valid) s = sight_of(a, row, len, count, l);
+    const bool sees = valid && s.lo < s.hi;
+    const int wave_lo = wave_min_int(sees ? s.lo : 0x7fffffff), wave_hi = -wave_min_int(sees ? -s.hi : 0);       // what some query of the wavefront sees
+    const int open_from = -wave_min_int(valid ? -(sees ? s.lo : 0x7fffffff) : 0), open_to = wave_min_int(valid ? s.hi : 0x7fffffff);    // what all of them see
+    if (lane == 0) {
+        range[0][wave] = wave_lo;
+        range[1][wave] = wave_hi;
     }
-    const bool none = s.hi <= s.lo;
-    a.out[(((size_t)row * a.L + l) * a.Hq + hq) * HD + tid] = to_16<DT>(none ? 0.0f : acc / sum);
-    if (a.lse && tid == 0) a.lse[((size_t)row * a.Hq + hq) * a.L + l] = none ? -INFINITY : m + logf(sum);
+    __syncthreads();
+    int lo = range[0][0], hi = range[1][0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+        lo = min(lo, range[0][w]);
+        hi = max(hi, range[1][w]);
+    }
+    const int first = lo / BLOCK_TOKENS, blocks = max((hi + BLOCK_TOKENS - 1) / BLOCK_TOKENS - first, 0), share = (blocks + a.splits - 1) / a.splits;
+    const int b0 = __builtin_amdgcn_readfirstlane(first + split * share), mine = __builtin_amdgcn_readfirstlane(min(share, blocks - split * share));
+    const int full = len / BLOCK_TOKENS;
+
+    f16x8 q[8];                                                 // dims 16 st + 8 half + e
+    float qdown = 1.0f;
+    {
+        uint4 raw[8];
+        const uint16_t* src = a.q + row * a.qb + hq * a.qh + l * a.ql + 8 * half;
+#pragma unroll
+        for (int st = 0; st < 8; ++st) raw[st] = valid ? *reinterpret_cast<const uint4*>(src + 16 * st) : make_uint4(0, 0, 0, 0);
+        if constexpr (DT == ODMKV_BF16) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int st = 0; st < 8; ++st) top = max(top, abs_max8(raw[st]));
+            const auto o = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            const Power pw = power_for<DT>(max(o[0], o[1]));
+            qdown = pw.down;
+#pragma unroll
+            for (int st = 0; st < 8; ++st) q[st] = scaled_f16<DT>(raw[st], pw.up);
+        } else {
+#pragma unroll
+            for (int st = 0; st < 8; ++st) q[st] = __builtin_bit_cast(f16x8, raw[st]);
+        }
+    }
+    const float slope = !PLAIN && a.slopes && valid ? a.slopes[hq] * LOG2E : 0.0f;
+    const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const float qs = a.scaling * qdown * (PLAIN ? LOG2E : 1.0f);
+
+    float ref = -INFINITY, sum = 0.0f, vref = 0.0f;
+    f32x16 acc[4];                                              // dims 32 db + 8 (r / 4) + 4 half + r % 4 of query `col`
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] = 0.0f;
+
+    const auto values_up_to = [&](float v) {                    // the sums' values are in units of vref from here on
+        if (v <= vref) return;
+        const float old = vref / v;
+#pragma unroll
+        for (int db = 0; db < 4; ++db) acc[db] *= old;
+        vref = v;
+    };
+
+    // ---- a block on its way: pieces of 16 codes, a token's 16 dims or a dim's 16 tokens
+    constexpr int PIECES = PAGE_BYTES / 16 / THREADS;
+    uint4 kc[PIECES], vc[PIECES];
+    int page_of = 0;
+    const auto look_up = [&](int i) { return i + lane < mine && b0 + i + lane < full ? p.table[(size_t)slot * p.blocks + b0 + i + lane] : 0; };
+    const auto request = [&](int i) {                           // block b0 + i, which lies in a page
+        if ((i & 63) == 0) page_of = look_up(i);
+        const size_t at = page_at(p, a.layer, __builtin_amdgcn_readlane(page_of, i & 63), h);
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+            kc[c] = *reinterpret_cast<const uint4*>(p.kcodes + at + (size_t)(tid + c * THREADS) * 16);
+            vc[c] = *reinterpret_cast<const uint4*>(p.vcodes + at + (size_t)(tid + c * THREADS) * 16);
+        }
+    };
+    const auto key_piece = [&](uint8_t* buf, int token, int piece) { return reinterpret_cast<f16x8*>(buf + token * 256 + ((piece ^ (token & 15)) << 4)); };
+    const auto value_piece = [&](uint8_t* buf, int dim, int piece) { return buf + VALUES + dim * 128 + ((piece ^ (dim & 7)) << 4); };
+    const auto put = [&](uint8_t* buf) {
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+            const int i = tid + c * THREADS;
+            *key_piece(buf, i >> 3, 2 * (i & 7)) = codes_f16<KIND>(kc[c].x, kc[c].y);
+            *key_piece(buf, i >> 3, 2 * (i & 7) + 1) = codes_f16<KIND>(kc[c].z, kc[c].w);
+            *reinterpret_cast<f16x8*>(value_piece(buf, i >> 2, 2 * (i & 3))) = codes_f16<KIND>(vc[c].x, vc[c].z);
+            *reinterpret_cast<f16x8*>(value_piece(buf, i >> 2, 2 * (i & 3) + 1)) = codes_f16<KIND>(vc[c].y, vc[c].w);
+        }
+    };
+    float tail_k = 1.0f, tail_v = 0.0f;                         // what the open block's numbers in LDS are to be multiplied by
+    const auto put_tail = [&](uint8_t* buf) {
+        const uint4* kt = reinterpret_cast<const uint4*>(p.ktail + tail_at(p, a.layer, slot, h));
+        const uint4* vt = reinterpret_cast<const uint4*>(p.vtail + tail_at(p, a.layer, slot, h));
+        uint32_t top[2] = {0, 0};
+#pragma unroll 1
+        for (int i = tid; i < TAIL_ELEMS / 8; i += THREADS) {
+            top[0] = max(top[0], abs_max8(kt[i]));
+            top[1] = max(top[1], abs_max8(vt[i]));
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t t = larger_bits(top[x], true);
+            if (lane == 0) tops[x][wave] = t;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) top[x] = max(top[x], tops[x][w]);
+        const Power pk = power_for<DT>(top[0]), pv = power_for<DT>(top[1]);
+        tail_k = pk.down;
+        tail_v = top[1] > 0 ? pv.down : 0.0f;
+#pragma unroll 1
+        for (int i = tid; i < TAIL_ELEMS / 8; i += THREADS) {
+            const int dim = i >> 3, u = i & 7;
+            *key_piece(buf, i >> 4, i & 15) = scaled_f16<DT>(kt[i], pk.up);
+            const uint4 x = __builtin_bit_cast(uint4, scaled_f16<DT>(vt[i], pv.up));
+            *reinterpret_cast<uint2*>(value_piece(buf, dim, u & ~1) + 8 * (u & 1)) = make_uint2(x.x, x.y);
+            *reinterpret_cast<uint2*>(value_piece(buf, dim, u | 1) + 8 * (u & 1)) = make_uint2(x.z, x.w);
+        }
+    };
+
+    const int codes = min(mine, full - b0);                     // of the blocks those that lie in pages
+    if (codes > 0) request(0);
+    float ks_of = 0.0f, f_of = 0.0f;
+#pragma unroll 1
+    for (int i = -1; i < mine; ++i) {
+        uint8_t* buf = lds + (i & 1) * BUFFER;
+        __syncthreads();                                        // this block lies there, and nobody reads the one before any more
+        if (i + 1 < codes) put(lds + ((i + 1) & 1) * BUFFER);
+        else if (i + 1 < mine) put_tail(lds + ((i + 1) & 1) * BUFFER);
+        if (i + 2 < codes) request(i + 2);
+        if (i < 0) continue;
+        const int t0 = (b0 + i) * BLOCK_TOKENS;
+        float ks, f;
+        if (i < codes) {
+            if ((i & 63) == 0) {                                // 64 blocks' scales at a time
+                const bool in = i + lane < codes;
+                const int page = look_up(i);
+                const float vs = in ? p.vscale[scale_at(p, a.layer, page, h)] : 0.0f;
+                ks_of = in ? p.kscale[scale_at(p, a.layer, page, h)] : 0.0f;
+                values_up_to(wave_max(vs));
+                f_of = vref > 0.0f ? 128.0f * (vs / vref) : 0.0f;
+            }
+            ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_of), i & 63));
+            f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f_of), i & 63));
+        } else {
+            ks = tail_k;
+            values_up_to(tail_v);
+            f = tail_v > 0.0f ? 128.0f * (tail_v / vref) : 0.0f;
+        }
+        if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;      // (of the wavefront's own queries none sees the block)
+        f32x16 dot[2];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dot[tb][e] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < 8; ++st)
+                dot[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*key_piece(buf, 32 * tb + col, 2 * st + half), q[st], dot[tb], 0, 0, 0);
+        }
+        const float c = ks * qs;
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = dot[e >> 4][e & 15] * c;
+        const int tl = t0 + 4 * half;                           // token of x[e]: tl + 8 (e / 4) + e % 4
+        if constexpr (!PLAIN) {
+            if (inv_cap > 0.0f) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = a.cap * tanh_of(x[e] * inv_cap);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = __fmaf_rn(x[e], LOG2E, -slope * fabsf((float)(s.pos - tl - 8 * (e >> 2) - (e & 3))));
+        }
+        if (t0 < open_from || t0 + BLOCK_TOKENS > open_to) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const int t = tl + 8 * (e >> 2) + (e & 3);
+                x[e] = t >= s.lo && t < s.hi ? x[e] : -INFINITY;
+            }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) top = fmaxf(top, x[e]);
+        if (__any(top > ref + RISE)) {
+            const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const float to = fmaxf(ref, fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]))), by = to > -INFINITY ? to : 0.0f;
+            const float old = __builtin_amdgcn_exp2f(ref - by);
+            ref = to;
+            sum *= old;
+#pragma unroll
+            for (int db = 0; db < 4; ++db) acc[db] *= old;
+        }
+        const float by = ref > -INFINITY ? ref : 0.0f;
+        float z0 = 0.0f, z1 = 0.0f;
+        f16x8 w[4];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(x[e] - by), p1 = __builtin_amdgcn_exp2f(x[e + 1] - by);
+            z0 += p0;
+            z1 += p1;
+            w[e >> 3][e & 7] = (_Float16)(p0 * f);
+            w[e >> 3][(e & 7) + 1] = (_Float16)(p1 * f);
+        }
+        sum += z0 + z1;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(value_piece(buf, 32 * db + col, 2 * st + half)), w[st], acc[db], 0, 0, 0);
+    }
+
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+    if (!valid) return;
+    const bool none = sum == 0.0f;
+    const float unit = none ? 0.0f : vref * (1.0f / 128.0f) / sum, lse2 = none ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
+    if (a.splits > 1) {
+        const size_t unit_at = ((size_t)pair * a.splits + split) * R + r;
+        float* dst = a.part_out + unit_at * HD + 4 * half;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : acc[db][4 * g + e] * unit;
+                *reinterpret_cast<f32x4*>(dst + 32 * db + 8 * g) = v;
+            }
+        if (half == 0) a.part_lse[unit_at] = lse2;
+        return;
+    }
+    uint16_t* dst = a.out + (((size_t)row * a.L + l) * a.Hq + hq) * HD + 4 * half;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint32_t v[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                v[e] = none ? 0u : (uint32_t)to_16<DT>(acc[db][4 * g + 2 * e] * unit) | (uint32_t)to_16<DT>(acc[db][4 * g + 2 * e + 1] * unit) << 16;
+            *reinterpret_cast<uint2*>(dst + 32 * db + 8 * g) = make_uint2(v[0], v[1]);
+        }
+    if (a.lse && half == 0) a.lse[((size_t)row * a.Hq + hq) * a.L + l] = none ? -INFINITY : lse2 * LN2;
 }
 
-// Workgroups for a row and kv-head: two a compute unit in all, each with a block a wavefront at least.
-static int splits_of(const odmkv_pages_t& p, int max_length) {
-    const int blocks = max_length / BLOCK_TOKENS + 1, pairs = p.rows * p.Hkv;
-    return std::max(1, std::min((2 * compute_units() + pairs - 1) / pairs, blocks / NARROW_WAVES));
+// How a call is cut: wavefronts of a workgroup (0: the narrow kernel) and workgroups that share a row's blocks, two a compute unit in all,
+// each with a few blocks at least.
+struct Cut { int waves, splits; };
+static Cut cut_of(const odmkv_pages_t& p, int R, int max_length) {
+    const int blocks = max_length / BLOCK_TOKENS + 1, wanted = 2 * compute_units();
+    long long groups = (long long)p.rows * p.Hkv;
+    Cut c = {0, 1};
+    if (R > NARROW) {
+        c.waves = R > 128 ? WIDE_WAVES : 4;
+        groups *= (R + 32 * c.waves - 1) / (32 * c.waves);
+    }
+    c.splits = (int)std::max(1LL, std::min((wanted + groups - 1) / groups, (long long)blocks / 4));
+    return c;
 }
 
 extern "C" size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length) {
     if (!p || p->Hkv <= 0 || p->rows <= 0 || Hq <= 0 || L <= 0 || max_length < 0) return 0;
-    const int R = Hq / p->Hkv * L;
-    if (R > NARROW) return 0;
-    const int splits = splits_of(*p, max_length);
+    const int R = Hq / p->Hkv * L, splits = cut_of(*p, R, max_length).splits;
     return splits > 1 ? align_up((size_t)p->rows * p->Hkv * splits * R * (HD + 1) * sizeof(float), 256) : 0;
 }
 
 template <int DT, int KIND>
-static void launch_narrow(const AttendArgs& a, bool plain, hipStream_t st) {
-    const dim3 grid((unsigned)(a.p.rows * a.p.Hkv * a.splits)), block(NARROW_WAVES * 64);
-    if (plain) hipLaunchKernelGGL((attend_narrow_kernel<DT, KIND, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((attend_narrow_kernel<DT, KIND, false>), grid, block, 0, st, a);
-}
-static int launch_merge(const AttendArgs& a, hipStream_t st) {
-    const dim3 grid(a.G * a.L, a.p.Hkv, a.p.rows);
-    if (a.p.dtype == ODMKV_F16) hipLaunchKernelGGL(attend_merge_kernel<ODMKV_F16>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(attend_merge_kernel<ODMKV_BF16>, grid, dim3(256), 0, st, a);
+static int launch_attend(const AttendArgs& a, int waves, hipStream_t st) {
+    const bool plain = a.cap == 0.0f && !a.slopes;
+    const int pairs = a.p.rows * a.p.Hkv, R = a.G * a.L;
+    if (waves == 0) {
+        const dim3 grid((unsigned)(pairs * a.splits)), block(NARROW_WAVES * 64);
+        if (plain) hipLaunchKernelGGL((attend_narrow_kernel<DT, KIND, true>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((attend_narrow_kernel<DT, KIND, false>), grid, block, 0, st, a);
+        ODMKV_CHECK_LAUNCH("attend_narrow_kernel");
+    } else {
+        const long long groups = (long long)pairs * a.splits * ((R + 32 * waves - 1) / (32 * waves));
+        ODMKV_CHECK_ARG(groups < 0x7fffffffLL, "pages_attend: too many queries");
+        const dim3 grid((unsigned)groups), block(waves * 64);
+        const auto run = [&](auto kernel) -> int {
+            ODMKV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, WIDE_LDS));
+            hipLaunchKernelGGL(kernel, grid, block, WIDE_LDS, st, a);
+            return 0;
+        };
+        int rc;
+        if (waves == 4) rc = plain ? run(attend_wide_kernel<DT, KIND, true, 4>) : run(attend_wide_kernel<DT, KIND, false, 4>);
+        else rc = plain ? run(attend_wide_kernel<DT, KIND, true, WIDE_WAVES>) : run(attend_wide_kernel<DT, KIND, false, WIDE_WAVES>);
+        if (rc) return rc;
+        ODMKV_CHECK_LAUNCH("attend_wide_kernel");
+    }
+    if (a.splits == 1) return 0;
+    hipLaunchKernelGGL(attend_merge_kernel<DT>, dim3(R, a.p.Hkv, a.p.rows), dim3(256), 0, st, a);
     ODMKV_CHECK_LAUNCH("attend_merge_kernel");
     return 0;
 }
@@ -495,7 +726,7 @@ extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
     ODMKV_CHECK_ARG(p.kind == ODMKV_INT8 || p.kind == ODMKV_E4M3, "pages_attend: bad kind %d", p.kind);
     ODMKV_CHECK_ARG(d->layer >= 0 && d->layer < p.layers, "pages_attend: layer %d of %d", d->layer, p.layers);
     ODMKV_CHECK_ARG(d->Hq > 0 && d->Hq % p.Hkv == 0 && d->Hq / p.Hkv <= ODMKV_MAX_GROUP, "pages_attend: %d query heads over %d kv-heads", d->Hq, p.Hkv);
-    ODMKV_CHECK_ARG(d->L >= 0 && d->window >= 0 && d->max_length >= 0, "pages_attend: bad length");
+    ODMKV_CHECK_ARG(d->L >= 0 && d->L <= (1 << 26) && d->window >= 0 && d->max_length >= 0, "pages_attend: bad length");
     ODMKV_CHECK_ARG(d->cap >= 0.0f && d->cap < INFINITY, "pages_attend: bad cap");
     if (d->L == 0) return 0;
     ODMKV_CHECK_ARG(d->q && d->out, "pages_attend: null pointer");
@@ -509,24 +740,11 @@ extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
         odmkv_set_error("pages_attend: workspace too small");
         return ODMKV_ENOSPACE;
     }
-    if (a.G * a.L <= NARROW) {
-        a.splits = splits_of(p, d->max_length);
-        a.part_out = (float*)d->workspace;
-        a.part_lse = a.part_out + (size_t)p.rows * p.Hkv * a.splits * a.G * a.L * HD;
-        const bool plain = a.cap == 0.0f && !a.slopes;
-        if (p.dtype == ODMKV_F16 && p.kind == ODMKV_INT8) launch_narrow<ODMKV_F16, ODMKV_INT8>(a, plain, (hipStream_t)stream);
-        else if (p.dtype == ODMKV_F16) launch_narrow<ODMKV_F16, ODMKV_E4M3>(a, plain, (hipStream_t)stream);
-        else if (p.kind == ODMKV_INT8) launch_narrow<ODMKV_BF16, ODMKV_INT8>(a, plain, (hipStream_t)stream);
-        else launch_narrow<ODMKV_BF16, ODMKV_E4M3>(a, plain, (hipStream_t)stream);
-        ODMKV_CHECK_LAUNCH("attend_narrow_kernel");
-        return a.splits > 1 ? launch_merge(a, (hipStream_t)stream) : 0;
-    }
-    const dim3 grid(d->L, d->Hq, p.rows);
+    const Cut cut = cut_of(p, a.G * a.L, d->max_length);
+    a.splits = cut.splits;
+    a.part_out = (float*)d->workspace;
+    a.part_lse = a.part_out + (size_t)p.rows * p.Hkv * a.splits * a.G * a.L * HD;
     hipStream_t st = (hipStream_t)stream;
-    if (p.dtype == ODMKV_F16 && p.kind == ODMKV_INT8) hipLaunchKernelGGL((attend_simple_kernel<ODMKV_F16, ODMKV_INT8>), grid, dim3(128), 0, st, a);
-    else if (p.dtype == ODMKV_F16) hipLaunchKernelGGL((attend_simple_kernel<ODMKV_F16, ODMKV_E4M3>), grid, dim3(128), 0, st, a);
-    else if (p.kind == ODMKV_INT8) hipLaunchKernelGGL((attend_simple_kernel<ODMKV_BF16, ODMKV_INT8>), grid, dim3(128), 0, st, a);
-    else hipLaunchKernelGGL((attend_simple_kernel<ODMKV_BF16, ODMKV_E4M3>), grid, dim3(128), 0, st, a);
-    ODMKV_CHECK_LAUNCH("attend_simple_kernel");
-    return 0;
+    if (p.dtype == ODMKV_F16) return p.kind == ODMKV_INT8 ? launch_attend<ODMKV_F16, ODMKV_INT8>(a, cut.waves, st) : launch_attend<ODMKV_F16, ODMKV_E4M3>(a, cut.waves, st);
+    return p.kind == ODMKV_INT8 ? launch_attend<ODMKV_BF16, ODMKV_INT8>(a, cut.waves, st) : launch_attend<ODMKV_BF16, ODMKV_E4M3>(a, cut.waves, st);
 }

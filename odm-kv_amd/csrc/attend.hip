@@ -670,14 +670,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
 // each with a few blocks at least.
 struct Cut { int waves, splits; };
 static Cut cut_of(const odmkv_pages_t& p, int R, int max_length) {
-    const int blocks = max_length / BLOCK_TOKENS + 1, wanted = 2 * compute_units();
+    const int blocks = max_length / BLOCK_TOKENS + 1;
     long long groups = (long long)p.rows * p.Hkv;
     Cut c = {0, 1};
     if (R > NARROW) {
         c.waves = R > 128 ? WIDE_WAVES : 4;
         groups *= (R + 32 * c.waves - 1) / (32 * c.waves);
     }
-    c.splits = (int)std::max(1LL, std::min((wanted + groups - 1) / groups, (long long)blocks / 4));
+    const int wanted = (c.waves == WIDE_WAVES ? 1 : 2) * compute_units();
+    c.splits = (int)std::max(1LL, std::min(wanted / groups, (long long)blocks / 4));
     return c;
 }
 

@@ -16,6 +16,7 @@ _LAZY = {
     "TurboQuantBackendPress": "kvquant.backend_press",
     "TurboQuantPerTokenPress": "kvquant.press",
     "PackedCacheLayer": "kvquant.hf_cache",          # not in the reference: a cache layer without a dense copy
+    "PagedCache": "kvquant.hf_cache",                # not in the reference: a model's cache over the next
     "PagedKVCache": "kvquant.paged_cache",           # not in the reference: 8 bits a value, rows that share pages
 }
 

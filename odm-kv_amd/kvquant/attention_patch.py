@@ -1,6 +1,6 @@
-"""Attention-function patch: fused packed-cache decode, and head-wise masking for the dense path.
+"""Attention-function patch: fused packed-cache decode, the paged cache, and head-wise masking for the dense path.
 
-Stands where the reference's kvquant/attention_patch.py:13-62 stands.  Two behaviours:
+Stands where the reference's kvquant/attention_patch.py:13-62 stands.  Three behaviours:
 
 * decode (one query token, or a block of new tokens such as the question after a prefill) on a module
   whose layer has a packed store attached (``module._odmkv_state``): the attention output comes from
@@ -9,6 +9,7 @@ Stands where the reference's kvquant/attention_patch.py:13-62 stands.  Two behav
   except for the new tokens, which the store does not hold yet when the attention function runs (the
   press appends them in its forward hook, afterwards).  Evicted tokens are absent from the store, so
   no fake keys are needed.
+* new tokens of a `PagedCache` (kvquant/hf_cache.py) attend over its pages (``PagedKVCache.attend``);
 * everything else goes to the wrapped attention function as in the reference, with evicted keys
   replaced by a fake key whose weight underflows to zero (``search_hyperplane``).
 """
@@ -31,6 +32,7 @@ _NATIVE_PAIRS = 3 << 20
 _PATCH_ATTR = "_kvtoken_quant_attention_patched"
 # how many decode calls took the fused kernel / the wrapped attention function (diagnostics)
 call_counts = {"fused": 0, "dense": 0}
+paged_counts = {"paged": 0}                              # and the paged cache's kernels
 
 
 def search_hyperplane(x: torch.Tensor, max_iter: int = 1000) -> torch.Tensor:
@@ -163,12 +165,60 @@ def _fused_block(state, query, key, value, attention_mask, scaling, k_len, layer
     return out.to(query.dtype).transpose(1, 2).contiguous()                      # [B, L, Hq, D]
 
 
+_paged_masks: dict = {}
+
+
+def _paged_starts(mask: torch.Tensor, B: int, L: int, k_len: int, window, layer):
+    """The first token that each row sees (int32 [B], or None: the first), if `mask` is what a causal call over rows padded in front makes of it, else False.
+    The look waits for the device; its answer serves the layers above, as `_store_part_is_open`'s does."""
+    version = None if mask.is_inference() else mask._version
+    hit = _paged_masks.get(window)
+    if hit is not None and hit[0] is mask and hit[1] == version and layer is not None and hit[2] is not None and layer > hit[2]:
+        return hit[3]
+    found = False
+    if mask.dim() == 4 and mask.shape[0] in (1, B) and mask.shape[1] == 1 and mask.shape[-2] == L and mask.shape[-1] == k_len:
+        seen = mask[:, 0] if mask.dtype == torch.bool else mask[:, 0] == 0
+        j = torch.arange(k_len, device=mask.device)
+        i = j[k_len - L:, None]
+        causal = j <= i if window is None else (j <= i) & (j > i - window)
+        # the first token that counts: every later query sees it, unless a window has passed it by
+        any_seen = seen.any(dim=1)
+        starts = any_seen.to(torch.uint8).argmax(dim=-1)
+        if window is not None:
+            starts = torch.where(starts <= max(k_len - L - window + 1, 0), torch.zeros_like(starts), starts)
+        same = (seen == (causal & (j >= starts[:, None, None]))).all()
+        if mask.dtype != torch.bool:                     # what is not open is closed altogether, not biased
+            same = same & ((mask[:, 0] == 0) | (mask[:, 0] <= torch.finfo(mask.dtype).min / 2)).all()
+        if bool(same):
+            found = starts.to(torch.int32).expand(B).contiguous() if bool((starts > 0).any()) else None
+    _paged_masks[window] = (mask, version, layer, found)
+    return found
+
+
+def _paged_attention(paged, module, query, attention_mask, dropout, kwargs):
+    """Attention output [B, L, Hq, D] over a `PagedCache`, whose pages and tails hold the new tokens already."""
+    pool, index, k_len = paged
+    window = kwargs.get("sliding_window")
+    starts = None
+    if attention_mask is not None:
+        starts = _paged_starts(attention_mask, query.shape[0], query.shape[2], k_len, window, getattr(module, "layer_idx", None))
+    if dropout or starts is False or kwargs.get("s_aux") is not None:
+        raise RuntimeError("this call cannot be answered from the paged cache: it takes causal attention, with padding in front, a sliding window or a soft cap, "
+                           "but no dropout, attention sinks as parameters or other masks")
+    out = pool.attend(index, query, scaling=kwargs.get("scaling"), softcap=kwargs.get("softcap"), window=window, starts=starts)
+    paged_counts["paged"] += 1
+    return out
+
+
 def _attention_patch(func):
     if getattr(func, _PATCH_ATTR, False):
         return func
 
     @functools.wraps(func)
     def wrapper(module, query, key, value, attention_mask, dropout=0.0, **kwargs):
+        paged = getattr(key, "_odmkv_paged", None)       # new tokens of a PagedCache, which holds them and all before them
+        if paged is not None:
+            return _paged_attention(paged, module, query, attention_mask, dropout, kwargs), None
         # a decode step like the layer's last one: the native block checks the call, stores the token and attends
         state = module.__dict__.get("_odmkv_state")
         fast = None if state is None else getattr(state, "_fast", None)

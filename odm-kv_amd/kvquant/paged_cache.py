@@ -34,6 +34,10 @@ KINDS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 Counts = Union[int, Sequence[int], torch.Tensor]
 
 
+class OutOfPages(ValueError):
+    """The pool has too few free pages for a call: `compacted` gives a larger one."""
+
+
 def _blocks(tokens: int) -> int:
     return (tokens + BLOCK - 1) // BLOCK
 
@@ -162,7 +166,7 @@ class PagedKVCache:
             if attempt:
                 if max(after) > self.max_tokens:
                     raise ValueError(f"a row of {max(after)} tokens does not fit max_tokens={self.max_tokens}")
-                raise ValueError(f"out of pages: {self._shared['used']} of {self.pages} in use, {need} more wanted")
+                raise OutOfPages(f"out of pages: {self._shared['used']} of {self.pages} in use, {need} more wanted")
             self.refresh()
             self._loose = False
         self._bounds[:] = after

@@ -622,6 +622,7 @@ int odmkv_decode_attn_static(const void* q, int q_dtype, int B, int Hq, float sc
 #define ODMKV_INT8 0
 #define ODMKV_E4M3 1
 #define ODMKV_PAGES_MAX_ROWS 1024
+#define ODMKV_PAGES_HOST_ROWS 512     /* batches up to here can have a row's number each (a count, a length, a parent) from the host, in the launch's arguments */
 
 typedef struct odmkv_pages {
     int32_t layers, rows, Hkv, pages, blocks;    /* blocks: places of a table row, so at most blocks * 64 + 63 tokens a row */
@@ -643,27 +644,27 @@ typedef struct odmkv_pages {
 
 /* An empty cache: lengths 0, row b in slot b, all pages free, table and tails cleared. */
 int odmkv_pages_init(const odmkv_pages_t* p, void* stream);
-/* Every row grows by its count of tokens: device int32 [rows], or NULL: `count` for all.  Blocks that become full get the
+/* Every row grows by its count of tokens: device int32 [rows], or host int32 [rows] (at most ODMKV_PAGES_HOST_ROWS; read before the call returns), or both NULL: `count` for all.  Blocks that become full get the
  * lowest free pages, row after row.  max_count: no count is larger (a larger or negative one refuses the call). */
-int odmkv_pages_extend(const odmkv_pages_t* p, const int32_t* counts, int count, int max_count, void* stream);
+int odmkv_pages_extend(const odmkv_pages_t* p, const int32_t* counts, const int32_t* counts_host, int count, int max_count, void* stream);
 /* The tokens that the last extend made room for, of one layer (once a layer and extend): K, V [rows, Hkv, T, 128] of the
  * cache's dtype with element strides (multiples of 8, 16-byte aligned), row b's tokens at t < its count; T at least max_count. */
 int odmkv_pages_write(const odmkv_pages_t* p, int layer, const void* K, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t,
                       const void* V, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, int T, void* stream);
 /* Dense keys and values of one layer, [rows, Hkv, T, 128] contiguous of out_dtype (any), 0 behind a row's length. */
 int odmkv_pages_read(const odmkv_pages_t* p, int layer, void* K, void* V, int out_dtype, int T, void* stream);
-/* Row b becomes a copy of row parents[b] (device int64 [rows], all at once): full blocks are shared, tails copied.  A row
+/* Row b becomes a copy of row parents[b] (device int64 [rows], or host int32 [rows], all at once): full blocks are shared, tails copied.  A row
  * that stays, or else the first copy of one that does not, keeps its place.  A parent out of range refuses the call. */
 size_t odmkv_pages_reorder_workspace_bytes(int rows);
-int odmkv_pages_reorder(const odmkv_pages_t* p, const int64_t* parents, void* workspace, size_t workspace_bytes, void* stream);
+int odmkv_pages_reorder(const odmkv_pages_t* p, const int64_t* parents, const int32_t* parents_host, void* workspace, size_t workspace_bytes, void* stream);
 /* The rows of `to` (another batch over the same pages: same codes, scales, refs, status; its own table, tails, length, start,
  * slot, rows; its rows hold nothing yet) become copies of rows parents[b] of p (device int64 [to->rows]).  p's rows stay. */
 int odmkv_pages_select(const odmkv_pages_t* p, const odmkv_pages_t* to, const int64_t* parents, void* workspace,
                        size_t workspace_bytes, void* stream);
-/* Rows shrink to a length (device int32 [rows], or NULL: `length` for all; a longer one leaves the row): pages that nobody
+/* Rows shrink to a length (device int32 [rows], or host int32 [rows], or both NULL: `length` for all; a longer one leaves the row): pages that nobody
  * holds any more are free; a full block that is cut becomes the tail, as the values that it stands for.  row_mask: host
  * uint32 [32], bit b of word b / 32 set for the rows meant, or NULL: all. */
-int odmkv_pages_truncate(const odmkv_pages_t* p, const int32_t* lengths, int length, const uint32_t* row_mask, void* stream);
+int odmkv_pages_truncate(const odmkv_pages_t* p, const int32_t* lengths, const int32_t* lengths_host, int length, const uint32_t* row_mask, void* stream);
 /* `to` (pages of its own, at least as many as p has in use; blocks of its own, at least what p's rows need; the rest as p's)
  * becomes what p is, its pages in use one behind the other in their order.  workspace: 4 bytes a page of p. */
 size_t odmkv_pages_compact_workspace_bytes(int pages);

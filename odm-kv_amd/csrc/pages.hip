@@ -24,6 +24,23 @@ static int check_layer(const char* who, const odmkv_pages_t* p, int layer) {
     return 0;
 }
 
+// one whole number a row: from the device, from the host by way of the launch's arguments, or the same for all
+struct RowInts {
+    const int32_t* device;
+    int all, from_host;
+    int32_t host[ODMKV_PAGES_HOST_ROWS];
+};
+__device__ static inline int row_int(const RowInts& a, int row) { return a.device ? a.device[row] : a.from_host ? a.host[row] : a.all; }
+static int make_row_ints(const char* who, RowInts& a, int rows, const int32_t* device, const int32_t* host, int all) {
+    ODMKV_CHECK_ARG(!device || !host, "%s: numbers from the device and from the host", who);
+    ODMKV_CHECK_ARG(!host || rows <= ODMKV_PAGES_HOST_ROWS, "%s: %d rows' numbers from the host", who, rows);
+    a.device = device;
+    a.all = all;
+    a.from_host = host != nullptr;
+    for (int i = 0; i < ODMKV_PAGES_HOST_ROWS; ++i) a.host[i] = host && i < rows ? host[i] : 0;
+    return 0;
+}
+
 // ---- bookkeeping ----------------------------------------------------------------------------------
 // inclusive prefix sum over the workgroup's threads; total: of all.  part: one int a wavefront.
 __device__ static inline int book_scan(int v, int* part, int& total) {
@@ -75,7 +92,7 @@ extern "C" int odmkv_pages_init(const odmkv_pages_t* p, void* stream) {
 
 // One workgroup, a thread a row; the lowest free pages are found by going over the holders' counts from the hint on, and each goes to
 // the row and block of its rank.
-__global__ __launch_bounds__(BOOK_THREADS) void pages_extend_kernel(odmkv_pages_t p, const int32_t* counts, int count, int max_count) {
+__global__ __launch_bounds__(BOOK_THREADS) void pages_extend_kernel(odmkv_pages_t p, RowInts counts, int max_count) {
     __shared__ int part[BOOK_THREADS / 64], upto[MAX_ROWS], first[MAX_ROWS], slots[MAX_ROWS];
     __shared__ int refused, last;
     const int tid = threadIdx.x;
@@ -84,7 +101,7 @@ __global__ __launch_bounds__(BOOK_THREADS) void pages_extend_kernel(odmkv_pages_
     if (tid == 0) refused = last = 0;
     if (tid < p.rows) {
         len = p.length[tid];
-        c = counts ? counts[tid] : count;
+        c = row_int(counts, tid);
         bad = c < 0 || c > max_count;
         if (bad) c = 0;
         bad = bad || (long long)len + c > (long long)p.blocks * BLOCK_TOKENS + BLOCK_TOKENS - 1;
@@ -131,10 +148,12 @@ __global__ __launch_bounds__(BOOK_THREADS) void pages_extend_kernel(odmkv_pages_
     }
 }
 
-extern "C" int odmkv_pages_extend(const odmkv_pages_t* p, const int32_t* counts, int count, int max_count, void* stream) {
+extern "C" int odmkv_pages_extend(const odmkv_pages_t* p, const int32_t* counts, const int32_t* counts_host, int count, int max_count, void* stream) {
     if (int rc = check_pages("pages_extend", p)) return rc;
-    ODMKV_CHECK_ARG(max_count >= 0 && (counts || (count >= 0 && count <= max_count)), "pages_extend: bad count");
-    hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(BOOK_THREADS), 0, (hipStream_t)stream, *p, counts, count, max_count);
+    ODMKV_CHECK_ARG(max_count >= 0 && (counts || counts_host || (count >= 0 && count <= max_count)), "pages_extend: bad count");
+    RowInts c;
+    if (int rc = make_row_ints("pages_extend", c, p->rows, counts, counts_host, count)) return rc;
+    hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(BOOK_THREADS), 0, (hipStream_t)stream, *p, c, max_count);
     ODMKV_CHECK_LAUNCH("pages_extend_kernel");
     return 0;
 }
@@ -385,7 +404,7 @@ struct Move { int from, to, length, dropped; };      // to < 0: nothing
 
 // One workgroup, a thread a row.  A parent's slot goes to the row itself if it stays, or else to its first child; every other row takes a
 // slot that no row uses any more, both in ascending order.
-__global__ __launch_bounds__(BOOK_THREADS) void pages_plan_kernel(odmkv_pages_t p, const int64_t* parents, Move* moves) {
+__global__ __launch_bounds__(BOOK_THREADS) void pages_plan_kernel(odmkv_pages_t p, const int64_t* parents, RowInts known, Move* moves) {
     __shared__ int part[BOOK_THREADS / 64], slots[MAX_ROWS], lengths[MAX_ROWS], heir[MAX_ROWS], owner[MAX_ROWS], unused[MAX_ROWS];
     __shared__ int refused;
     const int tid = threadIdx.x, rows = p.rows;
@@ -396,7 +415,7 @@ __global__ __launch_bounds__(BOOK_THREADS) void pages_plan_kernel(odmkv_pages_t 
     if (mine) {
         slots[tid] = p.slot[tid];
         lengths[tid] = p.length[tid];
-        parent = parents[tid];
+        parent = parents ? parents[tid] : row_int(known, tid);
     }
     __syncthreads();
     if (mine) owner[slots[tid]] = tid;                         // which row a slot belongs to
@@ -454,11 +473,21 @@ __global__ __launch_bounds__(BOOK_THREADS) void pages_plan_select_kernel(odmkv_p
     to.length[tid] = to.start[tid] = len;
 }
 
-// one holder less of a page; the last one frees it
-__device__ static inline void drop_page(const odmkv_pages_t& p, int page) {
+// Pages that lose a holder; those that lose their last are free.  A wavefront's are counted together before the pool's words are touched.
+struct Freed { int count, lowest; };
+__device__ static inline void drop_page(const odmkv_pages_t& p, int page, Freed& f) {
     if (atomicSub(&p.refs[page], 1) == 1) {
-        atomicAdd(&p.status[ST_FREE], 1);
-        atomicMin(&p.status[ST_HINT], page);
+        f.count += 1;
+        f.lowest = min(f.lowest, page);
+    }
+}
+__device__ static inline void give_back(const odmkv_pages_t& p, const Freed& f) {      // by all lanes of a wavefront
+    const auto add = [](float x, float y) { return __int_as_float(__float_as_int(x) + __float_as_int(y)); };
+    const auto less = [](float x, float y) { return __int_as_float(min(__float_as_int(x), __float_as_int(y))); };
+    const int count = __float_as_int(wave_fold(__int_as_float(f.count), add)), lowest = __float_as_int(wave_fold(__int_as_float(f.lowest), less));
+    if (count > 0 && (threadIdx.x & 63) == 0) {
+        atomicAdd(&p.status[ST_FREE], count);
+        atomicMin(&p.status[ST_HINT], lowest);
     }
 }
 
@@ -472,12 +501,14 @@ __global__ __launch_bounds__(256) void pages_move_kernel(odmkv_pages_t p, odmkv_
         const int full = m.length / BLOCK_TOKENS;
         const int32_t* src = p.table + (size_t)m.from * p.blocks;
         int32_t* dst = to.table + (size_t)m.to * to.blocks;
+        Freed freed = {0, 0x7fffffff};
         for (int j = tid; j < to.blocks; j += 256) {
             const int was = j < m.dropped ? dst[j] : -1, is = src[j];
             dst[j] = is;
             if (j < full) atomicAdd(&p.refs[is], 1);
-            if (was >= 0) drop_page(p, was);
+            if (was >= 0) drop_page(p, was, freed);
         }
+        give_back(p, freed);
         return;
     }
     const int lh = blockIdx.y - 1, layer = lh / p.Hkv, h = lh % p.Hkv;
@@ -497,15 +528,18 @@ static int launch_moves(const odmkv_pages_t* p, const odmkv_pages_t* to, const M
     return 0;
 }
 
-extern "C" int odmkv_pages_reorder(const odmkv_pages_t* p, const int64_t* parents, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int odmkv_pages_reorder(const odmkv_pages_t* p, const int64_t* parents, const int32_t* parents_host, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
     if (int rc = check_pages("pages_reorder", p)) return rc;
-    ODMKV_CHECK_ARG(parents != nullptr, "pages_reorder: null pointer");
+    ODMKV_CHECK_ARG((parents != nullptr) != (parents_host != nullptr), "pages_reorder: parents from the device or from the host");
+    RowInts known;
+    if (int rc = make_row_ints("pages_reorder", known, p->rows, nullptr, parents_host, 0)) return rc;
     ODMKV_CHECK_ARG((long long)p->layers * p->Hkv < 65535, "pages_reorder: more than 65534 layers and heads");
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < odmkv_pages_reorder_workspace_bytes(p->rows)) {
         odmkv_set_error("pages_reorder: workspace too small");
         return ODMKV_ENOSPACE;
     }
-    hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(BOOK_THREADS), 0, (hipStream_t)stream, *p, parents, (Move*)workspace);
+    hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(BOOK_THREADS), 0, (hipStream_t)stream, *p, parents, known, (Move*)workspace);
     ODMKV_CHECK_LAUNCH("pages_plan_kernel");
     return launch_moves(p, p, (const Move*)workspace, (hipStream_t)stream);
 }
@@ -533,13 +567,12 @@ extern "C" int odmkv_pages_select(const odmkv_pages_t* p, const odmkv_pages_t* t
 // ---- rewinds --------------------------------------------------------------------------------------
 struct TruncateArgs {
     odmkv_pages_t p;
-    const int32_t* lengths;
-    int length;
+    RowInts lengths;
     uint32_t rows[MAX_ROWS / 32];
 };
 __device__ static inline int cut_length(const TruncateArgs& a, int row, int len) {
     if (!(a.rows[row >> 5] >> (row & 31) & 1u)) return len;
-    return min(len, max(a.lengths ? a.lengths[row] : a.length, 0));
+    return min(len, max(row_int(a.lengths, row), 0));
 }
 
 // blockIdx.y == 0: the pages given up; from 1 on: a layer and head of the block that becomes the tail
@@ -550,7 +583,9 @@ __global__ __launch_bounds__(256) void pages_truncate_kernel(TruncateArgs a) {
     const int keep = cut / BLOCK_TOKENS, full = len / BLOCK_TOKENS, slot = p.slot[row];
     if (keep >= full) return;
     if (blockIdx.y == 0) {
-        for (int j = keep + tid; j < full; j += 256) drop_page(p, p.table[(size_t)slot * p.blocks + j]);
+        Freed freed = {0, 0x7fffffff};
+        for (int j = keep + tid; j < full; j += 256) drop_page(p, p.table[(size_t)slot * p.blocks + j], freed);
+        give_back(p, freed);
         return;
     }
     if (cut == keep * BLOCK_TOKENS) return;
@@ -582,16 +617,16 @@ __global__ __launch_bounds__(BOOK_THREADS) void pages_cut_kernel(TruncateArgs a)
     a.p.length[row] = a.p.start[row] = cut_length(a, row, a.p.length[row]);
 }
 
-extern "C" int odmkv_pages_truncate(const odmkv_pages_t* p, const int32_t* lengths, int length, const uint32_t* row_mask, void* stream) {
+extern "C" int odmkv_pages_truncate(const odmkv_pages_t* p, const int32_t* lengths, const int32_t* lengths_host, int length, const uint32_t* row_mask,
+                                    void* stream) {
     if (int rc = check_pages("pages_truncate", p)) return rc;
-    ODMKV_CHECK_ARG(lengths || length >= 0, "pages_truncate: bad length");
+    ODMKV_CHECK_ARG(lengths || lengths_host || length >= 0, "pages_truncate: bad length");
     ODMKV_CHECK_ARG((long long)p->layers * p->Hkv < 65535, "pages_truncate: more than 65534 layers and heads");
     TruncateArgs a;
     a.p = *p;
-    a.lengths = lengths;
-    a.length = length;
+    if (int rc = make_row_ints("pages_truncate", a.lengths, p->rows, lengths, lengths_host, length)) return rc;
     for (int i = 0; i < MAX_ROWS / 32; ++i) a.rows[i] = row_mask ? row_mask[i] : 0xffffffffu;
-    const int tails = lengths || length % BLOCK_TOKENS ? p->layers * p->Hkv : 0;
+    const int tails = lengths || lengths_host || length % BLOCK_TOKENS ? p->layers * p->Hkv : 0;
     PAGES_DISPATCH(pages_truncate_kernel, p, dim3(p->rows, 1 + tails), dim3(256), 0, (hipStream_t)stream, a);
     ODMKV_CHECK_LAUNCH("pages_truncate_kernel");
     hipLaunchKernelGGL(pages_cut_kernel, dim3(1), dim3(BOOK_THREADS), 0, (hipStream_t)stream, a);

@@ -101,8 +101,8 @@ PyObject* run(Step* s, const at::Tensor& q, const at::Tensor& k, const at::Tenso
     return THPVariable_Wrap(std::move(out));
 }
 
-#define GUARDED(body)                                                  \
-    try { body } catch (const std::exception& e) {                     \
+#define GUARDED(...)                                                   \
+    try { __VA_ARGS__ } catch (const std::exception& e) {                     \
         PyErr_SetString(PyExc_RuntimeError, e.what());                 \
         return nullptr;                                                \
     }
@@ -216,7 +216,122 @@ PyObject* native_alias(PyObject*, PyObject* const* a, Py_ssize_t n) {
     )
 }
 
+// ---- the paged cache's calls of every layer and step: None where a call does not fit as it is, and Python checks, copies or refuses
+typedef int (*write_fn)(const odmkv_pages_t*, int, const void*, int64_t, int64_t, int64_t, const void*, int64_t, int64_t, int64_t, int, void*);
+typedef int (*attend_fn)(const odmkv_attend_t*, void*);
+typedef size_t (*attend_bytes_fn)(const odmkv_pages_t*, int, int, int);
+
+// rows of 128 of the cache's type on its device that start on 16 bytes
+bool rows_fit(const odmkv_pages_t* p, const at::Tensor& t, int device) {
+    if (t.dim() != 4 || !t.is_cuda() || t.get_device() != device || t.scalar_type() != scalar_of(p->dtype)) return false;
+    const auto z = t.sizes(); const auto r = t.strides();
+    return z[0] == p->rows && z[3] == ODMKV_HEAD_DIM && r[3] == 1 && ((r[0] | r[1] | r[2]) & 7) == 0 && ((uintptr_t)t.data_ptr() & 15) == 0;
+}
+
+PyObject* raise_odmkv(int rc, const char* what) {
+    return PyErr_Format(rc == ODMKV_EHIP ? PyExc_RuntimeError : PyExc_ValueError, "odmkv: %s failed (code %d)", what, rc);
+}
+
+// paged_write(entry, pages, device, layer, keys, values, stream): True, or None
+PyObject* native_paged_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 7 || !THPVariable_Check(a[4]) || !THPVariable_Check(a[5])) {
+        PyErr_SetString(PyExc_TypeError, "paged_write(entry, pages, device, layer, keys, values, stream)");
+        return nullptr;
+    }
+    const write_fn fn = (write_fn)(uintptr_t)PyLong_AsUnsignedLongLong(a[0]);
+    const odmkv_pages_t* p = (const odmkv_pages_t*)(uintptr_t)PyLong_AsUnsignedLongLong(a[1]);
+    const int device = (int)PyLong_AsLong(a[2]);
+    const long layer = PyLong_AsLong(a[3]);
+    const unsigned long long stream = PyLong_AsUnsignedLongLong(a[6]);
+    if (PyErr_Occurred()) return nullptr;
+    GUARDED(
+        const at::Tensor& k = THPVariable_Unpack(a[4]);
+        const at::Tensor& v = THPVariable_Unpack(a[5]);
+        if (layer < 0 || layer >= p->layers || !rows_fit(p, k, device) || !rows_fit(p, v, device) || k.sizes() != v.sizes() || k.size(1) != p->Hkv
+            || k.size(2) > INT32_MAX) Py_RETURN_NONE;
+        const int rc = fn(p, (int)layer, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2),
+                          (int)k.size(2), (void*)(uintptr_t)stream);
+        if (rc) return raise_odmkv(rc, "storing tokens");
+        Py_RETURN_TRUE;
+    )
+}
+
+// paged_attend(attend entry, workspace entry, pages, device, layer, query, scaling, cap, window, max_length, want_lse, counts, slopes, prefix, starts,
+// stream): out, or (out, lse), or None.  counts, slopes, prefix, starts: None, or tensors of the right type and shape, contiguous.
+PyObject* native_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 16 || !THPVariable_Check(a[5])) {
+        PyErr_SetString(PyExc_TypeError, "paged_attend(attend, bytes, pages, device, layer, query, scaling, cap, window, max_length, want_lse, counts, "
+                                         "slopes, prefix, starts, stream)");
+        return nullptr;
+    }
+    const attend_fn fn = (attend_fn)(uintptr_t)PyLong_AsUnsignedLongLong(a[0]);
+    const attend_bytes_fn bytes_of = (attend_bytes_fn)(uintptr_t)PyLong_AsUnsignedLongLong(a[1]);
+    const odmkv_pages_t* p = (const odmkv_pages_t*)(uintptr_t)PyLong_AsUnsignedLongLong(a[2]);
+    const int device = (int)PyLong_AsLong(a[3]);
+    const long layer = PyLong_AsLong(a[4]);
+    const double scaling = PyFloat_AsDouble(a[6]);
+    const double cap = PyFloat_AsDouble(a[7]);
+    const long long window = PyLong_AsLongLong(a[8]);
+    const long long longest = PyLong_AsLongLong(a[9]);
+    const int want_lse = PyObject_IsTrue(a[10]);
+    const unsigned long long stream = PyLong_AsUnsignedLongLong(a[15]);
+    if (PyErr_Occurred()) return nullptr;
+    GUARDED(
+        const at::Tensor& q = THPVariable_Unpack(a[5]);
+        if (layer < 0 || layer >= p->layers || !rows_fit(p, q, device)) Py_RETURN_NONE;
+        const int64_t Hq = q.size(1);
+        const int64_t L = q.size(2);
+        if (Hq <= 0 || Hq % p->Hkv || Hq / p->Hkv > ODMKV_MAX_GROUP || L < 1 || L > (1 << 26)) Py_RETURN_NONE;
+        const void* small[4];
+        for (int i = 0; i < 4; ++i) {
+            small[i] = nullptr;
+            if (a[11 + i] == Py_None) continue;
+            if (!THPVariable_Check(a[11 + i])) Py_RETURN_NONE;
+            const at::Tensor& t = THPVariable_Unpack(a[11 + i]);
+            const int64_t want = i == 1 ? Hq : p->rows;
+            if (!t.is_cuda() || t.get_device() != device || t.scalar_type() != (i == 1 ? at::kFloat : at::kInt) || !t.is_contiguous() || t.dim() < 1
+                || t.size(0) != want || (i < 3 ? t.dim() != 1 : t.dim() > 2 || (t.dim() == 2 && t.size(1) != L))) Py_RETURN_NONE;
+            small[i] = t.data_ptr();
+        }
+        const bool some = a[11] != Py_None;                   // (rows behind a count come back as 0)
+        const int64_t shape[4] = {p->rows, L, Hq, ODMKV_HEAD_DIM};
+        const int64_t lse_shape[3] = {p->rows, Hq, L};
+        const auto make = [&](at::IntArrayRef z, at::ScalarType type) { return some ? at::zeros(z, q.options().dtype(type)) : at::empty(z, q.options().dtype(type)); };
+        at::Tensor out = make(at::IntArrayRef(shape, 4), q.scalar_type());
+        at::Tensor lse;
+        if (want_lse) lse = make(at::IntArrayRef(lse_shape, 3), at::kFloat);
+        const size_t bytes = bytes_of(p, (int)Hq, (int)L, (int)longest);
+        at::Tensor ws;
+        if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));      // (of its own for every call: a graph's is the graph's)
+        odmkv_attend_t d;
+        memset(&d, 0, sizeof d);
+        d.pages = p; d.q = q.data_ptr(); d.q_stride_b = q.stride(0); d.q_stride_h = q.stride(1); d.q_stride_l = q.stride(2);
+        d.out = out.data_ptr();
+        d.lse = want_lse ? (float*)lse.data_ptr() : nullptr;
+        d.counts = (const int32_t*)small[0]; d.slopes = (const float*)small[1]; d.prefix = (const int32_t*)small[2]; d.starts = (const int32_t*)small[3];
+        if (small[3]) {
+            const at::Tensor& t = THPVariable_Unpack(a[14]);
+            d.start_stride_b = t.stride(0);
+            d.start_stride_l = t.dim() == 2 ? t.stride(1) : 0;
+        }
+        d.workspace = bytes ? ws.data_ptr() : nullptr; d.workspace_bytes = bytes;
+        d.layer = (int)layer; d.L = (int)L; d.Hq = (int)Hq; d.window = (int)window; d.max_length = (int)longest;
+        d.scaling = (float)scaling; d.cap = (float)cap;
+        const int rc = fn(&d, (void*)(uintptr_t)stream);
+        if (rc) return raise_odmkv(rc, "attention over the paged cache");
+        if (!want_lse) return THPVariable_Wrap(std::move(out));
+        PyObject* both = PyTuple_New(2);
+        if (both) {
+            PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(out)));
+            PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(lse)));
+        }
+        return both;
+    )
+}
+
 PyMethodDef module_methods[] = {
+    {"paged_write", (PyCFunction)(void*)native_paged_write, METH_FASTCALL, nullptr},
+    {"paged_attend", (PyCFunction)(void*)native_paged_attend, METH_FASTCALL, nullptr},
     {"alias", (PyCFunction)(void*)native_alias, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, module_methods};

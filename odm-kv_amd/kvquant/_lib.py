@@ -177,13 +177,13 @@ def _load() -> C.CDLL:
         "odmkv_flush_score": (C.c_int, [vp, vp, i32, i32, i32, vp, f32, f32, i32, vp, vp, vp, vp]),
         "odmkv_flush_rank": (C.c_int, [vp, vp, i32, i32, i32, vp, vp, vp]),
         "odmkv_pages_init": (C.c_int, [C.POINTER(Pages), vp]),
-        "odmkv_pages_extend": (C.c_int, [C.POINTER(Pages), vp, i32, i32, vp]),
+        "odmkv_pages_extend": (C.c_int, [C.POINTER(Pages), vp, vp, i32, i32, vp]),
         "odmkv_pages_write": (C.c_int, [C.POINTER(Pages), i32, vp, i64, i64, i64, vp, i64, i64, i64, i32, vp]),
         "odmkv_pages_read": (C.c_int, [C.POINTER(Pages), i32, vp, vp, i32, i32, vp]),
         "odmkv_pages_reorder_workspace_bytes": (sz, [i32]),
-        "odmkv_pages_reorder": (C.c_int, [C.POINTER(Pages), vp, vp, sz, vp]),
+        "odmkv_pages_reorder": (C.c_int, [C.POINTER(Pages), vp, vp, vp, sz, vp]),
         "odmkv_pages_select": (C.c_int, [C.POINTER(Pages), C.POINTER(Pages), vp, vp, sz, vp]),
-        "odmkv_pages_truncate": (C.c_int, [C.POINTER(Pages), vp, i32, vp, vp]),
+        "odmkv_pages_truncate": (C.c_int, [C.POINTER(Pages), vp, vp, i32, vp, vp]),
         "odmkv_pages_compact_workspace_bytes": (sz, [i32]),
         "odmkv_pages_compact": (C.c_int, [C.POINTER(Pages), C.POINTER(Pages), vp, sz, vp]),
         "odmkv_pages_attend_workspace_bytes": (sz, [C.POINTER(Pages), i32, i32, i32]),
@@ -198,6 +198,7 @@ def _load() -> C.CDLL:
 
 lib = _load()
 STEP_ENTRY = C.cast(lib.odmkv_decode_step, C.c_void_p).value      # what _native.Step calls
+PAGES_ENTRIES = tuple(C.cast(f, C.c_void_p).value for f in (lib.odmkv_pages_write, lib.odmkv_pages_attend, lib.odmkv_pages_attend_workspace_bytes))
 EXPORTS = ("odmkv_version", "odmkv_last_error", "odmkv_score_workspace_bytes", "odmkv_score", "odmkv_score_model_dtype", "odmkv_score_expected", "odmkv_token_mean_workspace_bytes", "odmkv_token_mean", "odmkv_average_rope",
            "odmkv_project_rows", "odmkv_prompt_scores_workspace_bytes", "odmkv_prompt_scores", "odmkv_query_covariance_workspace_bytes", "odmkv_query_covariance", "odmkv_rotate_queries",
            "odmkv_normalize_workspace_bytes", "odmkv_normalize_scores",

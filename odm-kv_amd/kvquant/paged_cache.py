@@ -28,8 +28,15 @@ from ._lib import HEAD_DIM, lib
 
 BLOCK = 64                                    # tokens of a page
 MAX_ROWS = 1024                               # the bookkeeping runs in one workgroup, a thread a row
+HOST_ROWS = 512                               # batches up to here have a row's number each travel in the launch's arguments
 MAX_GROUP = 8
 KINDS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
+
+_SCALING = HEAD_DIM ** -0.5
+_FAR = 2 ** 30                                # a window past everything
+_WRITE, _ATTEND, _ATTEND_BYTES = _lib.PAGES_ENTRIES
+_native = _lib._native
+_device = torch.cuda.current_device
 
 Counts = Union[int, Sequence[int], torch.Tensor]
 
@@ -104,6 +111,7 @@ class PagedKVCache:
         self._p = _lib.Pages(self.layers, self.batch, self.kv_heads, self.pages, self.table.shape[1], _lib._DT[self.dtype], KINDS[self.kind][0],
                              *(t.data_ptr() for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.table,
                                                       self.length, self.start, self.slot, self.refs, self.status)))
+        self._at = C.addressof(self._p)
 
     def _sibling(self, batch: int) -> "PagedKVCache":
         new = object.__new__(PagedKVCache)
@@ -121,21 +129,28 @@ class PagedKVCache:
         else:
             _lib.check(fn(*args, _lib.stream_ptr(self.device)))
 
-    def _ints(self, values, dtype, what: str) -> torch.Tensor:
-        """A device tensor of one whole number a row."""
-        if not (isinstance(values, torch.Tensor) and values.is_cuda) and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"{what} must lie on the device while a graph is captured: every replay would read the host's memory again")
-        if isinstance(values, torch.Tensor):
+    def _ints(self, values, n: int, dtype, what: str):
+        """One whole number a row: (device tensor or None, host int32 array or None, the same as a list where the host knows it)."""
+        if isinstance(values, torch.Tensor) and values.is_cuda:
             if values.is_floating_point() or values.is_complex() or values.dtype == torch.bool:
                 raise ValueError(f"{what} must be whole numbers, got {values.dtype}")
-            if values.device.type == "cuda" and values.device != self.device:
+            if values.device != self.device:
                 raise ValueError(f"{what} lie on {values.device}, the cache on {self.device}")
-            values = values.to(device=self.device, dtype=dtype)
-        else:
-            values = torch.tensor([int(v) for v in values], dtype=dtype, pin_memory=True).to(self.device, non_blocking=True)
-        if values.dim() != 1:
-            raise ValueError(f"{what} must be one number a row, got {tuple(values.shape)}")
-        return values.contiguous()
+            if values.shape != (n,):
+                raise ValueError(f"{what} must be one number a row, [{n}], got {list(values.shape)}")
+            return values.to(dtype).contiguous(), None, None
+        if isinstance(values, torch.Tensor) and (values.is_floating_point() or values.is_complex() or values.dtype == torch.bool):
+            raise ValueError(f"{what} must be whole numbers, got {values.dtype}")
+        known = [int(v) for v in values]
+        if len(known) != n:
+            raise ValueError(f"{len(known)} {what} for {n} rows")
+        if known and not -2 ** 31 <= min(known) <= max(known) < 2 ** 31:
+            raise ValueError(f"{what} must fit 32 bits")
+        if n <= HOST_ROWS:
+            return None, (C.c_int32 * n)(*known), known
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} of more than {HOST_ROWS} rows must lie on the device while a graph is captured: every replay would read the host's memory again")
+        return torch.tensor(known, dtype=dtype, pin_memory=True).to(self.device, non_blocking=True), None, known
 
     # ------------------------------------------------------------------ what the host knows
     @property
@@ -182,38 +197,35 @@ class PagedKVCache:
             if counts < 0:
                 raise ValueError(f"counts must not be negative, got {counts}")
             self._make_room([counts] * self.batch)
-            self._call(lib.odmkv_pages_extend, C.byref(self._p), None, counts, counts)
+            self._call(lib.odmkv_pages_extend, C.byref(self._p), None, None, counts, counts)
             return
-        if isinstance(counts, torch.Tensor) and counts.is_cuda:
+        on_device, host, known = self._ints(counts, self.batch, torch.int32, "counts")
+        if known is None:
             if bound is None or bound < 0:
                 raise ValueError("counts on the device need a bound that none of them is above")
-            on_device = self._ints(counts, torch.int32, "counts")
-            if on_device.shape[0] != self.batch:
-                raise ValueError(f"{on_device.shape[0]} counts for {self.batch} rows")
             try:
                 self._make_room([int(bound)] * self.batch)
             except ValueError:                               # not if every row grew by the bound: what they do grow by decides
-                known = on_device.tolist()
-                if min(known) < 0 or max(known) > bound:
-                    raise ValueError(f"counts must be 0 to bound={bound}, got {min(known)} to {max(known)}") from None
-                self._make_room(known)
+                read = on_device.tolist()
+                if min(read) < 0 or max(read) > bound:
+                    raise ValueError(f"counts must be 0 to bound={bound}, got {min(read)} to {max(read)}") from None
+                self._make_room(read)
             self._loose = True
         else:
-            counts = [int(c) for c in counts]
-            if len(counts) != self.batch:
-                raise ValueError(f"{len(counts)} counts for {self.batch} rows")
-            if min(counts) < 0:
-                raise ValueError(f"counts must not be negative, got {min(counts)}")
-            bound = max(counts) if bound is None else int(bound)
-            if max(counts) > bound:
-                raise ValueError(f"a count of {max(counts)} is above bound={bound}")
-            on_device = self._ints(counts, torch.int32, "counts")
-            self._make_room(counts)
-        self._call(lib.odmkv_pages_extend, C.byref(self._p), on_device.data_ptr(), 0, int(bound))
+            if min(known) < 0:
+                raise ValueError(f"counts must not be negative, got {min(known)}")
+            if bound is not None and max(known) > bound:
+                raise ValueError(f"a count of {max(known)} is above bound={bound}")
+            bound = max(known)
+            self._make_room(known)
+        self._call(lib.odmkv_pages_extend, C.byref(self._p), _lib.ptr(on_device), host, 0, int(bound))
 
     def write(self, layer: int, keys: torch.Tensor, values: torch.Tensor) -> None:
         """Stores the tokens of the last ``extend`` in one layer: keys, values [B, Hkv, T, 128] of the cache's dtype, row b's at t < its count, T at least
         the largest count.  Once a layer and extend: a second call would take the new tail for the old one."""
+        if _device() == self.device.index and isinstance(keys, torch.Tensor) and isinstance(values, torch.Tensor) and _native.paged_write(
+                _WRITE, self._at, self.device.index, layer, keys, values, _lib.stream_ptr(self.device)):
+            return
         self._check_layer(layer)
         for t, what in ((keys, "keys"), (values, "values")):
             if t.dim() != 4 or t.shape[0] != self.batch or t.shape[1] != self.kv_heads or t.shape[3] != HEAD_DIM:
@@ -277,6 +289,13 @@ class PagedKVCache:
         i - window + 1; hi is i + 1, or `prefix` (int32 [B]: tokens that everybody sees) where that is more, within the row.  Scores are scaling * q.k
         (default 128 ** -0.5), then softcap * tanh(x / softcap), then less slope * |i - j| (`slopes`, fp32 [Hq]).  Queries that see nothing
         get 0, and -inf for lse."""
+        if _device() == self.device.index and isinstance(query, torch.Tensor) and (softcap is None or 0.0 < softcap < math.inf) and (window is None or window >= 1):
+            # (everything as the kernels take it: one native call)
+            done = _native.paged_attend(_ATTEND, _ATTEND_BYTES, self._at, self.device.index, layer, query, _SCALING if scaling is None else scaling,
+                                        0.0 if softcap is None else softcap, 0 if window is None else min(window, _FAR), max(self._bounds), return_lse,
+                                        counts, slopes, prefix, starts, _lib.stream_ptr(self.device))
+            if done is not None:
+                return done
         self._check_layer(layer)
         if query.dim() != 4 or query.shape[0] != self.batch or query.shape[3] != HEAD_DIM:
             raise ValueError(f"query must be [{self.batch}, Hq, L, {HEAD_DIM}], got {tuple(query.shape)}")
@@ -288,7 +307,7 @@ class PagedKVCache:
             raise ValueError(f"softcap must be positive, got {softcap}")
         if window is not None and window < 1:
             raise ValueError(f"window must be positive, got {window}")
-        scaling = HEAD_DIM ** -0.5 if scaling is None else float(scaling)
+        scaling = _SCALING if scaling is None else float(scaling)
         query = self._rows_ok(query)
         slopes = self._small(slopes, "slopes", torch.float32, ((Hq,),))
         prefix = self._small(prefix, "prefix", torch.int32, ((B,),))
@@ -304,7 +323,7 @@ class PagedKVCache:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
             a = _lib.Attend(C.pointer(self._p), query.data_ptr(), *query.stride()[:3], out.data_ptr(), _lib.ptr(lse), _lib.ptr(counts), _lib.ptr(slopes),
                             _lib.ptr(prefix), _lib.ptr(starts), 0 if starts is None else starts.stride(0),
-                            0 if starts is None or starts.dim() == 1 else starts.stride(1), _lib.ptr(ws), nbytes, layer, L, Hq, window or 0, longest,
+                            0 if starts is None or starts.dim() == 1 else starts.stride(1), _lib.ptr(ws), nbytes, layer, L, Hq, min(window or 0, _FAR), longest,
                             scaling, 0.0 if softcap is None else float(softcap))
             self._call(lib.odmkv_pages_attend, C.byref(a))
         return (out, lse) if return_lse else out
@@ -325,16 +344,16 @@ class PagedKVCache:
     def reorder(self, parents) -> None:
         """Row b becomes a copy of row parents[b], all at once (beam search, samples of one prompt): full blocks are shared, tails copied.
         `parents`: a list, or whole numbers on the device (an index out of range is then refused there: see ``refresh``)."""
-        parents = self._parents(parents, self.batch)
-        if parents[1] is None:                               # indices that only the device knows
+        on_device, host, known = self._parents(parents, self.batch)
+        if known is None:                                    # indices that only the device knows
             self._bounds[:] = [self.max_length] * self.batch
             self._loose = True
         else:
-            self._bounds[:] = [self._bounds[b] for b in parents[1]]
+            self._bounds[:] = [self._bounds[b] for b in known]
         self._used_at_most()
         nbytes = lib.odmkv_pages_reorder_workspace_bytes(self.batch)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        self._call(lib.odmkv_pages_reorder, C.byref(self._p), parents[0].data_ptr(), ws.data_ptr(), nbytes)
+        self._call(lib.odmkv_pages_reorder, C.byref(self._p), _lib.ptr(on_device), host, ws.data_ptr(), nbytes)
 
     def select(self, parents) -> "PagedKVCache":
         """A batch of its own over the same pages, whose row b is a copy of this one's row parents[b]; this one's rows stay (``free`` them where they are
@@ -342,7 +361,9 @@ class PagedKVCache:
         n = int(parents.shape[0]) if isinstance(parents, torch.Tensor) and parents.dim() == 1 else len(parents)
         if not 1 <= n <= MAX_ROWS:
             raise ValueError(f"a batch must be 1 to {MAX_ROWS} rows, got {n}")
-        parents = self._parents(parents, n)
+        on_device, host, known = self._parents(parents, n)
+        if on_device is None:
+            on_device = torch.tensor(known, dtype=torch.int64).to(self.device)
         new = self._sibling(n)
         for name in ("pages", "k_codes", "v_codes", "k_scale", "v_scale", "refs", "status", "_shared"):
             setattr(new, name, getattr(self, name))
@@ -351,27 +372,18 @@ class PagedKVCache:
             t.zero_()
         new.slot.copy_(torch.arange(n, dtype=torch.int32, device=self.device))
         new._struct()
-        new._bounds[:] = [self.max_length] * n if parents[1] is None else [self._bounds[b] for b in parents[1]]
-        new._loose = self._loose or parents[1] is None
+        new._bounds[:] = [self.max_length] * n if known is None else [self._bounds[b] for b in known]
+        new._loose = self._loose or known is None
         nbytes = lib.odmkv_pages_reorder_workspace_bytes(n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        self._call(lib.odmkv_pages_select, C.byref(self._p), C.byref(new._p), parents[0].data_ptr(), ws.data_ptr(), nbytes)
+        self._call(lib.odmkv_pages_select, C.byref(self._p), C.byref(new._p), on_device.data_ptr(), ws.data_ptr(), nbytes)
         return new
 
     def _parents(self, parents, n: int):
-        """(device int64 [n], the same as a list or None)"""
-        known = None
-        if not (isinstance(parents, torch.Tensor) and parents.is_cuda):
-            known = [int(b) for b in parents]
-            if len(known) != n:
-                raise ValueError(f"{len(known)} parents for {n} rows")
-            if known and not (0 <= min(known) and max(known) < self.batch):
-                raise ValueError(f"parents must be rows 0 to {self.batch - 1}, got {min(known)} to {max(known)}")
-            parents = known
-        on_device = self._ints(parents, torch.int64, "parents")
-        if on_device.shape[0] != n:
-            raise ValueError(f"{on_device.shape[0]} parents for {n} rows")
-        return on_device, known
+        on_device, host, known = self._ints(parents, n, torch.int64, "parents")
+        if known is not None and not (0 <= min(known) and max(known) < self.batch):
+            raise ValueError(f"parents must be rows 0 to {self.batch - 1}, got {min(known)} to {max(known)}")
+        return on_device, host, known
 
     def truncate(self, lengths: Counts, rows: Optional[Sequence[int]] = None) -> None:
         """Rows shrink to a length (one for all, a list of one a row, or int32 on the device); rows that are not longer stay as they are.  A full block that is
@@ -385,17 +397,12 @@ class PagedKVCache:
                 mask[b >> 5] |= 1 << (b & 31)
         meant = range(self.batch) if rows is None else set(rows)
         if isinstance(lengths, int):
-            if lengths < 0:
-                raise ValueError(f"a length must not be negative, got {lengths}")
-            on_device, known = None, [lengths] * self.batch
+            on_device, host, known = None, None, [lengths] * self.batch
         else:
-            known = None if isinstance(lengths, torch.Tensor) and lengths.is_cuda else [int(n) for n in lengths]
-            if known is not None and known and min(known) < 0:
-                raise ValueError(f"a length must not be negative, got {min(known)}")
-            on_device = self._ints(lengths if known is None else known, torch.int32, "lengths")
-            if on_device.shape[0] != self.batch:
-                raise ValueError(f"{on_device.shape[0]} lengths for {self.batch} rows")
-        self._call(lib.odmkv_pages_truncate, C.byref(self._p), _lib.ptr(on_device), lengths if on_device is None else 0, mask)
+            on_device, host, known = self._ints(lengths, self.batch, torch.int32, "lengths")
+        if known is not None and min(known) < 0:
+            raise ValueError(f"a length must not be negative, got {min(known)}")
+        self._call(lib.odmkv_pages_truncate, C.byref(self._p), _lib.ptr(on_device), host, lengths if isinstance(lengths, int) else 0, mask)
         if known is not None:
             for b in meant:
                 self._bounds[b] = min(self._bounds[b], known[b])

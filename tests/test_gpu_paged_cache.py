@@ -495,12 +495,30 @@ def test_a_replay_without_room_is_refused():
     assert c.refresh() == [120]
 
 
-def test_a_list_from_the_host_is_not_captured():
-    c = _cache(2, 1, 200)
+def test_numbers_from_the_host_in_a_graph():
+    """Up to 512 rows they are part of the launch and the same at every replay; beyond that the host's memory would be read again, which is refused."""
+    r = _Rows([200, 64, 130], layers=1)
+    k, v = (x.to(DEV) for x in _rows(90, 3, 2, 70, torch.float16))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r.c.reorder([0, 0, 1])
+        r.c.truncate([100, 1000, 3])
+        r.c.extend([1, 70, 64])
+        r.c.write(0, k, v)
+    junk = [torch.full((1 << 16,), i, pin_memory=True) for i in range(4)]       # (what pinned memory was about would be overwritten)
+    for _ in range(3):
+        graph.replay()
+        rows = [r.rows[0][b] for b in (0, 0, 1)]
+        rows = [tuple(plain.cut(x, n, r.kind) for x in row) for row, n in zip(rows, (100, 1000, 3))]
+        r.rows[0] = [tuple(torch.cat([x, y[b, :, :n].cpu()], dim=1) for x, y in zip(row, (k, v))) for b, (row, n) in enumerate(zip(rows, (1, 70, 64)))]
+        assert r.c.refresh() == [x[0].shape[1] for x in r.rows[0]]
+        r.check()
+    assert len(junk) == 4
+    wide = _cache(600, 1, 70)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         torch.zeros(1, device=DEV)
-        for call in (lambda: c.reorder([0, 0]), lambda: c.truncate([3, 4]), lambda: c.extend([1, 2])):
+        for call in (lambda: wide.reorder([0] * 600), lambda: wide.truncate([3] * 600), lambda: wide.extend([1] * 600)):
             with pytest.raises(RuntimeError, match="captured"):
                 call()
 

@@ -3,6 +3,7 @@
 //
 //   x_j = scaling * s_k (q . c_j), capped and biased;  out = sum_j softmax(x)_j s_v v_j over lo <= j < hi
 #include <algorithm>
+#include <type_traits>
 #include "pages.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -22,9 +23,9 @@ struct AttendArgs {
     int64_t sb, sl;
     int layer, L, Hq, G, window;
     float scaling, cap;
-    int splits;          // workgroups that share a row and kv-head's blocks
-    float* part_out;     // [rows, Hkv, splits, G L, 128]
-    float* part_lse;     // [rows, Hkv, splits, G L], base 2
+    int splits;          // workgroups of a kv-head (narrow), or that share a row and kv-head's blocks (wide)
+    float* part_out;     // narrow [Hkv, splits, G L, 128], wide [rows, Hkv, splits, G L, 128]
+    float* part_lse;     // the same without the 128, base 2
 };
 
 #define LOG2E 1.4426950408889634f
@@ -55,6 +56,15 @@ __device__ static inline float tanh_of(float t) {
     return a < 0.3f ? __fmaf_rn(t * b, f, t) : far;
 }
 
+// a piece of codes; STREAM: read once, so that the caches need not keep it
+template <bool STREAM>
+__device__ static inline uint4 piece16(const uint8_t* at) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    if (!STREAM) return *reinterpret_cast<const uint4*>(at);
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 // eight codes as fp16, all of them exactly.  int8: c + 128 is the low byte of the fp16 number 1024 + (c + 128)
 template <int KIND>
 __device__ static inline f16x8 codes_f16(uint32_t w0, uint32_t w1) {
@@ -76,25 +86,24 @@ __device__ static inline f16x8 codes_f16(uint32_t w0, uint32_t w1) {
     return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
 
-// 16-bit numbers on the fp16 matrix cores: times a power of two that takes the largest of them (its bits: `top`) to 64 .. 128.  Nothing that counts
-// is lost: what falls out of fp16's range is 2^-31 of the largest and less.
+// 16-bit numbers on the fp16 matrix cores: times a power of two that takes the largest of them (its bits: `top`) to 64 .. 128 (fp16 numbers: by 2^15 at the
+// most, which loses nothing either).  Nothing that counts is lost: what falls out of fp16's range is 2^-30 of the largest and less.
 struct Power { float up, down; };
 template <int DT>
 __device__ static inline Power power_for(uint32_t top) {
     const float t = Elem<DT>::to_f32((uint16_t)top);
-    const int e = min(max((int)(__float_as_uint(t) >> 23) - 127, -100), 127);
+    const int e = min(max((int)(__float_as_uint(t) >> 23) - 127, DT == ODMKV_F16 ? -9 : -100), 127);
     return {__uint_as_float((uint32_t)(127 + 6 - e) << 23), __uint_as_float((uint32_t)(127 - 6 + e) << 23)};
 }
 template <int DT>
 __device__ static inline f16x8 scaled_f16(const uint4& v, float up) {
+    if constexpr (DT == ODMKV_F16) return __builtin_bit_cast(f16x8, v) * (_Float16)up;
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    f16x8 h;
+    uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        h[2 * i] = (_Float16)(Elem<DT>::to_f32((uint16_t)(w[i] & 0xffffu)) * up);
-        h[2 * i + 1] = (_Float16)(Elem<DT>::to_f32((uint16_t)(w[i] >> 16)) * up);
-    }
-    return h;
+    for (int i = 0; i < 4; ++i)                                 // (towards zero: exact but for the numbers that fall out of the range)
+        h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up));
+    return __builtin_bit_cast(f16x8, make_uint4(h[0], h[1], h[2], h[3]));
 }
 __device__ static inline uint32_t abs_max8(const uint4& v) {
     return max(max(abs_max_pair(v.x), abs_max_pair(v.y)), max(abs_max_pair(v.z), abs_max_pair(v.w)));
@@ -127,18 +136,74 @@ __device__ static inline int wave_min_int(int v) {
 // Codes are exact in fp16, queries as they are (bf16: times a power of two each), products and sums fp32; a block's scale joins the scores and, for values,
 // the weights: weights are rounded to fp16 (half a step, 2^-12 to 2^-11 of themselves) times 2^7 s / (largest s of the wavefront's blocks).
 //
-// A wavefront takes every fourth block of its workgroup's share, its pages and scales looked up 64 at a time, the next block's keys and values requested
+// A wavefront takes every fourth (or eighth) block of its workgroup's share, its pages and scales looked up 64 at a time, the next block's keys and values requested
 // as soon as this one's are used.  Bound by memory (256 bytes a token and head); the arithmetic of a block is about a third of the time its bytes take.
 #define NARROW 16
-#define NARROW_WAVES 4
 #define RISE 8.0f            // how far scores may pass the reference (base 2) before the sums are brought to a new one
+#define NARROW_LDS(waves) ((waves) * NARROW * (HD + 4 + 2) * 4)
 
-template <int DT, int KIND, bool PLAIN>
-__global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(AttendArgs a) {
+// The workgroups of a kv-head, `splits` of them, go to the rows by their lengths: one each, the others in proportion.  Given a workgroup (`at`): its row;
+// given a row: its first workgroup; and how many it has.  A wavefront does this by itself, 64 rows at a time.
+struct Share { int row, first, count; };
+__device__ static inline int wave_scan(int v) {                 // inclusive
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+template <bool BY_ROW>
+__device__ static inline Share share_of(const AttendArgs& a, int at) {
     const odmkv_pages_t& p = a.p;
-    __shared__ __align__(16) float acc_of[NARROW_WAVES][NARROW][HD + 4];
-    __shared__ float ref_of[NARROW_WAVES][NARROW], sum_of[NARROW_WAVES][NARROW];
-    const int split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits, row = pair / p.Hkv, h = pair % p.Hkv;
+    const int lane = threadIdx.x & 63;
+    if (p.rows == 1) return {0, 0, a.splits};
+    if (a.splits == p.rows) return {at, at, 1};
+    const auto blocks = [&](int row) {
+        if (row >= p.rows) return 0;
+        const int len = p.length[row];
+        return (a.window > 0 ? min(len, min(a.window, 1 << 29) + a.L) : len) / BLOCK_TOKENS + 1;
+    };
+    long long total = 0;
+    int mine = 0;
+    for (int r0 = 0; r0 < p.rows; r0 += 64) {
+        mine = blocks(r0 + lane);
+        total += __builtin_amdgcn_readlane(wave_scan(mine), 63);
+    }
+    const int spare = a.splits - p.rows;
+    int before = 0;
+    for (int r0 = 0; r0 < p.rows; r0 += 64) {
+        if (p.rows > 64) mine = blocks(r0 + lane);
+        const int count = r0 + lane < p.rows ? 1 + (int)((long long)mine * spare / total) : 0;
+        const int upto = before + wave_scan(count);
+        if (BY_ROW) {
+            if (at < r0 + 64) return {at, __builtin_amdgcn_readlane(upto - count, at - r0), __builtin_amdgcn_readlane(count, at - r0)};
+        } else {
+            const unsigned long long behind = __ballot(upto > at);
+            if (behind) {
+                const int l = __builtin_ctzll(behind);
+                return {r0 + l, __builtin_amdgcn_readlane(upto - count, l), __builtin_amdgcn_readlane(count, l)};
+            }
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return {-1, 0, 0};
+}
+
+template <int DT, int KIND, bool PLAIN, int WAVES, bool STREAM>
+__global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs a) {
+    const odmkv_pages_t& p = a.p;
+    extern __shared__ __align__(16) float narrow_lds[];
+    float (*acc_of)[NARROW][HD + 4] = reinterpret_cast<float (*)[NARROW][HD + 4]>(narrow_lds);      // [WAVES]
+    float (*ref_of)[NARROW] = reinterpret_cast<float (*)[NARROW]>(narrow_lds + WAVES * NARROW * (HD + 4));
+    float (*sum_of)[NARROW] = ref_of + WAVES;
+    // heads vary fastest: every head's longest row first, all heads alike
+    const int h = blockIdx.x % p.Hkv, group = blockIdx.x / p.Hkv;
+    const Share own = share_of<false>(a, group);
+    const int row = __builtin_amdgcn_readfirstlane(own.row), splits = __builtin_amdgcn_readfirstlane(own.count);
+    if (row < 0) return;
+    const int split = group - __builtin_amdgcn_readfirstlane(own.first);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, j = lane >> 4;
     const int R = a.G * a.L, len = p.length[row], count = a.counts ? min(max(a.counts[row], 0), a.L) : a.L, slot = p.slot[row];
     const int l = n / a.G, hq = h * a.G + n - l * a.G;
@@ -151,17 +216,28 @@ __global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(Att
     // blocks from lo_max on and up to hi_min are seen by every query
     const int lo_max = valid && !sees ? 0x7fffffff : s.lo;
     const int open_from = -wave_min_int(valid ? -lo_max : 0), open_to = wave_min_int(valid ? s.hi : 0x7fffffff);
-    const int blocks = max(last - first, 0), share = (blocks + a.splits - 1) / a.splits;
+    const int blocks = max(last - first, 0), share = (blocks + splits - 1) / splits;
     const int b0 = first + split * share, mine = min(share, blocks - split * share);             // may be negative: nothing to do
-    const int full = len / BLOCK_TOKENS;
+    const int full = len / BLOCK_TOKENS, codes = min(mine, full - b0);                           // of the blocks those that lie in pages
+    // 64 blocks of this wavefront at a time: their pages
+    const auto pages_at = [&](int g0) {
+        const int at = g0 + WAVES * lane;
+        return at < codes ? p.table[(size_t)slot * p.blocks + b0 + at] : 0;
+    };
+    int page_of = pages_at(wave);                               // (asked for ahead of the queries: the codes wait for it)
 
     f16x8 q[4];
     float qdown = 1.0f;
+    uint4 raw[4];
     {
-        uint4 raw[4];
         const uint16_t* src = a.q + row * a.qb + hq * a.qh + l * a.ql + 32 * j;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) raw[kk] = valid ? *reinterpret_cast<const uint4*>(src + 8 * kk) : make_uint4(0, 0, 0, 0);
+    }
+    const float slope = !PLAIN && a.slopes && valid ? a.slopes[hq] * LOG2E : 0.0f;
+    const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    float qs = 0.0f;
+    const auto take_queries = [&]() {
         if constexpr (DT == ODMKV_BF16) {
             const uint32_t top = larger_bits(max(max(abs_max8(raw[0]), abs_max8(raw[1])), max(abs_max8(raw[2]), abs_max8(raw[3]))), false);
             const Power pw = power_for<DT>(top);
@@ -172,10 +248,8 @@ __global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(Att
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) q[kk] = __builtin_bit_cast(f16x8, raw[kk]);
         }
-    }
-    const float slope = !PLAIN && a.slopes && valid ? a.slopes[hq] * LOG2E : 0.0f;
-    const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
-    const float qs = a.scaling * qdown * (PLAIN ? LOG2E : 1.0f);
+        qs = a.scaling * qdown * (PLAIN ? LOG2E : 1.0f);
+    };
 
     float ref = -INFINITY, sum = 0.0f, vref = 0.0f;
     f32x4 acc[8];
@@ -232,27 +306,29 @@ __global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(Att
         vref = v;
     };
 
-    const int codes = min(mine, full - b0);                     // of the blocks of this workgroup those that lie in pages
     const size_t kat = (size_t)(16 * (n >> 2) + (n & 3)) * HD + 32 * j, vat = (size_t)n * BLOCK_TOKENS + 16 * j;
+    bool first_group = true;
 #pragma unroll 1
-    for (int g0 = wave; g0 < codes; g0 += 64 * NARROW_WAVES) {  // 64 blocks of this wavefront at a time
-        const int at = g0 + NARROW_WAVES * lane, todo = min((codes - g0 + NARROW_WAVES - 1) / NARROW_WAVES, 64);
-        const int page_of = at < codes ? p.table[(size_t)slot * p.blocks + b0 + at] : 0;
-        const float ks_of = at < codes ? p.kscale[scale_at(p, a.layer, page_of, h)] : 0.0f;
-        const float vs_of = at < codes ? p.vscale[scale_at(p, a.layer, page_of, h)] : 0.0f;
+    for (int g0 = wave; g0 < codes; g0 += 64 * WAVES) {
+        const int at = g0 + WAVES * lane, todo = min((codes - g0 + WAVES - 1) / WAVES, 64);
+        if (!first_group) page_of = pages_at(g0);
         uint4 k[8], v[8];
         const auto request_keys = [&](int i) {
             const uint8_t* src = p.kcodes + page_at(p, a.layer, __builtin_amdgcn_readlane(page_of, i), h) + kat;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) k[c] = *reinterpret_cast<const uint4*>(src + (c >> 1) * 4 * HD + (c & 1) * 16);
+            for (int c = 0; c < 8; ++c) k[c] = piece16<STREAM>(src + (c >> 1) * 4 * HD + (c & 1) * 16);
         };
         const auto request_values = [&](int i) {
             const uint8_t* src = p.vcodes + page_at(p, a.layer, __builtin_amdgcn_readlane(page_of, i), h) + vat;
 #pragma unroll
-            for (int m = 0; m < 8; ++m) v[m] = *reinterpret_cast<const uint4*>(src + m * 16 * BLOCK_TOKENS);
+            for (int m = 0; m < 8; ++m) v[m] = piece16<STREAM>(src + m * 16 * BLOCK_TOKENS);
         };
         request_keys(0);
+        const float ks_of = at < codes ? p.kscale[scale_at(p, a.layer, page_of, h)] : 0.0f;
+        const float vs_of = at < codes ? p.vscale[scale_at(p, a.layer, page_of, h)] : 0.0f;
         request_values(0);
+        if (first_group) take_queries();
+        first_group = false;
         values_up_to(wave_max(vs_of));
         const float f_of = vref > 0.0f ? 128.0f * (vs_of / vref) : 0.0f;
 #pragma unroll 1
@@ -269,7 +345,7 @@ __global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(Att
             }
             if (i + 1 < todo) request_keys(i + 1);
             f16x8 w[2];
-            weigh(dot, b0 + g0 + NARROW_WAVES * i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_of), i)),
+            weigh(dot, b0 + g0 + WAVES * i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_of), i)),
                   __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f_of), i)), w);
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
@@ -280,40 +356,46 @@ __global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(Att
         }
     }
     // the open block, by the wavefront whose turn it is
-    if (mine > 0 && b0 + mine > full && (mine - 1) % NARROW_WAVES == wave) {
+    if (mine > 0 && b0 + mine > full && (mine - 1) % WAVES == wave) {
         const uint16_t* kt = p.ktail + tail_at(p, a.layer, slot, h) + kat;
         const uint16_t* vt = p.vtail + tail_at(p, a.layer, slot, h) + vat;
-        uint4 k[16];
-        uint32_t top = 0;
+        uint4 k[16], v[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-            k[c] = *reinterpret_cast<const uint4*>(kt + (c >> 2) * 4 * HD + (c & 3) * 8);
-            top = max(top, abs_max8(k[c]));
+        for (int c = 0; c < 16; ++c) k[c] = *reinterpret_cast<const uint4*>(kt + (c >> 2) * 4 * HD + (c & 3) * 8);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = *reinterpret_cast<const uint4*>(vt + (c >> 1) * 16 * BLOCK_TOKENS + (c & 1) * 8);
+        if (first_group) take_queries();
+        Power pk = {1.0f, 1.0f};
+        if constexpr (DT == ODMKV_BF16) {                       // (fp16 keys are taken as they are)
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) top = max(top, abs_max8(k[c]));
+            pk = power_for<DT>(larger_bits(top, true));
         }
-        Power pw = power_for<DT>(larger_bits(top, true));
         f32x4 dot[4];
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) {
             dot[tb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) dot[tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(k[4 * tb + kk], pw.up), q[kk], dot[tb], 0, 0, 0);
+            for (int kk = 0; kk < 4; ++kk) {
+                f16x8 x;
+                if constexpr (DT == ODMKV_BF16) x = scaled_f16<DT>(k[4 * tb + kk], pk.up);
+                else x = __builtin_bit_cast(f16x8, k[4 * tb + kk]);
+                dot[tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[kk], dot[tb], 0, 0, 0);
+            }
         }
-        const float kdown = pw.down;
-        top = 0;
+        uint32_t top = 0;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-            k[c] = *reinterpret_cast<const uint4*>(vt + (c >> 1) * 16 * BLOCK_TOKENS + (c & 1) * 8);
-            top = max(top, abs_max8(k[c]));
-        }
+        for (int c = 0; c < 16; ++c) top = max(top, abs_max8(v[c]));
         top = larger_bits(top, true);
-        pw = power_for<DT>(top);
-        if (top > 0) values_up_to(pw.down);
+        const Power pv = power_for<DT>(top);
+        if (top > 0) values_up_to(pv.down);
         f16x8 w[2];
-        weigh(dot, full, kdown, top > 0 ? 128.0f * (pw.down / vref) : 0.0f, w);
+        weigh(dot, full, pk.down, top > 0 ? 128.0f * (pv.down / vref) : 0.0f, w);
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
-            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(k[2 * m], pw.up), w[0], acc[m], 0, 0, 0);
-            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(k[2 * m + 1], pw.up), w[1], acc[m], 0, 0, 0);
+            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(v[2 * m], pv.up), w[0], acc[m], 0, 0, 0);
+            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(v[2 * m + 1], pv.up), w[1], acc[m], 0, 0, 0);
         }
     }
 
@@ -328,15 +410,15 @@ __global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(Att
     __syncthreads();
     // a thread takes eight dims of a query
     const int r = tid >> 4, d = (tid & 15) * 8, rl = r / a.G, rh = h * a.G + r - rl * a.G;
-    if (r >= R || rl >= count) return;
+    if (r >= R || rl >= count) return;                          // (of eight wavefronts the last four have no query)
     float to = ref_of[0][r], total = 0.0f, o[8];
 #pragma unroll
-    for (int w = 1; w < NARROW_WAVES; ++w) to = fmaxf(to, ref_of[w][r]);
+    for (int w = 1; w < WAVES; ++w) to = fmaxf(to, ref_of[w][r]);
     const float by = to > -INFINITY ? to : 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < NARROW_WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         const float f = __builtin_amdgcn_exp2f(ref_of[w][r] - by);
         // (a query that is not a number has a sum that is not, and a reference that may be anything)
         total += sum_of[w][r] == 0.0f ? 0.0f : sum_of[w][r] * f;
@@ -347,8 +429,8 @@ __global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(Att
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = total == 0.0f ? 0.0f : o[e] * inv;
     const float lse2 = total == 0.0f ? -INFINITY : to + __builtin_amdgcn_logf(total);
-    if (a.splits > 1) {
-        const size_t unit_at = ((size_t)pair * a.splits + split) * R + r;
+    if (splits > 1) {
+        const size_t unit_at = ((size_t)h * a.splits + group) * R + r;
         f32x4* dst = reinterpret_cast<f32x4*>(a.part_out + unit_at * HD + d);
         dst[0] = f32x4{o[0], o[1], o[2], o[3]};
         dst[1] = f32x4{o[4], o[5], o[6], o[7]};
@@ -363,21 +445,28 @@ __global__ __launch_bounds__(NARROW_WAVES * 64, 2) void attend_narrow_kernel(Att
 }
 
 // The shares of a row and kv-head's blocks, put together: a workgroup a query, its four wavefronts every fourth share, a lane two dims.
-template <int DT>
+template <int DT, bool NARROW_PARTS>
 __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
     const odmkv_pages_t& p = a.p;
     const int R = a.G * a.L, r = blockIdx.x, h = blockIdx.y, row = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int l = r / a.G, hq = h * a.G + r - l * a.G;
     if (l >= (a.counts ? min(max(a.counts[row], 0), a.L) : a.L)) return;
     __shared__ float part[4][HD], top_of[4], sum_of[4];
-    const size_t at = ((size_t)row * p.Hkv + h) * a.splits * R + r;
+    int splits = a.splits;
+    size_t at = ((size_t)row * p.Hkv + h) * a.splits * R + r;
+    if (NARROW_PARTS) {
+        const Share own = share_of<true>(a, row);
+        if (own.count == 1) return;                             // that workgroup has written the result
+        splits = own.count;
+        at = ((size_t)h * a.splits + own.first) * R + r;
+    }
     float top = -INFINITY;
-    for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, a.part_lse[at + (size_t)i * R]);
+    for (int i = lane; i < splits; i += 64) top = fmaxf(top, a.part_lse[at + (size_t)i * R]);
     top = wave_max(top);
     const float by = top > -INFINITY ? top : 0.0f;
     float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
 #pragma unroll 4
-    for (int i = wave; i < a.splits; i += 4) {
+    for (int i = wave; i < splits; i += 4) {
         const float lse = a.part_lse[at + (size_t)i * R];
         const float2 v = *reinterpret_cast<const float2*>(a.part_out + (at + (size_t)i * R) * HD + 2 * lane);
         const float w = __builtin_amdgcn_exp2f(lse - by);
@@ -668,52 +757,63 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
 
 // How a call is cut: wavefronts of a workgroup (0: the narrow kernel) and workgroups that share a row's blocks, two a compute unit in all,
 // each with a few blocks at least.
-struct Cut { int waves, splits; };
+struct Cut { int waves, splits; bool wide, stream; size_t parts; };     // stream: pages pass by the caches; parts: partial results
 static Cut cut_of(const odmkv_pages_t& p, int R, int max_length) {
-    const int blocks = max_length / BLOCK_TOKENS + 1;
-    long long groups = (long long)p.rows * p.Hkv;
-    Cut c = {0, 1};
-    if (R > NARROW) {
+    const int blocks = max_length / BLOCK_TOKENS + 1, units = compute_units();
+    Cut c = {4, 1, R > NARROW, false, 0};
+    if (c.wide) {
         c.waves = R > 128 ? WIDE_WAVES : 4;
-        groups *= (R + 32 * c.waves - 1) / (32 * c.waves);
+        const long long groups = (long long)p.rows * p.Hkv * ((R + 32 * c.waves - 1) / (32 * c.waves));
+        c.splits = (int)std::max(1LL, std::min((c.waves == WIDE_WAVES ? 1 : 2) * units / groups, (long long)blocks / 4));
+        c.parts = c.splits > 1 ? (size_t)p.rows * p.Hkv * c.splits * R : 0;
+    } else {
+        // Pages that all layers together have too many of for the last-level cache (256 MB) to keep from one call to the next: nothing is gained by keeping any, and
+        // reads that do not ask for it reach 5.9 TB/s instead of 5.0 (268 MB a call 59.7 -> 51.4 us; 67 MB a call over three caches in turn, which do fit, 18.7 -> 20.2).
+        c.stream = (size_t)p.layers * p.pages * p.Hkv * 2 * PAGE_BYTES > ((size_t)128 << 20);
+        // Eight wavefronts where they hold a row's blocks by themselves, so that nothing is merged (500 tokens: 10.8 -> 9.7 us), and for one row so long that
+        // each has several (131071 tokens of 4 heads: 35.4 -> 33.2 us; half as many shares to merge); four otherwise: twice as many compute units for 2000 tokens
+        // (13.1 -> 11.2 us), finer shares for rows of their own lengths (16 of up to 8192: 50.6 -> 40.4 us).
+        c.waves = blocks <= 8 || (p.rows == 1 && (long long)blocks * p.Hkv >= 24LL * units) ? 8 : 4;
+        const long long most = (long long)p.rows * std::max(1, blocks / c.waves);
+        c.splits = (int)std::max((long long)p.rows, std::min((long long)(8 / c.waves) * units / p.Hkv, most));
+        c.parts = c.splits > p.rows ? (size_t)p.Hkv * c.splits * R : 0;
     }
-    const int wanted = (c.waves == WIDE_WAVES ? 1 : 2) * compute_units();
-    c.splits = (int)std::max(1LL, std::min(wanted / groups, (long long)blocks / 4));
     return c;
 }
 
 extern "C" size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length) {
     if (!p || p->Hkv <= 0 || p->rows <= 0 || Hq <= 0 || L <= 0 || max_length < 0) return 0;
-    const int R = Hq / p->Hkv * L, splits = cut_of(*p, R, max_length).splits;
-    return splits > 1 ? align_up((size_t)p->rows * p->Hkv * splits * R * (HD + 1) * sizeof(float), 256) : 0;
+    return align_up(cut_of(*p, Hq / p->Hkv * L, max_length).parts * (HD + 1) * sizeof(float), 256);
 }
 
 template <int DT, int KIND>
-static int launch_attend(const AttendArgs& a, int waves, hipStream_t st) {
+static int launch_attend(const AttendArgs& a, const Cut& cut, hipStream_t st) {
     const bool plain = a.cap == 0.0f && !a.slopes;
-    const int pairs = a.p.rows * a.p.Hkv, R = a.G * a.L;
-    if (waves == 0) {
-        const dim3 grid((unsigned)(pairs * a.splits)), block(NARROW_WAVES * 64);
-        if (plain) hipLaunchKernelGGL((attend_narrow_kernel<DT, KIND, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((attend_narrow_kernel<DT, KIND, false>), grid, block, 0, st, a);
-        ODMKV_CHECK_LAUNCH("attend_narrow_kernel");
-    } else {
-        const long long groups = (long long)pairs * a.splits * ((R + 32 * waves - 1) / (32 * waves));
-        ODMKV_CHECK_ARG(groups < 0x7fffffffLL, "pages_attend: too many queries");
-        const dim3 grid((unsigned)groups), block(waves * 64);
-        const auto run = [&](auto kernel) -> int {
-            ODMKV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, WIDE_LDS));
-            hipLaunchKernelGGL(kernel, grid, block, WIDE_LDS, st, a);
-            return 0;
-        };
-        int rc;
-        if (waves == 4) rc = plain ? run(attend_wide_kernel<DT, KIND, true, 4>) : run(attend_wide_kernel<DT, KIND, false, 4>);
-        else rc = plain ? run(attend_wide_kernel<DT, KIND, true, WIDE_WAVES>) : run(attend_wide_kernel<DT, KIND, false, WIDE_WAVES>);
-        if (rc) return rc;
-        ODMKV_CHECK_LAUNCH("attend_wide_kernel");
-    }
-    if (a.splits == 1) return 0;
-    hipLaunchKernelGGL(attend_merge_kernel<DT>, dim3(R, a.p.Hkv, a.p.rows), dim3(256), 0, st, a);
+    const int R = a.G * a.L;
+    const long long groups = cut.wide ? (long long)a.p.rows * a.p.Hkv * a.splits * ((R + 32 * cut.waves - 1) / (32 * cut.waves)) : (long long)a.p.Hkv * a.splits;
+    ODMKV_CHECK_ARG(groups < 0x7fffffffLL, "pages_attend: too many queries");
+    const size_t lds = cut.wide ? WIDE_LDS : NARROW_LDS(cut.waves);
+    const auto run = [&](auto kernel) -> int {
+        if (lds > 65536) ODMKV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(cut.waves * 64), lds, st, a);
+        ODMKV_CHECK_LAUNCH("attend kernel");
+        return 0;
+    };
+    const auto narrow = [&](auto plain_, auto waves_, auto stream_) { return run(attend_narrow_kernel<DT, KIND, plain_.value, waves_.value, stream_.value>); };
+    const auto narrow_of = [&](auto waves_) {
+        const std::true_type yes;
+        const std::false_type no;
+        return plain ? (cut.stream ? narrow(yes, waves_, yes) : narrow(yes, waves_, no)) : (cut.stream ? narrow(no, waves_, yes) : narrow(no, waves_, no));
+    };
+    int rc;
+    if (!cut.wide) {
+        rc = cut.waves == 4 ? narrow_of(std::integral_constant<int, 4>()) : narrow_of(std::integral_constant<int, 8>());
+    } else if (cut.waves == 4) rc = plain ? run(attend_wide_kernel<DT, KIND, true, 4>) : run(attend_wide_kernel<DT, KIND, false, 4>);
+    else rc = plain ? run(attend_wide_kernel<DT, KIND, true, WIDE_WAVES>) : run(attend_wide_kernel<DT, KIND, false, WIDE_WAVES>);
+    if (rc || !cut.parts) return rc;
+    const dim3 grid(R, a.p.Hkv, a.p.rows);
+    if (cut.wide) hipLaunchKernelGGL((attend_merge_kernel<DT, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attend_merge_kernel<DT, true>), grid, dim3(256), 0, st, a);
     ODMKV_CHECK_LAUNCH("attend_merge_kernel");
     return 0;
 }
@@ -744,8 +844,8 @@ extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
     const Cut cut = cut_of(p, a.G * a.L, d->max_length);
     a.splits = cut.splits;
     a.part_out = (float*)d->workspace;
-    a.part_lse = a.part_out + (size_t)p.rows * p.Hkv * a.splits * a.G * a.L * HD;
+    a.part_lse = a.part_out + cut.parts * HD;
     hipStream_t st = (hipStream_t)stream;
-    if (p.dtype == ODMKV_F16) return p.kind == ODMKV_INT8 ? launch_attend<ODMKV_F16, ODMKV_INT8>(a, cut.waves, st) : launch_attend<ODMKV_F16, ODMKV_E4M3>(a, cut.waves, st);
-    return p.kind == ODMKV_INT8 ? launch_attend<ODMKV_BF16, ODMKV_INT8>(a, cut.waves, st) : launch_attend<ODMKV_BF16, ODMKV_E4M3>(a, cut.waves, st);
+    if (p.dtype == ODMKV_F16) return p.kind == ODMKV_INT8 ? launch_attend<ODMKV_F16, ODMKV_INT8>(a, cut, st) : launch_attend<ODMKV_F16, ODMKV_E4M3>(a, cut, st);
+    return p.kind == ODMKV_INT8 ? launch_attend<ODMKV_BF16, ODMKV_INT8>(a, cut, st) : launch_attend<ODMKV_BF16, ODMKV_E4M3>(a, cut, st);
 }

@@ -1,0 +1,301 @@
+// Attention over the paged 8-bit cache for up to sixteen queries of a kv-head.
+//
+// A step of one token (G query heads share a kv-head's keys), or of a few.  The queries are the sixteen columns of the matrix instructions: keys times
+// queries (rows: 16 tokens), then values times weights (rows: 16 dims, contraction: 32 tokens).  Which token a row of the first product is, is free:
+// row 4 j + r of product tb is token 16 j + 4 tb + r, so that a lane ends with the weights of the sixteen tokens whose values of a dim it reads as
+// one piece of 16 bytes; and lane (n, j) takes dims 32 j .. 32 j + 31 of its token, 32 bytes that lie together.  No weight changes lanes.
+//
+// Codes are exact in fp16, queries as they are (bf16: times a power of two each), products and sums fp32; a block's scale joins the scores and, for values,
+// the weights: weights are rounded to fp16 (half a step, 2^-12 to 2^-11 of themselves) times 2^7 s / (largest s of the wavefront's blocks).
+//
+// A wavefront takes every fourth (or eighth) block of its workgroup's share, its pages and scales looked up 64 at a time, the next block's keys and values requested
+// as soon as this one's are used.  Bound by memory (256 bytes a token and head); the arithmetic of a block is about a third of the time its bytes take.
+#pragma once
+
+#include "attend.h"
+
+#define NARROW_LDS(waves) ((waves) * NARROW * (HD + 4 + 2) * 4)
+
+template <int DT, int KIND, bool PLAIN, int WAVES, bool STREAM>
+__global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs a) {
+    const odmkv_pages_t& p = a.p;
+    extern __shared__ __align__(16) float narrow_lds[];
+    float (*acc_of)[NARROW][HD + 4] = reinterpret_cast<float (*)[NARROW][HD + 4]>(narrow_lds);      // [WAVES]
+    float (*ref_of)[NARROW] = reinterpret_cast<float (*)[NARROW]>(narrow_lds + WAVES * NARROW * (HD + 4));
+    float (*sum_of)[NARROW] = ref_of + WAVES;
+    // heads vary fastest: every head's longest row first, all heads alike
+    const int h = blockIdx.x % p.Hkv, group = blockIdx.x / p.Hkv;
+    const Share own = share_of<false>(a, group);
+    const int row = __builtin_amdgcn_readfirstlane(own.row), splits = __builtin_amdgcn_readfirstlane(own.count);
+    if (row < 0) return;
+    const int split = group - __builtin_amdgcn_readfirstlane(own.first);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, j = lane >> 4;
+    const int R = a.G * a.L, len = p.length[row], count = a.counts ? min(max(a.counts[row], 0), a.L) : a.L, slot = p.slot[row];
+    const int l = n / a.G, hq = h * a.G + n - l * a.G;
+    const bool valid = n < R && l < count;
+    Sight s = {0, 0, 0};
+    if (valid) s = sight_of(a, row, len, count, l);
+    const bool sees = valid && s.lo < s.hi;
+    const int first = wave_min_int(sees ? s.lo : 0x7fffffff) / BLOCK_TOKENS;
+    const int last = (-wave_min_int(sees ? -s.hi : 0) + BLOCK_TOKENS - 1) / BLOCK_TOKENS;        // one past the last block that is seen
+    // blocks from lo_max on and up to hi_min are seen by every query
+    const int lo_max = valid && !sees ? 0x7fffffff : s.lo;
+    const int open_from = -wave_min_int(valid ? -lo_max : 0), open_to = wave_min_int(valid ? s.hi : 0x7fffffff);
+    const int blocks = max(last - first, 0), share = (blocks + splits - 1) / splits;
+    const int b0 = first + split * share, mine = min(share, blocks - split * share);             // may be negative: nothing to do
+    const int full = len / BLOCK_TOKENS, codes = min(mine, full - b0);                           // of the blocks those that lie in pages
+    // 64 blocks of this wavefront at a time: their pages
+    const auto pages_at = [&](int g0) {
+        const int at = g0 + WAVES * lane;
+        return at < codes ? p.table[(size_t)slot * p.blocks + b0 + at] : 0;
+    };
+    int page_of = pages_at(wave);                               // (asked for ahead of the queries: the codes wait for it)
+
+    f16x8 q[4];
+    float qdown = 1.0f;
+    uint4 raw[4];
+    {
+        const uint16_t* src = a.q + row * a.qb + hq * a.qh + l * a.ql + 32 * j;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) raw[kk] = valid ? *reinterpret_cast<const uint4*>(src + 8 * kk) : make_uint4(0, 0, 0, 0);
+    }
+    const float slope = !PLAIN && a.slopes && valid ? a.slopes[hq] * LOG2E : 0.0f;
+    const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const bool by_exp = !PLAIN && a.cap > 0.0f && a.cap <= CAP_BY_EXP;
+    const Cap cap = {a.cap * LOG2E, 2.0f * LOG2E * a.cap, 2.0f * LOG2E * inv_cap};
+    float qs = 0.0f;
+    const auto take_queries = [&]() {
+        if constexpr (DT == ODMKV_BF16) {
+            const uint32_t top = larger_bits(max(max(abs_max8(raw[0]), abs_max8(raw[1])), max(abs_max8(raw[2]), abs_max8(raw[3]))), false);
+            const Power pw = power_for<DT>(top);
+            qdown = pw.down;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) q[kk] = scaled_f16<DT>(raw[kk], pw.up);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) q[kk] = __builtin_bit_cast(f16x8, raw[kk]);
+        }
+        qs = a.scaling * qdown * (PLAIN ? LOG2E : 1.0f);
+    };
+
+    float ref = -INFINITY, sum = 0.0f, vref = 0.0f;
+    f32x4 acc[8];
+#pragma unroll
+    for (int m = 0; m < 8; ++m) acc[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // raw products of a block to weights: x [tb][r] is token 64 block + 16 j + 4 tb + r.  Back come the weights as operands, times f = 2^log2f_.
+    const auto weigh = [&](const f32x4* dot, int block, float ks, float log2f_, f16x8* w) {
+        float x[16];
+        const float c = scale_of(ks, qs);
+        const int t0 = block * BLOCK_TOKENS + 16 * j;
+        if constexpr (PLAIN) {                                  // (c is not negative: the largest product is the largest score)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = dot[i >> 2][i & 3];
+        } else {
+            if (by_exp) {
+                const float k = c * cap.plain;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = capped(dot[i >> 2][i & 3] * k, cap);
+            } else if (inv_cap > 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = cap.by * tanh_of(dot[i >> 2][i & 3] * (c * inv_cap));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = dot[i >> 2][i & 3] * (c * LOG2E);
+            }
+            if (a.slopes) {
+                const float ahead = (float)(s.pos - t0);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = __fmaf_rn(-slope, fabsf(ahead - (float)i), x[i]);
+            }
+        }
+        if (block * BLOCK_TOKENS < open_from || block * BLOCK_TOKENS + BLOCK_TOKENS > open_to) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = t0 + i >= s.lo && t0 + i < s.hi ? x[i] : -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+        if constexpr (PLAIN) top = top > -INFINITY ? top * c : top;
+        if (__any(top > ref + RISE)) {
+            const float to = fmaxf(ref, column_max(top)), by = to > -INFINITY ? to : 0.0f, old = __builtin_amdgcn_exp2f(ref - by);
+            ref = to;
+            sum *= old;
+#pragma unroll
+            for (int m = 0; m < 8; ++m) acc[m] *= old;
+        }
+        // weights times f come out of the exponential itself, the block's sum is freed of f
+        const float shift = log2f_ - (ref > -INFINITY ? ref : 0.0f);
+        float z0 = 0.0f, z1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            x[i] = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(x[i], c, shift) : x[i] + shift);
+            x[i + 1] = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(x[i + 1], c, shift) : x[i + 1] + shift);
+            z0 += x[i];
+            z1 += x[i + 1];
+        }
+        sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-log2f_), sum);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (_Float16)x[i];
+    };
+    const auto values_up_to = [&](float v) {                    // the sums' values are in units of vref from here on
+        if (v <= vref) return;
+        const float old = vref / v;
+#pragma unroll
+        for (int m = 0; m < 8; ++m) acc[m] *= old;
+        vref = v;
+    };
+
+    const size_t kat = (size_t)(16 * (n >> 2) + (n & 3)) * HD + 32 * j, vat = (size_t)n * BLOCK_TOKENS + 16 * j;
+    bool first_group = true;
+#pragma unroll 1
+    for (int g0 = wave; g0 < codes; g0 += 64 * WAVES) {
+        const int at = g0 + WAVES * lane, todo = min((codes - g0 + WAVES - 1) / WAVES, 64);
+        if (!first_group) page_of = pages_at(g0);
+        uint4 k[8], v[8];
+        const auto request_keys = [&](int i) {
+            const uint8_t* src = p.kcodes + page_at(p, a.layer, __builtin_amdgcn_readlane(page_of, i), h) + kat;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) k[c] = piece16<STREAM>(src + (c >> 1) * 4 * HD + (c & 1) * 16);
+        };
+        const auto request_values = [&](int i) {
+            const uint8_t* src = p.vcodes + page_at(p, a.layer, __builtin_amdgcn_readlane(page_of, i), h) + vat;
+#pragma unroll
+            for (int m = 0; m < 8; ++m) v[m] = piece16<STREAM>(src + m * 16 * BLOCK_TOKENS);
+        };
+        request_keys(0);
+        const float ks_of = at < codes ? p.kscale[scale_at(p, a.layer, page_of, h)] : 0.0f;
+        const float vs_of = at < codes ? p.vscale[scale_at(p, a.layer, page_of, h)] : 0.0f;
+        request_values(0);
+        if (first_group) take_queries();
+        first_group = false;
+        values_up_to(wave_max(vs_of));
+        const float f_of = log2_share(vs_of, vref);
+#pragma unroll 1
+        for (int i = 0; i < todo; ++i) {
+            f32x4 dot[4];
+#pragma unroll
+            for (int tb = 0; tb < 4; ++tb) {
+                dot[tb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    const uint4& c = k[2 * tb + (kk >> 1)];
+                    dot[tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk & 1 ? codes_f16<KIND>(c.z, c.w) : codes_f16<KIND>(c.x, c.y), q[kk], dot[tb], 0, 0, 0);
+                }
+            }
+            if (i + 1 < todo) request_keys(i + 1);
+            f16x8 w[2];
+            weigh(dot, b0 + g0 + WAVES * i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_of), i)),
+                  __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f_of), i)), w);
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16<KIND>(v[m].x, v[m].y), w[0], acc[m], 0, 0, 0);
+                acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16<KIND>(v[m].z, v[m].w), w[1], acc[m], 0, 0, 0);
+            }
+            if (i + 1 < todo) request_values(i + 1);
+        }
+    }
+    // the open block, by the wavefront whose turn it is
+    if (mine > 0 && b0 + mine > full && (mine - 1) % WAVES == wave) {
+        const uint16_t* kt = p.ktail + tail_at(p, a.layer, slot, h) + kat;
+        const uint16_t* vt = p.vtail + tail_at(p, a.layer, slot, h) + vat;
+        uint4 k[16], v[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) k[c] = *reinterpret_cast<const uint4*>(kt + (c >> 2) * 4 * HD + (c & 3) * 8);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = *reinterpret_cast<const uint4*>(vt + (c >> 1) * 16 * BLOCK_TOKENS + (c & 1) * 8);
+        if (first_group) take_queries();
+        Power pk = {1.0f, 1.0f};
+        if constexpr (DT == ODMKV_BF16) {                       // (fp16 keys are taken as they are)
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) top = max(top, abs_max8(k[c]));
+            pk = power_for<DT>(larger_bits(top, true));
+        }
+        f32x4 dot[4];
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb) {
+            dot[tb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                f16x8 x;
+                if constexpr (DT == ODMKV_BF16) x = scaled_f16<DT>(k[4 * tb + kk], pk.up);
+                else x = __builtin_bit_cast(f16x8, k[4 * tb + kk]);
+                dot[tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[kk], dot[tb], 0, 0, 0);
+            }
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) top = max(top, abs_max8(v[c]));
+        top = larger_bits(top, true);
+        const Power pv = power_for<DT>(top);
+        if (top > 0) values_up_to(pv.down);
+        f16x8 w[2];
+        weigh(dot, full, pk.down, log2_share(top > 0 ? pv.down : 0.0f, vref), w);
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(v[2 * m], pv.up), w[0], acc[m], 0, 0, 0);
+            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(v[2 * m + 1], pv.up), w[1], acc[m], 0, 0, 0);
+        }
+    }
+
+    sum = column_sum(sum);
+    const float unit = vref * (1.0f / 128.0f);
+#pragma unroll
+    for (int m = 0; m < 8; ++m) *reinterpret_cast<f32x4*>(&acc_of[wave][n][16 * m + 4 * j]) = acc[m] * unit;
+    if (j == 0) {
+        ref_of[wave][n] = ref;
+        sum_of[wave][n] = sum;
+    }
+    __syncthreads();
+    // a thread takes eight dims of a query
+    const int r = tid >> 4, d = (tid & 15) * 8, rl = r / a.G, rh = h * a.G + r - rl * a.G;
+    if (r >= R || rl >= count) return;                          // (of eight wavefronts the last four have no query)
+    float to = ref_of[0][r], total = 0.0f, o[8];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) to = fmaxf(to, ref_of[w][r]);
+    const float by = to > -INFINITY ? to : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float f = __builtin_amdgcn_exp2f(ref_of[w][r] - by);
+        // (a query that is not a number has a sum that is not, and a reference that may be anything)
+        total += sum_of[w][r] == 0.0f ? 0.0f : sum_of[w][r] * f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = __fmaf_rn(acc_of[w][r][d + e], f, o[e]);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = total == 0.0f ? 0.0f : o[e] * inv;
+    const float lse2 = total == 0.0f ? -INFINITY : to + __builtin_amdgcn_logf(total);
+    if (splits > 1) {
+        const size_t unit_at = ((size_t)h * a.splits + group) * R + r;
+        f32x4* dst = reinterpret_cast<f32x4*>(a.part_out + unit_at * HD + d);
+        dst[0] = f32x4{o[0], o[1], o[2], o[3]};
+        dst[1] = f32x4{o[4], o[5], o[6], o[7]};
+        if (d == 0) a.part_lse[unit_at] = lse2;
+        return;
+    }
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = (uint32_t)to_16<DT>(o[2 * e]) | (uint32_t)to_16<DT>(o[2 * e + 1]) << 16;
+    *reinterpret_cast<uint4*>(a.out + (((size_t)row * a.L + rl) * a.Hq + rh) * HD + d) = make_uint4(b[0], b[1], b[2], b[3]);
+    if (a.lse && d == 0) a.lse[((size_t)row * a.Hq + rh) * a.L + rl] = lse2 * LN2;
+}
+
+template <int DT>
+static int launch_narrow_of(const AttendArgs& a, const Cut& cut, hipStream_t st) {
+    const bool plain = a.cap == 0.0f && !a.slopes && a.scaling > 0.0f;
+    const auto run = [&](auto dt, auto kind, auto plain_, auto waves, auto stream) {
+        return launch_attend(attend_narrow_kernel<dt.value, kind.value, plain_.value, waves.value, stream.value>, a, (long long)a.p.Hkv * a.splits, waves.value,
+                             NARROW_LDS(waves.value), st);
+    };
+    const auto of_stream = [&](auto dt, auto kind, auto plain_, auto waves) {
+        return cut.stream ? run(dt, kind, plain_, waves, std::true_type()) : run(dt, kind, plain_, waves, std::false_type());
+    };
+    const auto of_waves = [&](auto dt, auto kind, auto plain_) { return cut.waves == 4 ? of_stream(dt, kind, plain_, Int<4>()) : of_stream(dt, kind, plain_, Int<8>()); };
+    const auto of_scores = [&](auto dt, auto kind) { return plain ? of_waves(dt, kind, std::true_type()) : of_waves(dt, kind, std::false_type()); };
+    const Int<DT> dt;
+    return a.p.kind == ODMKV_INT8 ? of_scores(dt, Int<ODMKV_INT8>()) : of_scores(dt, Int<ODMKV_E4M3>());
+}

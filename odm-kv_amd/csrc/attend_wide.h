@@ -1,0 +1,333 @@
+// Attention over the paged 8-bit cache for many queries of a kv-head.
+//
+// A wavefront holds 32 queries (the columns of v_mfma_f32_32x32x16_f16), a workgroup 32 WAVES of them, token by token with the G heads of a
+// token together, so that a workgroup's tokens lie together and blocks that none of them sees are passed over.  A block of 64 tokens is turned into fp16 once a workgroup
+// and lies in LDS, the next block's codes are on their way in registers; rows of the first product are tokens as they lie, and row r of a half
+// wavefront's sixteen (8 (r / 4) + 4 half + r % 4) decides the order in which values lie in LDS: what a lane holds of the weights is
+// then its operand of the second product.  16-byte pieces of a row are moved by the row's number (xor), so that no two of eight rows meet in a bank.
+#pragma once
+
+#include "attend.h"
+
+#define WIDE_LDS (2 * (BLOCK_TOKENS * HD * 2 * 2))
+// what becomes of a product besides its factor: nothing; a cap by the exponential; a bias by distance; any of it
+enum { SCORES_PLAIN, SCORES_CAPPED, SCORES_BIASED, SCORES_ANY };
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT, int KIND, int MODE, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a) {
+    const odmkv_pages_t& p = a.p;
+    constexpr bool PLAIN = MODE == SCORES_PLAIN;
+    extern __shared__ __align__(16) uint8_t lds[];              // [2][keys 64 x 256 bytes, values 128 x 128 bytes]
+    __shared__ int range[2][WAVES];
+    __shared__ uint32_t tops[2][WAVES];
+    constexpr int THREADS = WAVES * 64, BUFFER = BLOCK_TOKENS * HD * 4, VALUES = BLOCK_TOKENS * HD * 2;
+    const int pairs = p.rows * p.Hkv, R = a.G * a.L, tiles = (R + 32 * WAVES - 1) / (32 * WAVES);
+    // heads vary fastest (a die of the chip then keeps few heads' pages in its L2), the longest rows of blocks come first
+    const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs, split = rest % a.splits, tile = tiles - 1 - rest / a.splits;
+    const int row = pair / p.Hkv, h = pair % p.Hkv, tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int len = p.length[row], count = a.counts ? min(max(a.counts[row], 0), a.L) : a.L, slot = p.slot[row];
+    const int r0 = tile * 32 * WAVES + 32 * wave, r = r0 + col, l = r / a.G, hq = h * a.G + r - l * a.G;
+    const bool valid = r < R && l < count;
+    Sight s = {0, 0, 0};
+    if (valid) s = sight_of(a, row, len, count, l);
+    const bool sees = valid && s.lo < s.hi;
+    const int wave_lo = wave_min_int(sees ? s.lo : 0x7fffffff), wave_hi = -wave_min_int(sees ? -s.hi : 0);       // what some query of the wavefront sees
+    const int open_from = -wave_min_int(valid ? -(sees ? s.lo : 0x7fffffff) : 0), open_to = wave_min_int(valid ? s.hi : 0x7fffffff);    // what all of them see
+    if (lane == 0) {
+        range[0][wave] = wave_lo;
+        range[1][wave] = wave_hi;
+    }
+    __syncthreads();
+    int lo = range[0][0], hi = range[1][0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+        lo = min(lo, range[0][w]);
+        hi = max(hi, range[1][w]);
+    }
+    const int first = lo / BLOCK_TOKENS, blocks = max((hi + BLOCK_TOKENS - 1) / BLOCK_TOKENS - first, 0), share = (blocks + a.splits - 1) / a.splits;
+    const int b0 = __builtin_amdgcn_readfirstlane(first + split * share), mine = __builtin_amdgcn_readfirstlane(min(share, blocks - split * share));
+    const int full = len / BLOCK_TOKENS;
+
+    f16x8 q[8];                                                 // dims 16 st + 8 half + e
+    float qdown = 1.0f;
+    {
+        uint4 raw[8];
+        const uint16_t* src = a.q + row * a.qb + hq * a.qh + l * a.ql + 8 * half;
+#pragma unroll
+        for (int st = 0; st < 8; ++st) raw[st] = valid ? *reinterpret_cast<const uint4*>(src + 16 * st) : make_uint4(0, 0, 0, 0);
+        if constexpr (DT == ODMKV_BF16) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int st = 0; st < 8; ++st) top = max(top, abs_max8(raw[st]));
+            const auto o = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            const Power pw = power_for<DT>(max(o[0], o[1]));
+            qdown = pw.down;
+#pragma unroll
+            for (int st = 0; st < 8; ++st) q[st] = scaled_f16<DT>(raw[st], pw.up);
+        } else {
+#pragma unroll
+            for (int st = 0; st < 8; ++st) q[st] = __builtin_bit_cast(f16x8, raw[st]);
+        }
+    }
+    const float slope = !PLAIN && a.slopes && valid ? a.slopes[hq] * LOG2E : 0.0f;
+    const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const bool by_exp = MODE == SCORES_CAPPED || (!PLAIN && a.cap > 0.0f && a.cap <= CAP_BY_EXP);
+    const Cap cap = {a.cap * LOG2E, 2.0f * LOG2E * a.cap, 2.0f * LOG2E * inv_cap};
+    const float qs = a.scaling * qdown * (PLAIN ? LOG2E : 1.0f);
+
+    float ref = -INFINITY, sum = 0.0f, vref = 0.0f;
+    f32x16 acc[4];                                              // dims 32 db + 8 (r / 4) + 4 half + r % 4 of query `col`
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] = 0.0f;
+
+    const auto values_up_to = [&](float v) {                    // the sums' values are in units of vref from here on
+        if (v <= vref) return;
+        const float old = vref / v;
+#pragma unroll
+        for (int db = 0; db < 4; ++db) acc[db] *= old;
+        vref = v;
+    };
+
+    // ---- a block on its way: pieces of 16 codes, a token's 16 dims or a dim's 16 tokens
+    constexpr int PIECES = PAGE_BYTES / 16 / THREADS;
+    uint4 kc[PIECES], vc[PIECES];
+    int page_of = 0;
+    const auto look_up = [&](int i) { return i + lane < mine && b0 + i + lane < full ? p.table[(size_t)slot * p.blocks + b0 + i + lane] : 0; };
+    const auto request = [&](int i) {                           // block b0 + i, which lies in a page
+        if ((i & 63) == 0) page_of = look_up(i);
+        const size_t at = page_at(p, a.layer, __builtin_amdgcn_readlane(page_of, i & 63), h);
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+            kc[c] = *reinterpret_cast<const uint4*>(p.kcodes + at + (size_t)(tid + c * THREADS) * 16);
+            vc[c] = *reinterpret_cast<const uint4*>(p.vcodes + at + (size_t)(tid + c * THREADS) * 16);
+        }
+    };
+    const auto key_piece = [&](uint8_t* buf, int token, int piece) { return reinterpret_cast<f16x8*>(buf + token * 256 + ((piece ^ (token & 15)) << 4)); };
+    const auto value_piece = [&](uint8_t* buf, int dim, int piece) { return buf + VALUES + dim * 128 + ((piece ^ (dim & 7)) << 4); };
+    const auto put = [&](uint8_t* buf) {
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+            const int i = tid + c * THREADS;
+            *key_piece(buf, i >> 3, 2 * (i & 7)) = codes_f16<KIND>(kc[c].x, kc[c].y);
+            *key_piece(buf, i >> 3, 2 * (i & 7) + 1) = codes_f16<KIND>(kc[c].z, kc[c].w);
+            *reinterpret_cast<f16x8*>(value_piece(buf, i >> 2, 2 * (i & 3))) = codes_f16<KIND>(vc[c].x, vc[c].z);
+            *reinterpret_cast<f16x8*>(value_piece(buf, i >> 2, 2 * (i & 3) + 1)) = codes_f16<KIND>(vc[c].y, vc[c].w);
+        }
+    };
+    float tail_k = 1.0f, tail_v = 0.0f;                         // what the open block's numbers in LDS are to be multiplied by
+    const auto put_tail = [&](uint8_t* buf) {
+        const uint4* kt = reinterpret_cast<const uint4*>(p.ktail + tail_at(p, a.layer, slot, h));
+        const uint4* vt = reinterpret_cast<const uint4*>(p.vtail + tail_at(p, a.layer, slot, h));
+        uint32_t top[2] = {0, 0};
+#pragma unroll 1
+        for (int i = tid; i < TAIL_ELEMS / 8; i += THREADS) {
+            top[0] = max(top[0], abs_max8(kt[i]));
+            top[1] = max(top[1], abs_max8(vt[i]));
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t t = larger_bits(top[x], true);
+            if (lane == 0) tops[x][wave] = t;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) top[x] = max(top[x], tops[x][w]);
+        const Power pk = power_for<DT>(top[0]), pv = power_for<DT>(top[1]);
+        tail_k = pk.down;
+        tail_v = top[1] > 0 ? pv.down : 0.0f;
+#pragma unroll 1
+        for (int i = tid; i < TAIL_ELEMS / 8; i += THREADS) {
+            const int dim = i >> 3, u = i & 7;
+            *key_piece(buf, i >> 4, i & 15) = scaled_f16<DT>(kt[i], pk.up);
+            const uint4 x = __builtin_bit_cast(uint4, scaled_f16<DT>(vt[i], pv.up));
+            *reinterpret_cast<uint2*>(value_piece(buf, dim, u & ~1) + 8 * (u & 1)) = make_uint2(x.x, x.y);
+            *reinterpret_cast<uint2*>(value_piece(buf, dim, u | 1) + 8 * (u & 1)) = make_uint2(x.z, x.w);
+        }
+    };
+
+    const int codes = min(mine, full - b0);                     // of the blocks those that lie in pages
+    if (codes > 0) request(0);
+    if (WAVES == 8 && wave < 4) __builtin_amdgcn_s_setprio(2);
+    float ks_of = 0.0f, f_of = 0.0f;
+#pragma unroll 1
+    for (int i = -1; i < mine; ++i) {
+        uint8_t* buf = lds + (i & 1) * BUFFER;
+        __syncthreads();                                        // this block lies there, and nobody reads the one before any more
+        if (i + 1 < codes) put(lds + ((i + 1) & 1) * BUFFER);
+        else if (i + 1 < mine) put_tail(lds + ((i + 1) & 1) * BUFFER);
+        if (i + 2 < codes) request(i + 2);
+        if (i < 0) continue;
+        const int t0 = (b0 + i) * BLOCK_TOKENS;
+        float ks, log2f_;
+        if (i < codes) {
+            if ((i & 63) == 0) {                                // 64 blocks' scales at a time
+                const bool in = i + lane < codes;
+                const int page = look_up(i);
+                const float vs = in ? p.vscale[scale_at(p, a.layer, page, h)] : 0.0f;
+                ks_of = in ? p.kscale[scale_at(p, a.layer, page, h)] : 0.0f;
+                values_up_to(wave_max(vs));
+                f_of = log2_share(vs, vref);
+            }
+            ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_of), i & 63));
+            log2f_ = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f_of), i & 63));
+        } else {
+            ks = tail_k;
+            values_up_to(tail_v);
+            log2f_ = log2_share(tail_v, vref);
+        }
+        const float free_f = __builtin_amdgcn_exp2f(-log2f_);
+        if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;      // (of the wavefront's own queries none sees the block)
+        const float c = scale_of(ks, qs), shift_f = log2f_;
+        const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
+        f32x16 dot[2];
+        f16x8 w[4];
+        const auto multiply_keys = [&](int tb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dot[tb][e] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < 8; ++st)
+                dot[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*key_piece(buf, 32 * tb + col, 2 * st + half), q[st], dot[tb], 0, 0, 0);
+        };
+        const auto multiply_values = [&](int st) {
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(value_piece(buf, 32 * db + col, 2 * st + half)), w[st], acc[db], 0, 0, 0);
+        };
+        // products of half a block to scores, and the reference where it is to rise (what has been summed up, and weights that have not, come to the new one)
+        const auto look_over = [&](int tb) {
+            f32x16& x = dot[tb];
+            const int tl = t0 + 32 * tb + 4 * half;             // token of score e: tl + 8 (e / 4) + e % 4
+            if constexpr (!PLAIN) {
+                if (by_exp) {
+                    const float k = c * cap.plain;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = capped(x[e] * k, cap);
+                } else if (MODE == SCORES_ANY && inv_cap > 0.0f) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = cap.by * tanh_of(x[e] * (c * inv_cap));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] *= c * LOG2E;
+                }
+                if (MODE == SCORES_BIASED || (MODE == SCORES_ANY && a.slopes)) {
+                    const float ahead = (float)(s.pos - tl);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = __fmaf_rn(-slope, fabsf(ahead - (float)(8 * (e >> 2) + (e & 3))), x[e]);
+                }
+            }
+            if (cut) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int t = tl + 8 * (e >> 2) + (e & 3);
+                    x[e] = t >= s.lo && t < s.hi ? x[e] : -INFINITY;
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+            if constexpr (PLAIN) top = top > -INFINITY ? top * c : top;      // (c is not negative: the largest product is the largest score)
+            if (__any(top > ref + RISE)) {
+                const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                const float to = fmaxf(ref, fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]))), by = to > -INFINITY ? to : 0.0f;
+                const float old = __builtin_amdgcn_exp2f(ref - by);
+                ref = to;
+                sum *= old;
+#pragma unroll
+                for (int db = 0; db < 4; ++db) acc[db] *= old;
+                if (tb == 1) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) w[e >> 3][e & 7] = (_Float16)((float)w[e >> 3][e & 7] * old);
+                }
+            }
+        };
+        // weights times f come out of the exponential itself, the block's sum is freed of f
+        const auto weigh = [&](int tb) {
+            const float shift = shift_f - (ref > -INFINITY ? ref : 0.0f);
+            float z0 = 0.0f, z1 = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e], c, shift) : dot[tb][e] + shift);
+                const float p1 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e + 1], c, shift) : dot[tb][e + 1] + shift);
+                z0 += p0;
+                z1 += p1;
+                w[2 * tb + (e >> 3)][e & 7] = (_Float16)p0;
+                w[2 * tb + (e >> 3)][(e & 7) + 1] = (_Float16)p1;
+            }
+            sum = __fmaf_rn(z0 + z1, free_f, sum);
+        };
+        // The two halves' vector work stands beside the other half's matrix work: a matrix instruction takes 32 cycles, which some eight vector instructions fill.
+        multiply_keys(0);
+        look_over(0);
+        multiply_keys(1);
+        weigh(0);
+
+        look_over(1);
+        multiply_values(0);
+        multiply_values(1);
+        weigh(1);
+
+        multiply_values(2);
+        multiply_values(3);
+    }
+
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+    if (!valid) return;
+    const bool none = sum == 0.0f;
+    const float unit = none ? 0.0f : vref * (1.0f / 128.0f) / sum, lse2 = none ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
+    if (a.splits > 1) {
+        const size_t unit_at = ((size_t)pair * a.splits + split) * R + r;
+        float* dst = a.part_out + unit_at * HD + 4 * half;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : acc[db][4 * g + e] * unit;
+                *reinterpret_cast<f32x4*>(dst + 32 * db + 8 * g) = v;
+            }
+        if (half == 0) a.part_lse[unit_at] = lse2;
+        return;
+    }
+    uint16_t* dst = a.out + (((size_t)row * a.L + l) * a.Hq + hq) * HD + 4 * half;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint32_t v[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                v[e] = none ? 0u : (uint32_t)to_16<DT>(acc[db][4 * g + 2 * e] * unit) | (uint32_t)to_16<DT>(acc[db][4 * g + 2 * e + 1] * unit) << 16;
+            *reinterpret_cast<uint2*>(dst + 32 * db + 8 * g) = make_uint2(v[0], v[1]);
+        }
+    if (a.lse && half == 0) a.lse[((size_t)row * a.Hq + hq) * a.L + l] = none ? -INFINITY : lse2 * LN2;
+}
+
+template <int DT>
+static int launch_wide_of(const AttendArgs& a, const Cut& cut, hipStream_t st) {
+    const bool capped = a.cap > 0.0f;
+    const int R = a.G * a.L, mode = a.slopes ? (capped ? SCORES_ANY : SCORES_BIASED)
+                                  : capped ? (a.cap <= CAP_BY_EXP ? SCORES_CAPPED : SCORES_ANY) : a.scaling > 0.0f ? SCORES_PLAIN : SCORES_ANY;
+    const long long groups = (long long)a.p.rows * a.p.Hkv * a.splits * ((R + 32 * cut.waves - 1) / (32 * cut.waves));
+    const auto run = [&](auto dt, auto kind, auto mode_, auto waves) {
+        return launch_attend(attend_wide_kernel<dt.value, kind.value, mode_.value, waves.value>, a, groups, waves.value, WIDE_LDS, st);
+    };
+    const auto of_waves = [&](auto dt, auto kind, auto mode_) { return cut.waves == 4 ? run(dt, kind, mode_, Int<4>()) : run(dt, kind, mode_, Int<WIDE_WAVES>()); };
+    const auto of_mode = [&](auto dt, auto kind) {
+        switch (mode) {
+            case SCORES_PLAIN: return of_waves(dt, kind, Int<SCORES_PLAIN>());
+            case SCORES_CAPPED: return of_waves(dt, kind, Int<SCORES_CAPPED>());
+            case SCORES_BIASED: return of_waves(dt, kind, Int<SCORES_BIASED>());
+            default: return of_waves(dt, kind, Int<SCORES_ANY>());
+        }
+    };
+    const Int<DT> dt;
+    return a.p.kind == ODMKV_INT8 ? of_mode(dt, Int<ODMKV_INT8>()) : of_mode(dt, Int<ODMKV_E4M3>());
+}

@@ -2,6 +2,8 @@
 #include "attend.h"
 
 // The shares of a row and kv-head's blocks, put together: a workgroup a query, its four wavefronts every fourth share, a lane two dims.
+#define MERGE_AHEAD 8
+
 template <int DT, bool NARROW_PARTS>
 __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
     const odmkv_pages_t& p = a.p;
@@ -17,29 +19,57 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
         splits = own.count;
         at = ((size_t)h * a.splits + own.first) * R + r;
     }
-    float top = -INFINITY;
-    for (int i = lane; i < splits; i += 64) top = fmaxf(top, a.part_lse[at + (size_t)i * R]);
-    top = wave_max(top);
-    const float by = top > -INFINITY ? top : 0.0f;
-    float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-#pragma unroll 4
-    for (int i = wave; i < splits; i += 4) {
-        const float lse = a.part_lse[at + (size_t)i * R];
-        const float2 v = *reinterpret_cast<const float2*>(a.part_out + (at + (size_t)i * R) * HD + 2 * lane);
-        const float w = __builtin_amdgcn_exp2f(lse - by);
-        sum += w;
-        o0 = __fmaf_rn(w, v.x, o0);
-        o1 = __fmaf_rn(w, v.y, o1);
+    // (each wavefront by its own largest: the partial results need not wait for the largest of all)
+    float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    for (int i0 = wave; i0 < splits; i0 += 4 * MERGE_AHEAD) {
+        float lse[MERGE_AHEAD];
+        float2 v[MERGE_AHEAD];
+#pragma unroll
+        for (int k = 0; k < MERGE_AHEAD; ++k) {
+            const size_t from = at + (size_t)min(i0 + 4 * k, splits - 1) * R;
+            lse[k] = a.part_lse[from];
+            v[k] = *reinterpret_cast<const float2*>(a.part_out + from * HD + 2 * lane);
+        }
+        float to = top;
+#pragma unroll
+        for (int k = 0; k < MERGE_AHEAD; ++k) {
+            if (i0 + 4 * k >= splits) lse[k] = -INFINITY;
+            to = fmaxf(to, lse[k]);
+        }
+        const float by = to > -INFINITY ? to : 0.0f, old = __builtin_amdgcn_exp2f(top - by);
+        top = to;
+        sum *= old;
+        o0 *= old;
+        o1 *= old;
+#pragma unroll
+        for (int k = 0; k < MERGE_AHEAD; ++k) {
+            const float w = __builtin_amdgcn_exp2f(lse[k] - by);
+            sum += w;
+            o0 = __fmaf_rn(w, v[k].x, o0);
+            o1 = __fmaf_rn(w, v[k].y, o1);
+        }
     }
     part[wave][2 * lane] = o0;
     part[wave][2 * lane + 1] = o1;
-    if (lane == 0) sum_of[wave] = sum;
+    if (lane == 0) {
+        sum_of[wave] = sum;
+        top_of[wave] = top;
+    }
     __syncthreads();
     if (tid >= 64) return;
-    sum = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+    top = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
+    const float by = top > -INFINITY ? top : 0.0f;
+    sum = o0 = o1 = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(top_of[w] - by);
+        sum = __fmaf_rn(f, sum_of[w], sum);
+        o0 = __fmaf_rn(f, part[w][2 * lane], o0);
+        o1 = __fmaf_rn(f, part[w][2 * lane + 1], o1);
+    }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    o0 = ((part[0][2 * lane] + part[1][2 * lane]) + (part[2][2 * lane] + part[3][2 * lane])) * inv;
-    o1 = ((part[0][2 * lane + 1] + part[1][2 * lane + 1]) + (part[2][2 * lane + 1] + part[3][2 * lane + 1])) * inv;
+    o0 *= inv;
+    o1 *= inv;
     *reinterpret_cast<uint32_t*>(a.out + (((size_t)row * a.L + l) * a.Hq + hq) * HD + 2 * lane) = (uint32_t)to_16<DT>(o0) | (uint32_t)to_16<DT>(o1) << 16;
     if (a.lse && lane == 0) a.lse[((size_t)row * a.Hq + hq) * a.L + l] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }

@@ -191,14 +191,17 @@ __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
         const int old = max(start - block * BLOCK_TOKENS, 0);  // tokens of the block that the tail holds
         uint4 k[2][2];                                         // sixteen dims of two tokens
         uint32_t ka = 0, va = 0;
+        uint16_t was[2][16];
+        if (old > 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) __builtin_memcpy(was[i], vtail + ((tid >> 2) + 64 * i) * BLOCK_TOKENS + (tid & 3) * 16, 32);
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int t = (tid >> 3) + 32 * i, d = (tid & 7) * 16;
             if (t < old) {
                 k[i][0] = *reinterpret_cast<const uint4*>(ktail + t * HD + d);
                 k[i][1] = *reinterpret_cast<const uint4*>(ktail + t * HD + d + 8);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) vs[v_place(t, d + e)] = vtail[(d + e) * BLOCK_TOKENS + t];
             } else {
                 const int64_t at = block * (int64_t)BLOCK_TOKENS + t - start;
                 const uint16_t* ks = K + at * a.kt + d;
@@ -214,15 +217,17 @@ __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
                 ka = max(max(ka, max(abs_max_pair(k[i][c].x), abs_max_pair(k[i][c].y))), max(abs_max_pair(k[i][c].z), abs_max_pair(k[i][c].w)));
         }
         __syncthreads();
-        // values: thread (dim, quarter of the tokens) of either half of the dims
+        // values: thread (dim, quarter of the tokens) of either half of the dims; what the tail holds of them lies dim by dim already
         uint16_t v[2][16];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 v[i][e] = vs[v_place((tid & 3) * 16 + e, (tid >> 2) + 64 * i)];
+                if (old > 0) v[i][e] = (tid & 3) * 16 + e < old ? was[i][e] : v[i][e];
                 va = max(va, (uint32_t)(v[i][e] & 0x7fffu));
             }
+        }
         const int lane = tid & 63;
         const auto larger = [](float x, float y) { return __uint_as_float(max(__float_as_uint(x), __float_as_uint(y))); };
         ka = __float_as_uint(wave_fold(__uint_as_float(ka), larger));
@@ -581,6 +586,10 @@ __global__ __launch_bounds__(256) void pages_truncate_kernel(TruncateArgs a) {
     const odmkv_pages_t& p = a.p;
     const int row = blockIdx.x, tid = threadIdx.x, len = p.length[row], cut = cut_length(a, row, len);
     const int keep = cut / BLOCK_TOKENS, full = len / BLOCK_TOKENS, slot = p.slot[row];
+    if (gridDim.y == 1) {                                      // (the row is this workgroup's alone: no tail is made of any)
+        __syncthreads();
+        if (tid == 0) p.length[row] = p.start[row] = cut;
+    }
     if (keep >= full) return;
     if (blockIdx.y == 0) {
         Freed freed = {0, 0x7fffffff};
@@ -629,6 +638,7 @@ extern "C" int odmkv_pages_truncate(const odmkv_pages_t* p, const int32_t* lengt
     const int tails = lengths || lengths_host || length % BLOCK_TOKENS ? p->layers * p->Hkv : 0;
     PAGES_DISPATCH(pages_truncate_kernel, p, dim3(p->rows, 1 + tails), dim3(256), 0, (hipStream_t)stream, a);
     ODMKV_CHECK_LAUNCH("pages_truncate_kernel");
+    if (tails == 0) return 0;
     hipLaunchKernelGGL(pages_cut_kernel, dim3(1), dim3(BOOK_THREADS), 0, (hipStream_t)stream, a);
     ODMKV_CHECK_LAUNCH("pages_cut_kernel");
     return 0;

@@ -625,7 +625,7 @@ int odmkv_decode_attn_static(const void* q, int q_dtype, int B, int Hq, float sc
 #define ODMKV_PAGES_HOST_ROWS 512     /* batches up to here can have a row's number each (a count, a length, a parent) from the host, in the launch's arguments */
 
 typedef struct odmkv_pages {
-    int32_t layers, rows, Hkv, pages, blocks;    /* blocks: places of a table row, so at most blocks * 64 + 63 tokens a row */
+    int32_t layers, rows, Hkv, pages, blocks;    /* pages under 2^24; blocks: places of a table row, so at most blocks * 64 + 63 tokens a row */
     int32_t dtype;                               /* ODMKV_F16 / ODMKV_BF16: the tails, new tokens, queries */
     int32_t kind;                                /* ODMKV_INT8 / ODMKV_E4M3 */
     uint8_t* kcodes;                             /* device [layers, pages, Hkv, 64, 128] */
@@ -658,7 +658,7 @@ int odmkv_pages_read(const odmkv_pages_t* p, int layer, void* K, void* V, int ou
 size_t odmkv_pages_reorder_workspace_bytes(int rows);
 int odmkv_pages_reorder(const odmkv_pages_t* p, const int64_t* parents, const int32_t* parents_host, void* workspace, size_t workspace_bytes, void* stream);
 /* The rows of `to` (another batch over the same pages: same codes, scales, refs, status; its own table, tails, length, start,
- * slot, rows; its rows hold nothing yet) become copies of rows parents[b] of p (device int64 [to->rows]).  p's rows stay. */
+ * slot, rows; its rows hold nothing yet: length 0, row b in slot b) become copies of rows parents[b] of p (device int64 [to->rows]).  p's rows stay. */
 int odmkv_pages_select(const odmkv_pages_t* p, const odmkv_pages_t* to, const int64_t* parents, void* workspace,
                        size_t workspace_bytes, void* stream);
 /* Rows shrink to a length (device int32 [rows], or host int32 [rows], or both NULL: `length` for all; a longer one leaves the row): pages that nobody

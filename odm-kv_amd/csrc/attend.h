@@ -208,7 +208,7 @@ int launch_attend_wide_bf16(const AttendArgs& a, const Cut& cut, hipStream_t st)
 
 template <typename K>
 static int launch_attend(K kernel, const AttendArgs& a, long long groups, int waves, size_t lds, hipStream_t st) {
-    ODMKV_CHECK_ARG(groups < 0x7fffffffLL, "pages_attend: too many queries");
+    ODMKV_CHECK_ARG(groups * waves * 64 < 0x100000000LL, "pages_attend: too many queries");
     if (lds > 65536) ODMKV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(waves * 64), lds, st, a);
     ODMKV_CHECK_LAUNCH("pages_attend");

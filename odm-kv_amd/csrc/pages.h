@@ -81,3 +81,10 @@ __device__ static inline uint16_t to_16(float x) {
     constexpr float M = DT == ODMKV_F16 ? 65504.0f : 3.3895313892515355e38f;
     return Elem<DT>::from_f32(x > M ? M : x < -M ? -M : x);
 }
+// 16 bytes that are read once, or written for somebody else: the caches need not keep them
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ static inline uint4 load_once(const void* at) {
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ static inline void store_once(void* at, const uint4& v) { __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(at)); }

@@ -10,8 +10,8 @@ static int check_pages(const char* who, const odmkv_pages_t* p) {
     ODMKV_CHECK_ARG(p != nullptr, "%s: null pointer", who);
     ODMKV_CHECK_ARG(p->kcodes && p->vcodes && p->kscale && p->vscale && p->ktail && p->vtail && p->table && p->length && p->start &&
                     p->slot && p->refs && p->status, "%s: null pointer", who);
-    ODMKV_CHECK_ARG(p->layers > 0 && p->rows > 0 && p->rows <= MAX_ROWS && p->Hkv > 0 && p->Hkv <= 65535 && p->pages > 0 && p->blocks > 0 &&
-                    p->blocks <= (1 << 24) && p->layers <= 65535, "%s: bad shape", who);
+    ODMKV_CHECK_ARG(p->layers > 0 && p->rows > 0 && p->rows <= MAX_ROWS && p->Hkv > 0 && p->Hkv <= 65535 && p->pages > 0 && p->pages < (1 << 24) &&
+                    p->blocks > 0 && p->blocks <= (1 << 24) && p->layers <= 65535, "%s: bad shape", who);
     ODMKV_CHECK_ARG(p->dtype == ODMKV_F16 || p->dtype == ODMKV_BF16, "%s: bad dtype %d", who, p->dtype);
     ODMKV_CHECK_ARG(p->kind == ODMKV_INT8 || p->kind == ODMKV_E4M3, "%s: bad kind %d", who, p->kind);
     ODMKV_CHECK_ARG((((uintptr_t)p->kcodes | (uintptr_t)p->vcodes | (uintptr_t)p->ktail | (uintptr_t)p->vtail) & 15) == 0,
@@ -208,8 +208,8 @@ __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
                 const uint16_t* vsrc = V + at * a.vt + d;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    k[i][c] = finite8<DT>(*reinterpret_cast<const uint4*>(ks + 8 * c));
-                    *reinterpret_cast<uint4*>(vs + v_place(t, d + 8 * c)) = finite8<DT>(*reinterpret_cast<const uint4*>(vsrc + 8 * c));
+                    k[i][c] = finite8<DT>(load_once(ks + 8 * c));
+                    *reinterpret_cast<uint4*>(vs + v_place(t, d + 8 * c)) = finite8<DT>(load_once(vsrc + 8 * c));
                 }
             }
 #pragma unroll
@@ -693,8 +693,8 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(odmkv_pages_t p, odmkv_
     const int pieces = p.Hkv * (PAGE_BYTES / 16);
 #pragma unroll 4
     for (int i = tid; i < pieces; i += 256) {
-        reinterpret_cast<uint4*>(to.kcodes + at)[i] = reinterpret_cast<const uint4*>(p.kcodes + from)[i];
-        reinterpret_cast<uint4*>(to.vcodes + at)[i] = reinterpret_cast<const uint4*>(p.vcodes + from)[i];
+        store_once(to.kcodes + at + (size_t)i * 16, load_once(p.kcodes + from + (size_t)i * 16));
+        store_once(to.vcodes + at + (size_t)i * 16, load_once(p.vcodes + from + (size_t)i * 16));
     }
     for (int h = tid; h < p.Hkv; h += 256) {
         to.kscale[scale_at(to, layer, dst, h)] = p.kscale[scale_at(p, layer, page, h)];

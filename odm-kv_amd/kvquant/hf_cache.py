@@ -235,7 +235,7 @@ class PagedCache(Cache):
         if isinstance(indices, torch.Tensor) and indices.dtype == torch.bool:
             indices = indices.nonzero().view(-1)
         self.pool = old.select(indices.to(old.device) if isinstance(indices, torch.Tensor) else indices)
-        old.free()
+        old.release()
 
     def batch_repeat_interleave(self, repeats: int) -> None:
         if self.pool is not None:

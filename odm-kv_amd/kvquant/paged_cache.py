@@ -13,7 +13,7 @@ layers, one ``write`` a layer stores its tokens, one ``attend`` a layer reads th
 Lengths, tables and the count of every page's holders live on the device, so that a step can be captured into a graph and goes on from where
 the rows are at each replay.  The host keeps an upper bound of every row's length and of the pages in use, checks every call against them
 before anything is launched, and reads the device's only where those bounds do not settle it.  After replays of a captured ``extend`` the bounds are out
-of date: ``refresh`` reads them back (and raises if a replay found no room).
+of date: ``refresh`` reads them back (and raises if a replay found no room).  The cache is for inference: nothing records gradients.
 """
 from __future__ import annotations
 
@@ -93,7 +93,7 @@ class PagedKVCache:
         self.v_scale = torch.empty(self.layers, pages, self.kv_heads, dtype=torch.float32, **empty)
         self.refs = torch.empty(pages, dtype=torch.int32, **empty)
         self.status = torch.empty(4, dtype=torch.int32, **empty)
-        # what the batches over this pool share: an upper bound of the pages in use, and every batch's bounds
+        # what the batches over this pool share: an upper bound of the pages in use, and every batch's bounds (its own list, changed in place)
         self._shared = {"used": 0, "bounds": []}
 
     def _make_rows(self) -> None:
@@ -105,6 +105,7 @@ class PagedKVCache:
         self.start = torch.empty(B, dtype=torch.int32, **empty)
         self.slot = torch.empty(B, dtype=torch.int32, **empty)
         self._bounds = [0] * B                               # no row is longer
+        self._grown, self._written = 0, set()                # tokens a row at most of the last extend, and the layers that have stored them
         self._shared["bounds"].append(self._bounds)
 
     def _struct(self) -> None:
@@ -197,6 +198,7 @@ class PagedKVCache:
             if counts < 0:
                 raise ValueError(f"counts must not be negative, got {counts}")
             self._make_room([counts] * self.batch)
+            self._grown, self._written = counts, set()
             self._call(lib.odmkv_pages_extend, C.byref(self._p), None, None, counts, counts)
             return
         on_device, host, known = self._ints(counts, self.batch, torch.int32, "counts")
@@ -218,13 +220,18 @@ class PagedKVCache:
                 raise ValueError(f"a count of {max(known)} is above bound={bound}")
             bound = max(known)
             self._make_room(known)
+        self._grown, self._written = int(bound), set()
         self._call(lib.odmkv_pages_extend, C.byref(self._p), _lib.ptr(on_device), host, 0, int(bound))
 
     def write(self, layer: int, keys: torch.Tensor, values: torch.Tensor) -> None:
-        """Stores the tokens of the last ``extend`` in one layer: keys, values [B, Hkv, T, 128] of the cache's dtype, row b's at t < its count, T at least
-        the largest count.  Once a layer and extend: a second call would take the new tail for the old one."""
-        if _device() == self.device.index and isinstance(keys, torch.Tensor) and isinstance(values, torch.Tensor) and _native.paged_write(
-                _WRITE, self._at, self.device.index, layer, keys, values, _lib.stream_ptr(self.device)):
+        """Stores the tokens of the last ``extend`` in one layer, once: keys, values [B, Hkv, T, 128] of the cache's dtype, row b's at t < its count, T at least the
+        largest count (or its bound)."""
+        if layer in self._written:                           # (the new tail would be taken for the old one)
+            raise ValueError(f"layer {layer} has stored the tokens of this extend already")
+        if (isinstance(keys, torch.Tensor) and isinstance(values, torch.Tensor) and keys.dim() == 4 and keys.shape[2] >= self._grown
+                and _device() == self.device.index and _native.paged_write(_WRITE, self._at, self.device.index, layer, keys, values,
+                                                                           _lib.stream_ptr(self.device))):
+            self._written.add(layer)
             return
         self._check_layer(layer)
         for t, what in ((keys, "keys"), (values, "values")):
@@ -233,9 +240,12 @@ class PagedKVCache:
             self._check_tensor(t, what)
         if keys.shape[2] != values.shape[2]:
             raise ValueError(f"{keys.shape[2]} keys and {values.shape[2]} values a row")
+        if keys.shape[2] < self._grown:
+            raise ValueError(f"{keys.shape[2]} tokens a row, but rows have grown by up to {self._grown}")
         keys, values = self._rows_ok(keys), self._rows_ok(values)
         self._call(lib.odmkv_pages_write, C.byref(self._p), layer, keys.data_ptr(), *keys.stride()[:3], values.data_ptr(), *values.stride()[:3],
                    keys.shape[2])
+        self._written.add(layer)
 
     def append(self, keys: torch.Tensor, values: torch.Tensor, counts: Optional[Counts] = None) -> None:
         """``extend`` and ``write`` of a cache of one layer."""
@@ -346,8 +356,9 @@ class PagedKVCache:
         `parents`: a list, or whole numbers on the device (an index out of range is then refused there: see ``refresh``)."""
         on_device, host, known = self._parents(parents, self.batch)
         if known is None:                                    # indices that only the device knows
-            self._bounds[:] = [self.max_length] * self.batch
-            self._loose = True
+            if min(self._bounds) < self.max_length:          # (rows of one length stay that)
+                self._bounds[:] = [self.max_length] * self.batch
+                self._loose = True
         else:
             self._bounds[:] = [self._bounds[b] for b in known]
         self._used_at_most()
@@ -356,7 +367,7 @@ class PagedKVCache:
         self._call(lib.odmkv_pages_reorder, C.byref(self._p), _lib.ptr(on_device), host, ws.data_ptr(), nbytes)
 
     def select(self, parents) -> "PagedKVCache":
-        """A batch of its own over the same pages, whose row b is a copy of this one's row parents[b]; this one's rows stay (``free`` them where they are
+        """A batch of its own over the same pages, whose row b is a copy of this one's row parents[b]; this one's rows stay (``release`` it where it is
         not needed).  Both batches draw on the one pool."""
         n = int(parents.shape[0]) if isinstance(parents, torch.Tensor) and parents.dim() == 1 else len(parents)
         if not 1 <= n <= MAX_ROWS:
@@ -416,6 +427,11 @@ class PagedKVCache:
         """Rows (default all) hold nothing any more."""
         self.truncate(0, rows)
 
+    def release(self) -> None:
+        """Frees all rows and leaves the pool to the batches that share it: this one is not used any more."""
+        self.free()
+        self._shared["bounds"] = [bounds for bounds in self._shared["bounds"] if bounds is not self._bounds]
+
     def _used_at_most(self) -> None:
         self._shared["used"] = min(self._shared["used"], sum(n // BLOCK for bounds in self._shared["bounds"] for n in bounds))
 
@@ -435,6 +451,7 @@ class PagedKVCache:
         new._make_rows()
         new._struct()
         new._bounds[:], new._loose = self._bounds, self._loose
+        new._grown, new._written = self._grown, set(self._written)
         new._shared["used"] = self._shared["used"]
         nbytes = lib.odmkv_pages_compact_workspace_bytes(self.pages)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)

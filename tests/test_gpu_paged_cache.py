@@ -353,7 +353,9 @@ def test_select_makes_another_batch_over_the_same_pages():
         wide.write(layer, k.to(DEV), v.to(DEV))
         _holds(wide, layer, [tuple(torch.cat([x, y[i]], dim=1) for x, y in zip(r.rows[layer][b], (k, v))) for i, b in enumerate((0, 0, 2, 1, 2))], r.kind)
     narrow = wide.select(torch.tensor([4], device=DEV))
-    wide.free()
+    with pytest.raises(ValueError, match="shared"):
+        narrow.compacted()
+    wide.release()
     _pages_add_up(narrow, wide)
     small = narrow.compacted()
     for layer in range(2):
@@ -533,6 +535,37 @@ def test_another_stream():
         got = _filled(k, v, [300], "int8").attend(0, q)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, want)
+
+
+def test_tokens_are_stored_once_a_layer_and_extend():
+    k, v = _rows(1, 1, 1, 70, torch.float16)
+    k, v = k.to(DEV), v.to(DEV)
+    c = _cache(1, 1, 300)
+    c.extend(70)
+    with pytest.raises(ValueError, match="70"):
+        c.write(0, k[:, :, :69], v[:, :, :69])
+    c.write(0, k, v)
+    for args in ((k, v), (k.transpose(2, 3).contiguous().transpose(2, 3), v)):
+        with pytest.raises(ValueError, match="already"):
+            c.write(0, *args)
+    c.extend(torch.tensor([3], device=DEV), bound=5)
+    with pytest.raises(ValueError, match="5"):
+        c.write(0, k[:, :, :4], v[:, :, :4])
+    c.write(0, k[:, :, :6], v[:, :, :6])
+    _holds(c, 0, [tuple(torch.cat([x, x[:, :, :3]], dim=2)[0].cpu() for x in (k, v))], "int8")
+
+
+def test_beams_of_one_length_need_no_reading_back():
+    """Parents that only the device knows leave the host's bounds as they are where all rows are alike."""
+    k, v = _rows(1, 4, 1, 64, torch.float16)
+    c = _filled(k, v, [64] * 4, "int8", pages=9)
+    c.refresh = lambda: pytest.fail("read back")
+    for step in range(64):
+        c.reorder(torch.tensor([step % 4, 0, 1, 1], device=DEV))
+        c.extend(1)
+        c.write(0, k[:, :, :1].to(DEV), v[:, :, :1].to(DEV))
+    assert c.length.tolist() == [128] * 4
+    _pages_add_up(c)
 
 
 def test_refusals():

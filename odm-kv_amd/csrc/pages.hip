@@ -171,8 +171,7 @@ struct WriteArgs {
 // sixteen dims and four quarters that a wavefront reads at a time fall on distinct banks.
 __device__ static inline int v_place(int token, int dim) { return token * HD + (((dim >> 3) ^ ((token >> 4) << 1)) << 3) + (dim & 7); }
 
-// A workgroup stores one block of a row and kv-head; the one of the row's first touched block also stores the open block, behind it: the tail that
-// the first one is completed from is the tail that the open one goes to.
+// A workgroup stores one block of a row and kv-head.
 // Bound by memory: 16 bits read and 8 written a value.
 template <int DT, int KIND>
 __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
@@ -181,6 +180,8 @@ __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
     const int start = p.start[row], len = p.length[row];
     if (len <= start || len - start > a.T) return;
     const int block = start / BLOCK_TOKENS + blockIdx.x, open = len / BLOCK_TOKENS, slot = p.slot[row];
+    const int begun = start / BLOCK_TOKENS < open ? start % BLOCK_TOKENS : 0;      // tokens of the first block, if it is completed, that the tail holds
+    if (block > open) return;
     __shared__ __align__(16) uint16_t vs[BLOCK_TOKENS * HD];
     __shared__ uint32_t top[2][4];
     uint16_t* ktail = p.ktail + tail_at(p, a.layer, slot, h);
@@ -189,6 +190,7 @@ __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
     const uint16_t* V = a.V + row * a.vb + h * a.vh;
     if (block < open) {
         const int old = max(start - block * BLOCK_TOKENS, 0);  // tokens of the block that the tail holds
+        const int page = p.table[(size_t)slot * p.blocks + block];
         uint4 k[2][2];                                         // sixteen dims of two tokens
         uint32_t ka = 0, va = 0;
         uint16_t was[2][16];
@@ -241,7 +243,6 @@ __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
         va = max(max(top[1][0], top[1][1]), max(top[1][2], top[1][3]));
         const float sk = block_scale<KIND>(Elem<DT>::to_f32((uint16_t)ka)), sv = block_scale<KIND>(Elem<DT>::to_f32((uint16_t)va));
         const float ik = sk > 0.0f ? __fdiv_rn(1.0f, sk) : 0.0f, iv = sv > 0.0f ? __fdiv_rn(1.0f, sv) : 0.0f;
-        const int page = p.table[(size_t)slot * p.blocks + block];
         const size_t at = page_at(p, a.layer, page, h);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -266,19 +267,37 @@ __global__ __launch_bounds__(256) void pages_write_kernel(WriteArgs a) {
             p.vscale[scale_at(p, a.layer, page, h)] = sv;
         }
     }
-    if (blockIdx.x != 0) return;
-    __syncthreads();                                           // the old tail has been read
+    // The open block: by its own workgroup, or, where the row's first block is completed from the tail that the open one goes to, by that one, behind it.
+    if (begun > 0 ? blockIdx.x != 0 : block != open) return;
+    __syncthreads();                                           // the old tail, and what lay in LDS, have been read
     // (tokens that complete the block that the tail had begun, with none behind them, go there as well: a token at a time, the tail takes every one)
     const int newest = start > open * BLOCK_TOKENS - BLOCK_TOKENS && len == open * BLOCK_TOKENS ? len - BLOCK_TOKENS : open * BLOCK_TOKENS;
-    const int from = max(start, newest);
-    for (int i = tid; i < (len - from) * 16; i += 256) {
-        const int t = from + (i >> 4), d = (i & 15) * 8, place = t - newest;
-        const int64_t at = t - start;
-        *reinterpret_cast<uint4*>(ktail + place * HD + d) = finite8<DT>(*reinterpret_cast<const uint4*>(K + at * a.kt + d));
-        const uint4 v = finite8<DT>(*reinterpret_cast<const uint4*>(V + at * a.vt + d));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const int from = max(start, newest), n = len - from;
+    const bool fresh = from == newest;                         // nothing of the block lies in the tail yet: its values go there by whole pieces
+    if (n == 0) return;
+    for (int i = tid; i < (fresh ? BLOCK_TOKENS : n) * 16; i += 256) {
+        const int d = (i & 15) * 8, place = from - newest + (i >> 4);
+        const int64_t at = from - start + (i >> 4);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (i >> 4 < n) {
+            *reinterpret_cast<uint4*>(ktail + place * HD + d) = finite8<DT>(*reinterpret_cast<const uint4*>(K + at * a.kt + d));
+            v = finite8<DT>(*reinterpret_cast<const uint4*>(V + at * a.vt + d));
+        }
+        if (fresh) *reinterpret_cast<uint4*>(vs + v_place(place, d)) = v;
+        else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) vtail[(d + e) * BLOCK_TOKENS + place] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            for (int e = 0; e < 8; ++e) vtail[(d + e) * BLOCK_TOKENS + place] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        }
+    }
+    if (!fresh) return;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint16_t v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = vs[v_place((tid & 3) * 16 + e, (tid >> 2) + 64 * i)];
+        __builtin_memcpy(vtail + ((tid >> 2) + 64 * i) * BLOCK_TOKENS + (tid & 3) * 16, v, 32);
     }
 }
 
@@ -343,10 +362,13 @@ __global__ __launch_bounds__(256) void pages_read_kernel(odmkv_pages_t p, int la
                     v[e] *= sv;
                 }
             } else {
+                uint16_t kt[16], vt16[16];
+                __builtin_memcpy(kt, p.ktail + tat + t * HD + d, 32);
+                __builtin_memcpy(vt16, p.vtail + tat + vd * BLOCK_TOKENS + vt, 32);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    k[i][e] = t < held ? Elem<DT>::to_f32(p.ktail[tat + t * HD + d + e]) : 0.0f;
-                    v[e] = vt + e < held ? Elem<DT>::to_f32(p.vtail[tat + vd * BLOCK_TOKENS + vt + e]) : 0.0f;
+                    k[i][e] = t < held ? Elem<DT>::to_f32(kt[e]) : 0.0f;
+                    v[e] = vt + e < held ? Elem<DT>::to_f32(vt16[e]) : 0.0f;
                 }
             }
 #pragma unroll

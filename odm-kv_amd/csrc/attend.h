@@ -198,6 +198,7 @@ __device__ static inline Share share_of(const AttendArgs& a, int at) {
 // How a call is cut.
 struct Cut {
     int waves, splits;       // wavefronts of a workgroup; workgroups of a kv-head (narrow), or that share a row and kv-head's blocks (wide)
+    int groups;              // wide: 32s of queries of a workgroup; two for four wavefronts: two take the first half of every block, two the second
     bool wide, stream;       // stream: pages pass by the caches
     size_t parts;            // partial results
 };

@@ -91,10 +91,11 @@ static int launch_attend_merge(const AttendArgs& a, const Cut& cut, hipStream_t 
 // one of eight.  (A share more than that costs its partial results: with two of eight, 2048 queries over 4096 tokens took 330 us for 273, four of 777 145 for 51.)
 static Cut cut_of(const odmkv_pages_t& p, int R, int max_length) {
     const int blocks = max_length / BLOCK_TOKENS + 1, units = compute_units();
-    Cut c = {4, 1, R > NARROW, false, 0};
+    Cut c = {4, 1, 4, R > NARROW, false, 0};
     if (c.wide) {
         c.waves = R > 128 ? WIDE_WAVES : 4;
-        const long long groups = (long long)p.rows * p.Hkv * ((R + 32 * c.waves - 1) / (32 * c.waves));
+        c.groups = R <= 64 ? 2 : c.waves;
+        const long long groups = (long long)p.rows * p.Hkv * ((R + 32 * c.groups - 1) / (32 * c.groups));
         c.splits = (int)std::max(1LL, std::min((c.waves == WIDE_WAVES ? 1 : 2) * units / groups, (long long)blocks / 4));
         c.parts = c.splits > 1 ? (size_t)p.rows * p.Hkv * c.splits * R : 0;
     } else {

@@ -14,21 +14,22 @@
 enum { SCORES_PLAIN, SCORES_CAPPED, SCORES_BIASED, SCORES_ANY };
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <int DT, int KIND, int MODE, int WAVES>
+template <int DT, int KIND, int MODE, int WAVES, int GROUPS>
 __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a) {
     const odmkv_pages_t& p = a.p;
-    constexpr bool PLAIN = MODE == SCORES_PLAIN;
+    constexpr bool PLAIN = MODE == SCORES_PLAIN, HALVES = GROUPS < WAVES;
     extern __shared__ __align__(16) uint8_t lds[];              // [2][keys 64 x 256 bytes, values 128 x 128 bytes]
     __shared__ int range[2][WAVES];
     __shared__ uint32_t tops[2][WAVES];
     constexpr int THREADS = WAVES * 64, BUFFER = BLOCK_TOKENS * HD * 4, VALUES = BLOCK_TOKENS * HD * 2;
-    const int pairs = p.rows * p.Hkv, R = a.G * a.L, tiles = (R + 32 * WAVES - 1) / (32 * WAVES);
+    const int pairs = p.rows * p.Hkv, R = a.G * a.L, tiles = (R + 32 * GROUPS - 1) / (32 * GROUPS);
     // heads vary fastest (a die of the chip then keeps few heads' pages in its L2), the longest rows of blocks come first
     const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs, split = rest % a.splits, tile = tiles - 1 - rest / a.splits;
     const int row = pair / p.Hkv, h = pair % p.Hkv, tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave % GROUPS;
+    const int part = HALVES ? wave / GROUPS : 0;                // the half of every block that this wavefront takes
     const int len = p.length[row], count = a.counts ? min(max(a.counts[row], 0), a.L) : a.L, slot = p.slot[row];
-    const int r0 = tile * 32 * WAVES + 32 * wave, r = r0 + col, l = r / a.G, hq = h * a.G + r - l * a.G;
+    const int r = tile * 32 * GROUPS + 32 * group + col, l = r / a.G, hq = h * a.G + r - l * a.G;
     const bool valid = r < R && l < count;
     Sight s = {0, 0, 0};
     if (valid) s = sight_of(a, row, len, count, l);
@@ -187,22 +188,22 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
         const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
         f32x16 dot[2];
         f16x8 w[4];
-        const auto multiply_keys = [&](int tb) {
+        const auto multiply_keys = [&](int tb, int place) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) dot[tb][e] = 0.0f;
 #pragma unroll
             for (int st = 0; st < 8; ++st)
-                dot[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*key_piece(buf, 32 * tb + col, 2 * st + half), q[st], dot[tb], 0, 0, 0);
+                dot[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*key_piece(buf, 32 * place + col, 2 * st + half), q[st], dot[tb], 0, 0, 0);
         };
-        const auto multiply_values = [&](int st) {
+        const auto multiply_values = [&](int st, int place) {
 #pragma unroll
             for (int db = 0; db < 4; ++db)
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(value_piece(buf, 32 * db + col, 2 * st + half)), w[st], acc[db], 0, 0, 0);
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(value_piece(buf, 32 * db + col, 2 * place + half)), w[st], acc[db], 0, 0, 0);
         };
         // products of half a block to scores, and the reference where it is to rise (what has been summed up, and weights that have not, come to the new one)
-        const auto look_over = [&](int tb) {
+        const auto look_over = [&](int tb, int place) {
             f32x16& x = dot[tb];
-            const int tl = t0 + 32 * tb + 4 * half;             // token of score e: tl + 8 (e / 4) + e % 4
+            const int tl = t0 + 32 * place + 4 * half;             // token of score e: tl + 8 (e / 4) + e % 4
             if constexpr (!PLAIN) {
                 if (by_exp) {
                     const float k = c * cap.plain;
@@ -262,18 +263,40 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
             sum = __fmaf_rn(z0 + z1, free_f, sum);
         };
         // The two halves' vector work stands beside the other half's matrix work: a matrix instruction takes 32 cycles, which some eight vector instructions fill.
-        multiply_keys(0);
-        look_over(0);
-        multiply_keys(1);
-        weigh(0);
-
-        look_over(1);
-        multiply_values(0);
-        multiply_values(1);
-        weigh(1);
-
-        multiply_values(2);
-        multiply_values(3);
+        multiply_keys(0, part);
+        look_over(0, part);
+        if constexpr (HALVES) {
+            weigh(0);
+            multiply_values(0, 2 * part);
+            multiply_values(1, 2 * part + 1);
+        } else {
+            multiply_keys(1, 1);
+            weigh(0);
+            look_over(1, 1);
+            multiply_values(0, 0);
+            multiply_values(1, 1);
+            weigh(1);
+            multiply_values(2, 2);
+            multiply_values(3, 3);
+        }
+    }
+    if constexpr (HALVES) {                                     // the second half's sums join the first's, by way of LDS
+        float* const other = reinterpret_cast<float*>(lds) + group * 66 * 64 + lane;
+        __syncthreads();
+        if (part) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) other[64 * e] = acc[e >> 4][e & 15];
+            other[64 * 64] = ref;
+            other[65 * 64] = sum;
+        }
+        __syncthreads();
+        if (part) return;
+        const float to = fmaxf(ref, other[64 * 64]), by = to > -INFINITY ? to : 0.0f;
+        const float mine_by = __builtin_amdgcn_exp2f(ref - by), other_by = __builtin_amdgcn_exp2f(other[64 * 64] - by);
+        ref = to;
+        sum = __fmaf_rn(other[65 * 64], other_by, sum * mine_by);
+#pragma unroll
+        for (int e = 0; e < 64; ++e) acc[e >> 4][e & 15] = __fmaf_rn(other[64 * e], other_by, acc[e >> 4][e & 15] * mine_by);
     }
 
     const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
@@ -315,11 +338,14 @@ static int launch_wide_of(const AttendArgs& a, const Cut& cut, hipStream_t st) {
     const bool capped = a.cap > 0.0f;
     const int R = a.G * a.L, mode = a.slopes ? (capped ? SCORES_ANY : SCORES_BIASED)
                                   : capped ? (a.cap <= CAP_BY_EXP ? SCORES_CAPPED : SCORES_ANY) : a.scaling > 0.0f ? SCORES_PLAIN : SCORES_ANY;
-    const long long groups = (long long)a.p.rows * a.p.Hkv * a.splits * ((R + 32 * cut.waves - 1) / (32 * cut.waves));
-    const auto run = [&](auto dt, auto kind, auto mode_, auto waves) {
-        return launch_attend(attend_wide_kernel<dt.value, kind.value, mode_.value, waves.value>, a, groups, waves.value, WIDE_LDS, st);
+    const long long groups = (long long)a.p.rows * a.p.Hkv * a.splits * ((R + 32 * cut.groups - 1) / (32 * cut.groups));
+    const auto run = [&](auto dt, auto kind, auto mode_, auto waves, auto groups_) {
+        return launch_attend(attend_wide_kernel<dt.value, kind.value, mode_.value, waves.value, groups_.value>, a, groups, waves.value, WIDE_LDS, st);
     };
-    const auto of_waves = [&](auto dt, auto kind, auto mode_) { return cut.waves == 4 ? run(dt, kind, mode_, Int<4>()) : run(dt, kind, mode_, Int<WIDE_WAVES>()); };
+    const auto of_waves = [&](auto dt, auto kind, auto mode_) {
+        if (cut.groups == 2) return run(dt, kind, mode_, Int<4>(), Int<2>());
+        return cut.waves == 4 ? run(dt, kind, mode_, Int<4>(), Int<4>()) : run(dt, kind, mode_, Int<WIDE_WAVES>(), Int<WIDE_WAVES>());
+    };
     const auto of_mode = [&](auto dt, auto kind) {
         switch (mode) {
             case SCORES_PLAIN: return of_waves(dt, kind, Int<SCORES_PLAIN>());

@@ -99,9 +99,10 @@ static Cut cut_of(const odmkv_pages_t& p, int R, int max_length) {
         c.splits = (int)std::max(1LL, std::min((c.waves == WIDE_WAVES ? 1 : 2) * units / groups, (long long)blocks / 4));
         c.parts = c.splits > 1 ? (size_t)p.rows * p.Hkv * c.splits * R : 0;
     } else {
-        // Pages that all layers together have too many of for the last-level cache (256 MB) to keep from one call to the next: nothing is gained by keeping any, and
-        // reads that do not ask for it reach 5.9 TB/s instead of 5.0 (268 MB a call 59.7 -> 51.4 us; 67 MB a call over three caches in turn, which do fit, 18.7 -> 20.2).
-        c.stream = (size_t)p.layers * p.pages * p.Hkv * 2 * PAGE_BYTES > ((size_t)128 << 20);
+        // Pages that the last-level cache (256 MB) would not keep from one call to the next, with what else passes between: nothing is gained by keeping any, and reads
+        // that do not ask for it are faster (268 MB a call 59.7 -> 51.4 us; three caches of 134 MB in turn 33.3 -> 30.3).  Where they would be kept, it costs: 134 MB
+        // and nothing else 28.2 -> 28.7 us, three caches of 67 MB in turn 18.7 -> 20.2.
+        c.stream = (size_t)p.layers * p.pages * p.Hkv * 2 * PAGE_BYTES > ((size_t)96 << 20);
         // Eight wavefronts where they hold a row's blocks by themselves, so that nothing is merged (500 tokens: 10.8 -> 9.7 us), and for one row so long that
         // each has several (131071 tokens of 4 heads: 35.4 -> 33.2 us; half as many shares to merge); four otherwise: twice as many compute units for 2000 tokens
         // (13.1 -> 11.2 us), finer shares for rows of their own lengths (16 of up to 8192: 50.6 -> 40.4 us).

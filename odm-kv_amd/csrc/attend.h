@@ -124,6 +124,15 @@ __device__ static inline uint32_t abs_max8(const uint4& v) {
     return max(max(abs_max_pair(v.x), abs_max_pair(v.y)), max(abs_max_pair(v.z), abs_max_pair(v.w)));
 }
 
+// the first n of eight numbers, 0 for the rest: what a tail holds behind its row's end is of tokens that are gone, and must not decide a power of two
+__device__ static inline uint4 first_of8(int n) {                // as a mask
+    uint32_t m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = n > 2 * i + 1 ? 0xffffffffu : n > 2 * i ? 0xffffu : 0u;
+    return make_uint4(m[0], m[1], m[2], m[3]);
+}
+__device__ static inline uint4 masked8(const uint4& v, const uint4& m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
+
 // over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a query
 template <typename F>
 __device__ static inline float column_fold(float v, F f) {

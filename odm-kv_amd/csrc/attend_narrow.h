@@ -205,6 +205,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
 #pragma unroll
         for (int c = 0; c < 16; ++c) v[c] = *reinterpret_cast<const uint4*>(vt + (c >> 1) * 16 * BLOCK_TOKENS + (c & 1) * 8);
         if (first_group) take_queries();
+        const int held = len - full * BLOCK_TOKENS;
+        const uint4 low = first_of8(held - 16 * j), high = first_of8(held - 16 * j - 8);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            if (16 * (n >> 2) + (n & 3) + 4 * (c >> 2) >= held) k[c] = make_uint4(0, 0, 0, 0);
+            v[c] = masked8(v[c], c & 1 ? high : low);
+        }
         Power pk = {1.0f, 1.0f};
         if constexpr (DT == ODMKV_BF16) {                       // (fp16 keys are taken as they are)
             uint32_t top = 0;

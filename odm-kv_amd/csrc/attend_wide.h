@@ -123,11 +123,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
     const auto put_tail = [&](uint8_t* buf) {
         const uint4* kt = reinterpret_cast<const uint4*>(p.ktail + tail_at(p, a.layer, slot, h));
         const uint4* vt = reinterpret_cast<const uint4*>(p.vtail + tail_at(p, a.layer, slot, h));
+        const int held = len - full * BLOCK_TOKENS;
+        const auto keys_of = [&](int i) { return i >> 4 < held ? kt[i] : make_uint4(0, 0, 0, 0); };
+        const auto values_of = [&](int i) { return masked8(vt[i], first_of8(held - 8 * (i & 7))); };
         uint32_t top[2] = {0, 0};
 #pragma unroll 1
         for (int i = tid; i < TAIL_ELEMS / 8; i += THREADS) {
-            top[0] = max(top[0], abs_max8(kt[i]));
-            top[1] = max(top[1], abs_max8(vt[i]));
+            top[0] = max(top[0], abs_max8(keys_of(i)));
+            top[1] = max(top[1], abs_max8(values_of(i)));
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -145,8 +148,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
 #pragma unroll 1
         for (int i = tid; i < TAIL_ELEMS / 8; i += THREADS) {
             const int dim = i >> 3, u = i & 7;
-            *key_piece(buf, i >> 4, i & 15) = scaled_f16<DT>(kt[i], pk.up);
-            const uint4 x = __builtin_bit_cast(uint4, scaled_f16<DT>(vt[i], pv.up));
+            *key_piece(buf, i >> 4, i & 15) = scaled_f16<DT>(keys_of(i), pk.up);
+            const uint4 x = __builtin_bit_cast(uint4, scaled_f16<DT>(values_of(i), pv.up));
             *reinterpret_cast<uint2*>(value_piece(buf, dim, u & ~1) + 8 * (u & 1)) = make_uint2(x.x, x.y);
             *reinterpret_cast<uint2*>(value_piece(buf, dim, u | 1) + 8 * (u & 1)) = make_uint2(x.z, x.w);
         }

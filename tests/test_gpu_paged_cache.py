@@ -555,6 +555,28 @@ def test_tokens_are_stored_once_a_layer_and_extend():
     _holds(c, 0, [tuple(torch.cat([x, x[:, :, :3]], dim=2)[0].cpu() for x in (k, v))], "int8")
 
 
+@pytest.mark.parametrize("L", [1, 3, 20])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("how", ["freed", "cut"])
+def test_what_a_tail_held_before_decides_nothing(how, dtype, L):
+    """Tokens behind a row's end, as large as the type has them, beside small ones in the same tail."""
+    big = torch.finfo(dtype).max / 4
+    k, v = _rows(2, 1, 2, 40, dtype)
+    k, v = k * 2.0 ** -6, v * 2.0 ** -8                       # (fp16: v from 2^-24 on, of which a factor of 2^-9 would leave nothing)
+    old = torch.full((1, 2, 60, 128), big, dtype=dtype)
+    c = _cache(1, 2, 300, dtype=dtype)
+    if how == "freed":
+        c.append(old.to(DEV), old.to(DEV))
+        c.free()
+    else:
+        c.append(k[:, :, :7].to(DEV), v[:, :, :7].to(DEV))
+        c.append(old[:, :, :50].to(DEV), old[:, :, :50].to(DEV))
+        c.truncate(7)
+    have = c.length.tolist()[0]
+    c.append(k[:, :, have:21].to(DEV), v[:, :, have:21].to(DEV))
+    _check_attend(c, [(k[0, :, :21], v[0, :, :21])], "int8", _queries(1, 1, 8, L, dtype, 60.0))
+
+
 def test_beams_of_one_length_need_no_reading_back():
     """Parents that only the device knows leave the host's bounds as they are where all rows are alike."""
     k, v = _rows(1, 4, 1, 64, torch.float16)

@@ -49,6 +49,11 @@ def _blocks(tokens: int) -> int:
     return (tokens + BLOCK - 1) // BLOCK
 
 
+def _as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Whole numbers as another type; those that 32 bits do not hold stop at their end."""
+    return t.clamp(-2 ** 31, 2 ** 31 - 1).to(dtype) if dtype == torch.int32 and t.dtype == torch.int64 else t.to(dtype)
+
+
 class PagedKVCache:
     """`batch` rows of at most `max_tokens` tokens, `layers` layers of `kv_heads` heads of 128; `pages`: full blocks that there is room for in each layer
     (default: every row's longest).  `kind`: "int8" or "e4m3".  The tensors are attributes, laid out as include/odmkv.h says (struct odmkv_pages)."""
@@ -108,6 +113,9 @@ class PagedKVCache:
         self._grown, self._written = 0, set()                # tokens a row at most of the last extend, and the layers that have stored them
         self._shared["bounds"].append(self._bounds)
 
+    def _nothing_to_write(self) -> None:
+        self._grown, self._written = 0, range(self.layers)   # (rows have moved: what was to be stored is not there any more)
+
     def _struct(self) -> None:
         self._p = _lib.Pages(self.layers, self.batch, self.kv_heads, self.pages, self.table.shape[1], _lib._DT[self.dtype], KINDS[self.kind][0],
                              *(t.data_ptr() for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.table,
@@ -139,7 +147,7 @@ class PagedKVCache:
                 raise ValueError(f"{what} lie on {values.device}, the cache on {self.device}")
             if values.shape != (n,):
                 raise ValueError(f"{what} must be one number a row, [{n}], got {list(values.shape)}")
-            return values.to(dtype).contiguous(), None, None
+            return _as(values, dtype).contiguous(), None, None
         if isinstance(values, torch.Tensor) and (values.is_floating_point() or values.is_complex() or values.dtype == torch.bool):
             raise ValueError(f"{what} must be whole numbers, got {values.dtype}")
         known = [int(v) for v in values]
@@ -220,14 +228,15 @@ class PagedKVCache:
                 raise ValueError(f"a count of {max(known)} is above bound={bound}")
             bound = max(known)
             self._make_room(known)
-        self._grown, self._written = int(bound), set()
-        self._call(lib.odmkv_pages_extend, C.byref(self._p), _lib.ptr(on_device), host, 0, int(bound))
+        bound = min(int(bound), self.max_tokens)
+        self._grown, self._written = bound, set()
+        self._call(lib.odmkv_pages_extend, C.byref(self._p), _lib.ptr(on_device), host, 0, bound)
 
     def write(self, layer: int, keys: torch.Tensor, values: torch.Tensor) -> None:
-        """Stores the tokens of the last ``extend`` in one layer, once: keys, values [B, Hkv, T, 128] of the cache's dtype, row b's at t < its count, T at least the
+        """Stores the tokens of the last ``extend`` in one layer, once and before rows are moved or cut: keys, values [B, Hkv, T, 128] of the cache's dtype, row b's at t < its count, T at least the
         largest count (or its bound)."""
         if layer in self._written:                           # (the new tail would be taken for the old one)
-            raise ValueError(f"layer {layer} has stored the tokens of this extend already")
+            raise ValueError(f"layer {layer} has no tokens to store: it has stored those of the last extend already, or rows have been moved or cut since")
         if (isinstance(keys, torch.Tensor) and isinstance(values, torch.Tensor) and keys.dim() == 4 and keys.shape[2] >= self._grown
                 and _device() == self.device.index and _native.paged_write(_WRITE, self._at, self.device.index, layer, keys, values,
                                                                            _lib.stream_ptr(self.device))):
@@ -348,7 +357,7 @@ class PagedKVCache:
             raise ValueError(f"{what} lie on {t.device}, the cache on {self.device}")
         if dtype == torch.int32 and (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool):
             raise ValueError(f"{what} must be whole numbers, got {t.dtype}")
-        return t.to(dtype).contiguous()
+        return (_as(t, dtype) if dtype == torch.int32 else t.to(dtype)).contiguous()
 
     # ------------------------------------------------------------------ rows
     def reorder(self, parents) -> None:
@@ -362,6 +371,7 @@ class PagedKVCache:
         else:
             self._bounds[:] = [self._bounds[b] for b in known]
         self._used_at_most()
+        self._nothing_to_write()
         nbytes = lib.odmkv_pages_reorder_workspace_bytes(self.batch)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self._call(lib.odmkv_pages_reorder, C.byref(self._p), _lib.ptr(on_device), host, ws.data_ptr(), nbytes)
@@ -383,6 +393,7 @@ class PagedKVCache:
             t.zero_()
         new.slot.copy_(torch.arange(n, dtype=torch.int32, device=self.device))
         new._struct()
+        new._nothing_to_write()
         new._bounds[:] = [self.max_length] * n if known is None else [self._bounds[b] for b in known]
         new._loose = self._loose or known is None
         nbytes = lib.odmkv_pages_reorder_workspace_bytes(n)
@@ -413,7 +424,8 @@ class PagedKVCache:
             on_device, host, known = self._ints(lengths, self.batch, torch.int32, "lengths")
         if known is not None and min(known) < 0:
             raise ValueError(f"a length must not be negative, got {min(known)}")
-        self._call(lib.odmkv_pages_truncate, C.byref(self._p), _lib.ptr(on_device), host, lengths if isinstance(lengths, int) else 0, mask)
+        self._call(lib.odmkv_pages_truncate, C.byref(self._p), _lib.ptr(on_device), host, min(lengths, self.max_tokens) if isinstance(lengths, int) else 0, mask)
+        self._nothing_to_write()
         if known is not None:
             for b in meant:
                 self._bounds[b] = min(self._bounds[b], known[b])
@@ -451,7 +463,7 @@ class PagedKVCache:
         new._make_rows()
         new._struct()
         new._bounds[:], new._loose = self._bounds, self._loose
-        new._grown, new._written = self._grown, set(self._written)
+        new._grown, new._written = self._grown, set(self._written)       # (what is still to be stored can be stored there)
         new._shared["used"] = self._shared["used"]
         nbytes = lib.odmkv_pages_compact_workspace_bytes(self.pages)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)

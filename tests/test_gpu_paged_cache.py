@@ -577,6 +577,38 @@ def test_what_a_tail_held_before_decides_nothing(how, dtype, L):
     _check_attend(c, [(k[0, :, :21], v[0, :, :21])], "int8", _queries(1, 1, 8, L, dtype, 60.0))
 
 
+def test_tokens_of_rows_that_have_moved_are_not_stored():
+    k, v = _rows(1, 2, 1, 10, torch.float16)
+    k, v = k.to(DEV), v.to(DEV)
+    c = _cache(2, 1, 300)
+    for move in (lambda: c.reorder([1, 0]), lambda: c.truncate(3), lambda: c.free([1])):
+        c.free()
+        c.extend(10)
+        move()
+        with pytest.raises(ValueError, match="moved or cut"):
+            c.write(0, k, v)
+    c.extend(10)
+    new = c.select([0])
+    with pytest.raises(ValueError, match="moved or cut"):
+        new.write(0, k[:1], v[:1])
+    c.write(0, k, v)                                          # (the batch that was copied has not moved)
+
+
+def test_numbers_past_32_bits_stop_at_their_end():
+    k, v = _rows(3, 2, 1, 100, torch.float16)
+    c = _filled(k, v, [100, 100], "int8", room=50)
+    q = _queries(1, 2, 4, 3, torch.float16).to(DEV)
+    far = 2 ** 32 + 5
+    none, lse = c.attend(0, q, starts=torch.tensor([far, far], device=DEV), return_lse=True)
+    assert not none.any() and bool((lse == float("-inf")).all())
+    everything = c.attend(0, q, prefix=torch.tensor([100, 100], device=DEV))
+    assert torch.equal(c.attend(0, q, prefix=torch.tensor([far, far], device=DEV)), everything)
+    c.truncate(2 ** 32)
+    c.truncate(torch.tensor([far, far], device=DEV))
+    c.extend(torch.tensor([1, 2], device=DEV), bound=far)
+    assert c.refresh() == [101, 102]
+
+
 def test_beams_of_one_length_need_no_reading_back():
     """Parents that only the device knows leave the host's bounds as they are where all rows are alike."""
     k, v = _rows(1, 4, 1, 64, torch.float16)

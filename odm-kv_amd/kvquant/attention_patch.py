@@ -201,7 +201,8 @@ def _paged_attention(paged, module, query, attention_mask, dropout, kwargs):
     window = kwargs.get("sliding_window")
     starts = None
     if attention_mask is not None:
-        starts = _paged_starts(attention_mask, query.shape[0], query.shape[2], k_len, window, getattr(module, "layer_idx", None))
+        starts = isinstance(attention_mask, torch.Tensor) and _paged_starts(attention_mask, query.shape[0], query.shape[2], k_len, window,
+                                                                            getattr(module, "layer_idx", None))
     if dropout or starts is False or kwargs.get("s_aux") is not None:
         raise RuntimeError("this call cannot be answered from the paged cache: it takes causal attention, with padding in front, a sliding window or a soft cap, "
                            "but no dropout, attention sinks as parameters or other masks")

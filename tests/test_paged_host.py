@@ -117,3 +117,11 @@ def test_the_plain_statement(kind):
         assert torch.equal(codes, codes.float().to(torch.float8_e4m3fn).double())
         # half a step of e4m3 is 2^-4 of the value, and 2^-10 below its normal numbers
         assert bool(((codes - blocks / s[..., None, None]).abs() <= torch.maximum(codes.abs() * 2.0 ** -4, torch.tensor(2.0 ** -10))).all())
+
+
+@pytest.mark.parametrize("mask", [object(), torch.ones(1, 9, dtype=torch.bool), torch.ones(1, 1, 2, 8, dtype=torch.bool), torch.ones(1, 1, 2, 9, dtype=torch.bool)],
+                         ids=["no tensor", "two dims", "another length", "not causal"])
+def test_masks_that_the_pages_cannot_answer_are_refused(mask):
+    from kvquant.attention_patch import _paged_attention
+    with pytest.raises(RuntimeError, match="cannot be answered from the paged cache"):
+        _paged_attention((None, 0, 9), None, torch.zeros(1, 2, 2, 128), mask, 0.0, {})

@@ -1,7 +1,9 @@
 // The entry of the attention over the paged 8-bit cache: its checks, how a call is cut into workgroups, the merge of partial results.
 #include "attend.h"
 
-// The shares of a row and kv-head's blocks, put together: a workgroup a query, its four wavefronts every fourth share, a lane two dims.
+// The shares of a row and kv-head's blocks, put together: out = sum_s w_s out_s / sum_s w_s, w_s = exp(lse_s - largest).  A workgroup a query, its four wavefronts every
+// fourth share, eight shares of a wavefront on their way at a time, a lane two dims.  Bound by the latency of two dependent reads: 4.0 us behind a step over 32768 tokens
+// (32 queries, 64 shares each), 7.2 for 928 queries of 64 shares (31 MB).
 #define MERGE_AHEAD 8
 
 template <int DT, bool NARROW_PARTS>

@@ -407,6 +407,41 @@ def test_many_rows_and_long_tables():
     _pages_add_up(c)
 
 
+def test_pages_past_four_gigabytes():
+    """Pages whose codes lie beyond 2^32 bytes: stored, read, attended, forked, cut and compacted."""
+    H, far = 8, 65600                                         # 65600 pages of 8 heads: 2^32 bytes and a little more, keys and values each
+    k, v = _rows(4, 2, H, 300, torch.float16)
+    c = _cache(2, H, (far + 10) * 64, pages=far + 10)
+    c.extend([far * 64, 0])                                   # (never written: what is looked at lies behind)
+    c.append(k.to(DEV), v.to(DEV), [0, 300])
+    assert int(c.table[c.slot[1], 0]) == far and far * H * 64 * 128 > 2 ** 32
+    for L in (1, 20):
+        q = _queries(L, 2, 16, L, torch.float16)
+        nothing = torch.zeros(H, 0, 128, dtype=torch.float16)
+        _check_attend(c, [(nothing, nothing), (k[1], v[1])], "int8", q, counts=torch.tensor([0, L], dtype=torch.int32))
+    c.reorder([1, 1])
+    _holds(c, 0, [(k[1], v[1])] * 2, "int8")
+    c.truncate([300, 100])
+    _holds(c, 0, [(k[1], v[1]), tuple(plain.cut(x[1], 100, "int8") for x in (k, v))], "int8")
+    _pages_add_up(c)
+    small = c.compacted()
+    del c
+    assert small.pages == 4
+    _holds(small, 0, [(k[1], v[1]), tuple(plain.cut(x[1], 100, "int8") for x in (k, v))], "int8")
+
+
+@pytest.mark.parametrize("window", [None, 200])
+def test_attend_shares_of_many_rows(window):
+    """More rows than a wavefront has lanes, whose blocks are shared out by their lengths, rows without tokens among them."""
+    B = 150
+    g = torch.Generator().manual_seed(2)
+    lengths = [0 if b % 13 == 5 else int(n) for b, n in enumerate(torch.randint(1, 900, (B,), generator=g))]
+    k, v = _rows(6, B, 1, max(lengths), torch.float16)
+    c = _filled(k, v, lengths, "int8")
+    q = _queries(3, B, 2, 1, torch.float16)
+    _check_attend(c, [(k[b, :, :n], v[b, :, :n]) for b, n in enumerate(lengths)], "int8", q, **({} if window is None else {"window": window}))
+
+
 # ------------------------------------------------------------------------------------------------ bounds, refusals, graphs
 def test_room_is_checked_before_anything_is_launched():
     c = _cache(2, 1, 200, pages=4)

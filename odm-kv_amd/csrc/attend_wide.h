@@ -13,9 +13,10 @@
 // Codes and weights are treated as in the narrow kernel: codes exact in fp16, weights rounded to it (at most 2^-11 of themselves), products and sums fp32.
 //
 // Bound by the vector instructions of the softmax (a scale, a maximum, an exponential, a sum and a conversion a score; a cap takes a second exponential and a reciprocal) beside the matrix cores, which
-// are busy 37 % of the time with a window and a cap.  2048 tokens of 32 heads over 12000: 942 TFLOP/s (a bf16 product of 8192 reaches 1429), with a bias 695; over a
+// are busy 37 % of the time with a window and a cap.  2048 tokens of 32 heads over 12000: 942 TFLOP/s (a bf16 product of 8192 reaches 1429), with a bias 740; over a
 // window of 4096 with a cap 757; 4096 over themselves 869; 29 tokens over 32768 34.9 us and 7.2 of the merge.
-// The halves of a block, each one's vector work beside the other's products, brought 905 -> 942; a bias pays for it (470 -> 530 us).
+// The halves of a block, each one's vector work beside the other's products, brought 905 -> 942; where scores have a bias, one half's vector work behind the other's is
+// faster instead (543 -> 498 us, with a cap besides 628 -> 582).
 #pragma once
 
 #include "attend.h"
@@ -29,6 +30,7 @@ template <int DT, int KIND, int MODE, int WAVES, int GROUPS>
 __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a) {
     const odmkv_pages_t& p = a.p;
     constexpr bool PLAIN = MODE == SCORES_PLAIN, HALVES = GROUPS < WAVES;
+    constexpr bool SIDE = MODE == SCORES_PLAIN || MODE == SCORES_CAPPED;      // a half's vector work beside the other half's products
     extern __shared__ __align__(16) uint8_t lds[];              // [2][keys 64 x 256 bytes, values 128 x 128 bytes]
     __shared__ int range[2][WAVES];
     __shared__ uint32_t tops[2][WAVES];
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
                 sum *= old;
 #pragma unroll
                 for (int db = 0; db < 4; ++db) acc[db] *= old;
-                if (tb == 1) {
+                if (SIDE && tb == 1) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) w[e >> 3][e & 7] = (_Float16)((float)w[e >> 3][e & 7] * old);
                 }
@@ -276,13 +278,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
             }
             sum = __fmaf_rn(z0 + z1, free_f, sum);
         };
-        // The two halves' vector work stands beside the other half's matrix work: a matrix instruction takes 32 cycles, which some eight vector instructions fill.
+        // SIDE: the two halves' vector work stands beside the other half's matrix work: a matrix instruction takes 32 cycles, which some eight vector instructions fill.
         multiply_keys(0, part);
         look_over(0, part);
         if constexpr (HALVES) {
             weigh(0);
             multiply_values(0, 2 * part);
             multiply_values(1, 2 * part + 1);
+        } else if constexpr (!SIDE) {
+            multiply_keys(1, 1);
+            look_over(1, 1);
+            weigh(0);
+            weigh(1);
+#pragma unroll
+            for (int st = 0; st < 4; ++st) multiply_values(st, st);
         } else {
             multiply_keys(1, 1);
             weigh(0);

@@ -75,8 +75,43 @@ __device__ static inline float capped(float kx, const Cap& m) {
     return __fmaf_rn(-m.twice, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(kx)), m.by);
 }
 
-// What a block's weights are multiplied by, in base 2: 2^7 times its values' scale over the largest; a block whose values are all 0 takes any.
-__device__ static inline float log2_share(float vs, float vref) { return vs > 0.0f ? 7.0f + __builtin_amdgcn_logf(vs / vref) : 7.0f; }
+// What a query's sums are relative to: weights to 2^ref, values that are weighted to 2^(ref + unit - 8).  Both are whole numbers, so that a move of either changes no
+// digit, and both are made of tokens that the query sees: what else lies in the row, and what other queries of the wavefront see, changes nothing.
+//
+// The values' operand is fp16: weights go there times 2^8 s / 2^unit, s what a code of one stands for in their block.  unit follows the largest weight times s, as ref
+// follows the largest weight, so that this one is 2^7 at least and 2^15 at most; what falls out of fp16's range beside it is 2^-33 of it and less, whatever the scales are.
+struct Sums { float ref, sum, unit; };
+#define NO_UNIT -10000.0f
+#define RISE 8.0f            // how far scores may pass the reference (base 2) before the sums are brought to a new one
+#define UNIT_RISE 7.0f       // how far weights times s may pass the unit
+
+// log2 s, as a whole number and the rest; values that are all 0 take the smallest, whose weights have no say
+struct Log2 { float whole, rest; };
+__device__ static inline Log2 log2_of(float s) {
+    const uint32_t bits = __float_as_uint(s);
+    return s > 0.0f ? Log2{(float)((int)(bits >> 23) - 127), __builtin_amdgcn_logf(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u))} : Log2{-300.0f, 0.0f};
+}
+// codes of e4m3 go up to 448, of int8 to 127: a unit of theirs is four times as much
+template <int KIND> constexpr float UNIT_OF_KIND = KIND == ODMKV_E4M3 ? 2.0f : 0.0f;
+
+// A block's weights are multiplied by 2^of.  (Where s is nothing beside the unit, 2^-64 is as good, and the weights' sum, which is freed of the factor, does not lose them.
+// The upper end is met where no token has been seen yet alone.)
+__device__ static inline float share_of_unit(const Sums& s, const Log2& u) { return __builtin_amdgcn_fmed3f((u.whole - s.unit) + (u.rest + 8.0f), -64.0f, 1000.0f); }
+// scores above this one bring the sums to a new reference, or to a new unit
+template <int KIND>
+__device__ static inline float highest(const Sums& s, const Log2& u) {
+    return s.ref + fminf(RISE, UNIT_RISE - ((u.whole - s.unit) + (u.rest + UNIT_OF_KIND<KIND>)));
+}
+// The query's largest score, and its largest score plus log2 s, where they pass what they may; what the values' sums are to be multiplied by (a power of two).
+__device__ static inline float raise(Sums& s, float most, float most_valued) {
+    const bool up = most > s.ref + RISE || most_valued - s.ref > s.unit + UNIT_RISE;
+    const float to = up ? fmaxf(s.ref, ceilf(most)) : s.ref, rise = s.ref > -INFINITY ? to - s.ref : 0.0f;
+    const float at = s.unit - rise, next = up ? fmaxf(at, ceilf(most_valued - (to > -INFINITY ? to : 0.0f))) : at;
+    s = {to, s.sum * __builtin_amdgcn_exp2f(-rise), next};
+    return __builtin_amdgcn_exp2f(at - next);
+}
+// 2^(unit - 8) x, for sums over the sum of the weights
+__device__ static inline float in_unit(const Sums& s, float x) { return __builtin_amdgcn_ldexpf(x, (int)fmaxf(s.unit - 8.0f, -500.0f)); }
 // Products to scores; never 0, so that a place that is not seen (-inf) stays that (a block whose keys are all 0 has products of 0 alone).
 __device__ static inline float scale_of(float ks, float qs) { return ks * qs != 0.0f ? ks * qs : 0x1p-120f; }
 
@@ -147,6 +182,7 @@ __device__ static inline uint32_t larger_bits(uint32_t v, bool whole_wave) {
     const auto f = [](float x, float y) { return __uint_as_float(max(__float_as_uint(x), __float_as_uint(y))); };
     return __float_as_uint(whole_wave ? wave_fold(__uint_as_float(v), f) : column_fold(__uint_as_float(v), f));
 }
+__device__ static inline float read_float(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
 __device__ static inline int wave_min_int(int v) {
     return __float_as_int(wave_fold(__int_as_float(v), [](float x, float y) { return __int_as_float(min(__float_as_int(x), __float_as_int(y))); }));
 }
@@ -202,7 +238,6 @@ __device__ static inline Share share_of(const AttendArgs& a, int at) {
 
 #define NARROW 16            // queries of a kv-head that the narrow kernel takes
 #define WIDE_WAVES 8
-#define RISE 8.0f            // how far scores may pass the reference (base 2) before the sums are brought to a new one
 
 // How a call is cut.
 struct Cut {

@@ -6,7 +6,8 @@
 // one piece of 16 bytes; and lane (n, j) takes dims 32 j .. 32 j + 31 of its token, 32 bytes that lie together.  No weight changes lanes.
 //
 // Codes are exact in fp16, queries as they are (bf16: times a power of two each), products and sums fp32; a block's scale joins the scores and, for values,
-// the weights: weights are rounded to fp16 (half a step, 2^-12 to 2^-11 of themselves) times 2^7 s / (largest s of the wavefront's blocks).
+// the weights: weights are rounded to fp16 (half a step, 2^-12 to 2^-11 of themselves) in a unit of
+// each query's own, which the tokens that it sees decide (attend.h: Sums).
 //
 // A wavefront takes every fourth (or eighth) block of its workgroup's share, its pages and scales looked up 64 at a time, the next block's keys and values requested
 // as soon as this one's are used: no tile passes through LDS, which holds what the wavefronts join at the end alone.  Bound by memory (256 bytes a token and head) and
@@ -81,13 +82,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
         qs = a.scaling * qdown * (PLAIN ? LOG2E : 1.0f);
     };
 
-    float ref = -INFINITY, sum = 0.0f, vref = 0.0f;
+    Sums sums = {-INFINITY, 0.0f, NO_UNIT};
     f32x4 acc[8];
 #pragma unroll
     for (int m = 0; m < 8; ++m) acc[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // raw products of a block to weights: x [tb][r] is token 64 block + 16 j + 4 tb + r.  Back come the weights as operands, times f = 2^log2f_.
-    const auto weigh = [&](const f32x4* dot, int block, float ks, float log2f_, f16x8* w) {
+    // raw products of a block to weights: x [tb][r] is token 64 block + 16 j + 4 tb + r.  Back come the weights as operands, in the query's unit.
+    const auto weigh = [&](const f32x4* dot, int block, float ks, const Log2& u, f16x8* w) {
         float x[16];
         const float c = scale_of(ks, qs);
         const int t0 = block * BLOCK_TOKENS + 16 * j;
@@ -120,15 +121,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
         if constexpr (PLAIN) top = top > -INFINITY ? top * c : top;
-        if (__any(top > ref + RISE)) {
-            const float to = fmaxf(ref, column_max(top)), by = to > -INFINITY ? to : 0.0f, old = __builtin_amdgcn_exp2f(ref - by);
-            ref = to;
-            sum *= old;
+        if (__any(top > highest<KIND>(sums, u))) {
+            const float most = column_max(top), old = raise(sums, most, most + (u.whole + (u.rest + UNIT_OF_KIND<KIND>)));
 #pragma unroll
             for (int m = 0; m < 8; ++m) acc[m] *= old;
         }
-        // weights times f come out of the exponential itself, the block's sum is freed of f
-        const float shift = log2f_ - (ref > -INFINITY ? ref : 0.0f);
+        // the factor comes out of the exponential itself, the block's sum is freed of it
+        const float factor = share_of_unit(sums, u), shift = factor - (sums.ref > -INFINITY ? sums.ref : 0.0f);
         float z0 = 0.0f, z1 = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
@@ -137,16 +136,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
             z0 += x[i];
             z1 += x[i + 1];
         }
-        sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-log2f_), sum);
+        sums.sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-factor), sums.sum);
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (_Float16)x[i];
-    };
-    const auto values_up_to = [&](float v) {                    // the sums' values are in units of vref from here on
-        if (v <= vref) return;
-        const float old = vref / v;
-#pragma unroll
-        for (int m = 0; m < 8; ++m) acc[m] *= old;
-        vref = v;
     };
 
     const size_t kat = (size_t)(16 * (n >> 2) + (n & 3)) * HD + 32 * j, vat = (size_t)n * BLOCK_TOKENS + 16 * j;
@@ -172,8 +164,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
         request_values(0);
         if (first_group) take_queries();
         first_group = false;
-        values_up_to(wave_max(vs_of));
-        const float f_of = log2_share(vs_of, vref);
+        const Log2 u_of = log2_of(vs_of);
 #pragma unroll 1
         for (int i = 0; i < todo; ++i) {
             f32x4 dot[4];
@@ -188,8 +179,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
             }
             if (i + 1 < todo) request_keys(i + 1);
             f16x8 w[2];
-            weigh(dot, b0 + g0 + WAVES * i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_of), i)),
-                  __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f_of), i)), w);
+            weigh(dot, b0 + g0 + WAVES * i, read_float(ks_of, i), Log2{read_float(u_of.whole, i), read_float(u_of.rest, i)}, w);
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
                 acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16<KIND>(v[m].x, v[m].y), w[0], acc[m], 0, 0, 0);
@@ -239,9 +229,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
         for (int c = 0; c < 16; ++c) top = max(top, abs_max8(v[c]));
         top = larger_bits(top, true);
         const Power pv = power_for<DT>(top);
-        if (top > 0) values_up_to(pv.down);
         f16x8 w[2];
-        weigh(dot, full, pk.down, log2_share(top > 0 ? pv.down : 0.0f, vref), w);
+        weigh(dot, full, pk.down, log2_of(top > 0 ? pv.down : 0.0f), w);
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
             acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(v[2 * m], pv.up), w[0], acc[m], 0, 0, 0);
@@ -249,13 +238,16 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
         }
     }
 
-    sum = column_sum(sum);
-    const float unit = vref * (1.0f / 128.0f);
+    // every wavefront's result, of the sum of its own weights
+    sums.sum = column_sum(sums.sum);
+    const float own_inv = sums.sum == 0.0f ? 0.0f : 1.0f / sums.sum;
 #pragma unroll
-    for (int m = 0; m < 8; ++m) *reinterpret_cast<f32x4*>(&acc_of[wave][n][16 * m + 4 * j]) = acc[m] * unit;
+    for (int m = 0; m < 8; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc_of[wave][n][16 * m + 4 * j + e] = in_unit(sums, acc[m][e] * own_inv);
     if (j == 0) {
-        ref_of[wave][n] = ref;
-        sum_of[wave][n] = sum;
+        ref_of[wave][n] = sums.ref;
+        sum_of[wave][n] = sums.sum;
     }
     __syncthreads();
     // a thread takes eight dims of a query
@@ -269,9 +261,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
     for (int e = 0; e < 8; ++e) o[e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-        const float f = __builtin_amdgcn_exp2f(ref_of[w][r] - by);
         // (a query that is not a number has a sum that is not, and a reference that may be anything)
-        total += sum_of[w][r] == 0.0f ? 0.0f : sum_of[w][r] * f;
+        const float f = sum_of[w][r] == 0.0f ? 0.0f : sum_of[w][r] * __builtin_amdgcn_exp2f(ref_of[w][r] - by);
+        total += f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = __fmaf_rn(acc_of[w][r][d + e], f, o[e]);
     }

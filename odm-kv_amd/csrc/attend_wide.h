@@ -10,7 +10,8 @@
 // and lies in LDS, the next block's codes are on their way in registers; rows of the first product are tokens as they lie, and row r of a half
 // wavefront's sixteen (8 (r / 4) + 4 half + r % 4) decides the order in which values lie in LDS: what a lane holds of the weights is
 // then its operand of the second product.  16-byte pieces of a row are moved by the row's number (xor), so that no two of eight rows meet in a bank.
-// Codes and weights are treated as in the narrow kernel: codes exact in fp16, weights rounded to it (at most 2^-11 of themselves), products and sums fp32.
+// Codes and weights are treated as in the narrow kernel: codes exact in fp16, weights rounded to it once (at most 2^-11 of themselves) in a unit of each
+// query's own, products and sums fp32.
 //
 // Bound by the vector instructions of the softmax (a scale, a maximum, an exponential, a sum and a conversion a score; a cap takes a second exponential and a reciprocal) beside the matrix cores, which
 // are busy 37 % of the time with a window and a cap.  2048 tokens of 32 heads over 12000: 942 TFLOP/s (a bf16 product of 8192 reaches 1429), with a bias 740; over a
@@ -91,20 +92,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
     const Cap cap = {a.cap * LOG2E, 2.0f * LOG2E * a.cap, 2.0f * LOG2E * inv_cap};
     const float qs = a.scaling * qdown * (PLAIN ? LOG2E : 1.0f);
 
-    float ref = -INFINITY, sum = 0.0f, vref = 0.0f;
+    Sums sums = {-INFINITY, 0.0f, NO_UNIT};
     f32x16 acc[4];                                              // dims 32 db + 8 (r / 4) + 4 half + r % 4 of query `col`
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[db][i] = 0.0f;
-
-    const auto values_up_to = [&](float v) {                    // the sums' values are in units of vref from here on
-        if (v <= vref) return;
-        const float old = vref / v;
-#pragma unroll
-        for (int db = 0; db < 4; ++db) acc[db] *= old;
-        vref = v;
-    };
 
     // ---- a block on its way: pieces of 16 codes, a token's 16 dims or a dim's 16 tokens
     constexpr int PIECES = PAGE_BYTES / 16 / THREADS;
@@ -171,7 +164,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
     const int codes = min(mine, full - b0);                     // of the blocks those that lie in pages
     if (codes > 0) request(0);
     if (WAVES == 8 && wave < 4) __builtin_amdgcn_s_setprio(2);
-    float ks_of = 0.0f, f_of = 0.0f;
+    float ks_of = 0.0f;
+    Log2 u_of = {0.0f, 0.0f};
 #pragma unroll 1
     for (int i = -1; i < mine; ++i) {
         uint8_t* buf = lds + (i & 1) * BUFFER;
@@ -181,29 +175,33 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
         if (i + 2 < codes) request(i + 2);
         if (i < 0) continue;
         const int t0 = (b0 + i) * BLOCK_TOKENS;
-        float ks, log2f_;
+        float ks;
+        Log2 u;
         if (i < codes) {
             if ((i & 63) == 0) {                                // 64 blocks' scales at a time
                 const bool in = i + lane < codes;
                 const int page = look_up(i);
                 const float vs = in ? p.vscale[scale_at(p, a.layer, page, h)] : 0.0f;
                 ks_of = in ? p.kscale[scale_at(p, a.layer, page, h)] : 0.0f;
-                values_up_to(wave_max(vs));
-                f_of = log2_share(vs, vref);
+                u_of = log2_of(vs);
             }
-            ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_of), i & 63));
-            log2f_ = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f_of), i & 63));
+            ks = read_float(ks_of, i & 63);
+            u = {read_float(u_of.whole, i & 63), read_float(u_of.rest, i & 63)};
         } else {
             ks = tail_k;
-            values_up_to(tail_v);
-            log2f_ = log2_share(tail_v, vref);
+            u = log2_of(tail_v);
         }
-        const float free_f = __builtin_amdgcn_exp2f(-log2f_);
         if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;      // (of the wavefront's own queries none sees the block)
-        const float c = scale_of(ks, qs), shift_f = log2f_;
+        const float c = scale_of(ks, qs);
         const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
         f32x16 dot[2];
         f16x8 w[4];
+        float limit, factor;                                    // what scores may reach, and what weights are multiplied by (base 2)
+        const auto look_at_unit = [&]() {
+            limit = highest<KIND>(sums, u);
+            factor = share_of_unit(sums, u);
+        };
+        look_at_unit();
         const auto multiply_keys = [&](int tb, int place) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) dot[tb][e] = 0.0f;
@@ -249,12 +247,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
 #pragma unroll
             for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
             if constexpr (PLAIN) top = top > -INFINITY ? top * c : top;      // (c is not negative: the largest product is the largest score)
-            if (__any(top > ref + RISE)) {
+            if (__any(top > limit)) {
                 const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                const float to = fmaxf(ref, fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]))), by = to > -INFINITY ? to : 0.0f;
-                const float old = __builtin_amdgcn_exp2f(ref - by);
-                ref = to;
-                sum *= old;
+                const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+                const float old = raise(sums, most, most + (u.whole + (u.rest + UNIT_OF_KIND<KIND>)));
+                look_at_unit();
 #pragma unroll
                 for (int db = 0; db < 4; ++db) acc[db] *= old;
                 if (SIDE && tb == 1) {
@@ -263,9 +260,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
                 }
             }
         };
-        // weights times f come out of the exponential itself, the block's sum is freed of f
+        // the factor comes out of the exponential itself, the block's sum is freed of it
         const auto weigh = [&](int tb) {
-            const float shift = shift_f - (ref > -INFINITY ? ref : 0.0f);
+            const float shift = factor - (sums.ref > -INFINITY ? sums.ref : 0.0f);
             float z0 = 0.0f, z1 = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
@@ -276,7 +273,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
                 w[2 * tb + (e >> 3)][e & 7] = (_Float16)p0;
                 w[2 * tb + (e >> 3)][(e & 7) + 1] = (_Float16)p1;
             }
-            sum = __fmaf_rn(z0 + z1, free_f, sum);
+            sums.sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-factor), sums.sum);
         };
         // SIDE: the two halves' vector work stands beside the other half's matrix work: a matrix instruction takes 32 cycles, which some eight vector instructions fill.
         multiply_keys(0, part);
@@ -304,29 +301,33 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
         }
     }
     if constexpr (HALVES) {                                     // the second half's sums join the first's, by way of LDS
-        float* const other = reinterpret_cast<float*>(lds) + group * 66 * 64 + lane;
+        float* const other = reinterpret_cast<float*>(lds) + group * 67 * 64 + lane;
         __syncthreads();
         if (part) {
 #pragma unroll
             for (int e = 0; e < 64; ++e) other[64 * e] = acc[e >> 4][e & 15];
-            other[64 * 64] = ref;
-            other[65 * 64] = sum;
+            other[64 * 64] = sums.ref;
+            other[65 * 64] = sums.sum;
+            other[66 * 64] = sums.unit;
         }
         __syncthreads();
         if (part) return;
-        const float to = fmaxf(ref, other[64 * 64]), by = to > -INFINITY ? to : 0.0f;
-        const float mine_by = __builtin_amdgcn_exp2f(ref - by), other_by = __builtin_amdgcn_exp2f(other[64 * 64] - by);
-        ref = to;
-        sum = __fmaf_rn(other[65 * 64], other_by, sum * mine_by);
+        const Sums theirs = {other[64 * 64], other[65 * 64], other[66 * 64]};
+        const float to = fmaxf(sums.ref, theirs.ref), by = to > -INFINITY ? to : 0.0f;
+        const auto unit_at = [&](const Sums& s) { return s.ref > -INFINITY ? s.unit + (s.ref - by) : 2.0f * NO_UNIT; };
+        const float unit = fmaxf(unit_at(sums), unit_at(theirs));
+        const float mine_by = __builtin_amdgcn_exp2f(unit_at(sums) - unit), other_by = __builtin_amdgcn_exp2f(unit_at(theirs) - unit);
+        sums = {to, __fmaf_rn(theirs.sum, __builtin_amdgcn_exp2f(theirs.ref - by), sums.sum * __builtin_amdgcn_exp2f(sums.ref - by)), unit};
 #pragma unroll
         for (int e = 0; e < 64; ++e) acc[e >> 4][e & 15] = __fmaf_rn(other[64 * e], other_by, acc[e >> 4][e & 15] * mine_by);
     }
 
-    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-    sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sums.sum), __float_as_uint(sums.sum), false, false);
+    const float sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
     if (!valid) return;
     const bool none = sum == 0.0f;
-    const float unit = none ? 0.0f : vref * (1.0f / 128.0f) / sum, lse2 = none ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
+    const float inv = none ? 0.0f : 1.0f / sum, lse2 = none ? -INFINITY : sums.ref + __builtin_amdgcn_logf(sum);
+    const auto result = [&](int db, int e) { return none ? 0.0f : in_unit(sums, acc[db][e] * inv); };
     if (a.splits > 1) {
         const size_t unit_at = ((size_t)pair * a.splits + split) * R + r;
         float* dst = a.part_out + unit_at * HD + 4 * half;
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
             for (int g = 0; g < 4; ++g) {
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = none ? 0.0f : acc[db][4 * g + e] * unit;
+                for (int e = 0; e < 4; ++e) v[e] = result(db, 4 * g + e);
                 *reinterpret_cast<f32x4*>(dst + 32 * db + 8 * g) = v;
             }
         if (half == 0) a.part_lse[unit_at] = lse2;
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
             uint32_t v[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                v[e] = none ? 0u : (uint32_t)to_16<DT>(acc[db][4 * g + 2 * e] * unit) | (uint32_t)to_16<DT>(acc[db][4 * g + 2 * e + 1] * unit) << 16;
+                v[e] = (uint32_t)to_16<DT>(result(db, 4 * g + 2 * e)) | (uint32_t)to_16<DT>(result(db, 4 * g + 2 * e + 1)) << 16;
             *reinterpret_cast<uint2*>(dst + 32 * db + 8 * g) = make_uint2(v[0], v[1]);
         }
     if (a.lse && half == 0) a.lse[((size_t)row * a.Hq + hq) * a.L + l] = none ? -INFINITY : lse2 * LN2;

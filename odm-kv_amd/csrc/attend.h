@@ -79,30 +79,33 @@ __device__ static inline float capped(float kx, const Cap& m) {
 // digit, and both are made of tokens that the query sees: what else lies in the row, and what other queries of the wavefront see, changes nothing.
 //
 // The values' operand is fp16: weights go there times 2^8 s / 2^unit, s what a code of one stands for in their block.  unit follows the largest weight times s, as ref
-// follows the largest weight, so that this one is 2^7 at least and 2^15 at most; what falls out of fp16's range beside it is 2^-33 of it and less, whatever the scales are.
+// follows the largest weight, so that this one is 2^7 to 2^15 there (e4m3, whose codes are larger: 2^5 to 2^13); a weight below fp16's normal
+// numbers is off by 2^-25, 2^-32 of that (2^-30) at the most, whatever the scales are.
 struct Sums { float ref, sum, unit; };
 #define NO_UNIT -10000.0f
 #define RISE 8.0f            // how far scores may pass the reference (base 2) before the sums are brought to a new one
 #define UNIT_RISE 7.0f       // how far weights times s may pass the unit
 
-// log2 s, as a whole number and the rest; values that are all 0 take the smallest, whose weights have no say
-struct Log2 { float whole, rest; };
+// log2 s as a whole number and the rest, the latter 8 more; and what the unit has to follow: log2 s, 2 more for e4m3, whose codes go up to 448 where int8's end at 127.
+// Values that are all 0 take the smallest, whose weights have no say.
+struct Log2 { float whole, rest8, lift; };
+template <int KIND>
 __device__ static inline Log2 log2_of(float s) {
     const uint32_t bits = __float_as_uint(s);
-    return s > 0.0f ? Log2{(float)((int)(bits >> 23) - 127), __builtin_amdgcn_logf(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u))} : Log2{-300.0f, 0.0f};
+    const float whole = s > 0.0f ? (float)((int)(bits >> 23) - 127) : -300.0f;
+    const float rest = s > 0.0f ? __builtin_amdgcn_logf(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u)) : 0.0f;
+    return {whole, rest + 8.0f, whole + (rest + (KIND == ODMKV_E4M3 ? 2.0f : 0.0f))};
 }
-// codes of e4m3 go up to 448, of int8 to 127: a unit of theirs is four times as much
-template <int KIND> constexpr float UNIT_OF_KIND = KIND == ODMKV_E4M3 ? 2.0f : 0.0f;
-
-// A block's weights are multiplied by 2^of.  (Where s is nothing beside the unit, 2^-64 is as good, and the weights' sum, which is freed of the factor, does not lose them.
-// The upper end is met where no token has been seen yet alone.)
-__device__ static inline float share_of_unit(const Sums& s, const Log2& u) { return __builtin_amdgcn_fmed3f((u.whole - s.unit) + (u.rest + 8.0f), -64.0f, 1000.0f); }
-// scores above this one bring the sums to a new reference, or to a new unit
-template <int KIND>
-__device__ static inline float highest(const Sums& s, const Log2& u) {
-    return s.ref + fminf(RISE, UNIT_RISE - ((u.whole - s.unit) + (u.rest + UNIT_OF_KIND<KIND>)));
+// What goes for a block, until the sums move: a score above `limit` moves them; scores go to weights in the unit by `shift`, whose sum is freed of 2^factor.
+// (Where s is nothing beside the unit, 2^-64 is as good, and the sum does not lose them.  The upper end is met where no token has been seen yet alone.)
+struct Terms { float limit, factor, shift; };
+__device__ static inline Terms terms_of(const Sums& s, const Log2& u) {
+    const float factor = __builtin_amdgcn_fmed3f((u.whole - s.unit) + u.rest8, -64.0f, 1000.0f);
+    return {s.ref + fminf(RISE, (s.unit + UNIT_RISE) - u.lift), factor, factor - fmaxf(s.ref, -1e30f)};
 }
 // The query's largest score, and its largest score plus log2 s, where they pass what they may; what the values' sums are to be multiplied by (a power of two).
+// Each query by itself: brought to a new reference with any other of its wavefront, a query would have bits that hang on what the others see.  (That would save a
+// move here and there: documents 83.5 us for 86.6, 2048 queries over a window 185 for 189.)
 __device__ static inline float raise(Sums& s, float most, float most_valued) {
     const bool up = most > s.ref + RISE || most_valued - s.ref > s.unit + UNIT_RISE;
     const float to = up ? fmaxf(s.ref, ceilf(most)) : s.ref, rise = s.ref > -INFINITY ? to - s.ref : 0.0f;
@@ -110,8 +113,8 @@ __device__ static inline float raise(Sums& s, float most, float most_valued) {
     s = {to, s.sum * __builtin_amdgcn_exp2f(-rise), next};
     return __builtin_amdgcn_exp2f(at - next);
 }
-// 2^(unit - 8) x, for sums over the sum of the weights
-__device__ static inline float in_unit(const Sums& s, float x) { return __builtin_amdgcn_ldexpf(x, (int)fmaxf(s.unit - 8.0f, -500.0f)); }
+// 2^(unit - 8), all that it may be
+__device__ static inline int unit_power(const Sums& s) { return (int)fmaxf(s.unit - 8.0f, -500.0f); }
 // Products to scores; never 0, so that a place that is not seen (-inf) stays that (a block whose keys are all 0 has products of 0 alone).
 __device__ static inline float scale_of(float ks, float qs) { return ks * qs != 0.0f ? ks * qs : 0x1p-120f; }
 
@@ -136,8 +139,9 @@ __device__ static inline f16x8 codes_f16(uint32_t w0, uint32_t w1) {
     return f16x8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
 }
 
-// 16-bit numbers on the fp16 matrix cores: times a power of two that takes the largest of them (its bits: `top`) to 64 .. 128 (fp16 numbers: by 2^15 at the
-// most, which loses nothing either).  Nothing that counts is lost: what falls out of fp16's range is 2^-30 of the largest and less.
+// 16-bit numbers of a token (or a query) on the fp16 matrix cores: times a power of two that takes the largest of them (its bits: `top`) to 64 .. 128 (fp16 numbers:
+// by 2^15 at the most, which loses nothing either).  Nothing that counts is lost: what falls out of fp16's range is 2^-30 of the token's largest and less.  Tokens
+// of a tail have a power each, since there may be queries that see one of them and not the others.
 struct Power { float up, down; };
 template <int DT>
 __device__ static inline Power power_for(uint32_t top) {
@@ -159,7 +163,7 @@ __device__ static inline uint32_t abs_max8(const uint4& v) {
     return max(max(abs_max_pair(v.x), abs_max_pair(v.y)), max(abs_max_pair(v.z), abs_max_pair(v.w)));
 }
 
-// the first n of eight numbers, 0 for the rest: what a tail holds behind its row's end is of tokens that are gone, and must not decide a power of two
+// the first n of eight numbers, 0 for the rest: what a tail holds behind its row's end is of tokens that are gone
 __device__ static inline uint4 first_of8(int n) {                // as a mask
     uint32_t m[4];
 #pragma unroll
@@ -167,6 +171,44 @@ __device__ static inline uint4 first_of8(int n) {                // as a mask
     return make_uint4(m[0], m[1], m[2], m[3]);
 }
 __device__ static inline uint4 masked8(const uint4& v, const uint4& m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
+
+// Powers of two tokens (a pair) of 16-bit numbers each, as power_for's, from the bits of their largest |x|.  The units' logarithms come as the numbers' own exponent
+// fields, BIAS too large.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ static inline uint32_t magnitudes(uint32_t w) { return w & 0x7fff7fffu; }
+__device__ static inline uint32_t larger_pair(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <int DT, int PAIRS>
+struct TokenPowers {
+    static constexpr bool F16 = DT == ODMKV_F16;
+    static constexpr float BIAS = F16 ? 15 + 6 : 127 + 6;
+    uint32_t up[F16 ? PAIRS : 2 * PAIRS];       // fp16: pairs of fp16 numbers; bf16: fp32 numbers
+    float log2[2 * PAIRS];
+    __device__ inline void take(int pair, uint32_t top) {
+        constexpr uint16_t SHIFT = F16 ? 10 : 7, LEAST = F16 ? 15 - 9 : 127 - 100;
+        const u16x2 e = __builtin_elementwise_max(__builtin_bit_cast(u16x2, top) >> u16x2{SHIFT, SHIFT}, u16x2{LEAST, LEAST});
+        log2[2 * pair] = (float)e[0];
+        log2[2 * pair + 1] = (float)e[1];
+        if constexpr (F16) up[pair] = __builtin_bit_cast(uint32_t, (u16x2{36, 36} - e) << u16x2{10, 10});
+        else {
+            up[2 * pair] = (260u - e[0]) << 23;
+            up[2 * pair + 1] = (260u - e[1]) << 23;
+        }
+    }
+    // the tokens of four pairs
+    __device__ inline f16x8 scaled(const uint4& v, int pair) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (F16) h[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w[i]) * __builtin_bit_cast(f16x2, up[pair + i]));
+            else h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w[i] << 16) * __uint_as_float(up[2 * (pair + i)]),
+                                                                                __uint_as_float(w[i] & 0xffff0000u) * __uint_as_float(up[2 * (pair + i) + 1])));
+        }
+        return __builtin_bit_cast(f16x8, make_uint4(h[0], h[1], h[2], h[3]));
+    }
+};
 
 // over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a query
 template <typename F>
@@ -178,9 +220,16 @@ __device__ static inline float column_fold(float v, F f) {
 }
 __device__ static inline float column_max(float v) { return column_fold(v, [](float x, float y) { return fmaxf(x, y); }); }
 __device__ static inline float column_sum(float v) { return column_fold(v, [](float x, float y) { return x + y; }); }
-__device__ static inline uint32_t larger_bits(uint32_t v, bool whole_wave) {
-    const auto f = [](float x, float y) { return __uint_as_float(max(__float_as_uint(x), __float_as_uint(y))); };
-    return __float_as_uint(whole_wave ? wave_fold(__uint_as_float(v), f) : column_fold(__uint_as_float(v), f));
+__device__ static inline uint32_t column_larger(uint32_t v) {        // of 16-bit numbers' bits
+    return __float_as_uint(column_fold(__uint_as_float(v), [](float x, float y) { return __uint_as_float(max(__float_as_uint(x), __float_as_uint(y))); }));
+}
+// over the sixteen lanes of a row
+__device__ static inline uint32_t row_fold_pair(uint32_t v) {
+    const auto of = [](uint32_t x, auto step) { return larger_pair(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(step)::value, 0xf, 0xf, false)); };
+    v = of(v, std::integral_constant<int, 0xB1>());
+    v = of(v, std::integral_constant<int, 0x4E>());
+    v = of(v, std::integral_constant<int, 0x141>());
+    return of(v, std::integral_constant<int, 0x140>());
 }
 __device__ static inline float read_float(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
 __device__ static inline int wave_min_int(int v) {

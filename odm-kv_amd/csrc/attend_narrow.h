@@ -70,7 +70,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
     float qs = 0.0f;
     const auto take_queries = [&]() {
         if constexpr (DT == ODMKV_BF16) {
-            const uint32_t top = larger_bits(max(max(abs_max8(raw[0]), abs_max8(raw[1])), max(abs_max8(raw[2]), abs_max8(raw[3]))), false);
+            const uint32_t top = column_larger(max(max(abs_max8(raw[0]), abs_max8(raw[1])), max(abs_max8(raw[2]), abs_max8(raw[3]))));
             const Power pw = power_for<DT>(top);
             qdown = pw.down;
 #pragma unroll
@@ -121,22 +121,23 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
         if constexpr (PLAIN) top = top > -INFINITY ? top * c : top;
-        if (__any(top > highest<KIND>(sums, u))) {
-            const float most = column_max(top), old = raise(sums, most, most + (u.whole + (u.rest + UNIT_OF_KIND<KIND>)));
+        Terms z = terms_of(sums, u);
+        if (__any(top > z.limit)) {
+            const float most = column_max(top), old = raise(sums, most, most + u.lift);
+            z = terms_of(sums, u);
 #pragma unroll
             for (int m = 0; m < 8; ++m) acc[m] *= old;
         }
         // the factor comes out of the exponential itself, the block's sum is freed of it
-        const float factor = share_of_unit(sums, u), shift = factor - (sums.ref > -INFINITY ? sums.ref : 0.0f);
         float z0 = 0.0f, z1 = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-            x[i] = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(x[i], c, shift) : x[i] + shift);
-            x[i + 1] = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(x[i + 1], c, shift) : x[i + 1] + shift);
+            x[i] = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(x[i], c, z.shift) : x[i] + z.shift);
+            x[i + 1] = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(x[i + 1], c, z.shift) : x[i + 1] + z.shift);
             z0 += x[i];
             z1 += x[i + 1];
         }
-        sums.sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-factor), sums.sum);
+        sums.sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-z.factor), sums.sum);
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = (_Float16)x[i];
     };
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
         request_values(0);
         if (first_group) take_queries();
         first_group = false;
-        const Log2 u_of = log2_of(vs_of);
+        const Log2 u_of = log2_of<KIND>(vs_of);
 #pragma unroll 1
         for (int i = 0; i < todo; ++i) {
             f32x4 dot[4];
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
             }
             if (i + 1 < todo) request_keys(i + 1);
             f16x8 w[2];
-            weigh(dot, b0 + g0 + WAVES * i, read_float(ks_of, i), Log2{read_float(u_of.whole, i), read_float(u_of.rest, i)}, w);
+            weigh(dot, b0 + g0 + WAVES * i, read_float(ks_of, i), Log2{read_float(u_of.whole, i), read_float(u_of.rest8, i), read_float(u_of.lift, i)}, w);
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
                 acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16<KIND>(v[m].x, v[m].y), w[0], acc[m], 0, 0, 0);
@@ -205,12 +206,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
             if (16 * (n >> 2) + (n & 3) + 4 * (c >> 2) >= held) k[c] = make_uint4(0, 0, 0, 0);
             v[c] = masked8(v[c], c & 1 ? high : low);
         }
-        Power pk = {1.0f, 1.0f};
-        if constexpr (DT == ODMKV_BF16) {                       // (fp16 keys are taken as they are)
-            uint32_t top = 0;
+        // keys by their tokens' powers (fp16 ones as they are), and the powers to the lanes that have the tokens' products
+        float up_k[4], down_k[4];
+        if constexpr (DT == ODMKV_BF16) {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) top = max(top, abs_max8(k[c]));
-            pk = power_for<DT>(larger_bits(top, true));
+            for (int tb = 0; tb < 4; ++tb) {
+                const Power pk = power_for<DT>(column_larger(max(max(abs_max8(k[4 * tb]), abs_max8(k[4 * tb + 1])), max(abs_max8(k[4 * tb + 2]), abs_max8(k[4 * tb + 3])))));
+                up_k[tb] = pk.up;
+                down_k[tb] = pk.down;
+            }
         }
         f32x4 dot[4];
 #pragma unroll
@@ -219,22 +223,55 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
                 f16x8 x;
-                if constexpr (DT == ODMKV_BF16) x = scaled_f16<DT>(k[4 * tb + kk], pk.up);
+                if constexpr (DT == ODMKV_BF16) x = scaled_f16<DT>(k[4 * tb + kk], up_k[tb]);
                 else x = __builtin_bit_cast(f16x8, k[4 * tb + kk]);
                 dot[tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[kk], dot[tb], 0, 0, 0);
             }
         }
-        uint32_t top = 0;
+        // values: the largest of a token's 128 lie in the sixteen lanes of its quarter, which have its weights as well
+        TokenPowers<DT, 8> pv;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) top = max(top, abs_max8(v[c]));
-        top = larger_bits(top, true);
-        const Power pv = power_for<DT>(top);
+        for (int x = 0; x < 8; ++x) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                const uint4& p = v[2 * m + (x >> 2)];
+                top = larger_pair(top, magnitudes((x & 3) == 0 ? p.x : (x & 3) == 1 ? p.y : (x & 3) == 2 ? p.z : p.w));
+            }
+            pv.take(x, row_fold_pair(top));
+        }
+        // scores, in base 2
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float down = DT == ODMKV_BF16 ? __shfl(down_k[i >> 2], 4 * j + (i & 3)) : 1.0f, c = scale_of(down, qs), raw = dot[i >> 2][i & 3];
+            x[i] = PLAIN ? raw * c : by_exp ? capped(raw * (c * cap.plain), cap) : inv_cap > 0.0f ? cap.by * tanh_of(raw * (c * inv_cap)) : raw * (c * LOG2E);
+            const int t = full * BLOCK_TOKENS + 16 * j + i;
+            if (!PLAIN && a.slopes) x[i] = __fmaf_rn(-slope, fabsf((float)(s.pos - t)), x[i]);
+            x[i] = t >= s.lo && t < s.hi ? x[i] : -INFINITY;
+        }
+        float top = x[0], top_v = x[0] + pv.log2[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) {
+            top = fmaxf(top, x[i]);
+            top_v = fmaxf(top_v, x[i] + pv.log2[i]);
+        }
+        const float old = raise(sums, column_max(top), column_max(top_v) - pv.BIAS);
+#pragma unroll
+        for (int m = 0; m < 8; ++m) acc[m] *= old;
+        const float by = sums.ref > -INFINITY ? sums.ref : 0.0f, shift = 8.0f - pv.BIAS - sums.unit - by;
         f16x8 w[2];
-        weigh(dot, full, pk.down, log2_of(top > 0 ? pv.down : 0.0f), w);
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            z += __builtin_amdgcn_exp2f(x[i] - by);
+            w[i >> 3][i & 7] = (_Float16)__builtin_amdgcn_exp2f(x[i] + (pv.log2[i] + shift));
+        }
+        sums.sum += z;
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
-            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(v[2 * m], pv.up), w[0], acc[m], 0, 0, 0);
-            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(scaled_f16<DT>(v[2 * m + 1], pv.up), w[1], acc[m], 0, 0, 0);
+            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pv.scaled(v[2 * m], 0), w[0], acc[m], 0, 0, 0);
+            acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pv.scaled(v[2 * m + 1], 4), w[1], acc[m], 0, 0, 0);
         }
     }
 
@@ -244,7 +281,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
 #pragma unroll
     for (int m = 0; m < 8; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc_of[wave][n][16 * m + 4 * j + e] = in_unit(sums, acc[m][e] * own_inv);
+        for (int e = 0; e < 4; ++e) acc_of[wave][n][16 * m + 4 * j + e] = __builtin_amdgcn_ldexpf(acc[m][e] * own_inv, unit_power(sums));
     if (j == 0) {
         ref_of[wave][n] = sums.ref;
         sum_of[wave][n] = sums.sum;

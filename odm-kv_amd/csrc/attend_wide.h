@@ -17,7 +17,7 @@
 // are busy 37 % of the time with a window and a cap.  2048 tokens of 32 heads over 12000: 942 TFLOP/s (a bf16 product of 8192 reaches 1429), with a bias 740; over a
 // window of 4096 with a cap 757; 4096 over themselves 869; 29 tokens over 32768 34.9 us and 7.2 of the merge.
 // The halves of a block, each one's vector work beside the other's products, brought 905 -> 942; where scores have a bias, one half's vector work behind the other's is
-// faster instead (543 -> 498 us, with a cap besides 628 -> 582).
+// faster instead, both halves' scores under one look for a new reference (543 -> 479 us).
 #pragma once
 
 #include "attend.h"
@@ -34,7 +34,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
     constexpr bool SIDE = MODE == SCORES_PLAIN || MODE == SCORES_CAPPED;      // a half's vector work beside the other half's products
     extern __shared__ __align__(16) uint8_t lds[];              // [2][keys 64 x 256 bytes, values 128 x 128 bytes]
     __shared__ int range[2][WAVES];
-    __shared__ uint32_t tops[2][WAVES];
+    // of the tail's tokens: pairs of largest values by wavefront; what their keys' products are multiplied by, and log2 of their values' unit
+    __shared__ uint32_t tops[WAVES][BLOCK_TOKENS / 2];
+    __shared__ __align__(16) float tail_down[BLOCK_TOKENS], tail_log2[BLOCK_TOKENS];
     constexpr int THREADS = WAVES * 64, BUFFER = BLOCK_TOKENS * HD * 4, VALUES = BLOCK_TOKENS * HD * 2;
     const int pairs = p.rows * p.Hkv, R = a.G * a.L, tiles = (R + 32 * GROUPS - 1) / (32 * GROUPS);
     // heads vary fastest (a die of the chip then keeps few heads' pages in its L2), the longest rows of blocks come first
@@ -125,49 +127,75 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
             *reinterpret_cast<f16x8*>(value_piece(buf, i >> 2, 2 * (i & 3) + 1)) = codes_f16<KIND>(vc[c].y, vc[c].w);
         }
     };
-    float tail_k = 1.0f, tail_v = 0.0f;                         // what the open block's numbers in LDS are to be multiplied by
     const auto put_tail = [&](uint8_t* buf) {
         const uint4* kt = reinterpret_cast<const uint4*>(p.ktail + tail_at(p, a.layer, slot, h));
         const uint4* vt = reinterpret_cast<const uint4*>(p.vtail + tail_at(p, a.layer, slot, h));
         const int held = len - full * BLOCK_TOKENS;
         const auto keys_of = [&](int i) { return i >> 4 < held ? kt[i] : make_uint4(0, 0, 0, 0); };
         const auto values_of = [&](int i) { return masked8(vt[i], first_of8(held - 8 * (i & 7))); };
-        uint32_t top[2] = {0, 0};
+        uint32_t top[4] = {0, 0, 0, 0};                         // tokens 8 (tid % 8) + 2 x and the next
 #pragma unroll 1
         for (int i = tid; i < TAIL_ELEMS / 8; i += THREADS) {
-            top[0] = max(top[0], abs_max8(keys_of(i)));
-            top[1] = max(top[1], abs_max8(values_of(i)));
+            uint4 k = keys_of(i);
+            if constexpr (DT == ODMKV_BF16) {                   // (fp16 keys are taken as they are; a token's lie in sixteen lanes)
+                const Power pk = power_for<DT>(row_fold_pair(abs_max8(k)));
+                if ((i & 15) == 0) tail_down[i >> 4] = pk.down;
+                k = __builtin_bit_cast(uint4, scaled_f16<DT>(k, pk.up));
+            }
+            *key_piece(buf, i >> 4, i & 15) = __builtin_bit_cast(f16x8, k);
+            const uint4 v = values_of(i);
+            top[0] = larger_pair(top[0], magnitudes(v.x));
+            top[1] = larger_pair(top[1], magnitudes(v.y));
+            top[2] = larger_pair(top[2], magnitudes(v.z));
+            top[3] = larger_pair(top[3], magnitudes(v.w));
         }
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint32_t t = larger_bits(top[x], true);
-            if (lane == 0) tops[x][wave] = t;
+        for (int x = 0; x < 4; ++x) {
+#pragma unroll
+            for (int d = 8; d < 64; d <<= 1) top[x] = larger_pair(top[x], __shfl_xor(top[x], d));
+            if (lane < 8) tops[wave][4 * lane + x] = top[x];
         }
         __syncthreads();
+        TokenPowers<DT, 4> pv;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < 4; ++x) {
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) top[x] = max(top[x], tops[x][w]);
-        const Power pk = power_for<DT>(top[0]), pv = power_for<DT>(top[1]);
-        tail_k = pk.down;
-        tail_v = top[1] > 0 ? pv.down : 0.0f;
+            for (int w = 0; w < WAVES; ++w) top[x] = larger_pair(top[x], tops[w][4 * (tid & 7) + x]);
+            pv.take(x, top[x]);
+            if (tid < 8) {
+                tail_log2[8 * tid + 2 * x] = pv.log2[2 * x] - pv.BIAS;
+                tail_log2[8 * tid + 2 * x + 1] = pv.log2[2 * x + 1] - pv.BIAS;
+            }
+        }
 #pragma unroll 1
         for (int i = tid; i < TAIL_ELEMS / 8; i += THREADS) {
             const int dim = i >> 3, u = i & 7;
-            *key_piece(buf, i >> 4, i & 15) = scaled_f16<DT>(keys_of(i), pk.up);
-            const uint4 x = __builtin_bit_cast(uint4, scaled_f16<DT>(values_of(i), pv.up));
+            const uint4 x = __builtin_bit_cast(uint4, pv.scaled(values_of(i), 0));
             *reinterpret_cast<uint2*>(value_piece(buf, dim, u & ~1) + 8 * (u & 1)) = make_uint2(x.x, x.y);
             *reinterpret_cast<uint2*>(value_piece(buf, dim, u | 1) + 8 * (u & 1)) = make_uint2(x.z, x.w);
         }
+    };
+
+    // half a block's keys, a quarter's values
+    const auto keys_times_queries = [&](uint8_t* buf, f32x16& x, int place) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll
+        for (int st = 0; st < 8; ++st) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(*key_piece(buf, 32 * place + col, 2 * st + half), q[st], x, 0, 0, 0);
+    };
+    const auto values_times_weights = [&](uint8_t* buf, const f16x8& w, int place) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+            acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(value_piece(buf, 32 * db + col, 2 * place + half)), w, acc[db], 0, 0, 0);
     };
 
     const int codes = min(mine, full - b0);                     // of the blocks those that lie in pages
     if (codes > 0) request(0);
     if (WAVES == 8 && wave < 4) __builtin_amdgcn_s_setprio(2);
     float ks_of = 0.0f;
-    Log2 u_of = {0.0f, 0.0f};
+    Log2 u_of = {0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-    for (int i = -1; i < mine; ++i) {
+    for (int i = -1; i < codes; ++i) {
         uint8_t* buf = lds + (i & 1) * BUFFER;
         __syncthreads();                                        // this block lies there, and nobody reads the one before any more
         if (i + 1 < codes) put(lds + ((i + 1) & 1) * BUFFER);
@@ -175,47 +203,24 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
         if (i + 2 < codes) request(i + 2);
         if (i < 0) continue;
         const int t0 = (b0 + i) * BLOCK_TOKENS;
-        float ks;
-        Log2 u;
-        if (i < codes) {
-            if ((i & 63) == 0) {                                // 64 blocks' scales at a time
-                const bool in = i + lane < codes;
-                const int page = look_up(i);
-                const float vs = in ? p.vscale[scale_at(p, a.layer, page, h)] : 0.0f;
-                ks_of = in ? p.kscale[scale_at(p, a.layer, page, h)] : 0.0f;
-                u_of = log2_of(vs);
-            }
-            ks = read_float(ks_of, i & 63);
-            u = {read_float(u_of.whole, i & 63), read_float(u_of.rest, i & 63)};
-        } else {
-            ks = tail_k;
-            u = log2_of(tail_v);
+        if ((i & 63) == 0) {                                    // 64 blocks' scales at a time
+            const bool in = i + lane < codes;
+            const int page = look_up(i);
+            ks_of = in ? p.kscale[scale_at(p, a.layer, page, h)] : 0.0f;
+            u_of = log2_of<KIND>(in ? p.vscale[scale_at(p, a.layer, page, h)] : 0.0f);
         }
+        const float ks = read_float(ks_of, i & 63);
+        const Log2 u = {read_float(u_of.whole, i & 63), read_float(u_of.rest8, i & 63), read_float(u_of.lift, i & 63)};
         if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;      // (of the wavefront's own queries none sees the block)
         const float c = scale_of(ks, qs);
         const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
         f32x16 dot[2];
         f16x8 w[4];
-        float limit, factor;                                    // what scores may reach, and what weights are multiplied by (base 2)
-        const auto look_at_unit = [&]() {
-            limit = highest<KIND>(sums, u);
-            factor = share_of_unit(sums, u);
-        };
-        look_at_unit();
-        const auto multiply_keys = [&](int tb, int place) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dot[tb][e] = 0.0f;
-#pragma unroll
-            for (int st = 0; st < 8; ++st)
-                dot[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*key_piece(buf, 32 * place + col, 2 * st + half), q[st], dot[tb], 0, 0, 0);
-        };
-        const auto multiply_values = [&](int st, int place) {
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(value_piece(buf, 32 * db + col, 2 * place + half)), w[st], acc[db], 0, 0, 0);
-        };
-        // products of half a block to scores, and the reference where it is to rise (what has been summed up, and weights that have not, come to the new one)
-        const auto look_over = [&](int tb, int place) {
+        Terms z = terms_of(sums, u);
+        const auto multiply_keys = [&](int tb, int place) { keys_times_queries(buf, dot[tb], place); };
+        const auto multiply_values = [&](int st, int place) { values_times_weights(buf, w[st], place); };
+        // products of half a block to scores (PLAIN: they stay products); the largest score
+        const auto to_scores = [&](int tb, int place) {
             f32x16& x = dot[tb];
             const int tl = t0 + 32 * place + 4 * half;             // token of score e: tl + 8 (e / 4) + e % 4
             if constexpr (!PLAIN) {
@@ -246,58 +251,103 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
             float top = x[0];
 #pragma unroll
             for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-            if constexpr (PLAIN) top = top > -INFINITY ? top * c : top;      // (c is not negative: the largest product is the largest score)
-            if (__any(top > limit)) {
+            return PLAIN && top > -INFINITY ? top * c : top;         // (c is not negative: the largest product is the largest score)
+        };
+        // the sums where a score is to move them; weights that have not been summed up come along
+        const auto move_sums = [&](float top, bool pending) {
+            if (__any(top > z.limit)) {
                 const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                 const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-                const float old = raise(sums, most, most + (u.whole + (u.rest + UNIT_OF_KIND<KIND>)));
-                look_at_unit();
+                const float old = raise(sums, most, most + u.lift);
+                z = terms_of(sums, u);
 #pragma unroll
                 for (int db = 0; db < 4; ++db) acc[db] *= old;
-                if (SIDE && tb == 1) {
+                if (pending) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) w[e >> 3][e & 7] = (_Float16)((float)w[e >> 3][e & 7] * old);
+                    for (int e = 0; e < 16; ++e) w[e >> 3][e & 7] = __builtin_amdgcn_ldexph(w[e >> 3][e & 7], (int)(__float_as_uint(old) >> 23) - 127);
                 }
             }
         };
         // the factor comes out of the exponential itself, the block's sum is freed of it
         const auto weigh = [&](int tb) {
-            const float shift = factor - (sums.ref > -INFINITY ? sums.ref : 0.0f);
             float z0 = 0.0f, z1 = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e], c, shift) : dot[tb][e] + shift);
-                const float p1 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e + 1], c, shift) : dot[tb][e + 1] + shift);
+                const float p0 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e], c, z.shift) : dot[tb][e] + z.shift);
+                const float p1 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e + 1], c, z.shift) : dot[tb][e + 1] + z.shift);
                 z0 += p0;
                 z1 += p1;
                 w[2 * tb + (e >> 3)][e & 7] = (_Float16)p0;
                 w[2 * tb + (e >> 3)][(e & 7) + 1] = (_Float16)p1;
             }
-            sums.sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-factor), sums.sum);
+            sums.sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-z.factor), sums.sum);
         };
         // SIDE: the two halves' vector work stands beside the other half's matrix work: a matrix instruction takes 32 cycles, which some eight vector instructions fill.
         multiply_keys(0, part);
-        look_over(0, part);
+        const float top = to_scores(0, part);
         if constexpr (HALVES) {
+            move_sums(top, false);
             weigh(0);
             multiply_values(0, 2 * part);
             multiply_values(1, 2 * part + 1);
         } else if constexpr (!SIDE) {
             multiply_keys(1, 1);
-            look_over(1, 1);
+            move_sums(fmaxf(top, to_scores(1, 1)), false);
             weigh(0);
             weigh(1);
 #pragma unroll
             for (int st = 0; st < 4; ++st) multiply_values(st, st);
         } else {
+            move_sums(top, false);
             multiply_keys(1, 1);
             weigh(0);
-            look_over(1, 1);
+            move_sums(to_scores(1, 1), true);
             multiply_values(0, 0);
             multiply_values(1, 1);
             weigh(1);
             multiply_values(2, 2);
             multiply_values(3, 3);
+        }
+    }
+    // the open block, last of its row: a power of two a token, a half of it behind the other
+    if (mine > 0 && codes < mine) {
+        uint8_t* buf = lds + (codes & 1) * BUFFER;
+        __syncthreads();
+        const int t0 = full * BLOCK_TOKENS;
+        const bool none_seen = t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo;
+#pragma unroll 1
+        for (int place = part; !none_seen && place < (HALVES ? part + 1 : 2); ++place) {
+            f32x16 x;
+            keys_times_queries(buf, x, place);
+            const int tl = 32 * place + 4 * half;
+            float top = -INFINITY, top_v = -INFINITY, log2_v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int at = tl + 8 * (e >> 2) + (e & 3), t = t0 + at;
+                const float c = scale_of(DT == ODMKV_BF16 ? tail_down[at] : 1.0f, qs);
+                x[e] = PLAIN ? x[e] * c : by_exp ? capped(x[e] * (c * cap.plain), cap) : inv_cap > 0.0f ? cap.by * tanh_of(x[e] * (c * inv_cap)) : x[e] * (c * LOG2E);
+                if (!PLAIN && a.slopes) x[e] = __fmaf_rn(-slope, fabsf((float)(s.pos - t)), x[e]);
+                x[e] = t >= s.lo && t < s.hi ? x[e] : -INFINITY;
+                log2_v[e] = tail_log2[at];
+                top = fmaxf(top, x[e]);
+                top_v = fmaxf(top_v, x[e] + log2_v[e]);
+            }
+            const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const auto ov = __builtin_amdgcn_permlane32_swap(__float_as_uint(top_v), __float_as_uint(top_v), false, false);
+            const float old = raise(sums, fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1])), fmaxf(__uint_as_float(ov[0]), __uint_as_float(ov[1])));
+#pragma unroll
+            for (int db = 0; db < 4; ++db) acc[db] *= old;
+            const float by = sums.ref > -INFINITY ? sums.ref : 0.0f, shift = 8.0f - sums.unit - by;
+            f16x8 w[2];
+            float z = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                z += __builtin_amdgcn_exp2f(x[e] - by);
+                w[e >> 3][e & 7] = (_Float16)__builtin_amdgcn_exp2f(x[e] + (log2_v[e] + shift));
+            }
+            sums.sum += z;
+            values_times_weights(buf, w[0], 2 * place);
+            values_times_weights(buf, w[1], 2 * place + 1);
         }
     }
     if constexpr (HALVES) {                                     // the second half's sums join the first's, by way of LDS
@@ -326,8 +376,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
     const float sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
     if (!valid) return;
     const bool none = sum == 0.0f;
-    const float inv = none ? 0.0f : 1.0f / sum, lse2 = none ? -INFINITY : sums.ref + __builtin_amdgcn_logf(sum);
-    const auto result = [&](int db, int e) { return none ? 0.0f : in_unit(sums, acc[db][e] * inv); };
+    float by = none ? 0.0f : 1.0f / sum;
+    const float lse2 = none ? -INFINITY : sums.ref + __builtin_amdgcn_logf(sum);
+    if (__any(sums.unit < -60.0f)) {                            // (a factor of its own, which the reciprocal need not take to where fp32 ends)
+#pragma unroll
+        for (int e = 0; e < 64; ++e) acc[e >> 4][e & 15] = __builtin_amdgcn_ldexpf(acc[e >> 4][e & 15], unit_power(sums));
+    } else by *= __builtin_amdgcn_exp2f(sums.unit - 8.0f);
+    const auto result = [&](int db, int e) { return none ? 0.0f : acc[db][e] * by; };
     if (a.splits > 1) {
         const size_t unit_at = ((size_t)pair * a.splits + split) * R + r;
         float* dst = a.part_out + unit_at * HD + 4 * half;

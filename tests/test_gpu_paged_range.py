@@ -64,6 +64,31 @@ def test_values_of_another_document_change_nothing(up, dtype, L, kind):
     _check(out1[0, L // 2:], lse1[0, :, L // 2:], q[0, :, L // 2:], k[0], v[0], kind, starts=torch.tensor(at))
 
 
+@pytest.mark.parametrize("L", [3, 17, 40])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("far", [-1, 1])
+def test_tokens_of_a_tail_that_others_see_change_nothing(far, dtype, L):
+    """A tail whose tokens belong to two documents, and one whose newest tokens only the newest queries see: keys and values of either, larger or smaller."""
+    n, at = 64 * 3 + 30, 64 * 3 + 20
+    k, v = _rows(L, 1, 2, n, dtype)
+    k, v = k * 2.0 ** -2, v * 2.0 ** -2
+    by = 2.0 ** (far * FAR[dtype][1])
+    q = _queries(L, 1, 8, L, dtype)
+    for where, mine in ((slice(64 * 3, at), dict(starts=torch.tensor([at], dtype=torch.int32))), (slice(n - 1, n), {})):
+        got = []
+        for scale in (1.0, by):
+            x, w = k.clone(), v.clone()
+            x[:, :, where] *= scale
+            w[:, :, where] *= scale
+            got.append(_filled(x, w, [n], "int8").attend(0, q.to(DEV), return_lse=True, **{name: t.to(DEV) for name, t in mine.items()}))
+        last = L if mine else L - 1                           # (the newest query sees the newest token)
+        assert torch.equal(got[0][0][:, :last], got[1][0][:, :last]) and torch.equal(got[0][1][..., :last], got[1][1][..., :last])
+        if mine:
+            w = v.clone()
+            w[:, :, :at] = 0
+            _check(got[1][0][0], got[1][1][0], q[0], k[0], w[0], "int8", starts=torch.tensor(at))
+
+
 def _attend(k, v, q, kind):
     """out [L, Hq, 128] and lse [Hq, L] of one row; for a few queries among 63 more rows, so that a wavefront takes several of its blocks."""
     n, H, L = k.shape[2], k.shape[1], q.shape[2]

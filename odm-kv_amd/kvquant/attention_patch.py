@@ -195,6 +195,27 @@ def _paged_starts(mask: torch.Tensor, B: int, L: int, k_len: int, window, layer)
     return found
 
 
+# What a call over the pages answers, and what it cannot by its name; of the rest, numbers a model goes on with (positions, switches) bear on nothing, while
+# functions and tensors that are no whole numbers (a bias, a mask by another name) would be left out of the answer.
+_PAGED_ANSWERS = ("scaling", "softcap", "sliding_window", "is_causal")
+_PAGED_REFUSES = ("position_bias", "s_aux", "head_mask", "block_mask", "score_mod", "cu_seq_lens_q", "cu_seq_lens_k")
+
+
+def _paged_refuses(module, L, attention_mask, dropout, kwargs) -> bool:
+    """True where a call asks for something that the pages' attention does not do."""
+    causal = kwargs.get("is_causal")
+    if causal is None:
+        causal = getattr(module, "is_causal", True)
+    if dropout or (not causal and L > 1 and attention_mask is None):          # (a mask says by itself what is seen)
+        return True
+    for name, value in kwargs.items():
+        if value is None or name in _PAGED_ANSWERS:
+            continue
+        if name in _PAGED_REFUSES or callable(value) or (isinstance(value, torch.Tensor) and (value.is_floating_point() or value.is_complex() or value.dtype == torch.bool)):
+            return True
+    return False
+
+
 def _paged_attention(paged, module, query, attention_mask, dropout, kwargs):
     """Attention output [B, L, Hq, D] over a `PagedCache`, whose pages and tails hold the new tokens already."""
     pool, index, k_len = paged
@@ -203,9 +224,9 @@ def _paged_attention(paged, module, query, attention_mask, dropout, kwargs):
     if attention_mask is not None:
         starts = isinstance(attention_mask, torch.Tensor) and _paged_starts(attention_mask, query.shape[0], query.shape[2], k_len, window,
                                                                             getattr(module, "layer_idx", None))
-    if dropout or starts is False or kwargs.get("s_aux") is not None:
+    if starts is False or _paged_refuses(module, query.shape[2], attention_mask, dropout, kwargs):
         raise RuntimeError("this call cannot be answered from the paged cache: it takes causal attention, with padding in front, a sliding window or a soft cap, "
-                           "but no dropout, attention sinks as parameters or other masks")
+                           "but no dropout, position bias, attention sinks as parameters or other masks")
     out = pool.attend(index, query, scaling=kwargs.get("scaling"), softcap=kwargs.get("softcap"), window=window, starts=starts)
     paged_counts["paged"] += 1
     return out

@@ -1,0 +1,71 @@
+"""What the `transformers` side of the paged 8-bit cache passes on, and what it refuses: on the CPU, over a stand-in for the cache itself."""
+import pytest
+import torch
+from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+
+class _Pool:
+    """Stands for a `PagedKVCache`: notes what it is asked."""
+    batch = 1
+
+    def __init__(self):
+        self.asked = []
+
+    def attend(self, index, query, **how):
+        self.asked.append(how)
+        return torch.zeros(query.shape[0], query.shape[2], query.shape[1], 128)
+
+
+class _Module(torch.nn.Module):
+    layer_idx = 0
+    num_key_value_groups = 2
+
+
+def _tagged(n=9, L=3):
+    """Keys and values marked as the cache marks L new tokens of n."""
+    pool = _Pool()
+    k, v = (torch.zeros(1, 2, L, 128) for _ in range(2))
+    k._odmkv_paged = (pool, 0, n)
+    return pool, k, v
+
+
+def _sdpa():
+    from kvquant.attention_patch import patch_attention_functions
+    patch_attention_functions()
+    return ALL_ATTENTION_FUNCTIONS["sdpa"]
+
+
+REFUSED = {"position_bias": dict(position_bias=torch.zeros(1, 4, 3, 9)), "is_causal": dict(is_causal=False), "head_mask": dict(head_mask=torch.ones(4)),
+           "sinks": dict(s_aux=torch.zeros(4)), "some other bias": dict(alibi=torch.zeros(4, 9)), "a mask by another name": dict(block_mask=object()),
+           "a mask of another kind": dict(extra_mask=torch.ones(3, 9, dtype=torch.bool)), "packed rows": dict(cu_seq_lens_q=torch.tensor([0, 2, 3])),
+           "a score function": dict(score_mod=lambda s: s), "dropout": dict(dropout=0.1)}
+
+
+@pytest.mark.parametrize("name", sorted(REFUSED))
+def test_what_the_pages_cannot_answer_is_refused(name):
+    pool, k, v = _tagged()
+    with pytest.raises(RuntimeError, match="cannot be answered from the paged cache"):
+        _sdpa()(_Module(), torch.zeros(1, 4, 3, 128), k, v, None, **REFUSED[name])
+    assert not pool.asked
+
+
+def test_a_module_that_is_not_causal_is_refused():
+    pool, k, v = _tagged()
+    module = _Module()
+    module.is_causal = False
+    with pytest.raises(RuntimeError, match="cannot be answered from the paged cache"):
+        _sdpa()(module, torch.zeros(1, 4, 3, 128), k, v, None)
+    # one token sees all there is either way, and a mask says itself what is seen
+    pool, k, v = _tagged(L=1)
+    _sdpa()(module, torch.zeros(1, 4, 1, 128), k, v, None, is_causal=False)
+    pool, k, v = _tagged()
+    mask = (torch.arange(9) <= torch.arange(6, 9)[:, None])[None, None]
+    _sdpa()(module, torch.zeros(1, 4, 3, 128), k, v, mask)
+    assert pool.asked[0]["starts"] is None
+
+
+def test_what_does_not_bear_on_the_answer_is_passed_over():
+    pool, k, v = _tagged()
+    _sdpa()(_Module(), torch.zeros(1, 4, 3, 128), k, v, None, scaling=0.5, softcap=20.0, sliding_window=7, position_bias=None, is_causal=True, head_mask=None,
+            position_ids=torch.arange(6, 9)[None], cache_position=torch.arange(6, 9), use_cache=True, output_attentions=False)
+    assert pool.asked == [dict(scaling=0.5, softcap=20.0, window=7, starts=None)]

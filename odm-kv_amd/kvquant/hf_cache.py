@@ -109,6 +109,38 @@ def is_aliased(t: torch.Tensor) -> bool:
     return t.dim() == 4 and t.shape[2] > 1 and t.stride(2) == 0
 
 
+class PagedTokens(torch.Tensor):
+    """New tokens' keys or values as a `PagedCache` hands them out: a mark for the patched attention functions, which read everything from the pages.  They are not
+    all the keys that there are, so that whoever would compute with them (attention inside a model, an attention function that is not patched, a cast
+    or copy that leaves the mark behind) is told instead of being given the attention over the newest tokens alone."""
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        name = getattr(func, "__name__", "")
+        with torch._C.DisableTorchFunctionSubclass():
+            if name in _LOOKS or func in _FIELDS:
+                return func(*args, **(kwargs or {}))
+            if name in _KEEPS:                            # where nothing is to be done they hand the tensor itself on
+                out = func(*args, **(kwargs or {}))
+                if out is args[0]:
+                    return out
+        raise RuntimeError(f"{name}() of a PagedCache's keys or values: they are the newest tokens alone, the others lie in pages, which the attention functions that transformers "
+                           "registers read (attn_implementation=\"sdpa\"); casts, copies and attention inside the model cannot be answered")
+
+
+# what a look at a tensor is, and what may be a look
+_LOOKS = ("dim", "size", "stride", "numel", "is_contiguous", "is_floating_point", "is_complex", "data_ptr", "get_device", "element_size", "storage_offset", "__len__", "__hash__")
+_FIELDS = tuple(getattr(torch.Tensor, field).__get__ for field in ("shape", "dtype", "device", "ndim", "layout", "is_cuda", "is_cpu", "requires_grad", "grad_fn", "is_leaf", "grad"))
+_KEEPS = ("contiguous", "to", "type_as", "half", "bfloat16", "float", "cuda")
+
+
+def paged_tokens(keys: torch.Tensor, values: torch.Tensor, paged):
+    """Keys and values as `PagedTokens`, the keys with what the attention patch needs: (pool, layer, tokens of a row)."""
+    keys, values = keys.as_subclass(PagedTokens), values.as_subclass(PagedTokens)
+    keys._odmkv_paged = paged
+    return keys, values
+
+
 class PagedCacheLayer(CacheLayerMixin):
     """A model layer's part of a `PagedCache`."""
     is_sliding = False
@@ -124,7 +156,7 @@ class PagedCacheLayer(CacheLayerMixin):
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
         """Stores the new tokens.  The first ones of a row (the prompt) go back as they are, for the model's own attention in full precision; later ones go
-        back tagged, for the attention patch, which reads everything from the pages."""
+        back as `PagedTokens`, for the attention patch, which reads everything from the pages."""
         owner, T = self.owner, key_states.shape[-2]
         if self.length == 0:
             self.lazy_initialization(key_states, value_states)
@@ -133,8 +165,7 @@ class PagedCacheLayer(CacheLayerMixin):
         before, self.length = self.length, self.length + T
         if before == 0:
             return key_states, value_states
-        key_states._odmkv_paged = (owner.pool, self.index, self.length)
-        return key_states, value_states
+        return paged_tokens(key_states, value_states, (owner.pool, self.index, self.length))
 
     def get_seq_length(self) -> int:
         return self.length

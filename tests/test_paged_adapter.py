@@ -69,3 +69,22 @@ def test_what_does_not_bear_on_the_answer_is_passed_over():
     _sdpa()(_Module(), torch.zeros(1, 4, 3, 128), k, v, None, scaling=0.5, softcap=20.0, sliding_window=7, position_bias=None, is_causal=True, head_mask=None,
             position_ids=torch.arange(6, 9)[None], cache_position=torch.arange(6, 9), use_cache=True, output_attentions=False)
     assert pool.asked == [dict(scaling=0.5, softcap=20.0, window=7, starts=None)]
+
+
+def test_keys_that_lose_their_mark_are_refused():
+    """Whoever computes with the newest tokens as if they were all: a cast, a copy, another attention function, attention inside the model."""
+    from transformers.models.llama.modeling_llama import eager_attention_forward
+    from kvquant.hf_cache import paged_tokens
+    pool, q = _Pool(), torch.zeros(1, 4, 3, 128)
+    k, v = paged_tokens(torch.zeros(1, 2, 3, 128), torch.zeros(1, 2, 3, 128), (pool, 0, 9))
+    for call in (lambda: k.half(), lambda: k.to(torch.float16), lambda: k.clone(), lambda: k.transpose(1, 2).contiguous(), lambda: k[:, :, 1:], lambda: q[:, :2] @ k.transpose(2, 3),
+                 lambda: torch.cat([k, k], dim=2), lambda: torch.matmul(q[:, :2], v), lambda: v.float().half(), lambda: k.repeat_interleave(2, dim=1), lambda: k + 1,
+                 lambda: torch.nn.functional.scaled_dot_product_attention(q[:, :2], k, v), lambda: v.cpu().numpy(),
+                 lambda: eager_attention_forward(_Module(), q, k, v, None, 1.0)):
+        with pytest.raises(RuntimeError, match="PagedCache"):
+            call()
+    # looks, and steps that change nothing, leave them as they are
+    assert k.shape == (1, 2, 3, 128) and k.dtype == torch.float32 and k.device.type == "cpu" and k.dim() == 4 and k.size(2) == 3 and k.stride(3) == 1 and not k.is_cuda
+    assert k.contiguous() is k and k.to(torch.float32) is k and v.float() is v
+    _sdpa()(_Module(), q, k.contiguous(), v, None)
+    assert len(pool.asked) == 1

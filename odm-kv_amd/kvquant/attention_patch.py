@@ -9,7 +9,8 @@ Stands where the reference's kvquant/attention_patch.py:13-62 stands.  Three beh
   except for the new tokens, which the store does not hold yet when the attention function runs (the
   press appends them in its forward hook, afterwards).  Evicted tokens are absent from the store, so
   no fake keys are needed.
-* new tokens of a `PagedCache` (kvquant/hf_cache.py) attend over its pages (``PagedKVCache.attend``);
+* new tokens of a `PagedCache` (kvquant/hf_cache.py) attend over its pages (``PagedKVCache.attend``), and so does its prompt where
+  scores are capped;
 * everything else goes to the wrapped attention function as in the reference, with evicted keys
   replaced by a fake key whose weight underflows to zero (``search_hyperplane``).
 """
@@ -239,6 +240,8 @@ def _attention_patch(func):
     @functools.wraps(func)
     def wrapper(module, query, key, value, attention_mask, dropout=0.0, **kwargs):
         paged = getattr(key, "_odmkv_paged", None)       # new tokens of a PagedCache, which holds them and all before them
+        if paged is None and kwargs.get("softcap") is not None:
+            paged = getattr(key, "_odmkv_prompt", None)  # a prompt that such a cache holds: "sdpa" would leave the cap out
         if paged is not None:
             return _paged_attention(paged, module, query, attention_mask, dropout, kwargs), None
         # a decode step like the layer's last one: the native block checks the call, stores the token and attends

@@ -155,7 +155,8 @@ class PagedCacheLayer(CacheLayerMixin):
         self.is_initialized = True
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
-        """Stores the new tokens.  The first ones of a row (the prompt) go back as they are, for the model's own attention in full precision; later ones go
+        """Stores the new tokens.  The first ones of a row (the prompt) go back as they are, for the model's own attention in full precision, unless that caps scores, which
+        the registered functions that a model would use here leave out in silence (a call with `softcap` finds its way by the mark); these and all later ones go
         back as `PagedTokens`, for the attention patch, which reads everything from the pages."""
         owner, T = self.owner, key_states.shape[-2]
         if self.length == 0:
@@ -163,9 +164,11 @@ class PagedCacheLayer(CacheLayerMixin):
         owner._room(self.length + T)
         owner.pool.write(self.index, key_states, value_states)
         before, self.length = self.length, self.length + T
-        if before == 0:
+        paged = (owner.pool, self.index, self.length)
+        if before == 0 and not owner.capped:
+            key_states._odmkv_prompt = paged
             return key_states, value_states
-        return paged_tokens(key_states, value_states, (owner.pool, self.index, self.length))
+        return paged_tokens(key_states, value_states, paged)
 
     def get_seq_length(self) -> int:
         return self.length
@@ -196,7 +199,7 @@ class PagedCacheLayer(CacheLayerMixin):
 class PagedCache(Cache):
     """A `transformers` cache of 8 bits a value (``kvquant.PagedKVCache``: int8 or e4m3 codes, one scale for 64 tokens of a head): pass it as
     ``past_key_values``.  The prompt is attended in the model's own precision and stored; every later token attends over the pages, soft caps and sliding
-    windows included.  Beams and samples share the pages of what they have in common: ``reorder_cache``, ``batch_repeat_interleave`` and
+    windows included.  Where scores are capped, the prompt attends over the pages as well: one cap from the first token on.  Beams and samples share the pages of what they have in common: ``reorder_cache``, ``batch_repeat_interleave`` and
     ``batch_select_indices`` copy 16-bit tails and count holders.  The pool starts at the prompt's size and is grown as rows do.
 
     `config`: the model's; its attention must be one of the registered functions (not "eager", which cannot be told to read the pages)."""
@@ -215,6 +218,7 @@ class PagedCache(Cache):
         if kind not in KINDS:
             raise ValueError(f"kind must be one of {sorted(KINDS)}, got {kind!r}")
         patch_attention_functions()
+        self.capped = getattr(text, "attn_logit_softcapping", None) is not None
         self.max_tokens = int(text.max_position_embeddings if max_tokens is None else max_tokens)
         self.kind, self.pool, self._extended = kind, None, 0
         super().__init__(layers=[PagedCacheLayer(self, i) for i in range(text.num_hidden_layers)])

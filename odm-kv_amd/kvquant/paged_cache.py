@@ -277,10 +277,11 @@ class PagedKVCache:
 
     @staticmethod
     def _rows_ok(t: torch.Tensor) -> torch.Tensor:
-        """Rows of 128 that start on 16 bytes, copied where they do not."""
-        if t.stride(3) == 1 and not any(s % 8 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0:
-            return t
-        return t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+        """Rows of 128 that start on 16 bytes, copied where they do not.  (The stride of a dimension of one means nothing, and may be any number.)"""
+        strides = [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
+        if t.stride(3) != 1 or any(s % 8 for s in strides[:3]) or t.data_ptr() % 16:
+            return t.clone(memory_format=torch.contiguous_format)
+        return t.as_strided(t.shape, (*strides[:3], 1)) if any(s % 8 for s in t.stride()[:3]) else t
 
     # ------------------------------------------------------------------ tokens out
     def read(self, layer: int = 0, tokens: Optional[int] = None, dtype: Optional[torch.dtype] = None):

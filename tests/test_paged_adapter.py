@@ -88,3 +88,21 @@ def test_keys_that_lose_their_mark_are_refused():
     assert k.contiguous() is k and k.to(torch.float32) is k and v.float() is v
     _sdpa()(_Module(), q, k.contiguous(), v, None)
     assert len(pool.asked) == 1
+
+
+def test_rows_as_the_kernels_take_them():
+    """Strides of dimensions of one mean nothing; what cannot be read 16 bytes at a time is copied."""
+    from kvquant import PagedKVCache
+    fits = PagedKVCache._rows_ok
+    whole = torch.arange(2 * 4 * 6 * 256, dtype=torch.float16).view(2, 4, 6, 256)
+    odd = torch.arange(20000, dtype=torch.float16)
+    ok = [whole[..., :128], whole[:, :, 1:2, 128:], whole.transpose(1, 2)[..., :128], whole[:1, :1, :1, :128].expand(2, 4, 5, 128), torch.zeros(2, 4, 0, 128).half()]
+    single = [odd.as_strided((2, 4, 1, 128), (1024, 128, 3, 1)), odd.as_strided((1, 4, 2, 128), (7, 128, 512, 1)), odd.as_strided((1, 1, 1, 128), (1, 5, 9, 1)),
+              odd.as_strided((2, 1, 3, 128), (1024, 130, 256, 1))]
+    copied = [odd.as_strided((2, 4, 1, 128), (1028, 128, 3, 1)), odd[1:].as_strided((2, 2, 2, 128), (512, 256, 128, 1)), whole[..., :128].transpose(2, 3).contiguous().transpose(2, 3),
+              odd[1:].as_strided((1, 1, 1, 128), (3, 5, 7, 1))]
+    for i, t in enumerate(ok + single + copied):
+        f = fits(t)
+        assert torch.equal(f, t), i
+        assert f.stride(3) == 1 and not any(s % 8 for s in f.stride()[:3]) and f.data_ptr() % 16 == 0, (i, f.stride())
+        assert (f.data_ptr() == t.data_ptr()) or i >= len(ok + single), i

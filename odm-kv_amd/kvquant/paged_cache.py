@@ -268,6 +268,12 @@ class PagedKVCache:
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
 
+    def _check_stored(self, layer: int) -> None:
+        """Raises where a layer has not stored the tokens of the last `extend`: its rows would be read with what lay in their places before."""
+        if self._grown and layer not in self._written:
+            self._check_layer(layer)
+            raise ValueError(f"layer {layer} has not stored the tokens of the last extend: write them first")
+
     def _check_tensor(self, t: torch.Tensor, what: str) -> None:
         _lib.require_gpu(t, what)
         if t.device != self.device:
@@ -287,6 +293,7 @@ class PagedKVCache:
     def read(self, layer: int = 0, tokens: Optional[int] = None, dtype: Optional[torch.dtype] = None):
         """Dense keys and values of one layer, [B, Hkv, tokens, 128] (default: the longest row's bound), 0 behind a row's length."""
         self._check_layer(layer)
+        self._check_stored(layer)
         tokens = self.max_length if tokens is None else int(tokens)
         if tokens < 0:
             raise ValueError(f"tokens must not be negative, got {tokens}")
@@ -309,6 +316,7 @@ class PagedKVCache:
         i - window + 1; hi is i + 1, or `prefix` (int32 [B]: tokens that everybody sees) where that is more, within the row.  Scores are scaling * q.k
         (default 128 ** -0.5), then softcap * tanh(x / softcap), then less slope * |i - j| (`slopes`, fp32 [Hq]).  Queries that see nothing
         get 0, and -inf for lse."""
+        self._check_stored(layer)
         if _device() == self.device.index and isinstance(query, torch.Tensor) and (softcap is None or 0.0 < softcap < math.inf) and (window is None or window >= 1):
             # (everything as the kernels take it: one native call)
             done = _native.paged_attend(_ATTEND, _ATTEND_BYTES, self._at, self.device.index, layer, query, _SCALING if scaling is None else scaling,

@@ -22,3 +22,31 @@ def test_strides_of_single_rows_mean_nothing():
     one.copy_(k[:, :, :1])
     c.write(0, one, one)
     _holds(c, 0, [tuple(torch.cat([x[0], k[0, :, :1]], dim=1) for x in (k, v))], "int8")
+
+
+def test_a_layer_that_has_not_stored_its_tokens_is_not_read():
+    k, v = _rows(1, 2, 1, 70, torch.float16)
+    k, v = k.to(DEV), v.to(DEV)
+    q = _queries(1, 2, 4, 1, torch.float16).to(DEV)
+    c = _cache(2, 1, 300, layers=2)
+    c.attend(1, q)                                            # (empty rows see nothing)
+    c.extend(70)
+    c.write(0, k, v)
+    c.attend(0, q)
+    for call in (lambda: c.attend(1, q), lambda: c.attend(1, q, return_lse=True, window=5), lambda: c.read(1), lambda: c.attend(1, q[..., ::2])):
+        with pytest.raises(ValueError, match="layer 1 has not stored"):
+            call()
+    for layer in (2, -1):
+        with pytest.raises(ValueError, match="of 2"):
+            c.attend(layer, q)
+    c.write(1, k, v)
+    assert torch.equal(c.attend(1, q), c.attend(0, q))
+    c.extend(0)                                               # (nothing to store)
+    assert torch.equal(c.attend(1, q), c.attend(0, q))
+    c.extend([0, 1])
+    small = c.compacted()
+    for cache in (c, small):
+        with pytest.raises(ValueError, match="has not stored"):
+            cache.attend(0, q)
+        cache.write(0, k[:, :, :1], v[:, :, :1])
+        cache.attend(0, q)

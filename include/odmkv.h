@@ -616,7 +616,7 @@ int odmkv_decode_attn_static(const void* q, int q_dtype, int B, int Hq, float sc
  *
  * The bookkeeping (lengths, tables, counts of a page's holders) lies on the device and is shared by all layers: no call reads
  * anything back, and calls that are captured into a graph go on from where the rows are at each replay.  A call that cannot be
- * carried out (too few pages, a row longer than its table) changes nothing but status[2], which it sets to 1; callers that
+ * carried out (too few pages, a row longer than it may be) changes nothing but status[2], which it sets to 1; callers that
  * know the lengths see to it before the call.  All calls on a cache are ordered by the caller (one stream, or events).
  */
 #define ODMKV_INT8 0
@@ -640,6 +640,7 @@ typedef struct odmkv_pages {
     int32_t* slot;                               /* device [rows] where a row's table and tail lie */
     int32_t* refs;                               /* device [pages] how many rows hold a page */
     int32_t* status;                             /* device [4]: free pages, a page below which none is free, refused, live pages */
+    int32_t max_tokens;                          /* no row may be longer (0: as long as its table holds); an extend past it is refused */
 } odmkv_pages_t;
 
 /* An empty cache: lengths 0, row b in slot b, all pages free, table and tails cleared. */

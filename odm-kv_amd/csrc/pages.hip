@@ -11,7 +11,7 @@ static int check_pages(const char* who, const odmkv_pages_t* p) {
     ODMKV_CHECK_ARG(p->kcodes && p->vcodes && p->kscale && p->vscale && p->ktail && p->vtail && p->table && p->length && p->start &&
                     p->slot && p->refs && p->status, "%s: null pointer", who);
     ODMKV_CHECK_ARG(p->layers > 0 && p->rows > 0 && p->rows <= MAX_ROWS && p->Hkv > 0 && p->Hkv <= 65535 && p->pages > 0 && p->pages < (1 << 24) &&
-                    p->blocks > 0 && p->blocks <= (1 << 24) && p->layers <= 65535, "%s: bad shape", who);
+                    p->blocks > 0 && p->blocks <= (1 << 24) && p->layers <= 65535 && p->max_tokens >= 0, "%s: bad shape", who);
     ODMKV_CHECK_ARG(p->dtype == ODMKV_F16 || p->dtype == ODMKV_BF16, "%s: bad dtype %d", who, p->dtype);
     ODMKV_CHECK_ARG(p->kind == ODMKV_INT8 || p->kind == ODMKV_E4M3, "%s: bad kind %d", who, p->kind);
     ODMKV_CHECK_ARG((((uintptr_t)p->kcodes | (uintptr_t)p->vcodes | (uintptr_t)p->ktail | (uintptr_t)p->vtail) & 15) == 0,
@@ -105,7 +105,8 @@ __global__ __launch_bounds__(BOOK_THREADS) void pages_extend_kernel(odmkv_pages_
         c = row_int(counts, tid);
         bad = c < 0 || c > max_count;
         if (bad) c = 0;
-        bad = bad || (long long)len + c > (long long)p.blocks * BLOCK_TOKENS + BLOCK_TOKENS - 1;
+        const long long held = (long long)p.blocks * BLOCK_TOKENS + BLOCK_TOKENS - 1;
+        bad = bad || (long long)len + c > (p.max_tokens > 0 ? min((long long)p.max_tokens, held) : held);
         if (!bad) need = (len + c) / BLOCK_TOKENS - len / BLOCK_TOKENS;
         first[tid] = len / BLOCK_TOKENS;
         slots[tid] = p.slot[tid];

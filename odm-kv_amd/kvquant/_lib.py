@@ -85,7 +85,8 @@ class Pages(C.Structure):
     """struct odmkv_pages of include/odmkv.h."""
     _fields_ = ([(n, C.c_int32) for n in ("layers", "rows", "Hkv", "pages", "blocks", "dtype", "kind")]
                 + [(n, C.c_void_p) for n in ("kcodes", "vcodes", "kscale", "vscale", "ktail", "vtail", "table", "length", "start", "slot",
-                                             "refs", "status")])
+                                             "refs", "status")]
+                + [("max_tokens", C.c_int32)])
 
 
 class Attend(C.Structure):

@@ -119,7 +119,7 @@ class PagedKVCache:
     def _struct(self) -> None:
         self._p = _lib.Pages(self.layers, self.batch, self.kv_heads, self.pages, self.table.shape[1], _lib._DT[self.dtype], KINDS[self.kind][0],
                              *(t.data_ptr() for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.table,
-                                                      self.length, self.start, self.slot, self.refs, self.status)))
+                                                      self.length, self.start, self.slot, self.refs, self.status)), self.max_tokens)
         self._at = C.addressof(self._p)
 
     def _sibling(self, batch: int) -> "PagedKVCache":

@@ -50,3 +50,29 @@ def test_a_layer_that_has_not_stored_its_tokens_is_not_read():
             cache.attend(0, q)
         cache.write(0, k[:, :, :1], v[:, :, :1])
         cache.attend(0, q)
+
+
+@pytest.mark.parametrize("max_tokens", [200, 256, 192])
+def test_a_replay_past_max_tokens_is_refused(max_tokens):
+    """Rows may have max_tokens, whatever their table has places for; the replay that would pass it changes nothing and is reported."""
+    c = _cache(2, 1, max_tokens, pages=20)
+    c.extend([max_tokens - 10, 3])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.extend(5)
+    for n in (max_tokens - 5, max_tokens):
+        graph.replay()
+        assert c.refresh() == [n, n - max_tokens + 13]
+    for _ in range(2):
+        graph.replay()
+        with pytest.raises(RuntimeError, match="beyond max_tokens"):
+            c.refresh()
+        assert c.refresh() == [max_tokens, 13]
+    c.truncate(max_tokens - 4, rows=[0])
+    graph.replay()
+    with pytest.raises(RuntimeError, match="beyond max_tokens"):
+        c.refresh()
+    c.truncate(max_tokens - 5, rows=[0])
+    graph.replay()
+    assert c.refresh() == [max_tokens, 18]
+    _pages_add_up(c)

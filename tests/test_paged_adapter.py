@@ -106,3 +106,10 @@ def test_rows_as_the_kernels_take_them():
         assert torch.equal(f, t), i
         assert f.stride(3) == 1 and not any(s % 8 for s in f.stride()[:3]) and f.data_ptr() % 16 == 0, (i, f.stride())
         assert (f.data_ptr() == t.data_ptr()) or i >= len(ok + single), i
+
+
+def test_a_negative_limit_of_a_row_is_refused():
+    import ctypes as C
+    from kvquant._lib import Pages, lib
+    p = Pages(2, 3, 4, 10, 5, 0, 0, *[4096] * 12, -1)
+    assert lib.odmkv_pages_init(C.byref(p), None) == -1 and "shape" in lib.odmkv_last_error().decode()

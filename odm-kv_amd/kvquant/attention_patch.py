@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import functools
 import os
+import weakref
 
 import torch
 from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
@@ -166,33 +167,41 @@ def _fused_block(state, query, key, value, attention_mask, scaling, k_len, layer
     return out.to(query.dtype).transpose(1, 2).contiguous()                      # [B, L, Hq, D]
 
 
-_paged_masks: dict = {}
+_LOOK = 1 << 24                                          # places of a mask that are looked at together
 
 
-def _paged_starts(mask: torch.Tensor, B: int, L: int, k_len: int, window, layer):
+def _paged_starts(mask: torch.Tensor, B: int, L: int, k_len: int, window, layer, looked=None):
     """The first token that each row sees (int32 [B], or None: the first), if `mask` is what a causal call over rows padded in front makes of it, else False.
-    The look waits for the device; its answer serves the layers above, as `_store_part_is_open`'s does."""
+    The look waits for the device; its answer serves the layers above, as `_store_part_is_open`'s does.  `looked`: the cache's answers, by window; they go when it
+    goes, and do not keep a mask alive."""
     version = None if mask.is_inference() else mask._version
-    hit = _paged_masks.get(window)
-    if hit is not None and hit[0] is mask and hit[1] == version and layer is not None and hit[2] is not None and layer > hit[2]:
+    hit = None if looked is None else looked.get(window)
+    if hit is not None and hit[0]() is mask and hit[1] == version and layer is not None and hit[2] is not None and layer > hit[2]:
         return hit[3]
     found = False
     if mask.dim() == 4 and mask.shape[0] in (1, B) and mask.shape[1] == 1 and mask.shape[-2] == L and mask.shape[-1] == k_len:
-        seen = mask[:, 0] if mask.dtype == torch.bool else mask[:, 0] == 0
         j = torch.arange(k_len, device=mask.device)
-        i = j[k_len - L:, None]
-        causal = j <= i if window is None else (j <= i) & (j > i - window)
+        step = max(1, _LOOK // max(k_len * mask.shape[0], 1))
+        pieces = [mask[:, 0, at:at + step] for at in range(0, max(L, 1), step)]
+
+        def seen(piece):
+            return piece if mask.dtype == torch.bool else piece == 0
         # the first token that counts: every later query sees it, unless a window has passed it by
-        any_seen = seen.any(dim=1)
-        starts = any_seen.to(torch.uint8).argmax(dim=-1)
+        starts = torch.stack([seen(piece).any(dim=1) for piece in pieces]).any(dim=0).to(torch.uint8).argmax(dim=-1)
         if window is not None:
             starts = torch.where(starts <= max(k_len - L - window + 1, 0), torch.zeros_like(starts), starts)
-        same = (seen == (causal & (j >= starts[:, None, None]))).all()
-        if mask.dtype != torch.bool:                     # what is not open is closed altogether, not biased
-            same = same & ((mask[:, 0] == 0) | (mask[:, 0] <= torch.finfo(mask.dtype).min / 2)).all()
-        if bool(same):
-            found = starts.to(torch.int32).expand(B).contiguous() if bool((starts > 0).any()) else None
-    _paged_masks[window] = (mask, version, layer, found)
+        same = torch.ones((), dtype=torch.bool, device=mask.device)
+        for n, piece in enumerate(pieces):
+            i = torch.arange(k_len - L + n * step, k_len - L + n * step + piece.shape[1], device=mask.device)[:, None]
+            causal = j <= i if window is None else (j <= i) & (j > i - window)
+            same = same & (seen(piece) == (causal & (j >= starts[:, None, None]))).all()
+            if mask.dtype != torch.bool:                 # what is not open is closed altogether, not biased
+                same = same & ((piece == 0) | (piece <= torch.finfo(mask.dtype).min / 2)).all()
+        same, padded = torch.stack([same, (starts > 0).any()]).tolist()
+        if same:
+            found = starts.to(torch.int32).expand(B).contiguous() if padded else None
+    if looked is not None:
+        looked[window] = (weakref.ref(mask), version, layer, found)
     return found
 
 
@@ -224,7 +233,7 @@ def _paged_attention(paged, module, query, attention_mask, dropout, kwargs):
     starts = None
     if attention_mask is not None:
         starts = isinstance(attention_mask, torch.Tensor) and _paged_starts(attention_mask, query.shape[0], query.shape[2], k_len, window,
-                                                                            getattr(module, "layer_idx", None))
+                                                                            getattr(module, "layer_idx", None), getattr(pool, "_looked", None))
     if starts is False or _paged_refuses(module, query.shape[2], attention_mask, dropout, kwargs):
         raise RuntimeError("this call cannot be answered from the paged cache: it takes causal attention, with padding in front, a sliding window or a soft cap, "
                            "but no dropout, position bias, attention sinks as parameters or other masks")

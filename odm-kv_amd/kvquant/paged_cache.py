@@ -112,6 +112,7 @@ class PagedKVCache:
         self._bounds = [0] * B                               # no row is longer
         self._grown, self._written = 0, set()                # tokens a row at most of the last extend, and the layers that have stored them
         self._shared["bounds"].append(self._bounds)
+        self._looked: dict = {}                              # what the attention patch has found masks to say (kvquant/attention_patch.py)
 
     def _nothing_to_write(self) -> None:
         self._grown, self._written = 0, range(self.layers)   # (rows have moved: what was to be stored is not there any more)

@@ -113,3 +113,55 @@ def test_a_negative_limit_of_a_row_is_refused():
     from kvquant._lib import Pages, lib
     p = Pages(2, 3, 4, 10, 5, 0, 0, *[4096] * 12, -1)
     assert lib.odmkv_pages_init(C.byref(p), None) == -1 and "shape" in lib.odmkv_last_error().decode()
+
+
+def _mask(B, L, k_len, starts, window=None, dtype=torch.bool):
+    i, j = torch.arange(k_len - L, k_len)[:, None], torch.arange(k_len)
+    open_ = (j <= i) & (j >= torch.tensor(starts)[:, None, None])
+    if window is not None:
+        open_ = open_ & (j > i - window)
+    open_ = open_[:, None]
+    return open_ if dtype == torch.bool else torch.where(open_, torch.zeros((), dtype=dtype), torch.full((), torch.finfo(dtype).min, dtype=dtype))
+
+
+@pytest.mark.parametrize("look", [1 << 24, 64, 1])
+@pytest.mark.parametrize("dtype", [torch.bool, torch.float16, torch.float32])
+def test_masks_are_read_piece_by_piece(dtype, look, monkeypatch):
+    from kvquant import attention_patch
+    monkeypatch.setattr(attention_patch, "_LOOK", look)
+    starts_of = attention_patch._paged_starts
+    assert starts_of(_mask(2, 5, 20, [0, 0], dtype=dtype), 2, 5, 20, None, 0) is None
+    assert starts_of(_mask(3, 5, 20, [0, 7, 17], dtype=dtype), 3, 5, 20, None, 0).tolist() == [0, 7, 17]
+    assert starts_of(_mask(3, 20, 20, [0, 7, 17], dtype=dtype), 3, 20, 20, None, 0).tolist() == [0, 7, 17]        # (queries before a row's start see nothing)
+    assert starts_of(_mask(1, 5, 20, [3], dtype=dtype), 4, 5, 20, None, 0).tolist() == [3] * 4
+    assert starts_of(_mask(2, 5, 20, [0, 14], window=4, dtype=dtype), 2, 5, 20, 4, 0).tolist() == [0, 14]
+    assert starts_of(_mask(2, 5, 20, [0, 9], window=4, dtype=dtype), 2, 5, 20, 4, 0) is None                      # (before every query's window)
+    for l, at in ((0, 3), (4, 10), (2, 17)):
+        wrong = _mask(2, 5, 20, [0, 0], dtype=dtype)
+        wrong[1, 0, l, at] = torch.finfo(dtype).min if dtype != torch.bool and wrong[1, 0, l, at] == 0 else 0 if dtype != torch.bool else not wrong[1, 0, l, at]
+        assert starts_of(wrong, 2, 5, 20, None, 0) is False
+    if dtype != torch.bool:
+        biased = _mask(1, 5, 20, [0], dtype=dtype)
+        biased[0, 0, 1, 2] = -3.0
+        assert starts_of(biased, 1, 5, 20, None, 0) is False
+
+
+def test_a_look_at_a_mask_serves_the_layers_above_and_keeps_nothing():
+    import gc
+    import weakref
+    pool, k, v = _tagged()
+    pool._looked = {}
+    mask = _mask(1, 3, 9, [2])
+    modules = [_Module() for _ in range(3)]
+    for i, module in enumerate(modules):
+        module.layer_idx = i
+        _sdpa()(module, torch.zeros(1, 4, 3, 128), k, v, mask)
+    starts = [how["starts"] for how in pool.asked]
+    assert starts[0].tolist() == [2] and starts[1] is starts[0] and starts[2] is starts[0]
+    mask[0, 0, :, 2] = False                              # (written to between forwards: looked at again)
+    _sdpa()(modules[1], torch.zeros(1, 4, 3, 128), k, v, mask)
+    assert pool.asked[-1]["starts"].tolist() == [3]
+    gone = weakref.ref(mask)
+    del mask
+    gc.collect()
+    assert gone() is None

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import weakref
 from typing import Optional, Sequence, Union
 
 import torch
@@ -98,8 +99,9 @@ class PagedKVCache:
         self.v_scale = torch.empty(self.layers, pages, self.kv_heads, dtype=torch.float32, **empty)
         self.refs = torch.empty(pages, dtype=torch.int32, **empty)
         self.status = torch.empty(4, dtype=torch.int32, **empty)
-        # what the batches over this pool share: an upper bound of the pages in use, and every batch's bounds (its own list, changed in place)
-        self._shared = {"used": 0, "bounds": []}
+        # what the batches over this pool share: an upper bound of the pages in use, every batch's bounds (its own list, changed in place), and the rows of
+        # batches that were dropped without `release`, whose pages the next call on the pool takes back
+        self._shared = {"used": 0, "bounds": [], "left": []}
 
     def _make_rows(self) -> None:
         B, H, empty = self.batch, self.kv_heads, dict(device=self.device)
@@ -122,6 +124,9 @@ class PagedKVCache:
                              *(t.data_ptr() for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.table,
                                                       self.length, self.start, self.slot, self.refs, self.status)), self.max_tokens)
         self._at = C.addressof(self._p)
+        rows = (self.k_tail, self.v_tail, self.table, self.length, self.start, self.slot)
+        self._dropped = weakref.finalize(self, self._shared["left"].append, (self._bounds, self._p, rows))
+        self._dropped.atexit = False
 
     def _sibling(self, batch: int) -> "PagedKVCache":
         new = object.__new__(PagedKVCache)
@@ -173,6 +178,7 @@ class PagedKVCache:
         call since the last refresh was refused on the device (a replayed graph that found no room, a bad index on the device)."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the cache's bounds do not settle this call, and its lengths cannot be read while a graph is captured")
+        self._take_back()
         status, lengths = self.status.tolist(), self.length.tolist()
         self._bounds[:] = lengths
         self._shared["used"] = self.pages - status[0]
@@ -181,8 +187,21 @@ class PagedKVCache:
             raise RuntimeError("a call on the paged cache was refused on the device: no free page, a row beyond max_tokens, or an index out of range")
         return lengths
 
+    def _take_back(self) -> None:
+        """The pages of batches over this pool that were dropped: freed on the current stream, as the pool's other calls."""
+        if not self._shared["left"] or torch.cuda.is_current_stream_capturing():         # (a graph would free them at every replay)
+            return
+        while self._shared["left"]:
+            bounds, p, rows = self._shared["left"].pop()
+            self._call(lib.odmkv_pages_truncate, C.byref(p), None, None, 0, None)
+            for t in rows:
+                t.record_stream(torch.cuda.current_stream(self.device))
+            self._shared["bounds"] = [b for b in self._shared["bounds"] if b is not bounds]
+        self._used_at_most()
+
     def _make_room(self, counts) -> None:
         """Raises unless rows that grow by `counts` fit; afterwards the bounds include them."""
+        self._take_back()
         for attempt in (0, 1):
             after = [n + c for n, c in zip(self._bounds, counts)]
             need = sum((c + BLOCK - 1) // BLOCK if self._loose else a // BLOCK - n // BLOCK for n, a, c in zip(self._bounds, after, counts))
@@ -388,7 +407,7 @@ class PagedKVCache:
 
     def select(self, parents) -> "PagedKVCache":
         """A batch of its own over the same pages, whose row b is a copy of this one's row parents[b]; this one's rows stay (``release`` it where it is
-        not needed).  Both batches draw on the one pool."""
+        not needed; the pages of a batch that is dropped come back with the next ``extend``, ``refresh`` or ``compacted`` over the pool).  Both batches draw on the one pool."""
         n = int(parents.shape[0]) if isinstance(parents, torch.Tensor) and parents.dim() == 1 else len(parents)
         if not 1 <= n <= MAX_ROWS:
             raise ValueError(f"a batch must be 1 to {MAX_ROWS} rows, got {n}")
@@ -452,6 +471,7 @@ class PagedKVCache:
     def release(self) -> None:
         """Frees all rows and leaves the pool to the batches that share it: this one is not used any more."""
         self.free()
+        self._dropped.detach()
         self._shared["bounds"] = [bounds for bounds in self._shared["bounds"] if bounds is not self._bounds]
 
     def _used_at_most(self) -> None:
@@ -461,6 +481,7 @@ class PagedKVCache:
     def compacted(self, pages: Optional[int] = None) -> "PagedKVCache":
         """A copy with a pool of its own of `pages` pages (default: those in use, read back from the device), in which the pages in use lie one behind the other:
         to give memory back, or to have more of it.  This cache stays as it is until it is dropped."""
+        self._take_back()
         if any(any(bounds) for bounds in self._shared["bounds"] if bounds is not self._bounds):
             raise ValueError("the pool is shared with another batch (select): its pages cannot be renumbered for this one alone")
         if pages is None or self._shared["used"] > pages:

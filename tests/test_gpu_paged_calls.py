@@ -76,3 +76,50 @@ def test_a_replay_past_max_tokens_is_refused(max_tokens):
     graph.replay()
     assert c.refresh() == [max_tokens, 18]
     _pages_add_up(c)
+
+
+@pytest.mark.parametrize("first", ["selected", "original"])
+def test_a_dropped_batch_gives_its_pages_back(first):
+    """Without `release`: its pages are free again for the other batches over the pool, which can be compacted."""
+    k, v = _rows(1, 2, 2, 200, torch.float16)
+    c = _cache(2, 2, 400, pages=8)
+    c.append(k.to(DEV), v.to(DEV), [200, 130])
+    other = c.select([0, 0, 1])
+    other.extend(64)                                          # three pages, all that are left
+    other.write(0, k[:1, :, :64].expand(3, 2, 64, 128).to(DEV), v[:1, :, :64].expand(3, 2, 64, 128).to(DEV))
+    with pytest.raises(ValueError, match="out of pages"):
+        c.extend(64)
+    if first == "selected":
+        kept, rows = c, [(k[0], v[0]), (k[1, :, :130], v[1, :, :130])]
+        del other
+    else:
+        kept, rows = other, [tuple(torch.cat([x[b, :, :n], x[0, :, :64]], dim=1) for x in (k, v)) for b, n in ((0, 200), (0, 200), (1, 130))]
+        del c, other
+    gc.collect()
+    assert kept.refresh() == [r[0].shape[1] for r in rows]
+    _pages_add_up(kept)
+    _holds(kept, 0, rows, "int8")
+    if first == "selected":                                   # (the other one holds all eight pages still)
+        kept.extend([64, 128])
+    small = kept.compacted()
+    assert small.pages == int((kept.refs > 0).sum())
+    _pages_add_up(small)
+
+
+def test_a_batch_dropped_while_a_graph_is_captured_is_left_for_later():
+    k, v = _rows(2, 1, 1, 130, torch.float16)
+    c = _filled(k, v, [130], "int8", pages=4)
+    other = c.select([0])
+    other.extend(64)
+    side = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(side):
+        del other
+        gc.collect()
+        c.extend(1)
+    for n in (131, 132):
+        side.replay()
+        torch.cuda.synchronize()
+        assert c.length.tolist() == [n]
+    assert int((c.refs > 0).sum()) == 3
+    assert c.refresh() == [132] and int((c.refs > 0).sum()) == 2
+    _pages_add_up(c)

@@ -38,6 +38,7 @@ _FAR = 2 ** 30                                # a window past everything
 _WRITE, _ATTEND, _ATTEND_BYTES = _lib.PAGES_ENTRIES
 _native = _lib._native
 _device = torch.cuda.current_device
+_capturing = torch.cuda.is_current_stream_capturing
 
 Counts = Union[int, Sequence[int], torch.Tensor]
 
@@ -327,7 +328,8 @@ class PagedKVCache:
 
     def attend(self, layer: int, query: torch.Tensor, *, scaling: Optional[float] = None, softcap: Optional[float] = None,
                slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, prefix: Optional[torch.Tensor] = None,
-               starts: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, return_lse: bool = False):
+               starts: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, return_lse: bool = False,
+               longest: Optional[int] = None):
         """Attention of the newest tokens' queries, query [B, Hq, L, 128], over one layer, which holds those tokens already -> [B, L, Hq, 128] of
         the same type, and on request lse fp32 [B, Hq, L].
 
@@ -335,12 +337,20 @@ class PagedKVCache:
         tokens lo <= j < hi: lo is its start (`starts`, int32 [B] or [B, L]: where a document or the text behind padding begins; default 0), and not before
         i - window + 1; hi is i + 1, or `prefix` (int32 [B]: tokens that everybody sees) where that is more, within the row.  Scores are scaling * q.k
         (default 128 ** -0.5), then softcap * tanh(x / softcap), then less slope * |i - j| (`slopes`, fp32 [Hq]).  Queries that see nothing
-        get 0, and -inf for lse."""
+        get 0, and -inf for lse.
+
+        `longest`: about how long the longest row is, which decides how the work is cut and nothing else (default: the host's bound, and while a graph is captured
+        max_tokens, since the rows may be that long at a replay)."""
         self._check_stored(layer)
+        if longest is None:
+            longest = self.max_tokens if _capturing() else max(self._bounds)
+        elif longest < 0:
+            raise ValueError(f"longest must not be negative, got {longest}")
+        longest = min(longest, self.max_tokens)
         if _device() == self.device.index and isinstance(query, torch.Tensor) and (softcap is None or 0.0 < softcap < math.inf) and (window is None or window >= 1):
             # (everything as the kernels take it: one native call)
             done = _native.paged_attend(_ATTEND, _ATTEND_BYTES, self._at, self.device.index, layer, query, _SCALING if scaling is None else scaling,
-                                        0.0 if softcap is None else softcap, 0 if window is None else min(window, _FAR), max(self._bounds), return_lse,
+                                        0.0 if softcap is None else softcap, 0 if window is None else min(window, _FAR), longest, return_lse,
                                         counts, slopes, prefix, starts, _lib.stream_ptr(self.device))
             if done is not None:
                 return done
@@ -365,7 +375,6 @@ class PagedKVCache:
         out = make(B, L, Hq, HEAD_DIM, dtype=query.dtype, device=self.device)
         lse = make(B, Hq, L, dtype=torch.float32, device=self.device) if return_lse else None
         if L:
-            longest = self.max_length
             nbytes = lib.odmkv_pages_attend_workspace_bytes(C.byref(self._p), Hq, L, longest)
             # (of its own for every call: two graphs that share one would race, and a graph's is the graph's)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None

@@ -123,3 +123,44 @@ def test_a_batch_dropped_while_a_graph_is_captured_is_left_for_later():
     assert int((c.refs > 0).sum()) == 3
     assert c.refresh() == [132] and int((c.refs > 0).sum()) == 2
     _pages_add_up(c)
+
+
+@pytest.mark.parametrize("L", [1, 20])
+def test_a_captured_step_is_cut_for_rows_as_long_as_they_may_become(L, monkeypatch):
+    """A graph captured over short rows and replayed over long ones shares their blocks out as an eager call does."""
+    from kvquant import paged_cache
+    cuts, native = [], paged_cache._native
+
+    class Watched:
+        paged_write = staticmethod(native.paged_write)
+
+        @staticmethod
+        def paged_attend(*args):
+            cuts.append(args[9])
+            return native.paged_attend(*args)
+
+    monkeypatch.setattr(paged_cache, "_native", Watched)
+    m, n = 70, 9000
+    k, v = _rows(3, 1, 2, n, torch.float16)
+    c = _cache(1, 2, 10000)
+    c.append(k[:, :, :m].to(DEV), v[:, :, :m].to(DEV))
+    q = _queries(1, 1, 8, L, torch.float16).to(DEV)
+    c.attend(0, q)
+    c.attend(0, q, longest=5000)
+    c.attend(0, q, longest=10 ** 6)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = c.attend(0, q, return_lse=True)
+        c.attend(0, q, longest=300)
+    assert cuts == [m, 5000, 10000, 10000, 300]
+    c.append(k[:, :, m:].to(DEV), v[:, :, m:].to(DEV))
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_lse = c.attend(0, q, return_lse=True, longest=10000)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    _check_attend(c, [(k[0], v[0])], "int8", q.cpu())
+    for bad in (lambda: c.attend(0, q, longest=-1), lambda: c.attend(0, q[..., ::2], longest=-1)):
+        with pytest.raises(ValueError):
+            bad()

@@ -673,7 +673,8 @@ int odmkv_pages_compact(const odmkv_pages_t* p, const odmkv_pages_t* to, void* w
 
 /* Attention of the newest tokens' queries over the cache: query l of row b's n (counts[b], or L) stands at position
  * i = length - n + l and sees the tokens lo <= j < hi,
- *   lo = max(0, start of l, i - window + 1 if window > 0),  hi = min(max(i + 1, prefix), length):
+ *   lo = max(0, start of l, i - window + 1 if window > 0),  hi = min(max(i + 1, prefix), length);
+ * (a query in front of the row, i < 0, where there are more queries than tokens, sees nothing, nor a prefix):
  *   x_j = scaling * q . k_j;  cap > 0: x_j = cap * tanh(x_j / cap);  slopes: x_j -= slope * |i - j|;
  *   out = sum_j softmax(x)_j v_j,  lse = log sum_j exp(x_j);  a query that sees nothing: 0 and -inf.
  * q [rows, Hq, L, 128] of the cache's dtype with element strides (multiples of 8, 16-byte aligned), row b's queries at l < n;

@@ -335,7 +335,8 @@ class PagedKVCache:
 
         Row b's query l of its n (`counts`, int32 [B]; default L, what lies behind n is neither read nor written) stands at position i = length - n + l and sees
         tokens lo <= j < hi: lo is its start (`starts`, int32 [B] or [B, L]: where a document or the text behind padding begins; default 0), and not before
-        i - window + 1; hi is i + 1, or `prefix` (int32 [B]: tokens that everybody sees) where that is more, within the row.  Scores are scaling * q.k
+        i - window + 1; hi is i + 1, or `prefix` (int32 [B]: tokens that everybody sees) where that is more, within the row; a query in front of
+        the row (i < 0: more queries than tokens) sees nothing.  Scores are scaling * q.k
         (default 128 ** -0.5), then softcap * tanh(x / softcap), then less slope * |i - j| (`slopes`, fp32 [Hq]).  Queries that see nothing
         get 0, and -inf for lse.
 

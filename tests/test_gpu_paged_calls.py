@@ -164,3 +164,16 @@ def test_a_captured_step_is_cut_for_rows_as_long_as_they_may_become(L, monkeypat
     for bad in (lambda: c.attend(0, q, longest=-1), lambda: c.attend(0, q[..., ::2], longest=-1)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("L", [3, 40])
+def test_queries_in_front_of_a_row_see_no_prefix(L):
+    """More queries than tokens: those at i < 0 see nothing, whatever the prefix is."""
+    lengths = [2, L + 70, 0]
+    k, v = _rows(L, 3, 2, L + 70, torch.float16)
+    c = _filled(k, v, lengths, "int8")
+    rows = [(k[b, :, :n], v[b, :, :n]) for b, n in enumerate(lengths)]
+    q = _queries(L, 3, 8, L, torch.float16)
+    _check_attend(c, rows, "int8", q, prefix=torch.tensor([2, 50, 7], dtype=torch.int32))
+    out, lse = c.attend(0, q.to(DEV), prefix=torch.tensor([2, 50, 7], dtype=torch.int32, device=DEV), return_lse=True)
+    assert not out[0, :L - 2].any() and bool((lse[0, :, :L - 2] == float("-inf")).all()) and bool(torch.isfinite(lse[0, :, L - 2:]).all())

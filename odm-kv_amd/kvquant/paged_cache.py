@@ -418,6 +418,8 @@ class PagedKVCache:
     def select(self, parents) -> "PagedKVCache":
         """A batch of its own over the same pages, whose row b is a copy of this one's row parents[b]; this one's rows stay (``release`` it where it is
         not needed; the pages of a batch that is dropped come back with the next ``extend``, ``refresh`` or ``compacted`` over the pool).  Both batches draw on the one pool."""
+        if _capturing():
+            raise RuntimeError("select makes a new batch, whose pages every replay of a captured one would take again: call it outside, and capture what the batch goes on with")
         n = int(parents.shape[0]) if isinstance(parents, torch.Tensor) and parents.dim() == 1 else len(parents)
         if not 1 <= n <= MAX_ROWS:
             raise ValueError(f"a batch must be 1 to {MAX_ROWS} rows, got {n}")

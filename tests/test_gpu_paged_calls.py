@@ -177,3 +177,19 @@ def test_queries_in_front_of_a_row_see_no_prefix(L):
     _check_attend(c, rows, "int8", q, prefix=torch.tensor([2, 50, 7], dtype=torch.int32))
     out, lse = c.attend(0, q.to(DEV), prefix=torch.tensor([2, 50, 7], dtype=torch.int32, device=DEV), return_lse=True)
     assert not out[0, :L - 2].any() and bool((lse[0, :, :L - 2] == float("-inf")).all()) and bool(torch.isfinite(lse[0, :, L - 2:]).all())
+
+
+def test_select_is_not_captured():
+    """Every replay would take its pages again, and lose those of the one before."""
+    k, v = _rows(2, 1, 1, 130, torch.float16)
+    c = _filled(k, v, [130], "int8")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device=DEV)
+        for parents in ([0, 0], torch.tensor([0]), torch.zeros(2, dtype=torch.int64)):
+            with pytest.raises(RuntimeError, match="captured"):
+                c.select(parents)
+    graph.replay()
+    torch.cuda.synchronize()
+    _pages_add_up(c)
+    _pages_add_up(c, c.select([0, 0]))

@@ -691,7 +691,7 @@ typedef struct odmkv_attend {
     void* workspace; size_t workspace_bytes;
     int32_t layer, L, Hq, window;
     int32_t max_length;                          /* about how long the longest row is: how the work is cut, not what is seen */
-    float scaling, cap;                          /* cap 0: none */
+    float scaling, cap;                          /* cap 0: none; 2^-100 at least otherwise */
 } odmkv_attend_t;
 size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length);
 int odmkv_pages_attend(const odmkv_attend_t* a, void* stream);

@@ -131,7 +131,7 @@ extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
     ODMKV_CHECK_ARG(d->layer >= 0 && d->layer < p.layers, "pages_attend: layer %d of %d", d->layer, p.layers);
     ODMKV_CHECK_ARG(d->Hq > 0 && d->Hq % p.Hkv == 0 && d->Hq / p.Hkv <= ODMKV_MAX_GROUP, "pages_attend: %d query heads over %d kv-heads", d->Hq, p.Hkv);
     ODMKV_CHECK_ARG(d->L >= 0 && d->L <= (1 << 26) && d->window >= 0 && d->max_length >= 0, "pages_attend: bad length");
-    ODMKV_CHECK_ARG(d->cap >= 0.0f && d->cap < INFINITY, "pages_attend: bad cap");
+    ODMKV_CHECK_ARG(d->cap == 0.0f || (d->cap >= 0x1p-100f && d->cap < INFINITY), "pages_attend: bad cap");
     if (d->L == 0) return 0;
     ODMKV_CHECK_ARG(d->q && d->out, "pages_attend: null pointer");
     ODMKV_CHECK_ARG((((uintptr_t)d->q | (uintptr_t)d->out) & 15) == 0 && ((d->q_stride_b | d->q_stride_h | d->q_stride_l) & 7) == 0,

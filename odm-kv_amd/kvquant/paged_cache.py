@@ -35,6 +35,7 @@ KINDS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 
 _SCALING = HEAD_DIM ** -0.5
 _FAR = 2 ** 30                                # a window past everything
+_LEAST_CAP = 2.0 ** -100                      # (what 32 bits make 0 of would be no cap)
 _WRITE, _ATTEND, _ATTEND_BYTES = _lib.PAGES_ENTRIES
 _native = _lib._native
 _device = torch.cuda.current_device
@@ -348,7 +349,7 @@ class PagedKVCache:
         elif longest < 0:
             raise ValueError(f"longest must not be negative, got {longest}")
         longest = min(longest, self.max_tokens)
-        if _device() == self.device.index and isinstance(query, torch.Tensor) and (softcap is None or 0.0 < softcap < math.inf) and (window is None or window >= 1):
+        if _device() == self.device.index and isinstance(query, torch.Tensor) and (softcap is None or _LEAST_CAP <= softcap < math.inf) and (window is None or window >= 1):
             # (everything as the kernels take it: one native call)
             done = _native.paged_attend(_ATTEND, _ATTEND_BYTES, self._at, self.device.index, layer, query, _SCALING if scaling is None else scaling,
                                         0.0 if softcap is None else softcap, 0 if window is None else min(window, _FAR), longest, return_lse,
@@ -362,8 +363,8 @@ class PagedKVCache:
         B, Hq, L, _ = query.shape
         if Hq == 0 or Hq % self.kv_heads or Hq // self.kv_heads > MAX_GROUP:
             raise ValueError(f"{Hq} query heads over {self.kv_heads} kv heads: groups of 1 to {MAX_GROUP} are built")
-        if softcap is not None and not 0.0 < softcap < math.inf:
-            raise ValueError(f"softcap must be positive, got {softcap}")
+        if softcap is not None and not _LEAST_CAP <= softcap < math.inf:
+            raise ValueError(f"softcap must be positive, at least 2 ** -100, got {softcap}")
         if window is not None and window < 1:
             raise ValueError(f"window must be positive, got {window}")
         scaling = _SCALING if scaling is None else float(scaling)

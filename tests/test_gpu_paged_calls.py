@@ -193,3 +193,15 @@ def test_select_is_not_captured():
     torch.cuda.synchronize()
     _pages_add_up(c)
     _pages_add_up(c, c.select([0, 0]))
+
+
+@pytest.mark.parametrize("L", [1, 20])
+def test_the_smallest_caps(L):
+    """2^-100: every token weighs the same; what is less, 0 in 32 bits among it, is refused and is not taken for no cap."""
+    k, v = _rows(2, 1, 1, 130, torch.float16)
+    c = _filled(k, v, [130], "int8")
+    q = _queries(1, 1, 4, L, torch.float16)
+    _check_attend(c, [(k[0], v[0])], "int8", q, softcap=2.0 ** -100)
+    for cap in (1e-50, 2.0 ** -101, float("nan")):
+        with pytest.raises(ValueError, match="softcap"):
+            c.attend(0, q.to(DEV), softcap=cap)

@@ -165,3 +165,13 @@ def test_a_look_at_a_mask_serves_the_layers_above_and_keeps_nothing():
     del mask
     gc.collect()
     assert gone() is None
+
+
+def test_a_cap_too_small_for_32_bits_is_refused():
+    import ctypes as C
+    from kvquant._lib import Attend, Pages, lib
+    pages = Pages(2, 3, 4, 10, 5, 0, 0, *[4096] * 12)
+    a = Attend(C.pointer(pages), 4096, 1024, 128, 1024, 4096, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 8, 0, 100, 0.1, 0.0)
+    for cap in (1e-38, 2.0 ** -101, 1e-45):
+        a.cap = cap
+        assert lib.odmkv_pages_attend(C.byref(a), None) == -1 and "cap" in lib.odmkv_last_error().decode()

@@ -75,12 +75,12 @@ __device__ static inline float capped(float kx, const Cap& m) {
     return __fmaf_rn(-m.twice, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(kx)), m.by);
 }
 
-// What a query's sums are relative to: weights to 2^ref, values that are weighted to 2^(ref + unit - 8).  Both are whole numbers, so that a move of either changes no
-// digit, and both are made of tokens that the query sees: what else lies in the row, and what other queries of the wavefront see, changes nothing.
+// What a query's sums are relative to: weights to 2^ref, values that are weighted to 2^(ref + unit - 8).  Both are made of tokens that the query sees: what else lies in the
+// row, and what other queries of the wavefront see, changes nothing.
 //
-// The values' operand is fp16: weights go there times 2^8 s / 2^unit, s what a code of one stands for in their block.  unit follows the largest weight times s, as ref
-// follows the largest weight, so that this one is 2^7 to 2^15 there (e4m3, whose codes are larger: 2^5 to 2^13); a weight below fp16's normal
-// numbers is off by 2^-25, 2^-32 of that (2^-30) at the most, whatever the scales are.
+// The values' operand is fp16: weights go there times 2^8 s / 2^unit, s what a code of one stands for in their block.  unit follows the largest weight times s, as ref follows
+// the largest weight: where it is set that one is 2^8 exactly, so that a token that outweighs the others is not rounded at all, and it may grow to 2^15 (e4m3, whose codes are
+// larger: 2^6 and 2^13).  A weight below fp16's normal numbers is off by 2^-25, 2^-33 of that (2^-31) at the most, whatever the scales are.
 struct Sums { float ref, sum, unit; };
 #define NO_UNIT -10000.0f
 #define RISE 8.0f            // how far scores may pass the reference (base 2) before the sums are brought to a new one
@@ -103,18 +103,21 @@ __device__ static inline Terms terms_of(const Sums& s, const Log2& u) {
     const float factor = __builtin_amdgcn_fmed3f((u.whole - s.unit) + u.rest8, -64.0f, 1000.0f);
     return {s.ref + fminf(RISE, (s.unit + UNIT_RISE) - u.lift), factor, factor - fmaxf(s.ref, -1e30f)};
 }
-// The query's largest score, and its largest score plus log2 s, where they pass what they may; what the values' sums are to be multiplied by (a power of two).
+// The query's largest score, and the largest score plus log2 s as a sum of two, where they pass what they may; what the values' sums are to be multiplied by.
 // Each query by itself: brought to a new reference with any other of its wavefront, a query would have bits that hang on what the others see.  (That would save a
 // move here and there: documents 83.5 us for 86.6, 2048 queries over a window 185 for 189.)
-__device__ static inline float raise(Sums& s, float most, float most_valued) {
-    const bool up = most > s.ref + RISE || most_valued - s.ref > s.unit + UNIT_RISE;
-    const float to = up ? fmaxf(s.ref, ceilf(most)) : s.ref, rise = s.ref > -INFINITY ? to - s.ref : 0.0f;
-    const float at = s.unit - rise, next = up ? fmaxf(at, ceilf(most_valued - (to > -INFINITY ? to : 0.0f))) : at;
+__device__ static inline float raise(Sums& s, float most, float valued, float lift) {
+    const bool some = s.ref > -INFINITY, up = most > s.ref + RISE || (valued - s.ref) + lift > s.unit + UNIT_RISE;
+    const float to = up ? fmaxf(s.ref, most) : s.ref, rise = some ? to - s.ref : 0.0f;
+    const float at = s.unit - rise, want = (valued - to) + lift, next = up ? (some ? fmaxf(at, want) : want) : at;
     s = {to, s.sum * __builtin_amdgcn_exp2f(-rise), next};
     return __builtin_amdgcn_exp2f(at - next);
 }
-// 2^(unit - 8), all that it may be
-__device__ static inline int unit_power(const Sums& s) { return (int)fmaxf(s.unit - 8.0f, -500.0f); }
+// 2^(unit - 8) x, all that it may be
+__device__ static inline float in_unit(const Sums& s, float x) {
+    const float power = fmaxf(s.unit - 8.0f, -500.0f), whole = floorf(power);
+    return __builtin_amdgcn_ldexpf(x * __builtin_amdgcn_exp2f(power - whole), (int)whole);
+}
 // Products to scores; never 0, so that a place that is not seen (-inf) stays that (a block whose keys are all 0 has products of 0 alone).
 __device__ static inline float scale_of(float ks, float qs) { return ks * qs != 0.0f ? ks * qs : 0x1p-120f; }
 

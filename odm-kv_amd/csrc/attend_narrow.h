@@ -123,7 +123,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
         if constexpr (PLAIN) top = top > -INFINITY ? top * c : top;
         Terms z = terms_of(sums, u);
         if (__any(top > z.limit)) {
-            const float most = column_max(top), old = raise(sums, most, most + u.lift);
+            const float most = column_max(top), old = raise(sums, most, most, u.lift);
             z = terms_of(sums, u);
 #pragma unroll
             for (int m = 0; m < 8; ++m) acc[m] *= old;
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
             top = fmaxf(top, x[i]);
             top_v = fmaxf(top_v, x[i] + pv.log2[i]);
         }
-        const float old = raise(sums, column_max(top), column_max(top_v) - pv.BIAS);
+        const float old = raise(sums, column_max(top), column_max(top_v), -pv.BIAS);
 #pragma unroll
         for (int m = 0; m < 8; ++m) acc[m] *= old;
         const float by = sums.ref > -INFINITY ? sums.ref : 0.0f, shift = 8.0f - pv.BIAS - sums.unit - by;
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
 #pragma unroll
     for (int m = 0; m < 8; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc_of[wave][n][16 * m + 4 * j + e] = __builtin_amdgcn_ldexpf(acc[m][e] * own_inv, unit_power(sums));
+        for (int e = 0; e < 4; ++e) acc_of[wave][n][16 * m + 4 * j + e] = in_unit(sums, acc[m][e] * own_inv);
     if (j == 0) {
         ref_of[wave][n] = sums.ref;
         sum_of[wave][n] = sums.sum;

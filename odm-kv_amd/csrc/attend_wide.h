@@ -253,20 +253,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
             for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
             return PLAIN && top > -INFINITY ? top * c : top;         // (c is not negative: the largest product is the largest score)
         };
-        // the sums where a score is to move them; weights that have not been summed up come along
-        const auto move_sums = [&](float top, bool pending) {
-            if (__any(top > z.limit)) {
-                const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-                const float old = raise(sums, most, most + u.lift);
-                z = terms_of(sums, u);
+        // the sums' references where a score is to move them: what the values' sums are to be multiplied by, before weights of the new ones are, and behind those of the old
+        const auto move_sums = [&](float top, float& old) {
+            if (!__any(top > z.limit)) return false;
+            const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+            old = raise(sums, most, most, u.lift);
+            z = terms_of(sums, u);
+            return true;
+        };
+        const auto multiply_sums = [&](float old) {
 #pragma unroll
-                for (int db = 0; db < 4; ++db) acc[db] *= old;
-                if (pending) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) w[e >> 3][e & 7] = __builtin_amdgcn_ldexph(w[e >> 3][e & 7], (int)(__float_as_uint(old) >> 23) - 127);
-                }
-            }
+            for (int db = 0; db < 4; ++db) acc[db] *= old;
         };
         // the factor comes out of the exponential itself, the block's sum is freed of it
         const auto weigh = [&](int tb) {
@@ -285,26 +283,28 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
         // SIDE: the two halves' vector work stands beside the other half's matrix work: a matrix instruction takes 32 cycles, which some eight vector instructions fill.
         multiply_keys(0, part);
         const float top = to_scores(0, part);
+        float old;
         if constexpr (HALVES) {
-            move_sums(top, false);
+            if (move_sums(top, old)) multiply_sums(old);
             weigh(0);
             multiply_values(0, 2 * part);
             multiply_values(1, 2 * part + 1);
         } else if constexpr (!SIDE) {
             multiply_keys(1, 1);
-            move_sums(fmaxf(top, to_scores(1, 1)), false);
+            if (move_sums(fmaxf(top, to_scores(1, 1)), old)) multiply_sums(old);
             weigh(0);
             weigh(1);
 #pragma unroll
             for (int st = 0; st < 4; ++st) multiply_values(st, st);
         } else {
-            move_sums(top, false);
+            if (move_sums(top, old)) multiply_sums(old);
             multiply_keys(1, 1);
             weigh(0);
-            move_sums(to_scores(1, 1), true);
+            const bool moved = move_sums(to_scores(1, 1), old);
             multiply_values(0, 0);
             multiply_values(1, 1);
             weigh(1);
+            if (moved) multiply_sums(old);
             multiply_values(2, 2);
             multiply_values(3, 3);
         }
@@ -334,7 +334,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
             }
             const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             const auto ov = __builtin_amdgcn_permlane32_swap(__float_as_uint(top_v), __float_as_uint(top_v), false, false);
-            const float old = raise(sums, fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1])), fmaxf(__uint_as_float(ov[0]), __uint_as_float(ov[1])));
+            const float old = raise(sums, fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1])), fmaxf(__uint_as_float(ov[0]), __uint_as_float(ov[1])), 0.0f);
 #pragma unroll
             for (int db = 0; db < 4; ++db) acc[db] *= old;
             const float by = sums.ref > -INFINITY ? sums.ref : 0.0f, shift = 8.0f - sums.unit - by;
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_wide_kernel(AttendArgs a
     const float lse2 = none ? -INFINITY : sums.ref + __builtin_amdgcn_logf(sum);
     if (__any(sums.unit < -60.0f)) {                            // (a factor of its own, which the reciprocal need not take to where fp32 ends)
 #pragma unroll
-        for (int e = 0; e < 64; ++e) acc[e >> 4][e & 15] = __builtin_amdgcn_ldexpf(acc[e >> 4][e & 15], unit_power(sums));
+        for (int e = 0; e < 64; ++e) acc[e >> 4][e & 15] = in_unit(sums, acc[e >> 4][e & 15]);
     } else by *= __builtin_amdgcn_exp2f(sums.unit - 8.0f);
     const auto result = [&](int db, int e) { return none ? 0.0f : acc[db][e] * by; };
     if (a.splits > 1) {

@@ -21,10 +21,9 @@ def _blocks_largest(v, kind):
 
 def _check(out, lse, q, k, v, kind, **how):
     """One row's out [L, Hq, 128] and lse [Hq, L] against the definition, with a bound made of what a query sees:
-    scores and their sum as in paged_rows.attend; weights rounded to fp16 (2^-11 of themselves); those below its normal numbers are off by 2^-25, and by half of that once
-    more where the reference rises between the halves of a block, in a unit in which the largest P_j s_j is 2^7 at least (s_j: what a code of one stands for, 2^-7 of the largest
-    value of its block or, in the tail, 2^-6 of its token's), the values there at most 128: 1.5 * 2^-25 * 128 * 2^-7 * 2^-6 = 3 * 2^-32 of the largest P_j V_j a token; and
-    a tail's values, in fp16 with their token's largest at 64 or more, are off by 2^-24 of that unit at the most, 2^-30 of P_j V_j."""
+    scores and their sum as in paged_rows.attend; weights rounded to fp16 (2^-11 of themselves); those below its normal numbers are off by 2^-25 at most, in
+    a unit in which the largest P_j s_j is 2^6 at least (s_j: what a code of one stands for, 2^-7 of the largest value of its block or, in the tail, 2^-6 of its token's),
+    the values there at most 128: 2^-25 * 128 * 2^-6 * 2^-6 = 2^-30 * 2^-2 and so less than 3 * 2^-32 of the largest P_j V_j a token; and a tail's values, in fp16 with their token's largest at 64 or more, are off by 2^-24 of that unit at the most, 2^-30 of P_j V_j."""
     dtype, L, m = q.dtype, q.shape[1], k.shape[1]
     held_k, held_v = plain.held(k, kind), plain.held(v, kind)
     want, wl, _, tl = plain.attend(q, held_k, held_v, **how)
@@ -162,3 +161,23 @@ def test_weights_are_rounded_once():
     assert held == 1.7457275390625 and up / held > 1 + 2.0 ** -11
     out = _filled(k.half(), v, [n], "int8").attend(0, q.half().to(DEV)).cpu().double()
     assert float(out.max()) < up, ((out > up).any(dim=-1).sum(), out.max())
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("L", [1, 3, 17, 40, 130])
+@pytest.mark.parametrize("at", [3, 40, 200, 400, 447, 500])
+def test_a_token_that_outweighs_the_others_is_rounded_once(at, L, kind):
+    """A token 2^-40 of whose weight all others have together: the outputs are what is held of its values, rounded to fp16 and nothing else but what 32 bits leave (the
+    logarithm of a scale and its power: 2^-21, by which a value half-way between two fp16 numbers may go either way).  In either half of a block and in the tail."""
+    n = 508
+    k, v = _rows(at, 1, 2, n, torch.float16)
+    k[..., 0] = 0
+    k[0, :, at, 0] = 40
+    q = _queries(L, 1, 8, L, torch.float16, size=0.7)
+    q[..., 0] = 13.7
+    out = _filled(k, v, [n], kind).attend(0, q.to(DEV))[0].cpu().double()
+    want = plain.held(v[0], kind)[:, at].repeat_interleave(4, dim=0).expand(L, 8, 128)
+    sees = torch.arange(n - L, n) >= at
+    # half a step of fp16 at each value: 2^-11 of the power of two below it, 2^-25 for the smallest
+    half = (2.0 ** (torch.frexp(want.abs()).exponent - 12).double()).clamp(min=2.0 ** -25)
+    assert bool(sees.any()) and bool(((out - want).abs()[sees] <= (half + 2.0 ** -21 * want.abs())[sees]).all()), float(((out - want).abs() / half)[sees].max())

@@ -22,14 +22,16 @@ def _blocks_largest(v, kind):
 def _check(out, lse, q, k, v, kind, **how):
     """One row's out [L, Hq, 128] and lse [Hq, L] against the definition, with a bound made of what a query sees:
     scores and their sum as in paged_rows.attend; weights rounded to fp16 (2^-11 of themselves); those below its normal numbers are off by 2^-25 at most, in
-    a unit in which the largest P_j s_j is 2^6 at least (s_j: what a code of one stands for, 2^-7 of the largest value of its block or, in the tail, 2^-6 of its token's),
-    the values there at most 128: 2^-25 * 128 * 2^-6 * 2^-6 = 2^-30 * 2^-2 and so less than 3 * 2^-32 of the largest P_j V_j a token; and a tail's values, in fp16 with their token's largest at 64 or more, are off by 2^-24 of that unit at the most, 2^-30 of P_j V_j."""
+    a unit in which the largest P_j s_j is 2^8, and 2^6 in a block of e4m3 codes (s_j: what a code of one stands for, V_j / 127, V_j / 448, or in the tail V_j / 64 at most, V_j
+    the largest value of the block or the tail's token), times codes of at most 127, 448 and 128: the worst is a code of 448 beside a largest P_j V_j in the tail,
+    2^-25 * 448 * 2^-8 / 64 = 3.5 * 2^-32 of it, for every token.  A tail's values, in fp16 with their token's largest at 64 or more, are off by 2^-24 of that unit at the
+    most, 2^-30 of P_j V_j."""
     dtype, L, m = q.dtype, q.shape[1], k.shape[1]
     held_k, held_v = plain.held(k, kind), plain.held(v, kind)
     want, wl, _, tl = plain.attend(q, held_k, held_v, **how)
     mass = plain.attend(q, held_k, held_v.abs(), **how)[0]
     large = plain.attend(q, held_k, _blocks_largest(held_v, kind).expand_as(held_v), **how)[0]
-    tol = (2 * tl.T[..., None] + 2.0 ** -11 + 2 * m * 2.0 ** -24) * mass + (3 * m + 4) * 2.0 ** -32 * 1.01 * large
+    tol = (2 * tl.T[..., None] + 2.0 ** -11 + 2 * m * 2.0 ** -24) * mass + (3.5 * m + 4) * 2.0 ** -32 * 1.01 * large
     bound = tol + torch.finfo(dtype).eps / 2 * (want.abs() + tol) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     got, gl = out.cpu().double(), lse.cpu().double()
     assert torch.equal(torch.isinf(gl), torch.isinf(wl)) and torch.isfinite(got).all()

@@ -12,8 +12,8 @@
 // A wavefront takes every fourth (or eighth) block of its workgroup's share, its pages and scales looked up 64 at a time, the next block's keys and values requested
 // as soon as this one's are used: no tile passes through LDS, which holds what the wavefronts join at the end alone.  Bound by memory (256 bytes a token and head) and
 // by what a launch costs, the arithmetic of a block being about a third of the time its bytes take.  Four query heads to a kv-head, one token: 32768 tokens of 8 heads,
-// 67 MB, 15.2 us (4.4 TB/s) and 4.0 of the merge behind it; 16 rows of up to 8192 tokens, 165 MB, 36.1 (4.6 TB/s) and 5.0; 131071 tokens of 8 heads, 268 MB, 49.6
-// with its merge (5.4 TB/s; a plain read reaches 6.4); 500 tokens, one launch, 8.4, of which a call on empty rows takes 4.2.
+// 67 MB, 15.6 us (4.3 TB/s) and 4.0 of the merge behind it; 16 rows of up to 8192 tokens, 165 MB, 35.9 (4.6 TB/s) and 4.8; 131071 tokens of 8 heads, 268 MB, 50.8
+// with its merge (5.3 TB/s; a plain read reaches 6.4); 500 tokens, one launch, 8.4, of which a call on empty rows takes 4.2.
 #pragma once
 
 #include "attend.h"

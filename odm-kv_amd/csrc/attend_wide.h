@@ -3,7 +3,7 @@
 // A wavefront holds 32 queries (the columns of v_mfma_f32_32x32x16_f16), a workgroup 32 GROUPS of them, token by token with the G heads of a
 // token together, so that a workgroup's tokens lie together and blocks that none of them sees are passed over.  GROUPS is WAVES, or, for 64 queries at the most, half of
 // it: two wavefronts then share 32 queries, each with a half of every block, and join at the end (29 tokens of four heads take 116 queries, 20 tokens 80: those
-// fill four wavefronts).  Eight wavefronts turn a block into fp16 for twice as many queries as four: 2048 tokens of 32 heads over 12000 take 391 us for 432, over a
+// fill four wavefronts).  Eight wavefronts turn a block into fp16 for twice as many queries as four: 2048 tokens of 32 heads over 12000 took 391 us for 432, over a
 // window of 4096 with a cap 182 for 202; four rows of 777 with a prefix, which leave compute units without work, 46.4 for 45.9.
 //
 // A block of 64 tokens is turned into fp16 once a workgroup
@@ -13,11 +13,12 @@
 // Codes and weights are treated as in the narrow kernel: codes exact in fp16, weights rounded to it once (at most 2^-11 of themselves) in a unit of each
 // query's own, products and sums fp32.
 //
-// Bound by the vector instructions of the softmax (a scale, a maximum, an exponential, a sum and a conversion a score; a cap takes a second exponential and a reciprocal) beside the matrix cores, which
-// are busy 37 % of the time with a window and a cap.  2048 tokens of 32 heads over 12000: 942 TFLOP/s (a bf16 product of 8192 reaches 1429), with a bias 740; over a
-// window of 4096 with a cap 757; 4096 over themselves 869; 29 tokens over 32768 34.9 us and 7.2 of the merge.
-// The halves of a block, each one's vector work beside the other's products, brought 905 -> 942; where scores have a bias, one half's vector work behind the other's is
-// faster instead, both halves' scores under one look for a new reference (543 -> 479 us).
+// Bound by the vector instructions of the softmax (a scale, a maximum, an exponential, a sum and a conversion a score; a cap takes a second exponential and a reciprocal)
+// beside the matrix cores: over a window with a cap they take 64 % of the SIMDs' cycles and the matrix cores are busy 29 %; without either 48 and 39 %, with a bias 60 and 31 %.
+// 2048 tokens of 32 heads over 12000: 914 TFLOP/s (a bf16 product of 8192 reaches 1429), with a bias 778, with a cap besides 633; over a window of 4096 with a cap 746; 4096
+// over themselves 861; 29 tokens over 32768 35.4 us and 7.4 of the merge.
+// The halves of a block, each one's vector work beside the other's products, brought 905 -> 942 TFLOP/s; where scores have a bias, one half's vector work behind the other's
+// is faster instead, both halves' scores under one look for a new reference (543 -> 473 us).
 #pragma once
 
 #include "attend.h"

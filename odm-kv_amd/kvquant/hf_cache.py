@@ -129,7 +129,7 @@ class PagedTokens(torch.Tensor):
 
 
 # what a look at a tensor is, and what may be a look
-_LOOKS = ("dim", "size", "stride", "numel", "is_contiguous", "is_floating_point", "is_complex", "data_ptr", "get_device", "element_size", "storage_offset", "__len__", "__hash__")
+_LOOKS = ("dim", "size", "stride", "numel", "is_contiguous", "is_floating_point", "is_complex", "data_ptr", "get_device", "element_size", "storage_offset", "__len__", "__hash__", "__repr__")
 _FIELDS = tuple(getattr(torch.Tensor, field).__get__ for field in ("shape", "dtype", "device", "ndim", "layout", "is_cuda", "is_cpu", "requires_grad", "grad_fn", "is_leaf", "grad"))
 _KEEPS = ("contiguous", "to", "type_as", "half", "bfloat16", "float", "cuda")
 

@@ -219,6 +219,7 @@ class PagedKVCache:
         self._shared["used"] += need
 
     _loose = False                                           # the bounds may be above the lengths
+    _replayed = False                                        # a write has been captured: replays store what the host does not know of
 
     # ------------------------------------------------------------------ tokens in
     def extend(self, counts: Counts, *, bound: Optional[int] = None) -> None:
@@ -259,6 +260,8 @@ class PagedKVCache:
         largest count (or its bound)."""
         if layer in self._written:                           # (the new tail would be taken for the old one)
             raise ValueError(f"layer {layer} has no tokens to store: it has stored those of the last extend already, or rows have been moved or cut since")
+        if not self._replayed and _capturing():
+            self._replayed = True
         if (isinstance(keys, torch.Tensor) and isinstance(values, torch.Tensor) and keys.dim() == 4 and keys.shape[2] >= self._grown
                 and _device() == self.device.index and _native.paged_write(_WRITE, self._at, self.device.index, layer, keys, values,
                                                                            _lib.stream_ptr(self.device))):
@@ -292,7 +295,7 @@ class PagedKVCache:
 
     def _check_stored(self, layer: int) -> None:
         """Raises where a layer has not stored the tokens of the last `extend`: its rows would be read with what lay in their places before."""
-        if self._grown and layer not in self._written:
+        if self._grown and layer not in self._written and not self._replayed:
             self._check_layer(layer)
             raise ValueError(f"layer {layer} has not stored the tokens of the last extend: write them first")
 

@@ -205,3 +205,24 @@ def test_the_smallest_caps(L):
     for cap in (1e-50, 2.0 ** -101, float("nan")):
         with pytest.raises(ValueError, match="softcap"):
             c.attend(0, q.to(DEV), softcap=cap)
+
+
+def test_tokens_that_a_replay_stores_can_be_read():
+    """Room made by hand, tokens stored by a graph: the host does not know that they are there, and does not say that they are not."""
+    m = 60
+    k, v = _rows(5, 1, 2, m + 12, torch.float16)
+    c = _filled(k[:, :, :m], v[:, :, :m], [m], "int8")
+    kn, vn = (torch.zeros(1, 2, 3, 128, dtype=torch.float16, device=DEV) for _ in range(2))
+    c.extend(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.write(0, kn, vn)
+    q = _queries(1, 1, 8, 3, torch.float16)
+    for n in range(m, m + 12, 3):
+        kn.copy_(k[:, :, n:n + 3])
+        vn.copy_(v[:, :, n:n + 3])
+        c.extend(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        _holds(c, 0, [(k[0, :, :n + 3], v[0, :, :n + 3])], "int8")
+        _check_attend(c, [(k[0, :, :n + 3], v[0, :, :n + 3])], "int8", q)

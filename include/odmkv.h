@@ -652,6 +652,30 @@ int odmkv_pages_extend(const odmkv_pages_t* p, const int32_t* counts, const int3
  * cache's dtype with element strides (multiples of 8, 16-byte aligned), row b's tokens at t < its count; T at least max_count. */
 int odmkv_pages_write(const odmkv_pages_t* p, int layer, const void* K, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t,
                       const void* V, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, int T, void* stream);
+/* odmkv_pages_write of keys that are turned by their positions on the way, and the queries turned beside them, in one launch.  A pair (a, b) of a token at position
+ * p becomes (a c - b s, b c + a s), c and s the pair's in row p of cosine and sine: pairs of dims (i, i + turned / 2), or (2 i, 2 i + 1) where interleaved is not 0, i <
+ * turned / 2; dims from `turned` (a multiple of 16) on stay as they are.  Products and sums in 32 bits, each rounded, then once to 16: a key there to the type's end at the most, and 0 where 32 bits do not hold it.
+ * Row b's t-th new token stands at position start[b] + t (less starts[b], at least 0), or at positions[b, t]; what lies outside the table counts as its
+ * nearest row and sets status[2].  q [rows, Hq, T, 128], k, v [rows, Hkv, T, 128] with element strides (multiples of 8, 16-byte aligned), row b's tokens
+ * at t < its count.  With offsets (device int32 [rows + 1]) row b's tokens are those from offsets[b] to before offsets[b + 1] of `tokens` packed ones: strides of a row are not looked
+ * at, positions are [1, tokens], T is a row's largest count, and a row whose tokens are not as many as it has grown by, or do not lie within `tokens`, is not
+ * stored and sets status[2].
+ * q_out [rows, T, Hq, 128] and k_out [rows, T, Hkv, 128] (packed: [tokens, ...]) contiguous, 0 for what is no row's token.  q_out may be NULL where Hq is 0. */
+typedef struct odmkv_rotate {
+    const odmkv_pages_t* pages;
+    const void* q; int64_t q_stride_b, q_stride_h, q_stride_t;
+    const void* k; int64_t k_stride_b, k_stride_h, k_stride_t;
+    const void* v; int64_t v_stride_b, v_stride_h, v_stride_t;
+    void* q_out;
+    void* k_out;                                 /* or NULL */
+    const float* cosine;                         /* device [table, turned / 2] contiguous */
+    const float* sine;
+    const int32_t* offsets;                      /* device [rows + 1], or NULL */
+    const int32_t* positions; int64_t position_stride_b, position_stride_t;      /* device, or NULL */
+    const int32_t* starts;                       /* device [rows], or NULL; not beside positions */
+    int32_t layer, T, tokens, Hq, turned, interleaved, table;
+} odmkv_rotate_t;
+int odmkv_pages_write_rotated(const odmkv_rotate_t* r, void* stream);
 /* Dense keys and values of one layer, [rows, Hkv, T, 128] contiguous of out_dtype (any), 0 behind a row's length. */
 int odmkv_pages_read(const odmkv_pages_t* p, int layer, void* K, void* V, int out_dtype, int T, void* stream);
 /* Row b becomes a copy of row parents[b] (device int64 [rows], or host int32 [rows], all at once): full blocks are shared, tails copied.  A row

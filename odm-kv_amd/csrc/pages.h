@@ -88,3 +88,30 @@ __device__ static inline uint4 load_once(const void* at) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 __device__ static inline void store_once(void* at, const uint4& v) { __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(at)); }
+
+// what every entry point that writes, moves or reads rows asks of a cache
+static inline int check_pages(const char* who, const odmkv_pages_t* p) {
+    ODMKV_CHECK_ARG(p != nullptr, "%s: null pointer", who);
+    ODMKV_CHECK_ARG(p->kcodes && p->vcodes && p->kscale && p->vscale && p->ktail && p->vtail && p->table && p->length && p->start &&
+                    p->slot && p->refs && p->status, "%s: null pointer", who);
+    ODMKV_CHECK_ARG(p->layers > 0 && p->rows > 0 && p->rows <= MAX_ROWS && p->Hkv > 0 && p->Hkv <= 65535 && p->pages > 0 && p->pages < (1 << 24) &&
+                    p->blocks > 0 && p->blocks <= (1 << 24) && p->layers <= 65535 && p->max_tokens >= 0, "%s: bad shape", who);
+    ODMKV_CHECK_ARG(p->dtype == ODMKV_F16 || p->dtype == ODMKV_BF16, "%s: bad dtype %d", who, p->dtype);
+    ODMKV_CHECK_ARG(p->kind == ODMKV_INT8 || p->kind == ODMKV_E4M3, "%s: bad kind %d", who, p->kind);
+    ODMKV_CHECK_ARG((((uintptr_t)p->kcodes | (uintptr_t)p->vcodes | (uintptr_t)p->ktail | (uintptr_t)p->vtail) & 15) == 0,
+                    "%s: codes and tails must be 16-byte aligned", who);
+    return 0;
+}
+static inline int check_layer(const char* who, const odmkv_pages_t* p, int layer) {
+    if (int rc = check_pages(who, p)) return rc;
+    ODMKV_CHECK_ARG(layer >= 0 && layer < p->layers, "%s: layer %d of %d", who, layer, p->layers);
+    return 0;
+}
+
+#define PAGES_DISPATCH(kernel, p, grid, block, lds, st, ...)                                                                  \
+    do {                                                                                                                      \
+        if ((p)->dtype == ODMKV_F16 && (p)->kind == ODMKV_INT8) hipLaunchKernelGGL((kernel<ODMKV_F16, ODMKV_INT8>), grid, block, lds, st, __VA_ARGS__);        \
+        else if ((p)->dtype == ODMKV_F16) hipLaunchKernelGGL((kernel<ODMKV_F16, ODMKV_E4M3>), grid, block, lds, st, __VA_ARGS__);                              \
+        else if ((p)->kind == ODMKV_INT8) hipLaunchKernelGGL((kernel<ODMKV_BF16, ODMKV_INT8>), grid, block, lds, st, __VA_ARGS__);                             \
+        else hipLaunchKernelGGL((kernel<ODMKV_BF16, ODMKV_E4M3>), grid, block, lds, st, __VA_ARGS__);                                                          \
+    } while (0)

@@ -97,6 +97,14 @@ class Attend(C.Structure):
                 + [(n, C.c_int32) for n in ("layer", "L", "Hq", "window", "max_length")] + [("scaling", C.c_float), ("cap", C.c_float)])
 
 
+class Rotate(C.Structure):
+    """struct odmkv_rotate of include/odmkv.h."""
+    _fields_ = ([("pages", C.POINTER(Pages))] + [f for n in "qkv" for f in ((n, C.c_void_p), *((f"{n}_stride_{d}", C.c_int64) for d in "bht"))]
+                + [(n, C.c_void_p) for n in ("q_out", "k_out", "cosine", "sine", "offsets", "positions")]
+                + [("position_stride_b", C.c_int64), ("position_stride_t", C.c_int64), ("starts", C.c_void_p)]
+                + [(n, C.c_int32) for n in ("layer", "T", "tokens", "Hq", "turned", "interleaved", "table")])
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -180,6 +188,7 @@ def _load() -> C.CDLL:
         "odmkv_pages_init": (C.c_int, [C.POINTER(Pages), vp]),
         "odmkv_pages_extend": (C.c_int, [C.POINTER(Pages), vp, vp, i32, i32, vp]),
         "odmkv_pages_write": (C.c_int, [C.POINTER(Pages), i32, vp, i64, i64, i64, vp, i64, i64, i64, i32, vp]),
+        "odmkv_pages_write_rotated": (C.c_int, [C.POINTER(Rotate), vp]),
         "odmkv_pages_read": (C.c_int, [C.POINTER(Pages), i32, vp, vp, i32, i32, vp]),
         "odmkv_pages_reorder_workspace_bytes": (sz, [i32]),
         "odmkv_pages_reorder": (C.c_int, [C.POINTER(Pages), vp, vp, vp, sz, vp]),
@@ -211,7 +220,7 @@ EXPORTS = ("odmkv_version", "odmkv_last_error", "odmkv_score_workspace_bytes", "
            "odmkv_round_trip_workspace_bytes", "odmkv_round_trip_rows", "odmkv_lloyd_max", "odmkv_dequant", "odmkv_dequant_from", "odmkv_append_exact", "odmkv_append_exact_rows", "odmkv_drop_exact_tail", "odmkv_truncate",
            "odmkv_worklist_cut", "odmkv_decode_workspace_bytes", "odmkv_rotation_operands", "odmkv_decode_attn", "odmkv_decode_attn_static",
            "odmkv_decode_step", "odmkv_decode_block_workspace_bytes", "odmkv_decode_block", "odmkv_block_merge", "odmkv_exact_tail", "odmkv_flush_score", "odmkv_flush_rank",
-           "odmkv_pages_init", "odmkv_pages_extend", "odmkv_pages_write", "odmkv_pages_read", "odmkv_pages_reorder_workspace_bytes", "odmkv_pages_reorder", "odmkv_pages_select",
+           "odmkv_pages_init", "odmkv_pages_extend", "odmkv_pages_write", "odmkv_pages_write_rotated", "odmkv_pages_read", "odmkv_pages_reorder_workspace_bytes", "odmkv_pages_reorder", "odmkv_pages_select",
            "odmkv_pages_truncate", "odmkv_pages_compact_workspace_bytes", "odmkv_pages_compact", "odmkv_pages_attend_workspace_bytes", "odmkv_pages_attend")
 
 

@@ -281,6 +281,74 @@ class PagedKVCache:
                    keys.shape[2])
         self._written.add(layer)
 
+    def write_rotated(self, layer: int, query: Optional[torch.Tensor], keys: torch.Tensor, values: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor, *,
+                      offsets: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+                      interleaved: bool = False, return_keys: bool = False):
+        """``write`` of keys that are turned by their positions on the way, with the queries turned beside them: query [B, Hq, T, 128] (or None), keys and values
+        [B, Hkv, T, 128] as a model projects them -> the turned query of the same shape and type (for ``attend``), and on request the turned keys in 16 bits (for
+        ``kvquant.prompt_attention``), 0 behind a row's count.
+
+        A pair (a, b) of a token at position p becomes (a c - b s, b c + a s), c and s the pair's in row p of `cosine` and `sine` (fp32 [positions, R / 2], R a multiple of 16 up to 128):
+        the dims below R in pairs (i, i + R / 2), or (2 i, 2 i + 1) where `interleaved`; the others stay as they are.  Computed in 32 bits and rounded once to 16; keys are
+        stored as ``write`` stores them (not finite: 0; past the type's end: its end).
+
+        A row's new tokens stand where they lie in the row, less `starts` (int32 [B]: where the text behind padding begins; padding stands at 0), or at `positions` (int32
+        [B, T]).  Packed: with `offsets` (int32 [B + 1]) keys, values and query are [1, heads, N, 128], row b's tokens those from offsets[b] to before offsets[b + 1], as many as the row has
+        grown by, and positions [1, N].  The host checks the table against the rows' lengths; what only the device can see (positions that the table has no row for, which count as
+        its nearest, offsets that do not fit, whose rows are not stored) is raised by ``refresh``."""
+        if layer in self._written:                           # (the new tail would be taken for the old one)
+            raise ValueError(f"layer {layer} has no tokens to store: it has stored those of the last extend already, or rows have been moved or cut since")
+        self._check_layer(layer)
+        B = self.batch if offsets is None else 1
+        rows = f"[{B}, heads, {'T' if offsets is None else 'N'}, {HEAD_DIM}]"
+        given = [(keys, "keys"), (values, "values")] + ([] if query is None else [(query, "queries")])
+        for t, what in given:
+            if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[0] != B or t.shape[3] != HEAD_DIM or (what != "queries" and t.shape[1] != self.kv_heads):
+                raise ValueError(f"{what} must be {rows} with {self.kv_heads} heads of keys and values, got {tuple(getattr(t, 'shape', ())) or type(t).__name__}")
+            self._check_tensor(t, what)
+        if any(t.shape[2] != keys.shape[2] for t, _ in given):
+            raise ValueError(f"{' and '.join(f'{t.shape[2]} {what}' for t, what in given)} a row")
+        if torch.is_grad_enabled() and any(t.requires_grad for t, _ in given):
+            raise RuntimeError("the cache records no gradients: turn and store under torch.no_grad()")
+        T, Hq = keys.shape[2], 0 if query is None else query.shape[1]
+        if T < self._grown:
+            raise ValueError(f"{T} tokens{' a row' if offsets is None else ''}, but rows have grown by up to {self._grown}")
+        if query is not None and not 1 <= Hq <= 65535:
+            raise ValueError(f"{Hq} query heads")
+        half = cosine.shape[1] if isinstance(cosine, torch.Tensor) and cosine.dim() == 2 else 0
+        for t, what in ((cosine, "cosine"), (sine, "sine")):
+            if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape != cosine.shape or t.dtype != torch.float32 or not 8 <= half <= HEAD_DIM // 2 or half % 8 or t.shape[0] == 0:
+                raise ValueError(f"{what} must be float32 [positions, R / 2], R a multiple of 16 up to {HEAD_DIM}, got {getattr(t, 'dtype', type(t).__name__)} {tuple(getattr(t, 'shape', ()))}")
+            _lib.require_gpu(t, what)
+            if t.device != self.device:
+                raise ValueError(f"{what} lies on {t.device}, the cache on {self.device}")
+        if positions is not None and starts is not None:
+            raise ValueError("positions say where tokens stand: starts as well would say it twice")
+        if positions is None:
+            longest = self.max_tokens if _capturing() else self.max_length
+            if longest > cosine.shape[0] and not _capturing() and self._loose:
+                longest = max(self.refresh())
+            if longest > cosine.shape[0]:
+                raise ValueError(f"a table of {cosine.shape[0]} positions for rows of up to {longest} tokens")
+        if not self._replayed and _capturing():
+            self._replayed = True
+        offsets = self._small(offsets, "offsets", torch.int32, ((self.batch + 1,),))
+        positions = self._small(positions, "positions", torch.int32, ((B, T),))
+        starts = self._small(starts, "starts", torch.int32, ((self.batch,),))
+        keys, values, query = (None if t is None else self._rows_ok(t) for t in (keys, values, query))
+        cosine, sine = cosine.contiguous(), sine.contiguous()
+        turned, turned_keys = (torch.empty(B, T, heads, HEAD_DIM, dtype=self.dtype, device=self.device) if wanted else None
+                               for heads, wanted in ((Hq, query is not None), (self.kv_heads, return_keys)))
+        if T:
+            a = _lib.Rotate(C.pointer(self._p), *(x for t in (query, keys, values) for x in ((0, 0, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:3]))),
+                            _lib.ptr(turned), _lib.ptr(turned_keys), cosine.data_ptr(), sine.data_ptr(), _lib.ptr(offsets), _lib.ptr(positions),
+                            0 if positions is None or offsets is not None else positions.stride(0), 0 if positions is None else positions.stride(1), _lib.ptr(starts),
+                            layer, T if offsets is None else max(self._grown, 1), T, Hq, 2 * half, interleaved, cosine.shape[0])
+            self._call(lib.odmkv_pages_write_rotated, C.byref(a))
+        self._written.add(layer)
+        turned = None if turned is None else turned.transpose(1, 2)
+        return (turned, turned_keys.transpose(1, 2)) if return_keys else turned
+
     def append(self, keys: torch.Tensor, values: torch.Tensor, counts: Optional[Counts] = None) -> None:
         """``extend`` and ``write`` of a cache of one layer."""
         if self.layers != 1:

@@ -720,6 +720,35 @@ typedef struct odmkv_attend {
 size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length);
 int odmkv_pages_attend(const odmkv_attend_t* a, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Attention of whole prompts over their own keys and values in 16 bits.  No counterpart in the reference.
+ *
+ * Row b's query l of n stands at position i = m - n + l among the row's m keys (a prompt: n = m; a later chunk over all keys so far: n < m; where there are more queries
+ * than keys, the first ones stand in front and see nothing) and sees the keys lo <= j < hi, lo = max(0, starts[b], i - window + 1 if window > 0), hi = i + 1, or m where
+ * causal is 0 (no window then):
+ *   x_j = scaling * q . k_j;  cap > 0: x_j = cap * tanh(x_j / cap);  out = sum_j softmax(x)_j v_j,  lse = log sum_j exp(x_j);
+ * a query that sees nothing: 0 and -inf.  What a query does not see has no part in its result, infinities and NaN
+ * included (0 times them would be NaN).
+ * q [rows, Hq, L, 128], k, v [rows, Hkv, T, 128] of dtype (fp16, bf16) with element strides (multiples of 8, 16-byte aligned); out [rows, L, Hq, 128], lse fp32 [rows, Hq, L] contiguous.
+ * Packed, with offsets (device int32 [rows + 1], ascending): q [Hq, L, 128], L the queries of all rows, row b's from offsets[b] to before offsets[b + 1]; k, v
+ * [Hkv, T, 128] by key_offsets, or by offsets where that is NULL; out [L, Hq, 128], lse [Hq, L], 0 and -inf for queries that no row has; strides of a row are not looked at.  Nothing outside
+ * the tensors is read or written, whatever offsets and starts say. */
+typedef struct odmkv_prompt_attend {
+    const void* q; int64_t q_stride_b, q_stride_h, q_stride_t;
+    const void* k; int64_t k_stride_b, k_stride_h, k_stride_t;
+    const void* v; int64_t v_stride_b, v_stride_h, v_stride_t;
+    void* out;
+    float* lse;                                  /* or NULL */
+    const int32_t* offsets;                      /* device [rows + 1], or NULL */
+    const int32_t* key_offsets;                  /* device [rows + 1], or NULL */
+    const int32_t* starts;                       /* device [rows], or NULL */
+    void* workspace; size_t workspace_bytes;
+    int32_t dtype, rows, L, T, Hq, Hkv, causal, window;
+    float scaling, cap;                          /* cap 0: none; 2^-100 at least otherwise */
+} odmkv_prompt_attend_t;
+size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T);
+int odmkv_prompt_attend(const odmkv_prompt_attend_t* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,7 +25,7 @@ LIB = os.path.join(LIBDIR, "libodmkv.so")
 BENCH_LIB = os.path.join(LIBDIR, "libodmkv_bench.so")
 SOURCES = ["error.hip", "score.hip", "window.hip", "allocate.hip", "pack.hip", "rows.hip", "decode.hip", "flush.hip", "codebook.hip",
            "levels.hip", "query_stats.hip", "store_edit.hip", "pages.hip", "rotate.hip", "attend.hip", "attend_narrow_f16.hip", "attend_narrow_bf16.hip",
-           "attend_wide_f16.hip", "attend_wide_bf16.hip", "worklist.cpp"]
+           "attend_wide_f16.hip", "attend_wide_bf16.hip", "prompt.hip", "worklist.cpp"]
 BENCH_SOURCES = ["bench_hooks.hip"]
 NATIVE = os.path.join(HERE, "kvquant", "_native.so")          # the CPython extension of csrc/torch_step.cpp (host code only)
 FLAGS = [

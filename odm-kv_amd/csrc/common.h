@@ -115,3 +115,8 @@ __device__ static inline float wave_fold(float v, F f) {
 }
 __device__ static inline float wave_sum(float v) { return wave_fold(v, [](float x, float y) { return x + y; }); }
 __device__ static inline float wave_max(float v) { return wave_fold(v, [](float x, float y) { return fmaxf(x, y); }); }
+
+// a tile on its way from memory into LDS without passing through registers: 16 bytes a lane, a wavefront's 1024 bytes one behind the other from `to` on
+__device__ static inline void request_to_lds(const uint16_t* from, uint32_t to) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(to) : "memory");      // (m0 is the place in LDS)
+}

@@ -1,0 +1,425 @@
+// Attention of whole prompts over their own keys and values in 16 bits: grouped heads, sequences of their own lengths packed one behind the other, later chunks (fewer
+// queries than keys), with a cap and a window.
+//
+//   x_j = scaling q . k_j, capped;  out = sum_j softmax(x)_j v_j over lo <= j < hi
+//
+// A wavefront holds 32 queries (the columns of the 32x32x16 matrix instructions), a workgroup WAVES times as many, token by token with the G heads of a token together, so that
+// a workgroup's tokens lie together: a block of 64 keys and values serves all heads of the group, and few blocks lie across a query's end.  The rows of the first product are
+// tokens; what a lane holds of the weights is its operand of the second product as it is, whose other operand, values dim by dim, comes out of LDS by transposing reads.
+// Blocks go from memory into LDS without passing through registers, the next one on its way while this one is used: one barrier a block.
+#include "attend.h"
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+#define PROMPT_WAVES 8
+#define PROMPT_COLS(waves) (32 * (waves))
+#define PROMPT_TILE (BLOCK_TOKENS * HD * 2)                      // bytes of a block of keys, or of values
+#define PROMPT_LDS (4 * PROMPT_TILE)
+
+struct PromptArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    int64_t qb, qh, qt, kb, kh, kt, vb, vh, vt;
+    uint16_t* out;               // [rows, L, Hq, 128], packed [L, Hq, 128]
+    float* lse;                  // [rows, Hq, L], packed [Hq, L]
+    const int32_t* offsets;      // packed: where the rows' queries begin, rows + 1 of them; L and T are all rows' together then
+    const int32_t* key_offsets;
+    const int32_t* starts;
+    int rows, L, T, Hq, Hkv, G, causal, window;
+    float scaling, cap;
+    int splits;                  // workgroups that share a tile's blocks
+    float* part_out;             // [splits, queries in all, Hq, 128]
+    float* part_lse;             // the same without the 128, base 2
+};
+
+// a tile of queries: of row `row` (-1: of none, queries that no row has), n of them from q0 on, over m keys from k0 on
+struct Tile { int row, nth, q0, n, k0, m; };
+
+// Packed rows' tiles one behind the other, before and behind them those of the queries that no row has.  What offsets say is kept within what there is.
+template <int COLS>
+__device__ static inline Tile tile_of(const PromptArgs& a, int at) {
+    if (!a.offsets) {
+        const int tiles = (a.G * a.L + COLS - 1) / COLS, nth = tiles - 1 - at / a.rows;         // (the last tiles see most: they come first)
+        return {nth < 0 ? -2 : at % a.rows, nth, 0, a.L, 0, a.T};
+    }
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int s0 = -1; s0 <= a.rows; s0 += 64) {
+        const int s = s0 + lane;
+        int begin = 0, end = 0;
+        if (s <= a.rows) {
+            begin = s < 0 ? 0 : min(max(a.offsets[s], 0), a.L);
+            end = s == a.rows ? a.L : max(min(a.offsets[s + 1], a.L), begin);
+        }
+        const int count = (int)(((int64_t)a.G * (end - begin) + COLS - 1) / COLS), upto = before + wave_scan(count);
+        const unsigned long long behind = __ballot(upto > at);
+        if (behind) {
+            const int l = __builtin_ctzll(behind), row = s0 + l, nth = __builtin_amdgcn_readlane(upto, l) - 1 - at;
+            const int q0 = __builtin_amdgcn_readlane(begin, l), n = __builtin_amdgcn_readlane(end, l) - q0;
+            if (row < 0 || row >= a.rows) return {-1, nth, q0, n, 0, 0};
+            const int32_t* const of = a.key_offsets ? a.key_offsets : a.offsets;
+            const int k0 = min(max(of[row], 0), a.T), m = max(min(of[row + 1], a.T) - k0, 0);
+            return {row, nth, q0, n, k0, m};
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return {-2, 0, 0, 0, 0, 0};
+}
+
+// operands of the matrix instructions
+template <int DT>
+__device__ static inline f32x16 multiply(const uint4& x, const uint4& y, const f32x16& to) {
+    if constexpr (DT == ODMKV_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), to, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), to, 0, 0, 0);
+}
+template <int DT>
+__device__ static inline uint32_t pair_16(float x, float y) {
+    if constexpr (DT == ODMKV_F16) return __builtin_bit_cast(uint32_t, f16x2{(_Float16)x, (_Float16)y});
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((__attribute__((ext_vector_type(2))) float){x, y}, __attribute__((ext_vector_type(2))) __bf16));
+}
+
+// Weights go to 16 bits relative to a reference that follows the largest score of the query's own: it moves where a score passes it by more than RISE (base 2).  fp16: the
+// reference's weight is 2^8 and may grow to 2^15, so that a weight below fp16's normal numbers is off by 2^-33 of the largest at the most; bf16 has the range of 32 bits.
+template <int DT> struct Weights {
+    static constexpr float LIFT = DT == ODMKV_F16 ? 8.0f : 0.0f, RISE_BY = DT == ODMKV_F16 ? 7.0f : 8.0f;
+};
+
+template <int DT, int MODE, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
+    constexpr bool PLAIN = MODE == 0;                           // 1: a cap by the exponential; 2: any
+    constexpr int COLS = PROMPT_COLS(WAVES), PIECES = PROMPT_TILE / 16 / (WAVES * 64);
+    constexpr float LIFT = Weights<DT>::LIFT;
+    extern __shared__ __align__(16) uint8_t smem[];             // [2][keys 64 x 256 bytes, values 64 x 256 bytes]
+    __shared__ int range[2][WAVES];
+    // heads vary fastest: a die of the chip then keeps few heads' keys and values in its L2
+    const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % a.splits;
+    const Tile tile = tile_of<COLS>(a, rest / a.splits);
+    if (tile.row < -1) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+    const int r = tile.nth * COLS + 32 * wave + col, l = r / a.G, hq = h * a.G + r - l * a.G;
+    const bool valid = l < tile.n;
+    const int row = max(tile.row, 0), pos = tile.m - tile.n + l;
+    int lo = 0, hi = 0;
+    if (valid && tile.row >= 0) {
+        lo = a.starts ? max(a.starts[row], 0) : 0;
+        if (a.window > 0) lo = max(lo, pos - a.window + 1);
+        hi = a.causal ? max(pos + 1, 0) : tile.m;
+    }
+    const bool sees = lo < hi;
+    const int wave_lo = wave_min_int(sees ? lo : 0x7fffffff), wave_hi = -wave_min_int(sees ? -hi : 0);          // what some query of the wavefront sees
+    const int open_from = -wave_min_int(valid ? -(sees ? lo : 0x7fffffff) : 0), open_to = wave_min_int(valid ? hi : 0x7fffffff);    // what all of them see
+    if (lane == 0) {
+        range[0][wave] = wave_lo;
+        range[1][wave] = wave_hi;
+    }
+    __syncthreads();
+    int from = range[0][0], upto = range[1][0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+        from = min(from, range[0][w]);
+        upto = max(upto, range[1][w]);
+    }
+    const int first = from / BLOCK_TOKENS, blocks = max((upto + BLOCK_TOKENS - 1) / BLOCK_TOKENS - first, 0), share = (blocks + a.splits - 1) / a.splits;
+    const int b0 = __builtin_amdgcn_readfirstlane(first + split * share), mine = __builtin_amdgcn_readfirstlane(min(share, blocks - split * share));
+
+    // 16-byte piece p of token t lies at p ^ (t % 16) of the token's place; of values 32-byte pieces at p ^ (t % 8): what a wavefront reads at a time falls on distinct banks.
+    // Tokens behind the row's end repeat its last one and are masked.
+    const uint16_t* const K = a.k + (a.offsets ? tile.k0 * a.kt : row * a.kb) + h * a.kh;
+    const uint16_t* const V = a.v + (a.offsets ? tile.k0 * a.vt : row * a.vb) + h * a.vh;
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    const auto request = [&](int i) {
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+            const int e = tid + WAVES * 64 * c, t = e >> 4, p = e & 15;
+            const int64_t at = min((b0 + i) * BLOCK_TOKENS + t, tile.m - 1);
+            const uint32_t to = lds0 + (i & 1) * 2 * PROMPT_TILE + (WAVES * 64 * c + 64 * wave) * 16;
+            request_to_lds(K + at * a.kt + 8 * (p ^ (t & 15)), to);
+            request_to_lds(V + at * a.vt + 8 * (p ^ ((t & 7) << 1)), to + PROMPT_TILE);
+        }
+    };
+    if (mine > 0) request(0);
+
+    uint4 q[8];                                                 // dims 16 st + 8 half + e
+    {
+        const uint16_t* src = a.q + (a.offsets ? (int64_t)(tile.q0 + l) * a.qt : row * a.qb + l * a.qt) + hq * a.qh + 8 * half;
+#pragma unroll
+        for (int st = 0; st < 8; ++st) q[st] = valid ? *reinterpret_cast<const uint4*>(src + 16 * st) : make_uint4(0, 0, 0, 0);
+    }
+    const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const bool by_exp = MODE == 1 || (!PLAIN && a.cap > 0.0f && a.cap <= CAP_BY_EXP);
+    const Cap cap = {a.cap * LOG2E, 2.0f * LOG2E * a.cap, 2.0f * LOG2E * inv_cap};
+    const float c = PLAIN ? a.scaling * LOG2E : a.scaling;
+    const auto score = [&](float x) {                           // of a product, base 2
+        return PLAIN ? x * c : by_exp ? capped(x * (c * cap.plain), cap) : inv_cap > 0.0f ? cap.by * tanh_of(x * (c * inv_cap)) : x * (c * LOG2E);
+    };
+
+    float ref = -INFINITY, sum = 0.0f;
+    f32x16 acc[4];                                              // dims 32 db + 8 (e / 4) + 4 half + e % 4 of query `col`
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[db][e] = 0.0f;
+
+    const int key_at = col * 256 + ((half ^ (col & 15)) << 4);                                      // piece 2 st + half of token col
+    const int value_token = 4 * half + ((lane & 15) >> 2);                                          // a lane reads four dims of a token, and gets four tokens of a dim
+    const int value_at = value_token * 256 + (((lane >> 4 & 1) ^ value_token) << 5) + ((lane & 3) << 3);
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // this block has come, and nobody reads the one before any more
+        if (i + 1 < mine) request(i + 1);
+        const int t0 = (b0 + i) * BLOCK_TOKENS;
+        if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;                  // (of the wavefront's own queries none sees the block)
+        const uint8_t* const keys = smem + (i & 1) * 2 * PROMPT_TILE;
+        const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
+        f32x16 dot[2];
+        uint4 w[4];
+        const auto multiply_keys = [&](int tb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dot[tb][e] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < 8; ++st)
+                dot[tb] = multiply<DT>(*reinterpret_cast<const uint4*>(keys + 32 * 256 * tb + (key_at ^ (st << 5))), q[st], dot[tb]);
+        };
+        const auto multiply_values = [&](int st) {
+#pragma unroll
+            for (int db = 0; db < 4; ++db) {
+                typedef __attribute__((address_space(3))) s16x4* place;
+                const uint32_t at = lds0 + (i & 1) * 2 * PROMPT_TILE + PROMPT_TILE + 16 * 256 * st + (value_at ^ (db << 6));
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(size_t)at), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(size_t)(at + 8 * 256));
+                const uint2 u = __builtin_bit_cast(uint2, x), v = __builtin_bit_cast(uint2, y);
+                acc[db] = multiply<DT>(make_uint4(u.x, u.y, v.x, v.y), w[st], acc[db]);
+            }
+        };
+        // products of half a block to scores (PLAIN: they stay products); the largest score
+        const auto to_scores = [&](int tb) {
+            f32x16& x = dot[tb];
+            if constexpr (!PLAIN) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = score(x[e]);
+            }
+            if (cut) {
+                const int tl = t0 + 32 * tb + 4 * half;         // token of score e: tl + 8 (e / 4) + e % 4
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int t = tl + 8 * (e >> 2) + (e & 3);
+                    x[e] = t >= lo && t < hi ? x[e] : -INFINITY;
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+            return PLAIN && top > -INFINITY ? top * c : top;    // (c is positive: the largest product is the largest score)
+        };
+        // the reference where a score is to move it, each query by itself; what the sums are to be multiplied by
+        const auto move_sums = [&](float top, float& old) {
+            if (!__any(top > ref + Weights<DT>::RISE_BY)) return false;
+            const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+            const float to = most > ref + Weights<DT>::RISE_BY ? most : ref;
+            old = ref > -INFINITY ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
+            sum *= old;
+            ref = to;
+            return true;
+        };
+        const auto multiply_sums = [&](float old) {
+#pragma unroll
+            for (int db = 0; db < 4; ++db) acc[db] *= old;
+        };
+        const auto weigh = [&](int tb) {
+            const float shift = LIFT - (ref > -INFINITY ? ref : 0.0f);
+            float z0 = 0.0f, z1 = 0.0f;
+            uint32_t word[8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e], c, shift) : dot[tb][e] + shift);
+                const float p1 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e + 1], c, shift) : dot[tb][e + 1] + shift);
+                z0 += p0;
+                z1 += p1;
+                word[e >> 1] = pair_16<DT>(p0, p1);
+            }
+            w[2 * tb] = make_uint4(word[0], word[1], word[2], word[3]);
+            w[2 * tb + 1] = make_uint4(word[4], word[5], word[6], word[7]);
+            sum += z0 + z1;
+        };
+        // the two halves' vector work stands beside the other half's matrix work
+        float old;
+        multiply_keys(0);
+        if (move_sums(to_scores(0), old)) multiply_sums(old);
+        multiply_keys(1);
+        weigh(0);
+        const bool moved = move_sums(to_scores(1), old);
+        multiply_values(0);
+        multiply_values(1);
+        weigh(1);
+        if (moved) multiply_sums(old);
+        multiply_values(2);
+        multiply_values(3);
+    }
+
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    sum = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+    const bool none = sum == 0.0f;
+    float by = none ? 0.0f : 1.0f / sum;
+    const float lse2 = none ? -INFINITY : ref - LIFT + __builtin_amdgcn_logf(sum);
+    // A value that is not finite has spoilt the queries that do not see its token as well (0 times it is not 0), and bf16 values at the type's end may have passed 32 bits: their
+    // sums are made once more, token by token, of what is seen alone.
+    bool spoilt = false;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) spoilt |= !(fabsf(acc[db][e]) < INFINITY);
+    if (__any(spoilt && sum < INFINITY)) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[db][e] = 0.0f;
+        const int t_from = max(wave_lo, b0 * BLOCK_TOKENS), t_upto = min(wave_hi, (b0 + mine) * BLOCK_TOKENS);
+#pragma unroll 1
+        for (int t = t_from; t < t_upto; ++t) {
+            float x = 0.0f;
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                const uint4 u = *reinterpret_cast<const uint4*>(K + (int64_t)t * a.kt + 16 * st + 8 * half);
+                const uint32_t kw[4] = {u.x, u.y, u.z, u.w}, qw[4] = {q[st].x, q[st].y, q[st].z, q[st].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x = __fmaf_rn(Elem<DT>::to_f32((uint16_t)(kw[e] & 0xffff)), Elem<DT>::to_f32((uint16_t)(qw[e] & 0xffff)), x);
+                    x = __fmaf_rn(Elem<DT>::to_f32((uint16_t)(kw[e] >> 16)), Elem<DT>::to_f32((uint16_t)(qw[e] >> 16)), x);
+                }
+            }
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+            x = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+            const bool seen = t >= lo && t < hi;
+            const float p = seen ? __builtin_amdgcn_exp2f(score(x) - lse2) : 0.0f;
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(V + (int64_t)t * a.vt + 32 * db + 8 * g + 4 * half);
+                    const uint32_t vw[2] = {u.x, u.y};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = Elem<DT>::to_f32((uint16_t)(vw[e >> 1] >> (16 * (e & 1))));
+                        acc[db][4 * g + e] = seen ? __fmaf_rn(p, v, acc[db][4 * g + e]) : acc[db][4 * g + e];
+                    }
+                }
+        }
+        by = 1.0f;
+    }
+    if (!valid) return;
+    const auto result = [&](int db, int e) { return none ? 0.0f : acc[db][e] * by; };
+    const int64_t nth = (a.offsets ? 0 : (int64_t)row * a.L) + tile.q0 + l;                         // of all queries
+    if (a.splits > 1) {
+        const int64_t all = a.offsets ? a.L : (int64_t)a.rows * a.L, to = (split * all + nth) * a.Hq + hq;
+        float* dst = a.part_out + to * HD + 4 * half;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = result(db, 4 * g + e);
+                *reinterpret_cast<f32x4*>(dst + 32 * db + 8 * g) = x;
+            }
+        if (half == 0) a.part_lse[to] = lse2;
+        return;
+    }
+    uint16_t* dst = a.out + (nth * a.Hq + hq) * HD + 4 * half;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint32_t x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) x[e] = pair_16<DT>(result(db, 4 * g + 2 * e), result(db, 4 * g + 2 * e + 1));
+            *reinterpret_cast<uint2*>(dst + 32 * db + 8 * g) = make_uint2(x[0], x[1]);
+        }
+    if (a.lse && half == 0) a.lse[((a.offsets ? 0 : (int64_t)row * a.Hq) + hq) * a.L + tile.q0 + l] = lse2 * LN2;
+}
+
+// The shares of a query's blocks, put together: a wavefront a query, a lane two dims.
+template <int DT>
+__global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t all = a.offsets ? a.L : (int64_t)a.rows * a.L, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= all * a.Hq) return;
+    float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[s * all * a.Hq + at]);
+    const float by = top > -INFINITY ? top : 0.0f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float w = __builtin_amdgcn_exp2f(a.part_lse[s * all * a.Hq + at] - by);
+        const float2 v = *reinterpret_cast<const float2*>(a.part_out + (s * all * a.Hq + at) * HD + 2 * lane);
+        sum += w;
+        o0 = __fmaf_rn(w, v.x, o0);
+        o1 = __fmaf_rn(w, v.y, o1);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint32_t*>(a.out + at * HD + 2 * lane) = pair_16<DT>(o0 * inv, o1 * inv);
+    if (a.lse && lane == 0) {
+        const int64_t nth = at / a.Hq, row = a.offsets ? 0 : nth / a.L;
+        a.lse[(row * a.Hq + at % a.Hq) * a.L + nth - row * a.L] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
+    }
+}
+
+// How a call is cut: tiles of queries at the most, and workgroups that share a tile's blocks where there are too few tiles for the compute units.
+struct PromptCut { long long tiles; int splits; };
+static PromptCut cut_of(bool packed, int rows, int G, int Hkv, int L, int T) {
+    const long long cols = PROMPT_COLS(PROMPT_WAVES);
+    PromptCut c;
+    c.tiles = packed ? ((long long)G * L + cols - 1) / cols + rows + 2 : (long long)rows * (((long long)G * L + cols - 1) / cols);
+    const long long blocks = (packed ? T / rows : T) / BLOCK_TOKENS + 1;
+    c.splits = (int)std::max(1LL, std::min(compute_units() / std::max(1LL, c.tiles * Hkv), blocks / 4));
+    return c;
+}
+
+extern "C" size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T) {
+    if (rows <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || L <= 0 || T < 0) return 0;
+    const PromptCut c = cut_of(packed != 0, rows, Hq / Hkv, Hkv, L, T);
+    return c.splits > 1 ? align_up((size_t)c.splits * (packed ? 1 : rows) * L * Hq * (HD + 1) * sizeof(float), 256) : 0;
+}
+
+extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream) {
+    ODMKV_CHECK_ARG(d != nullptr, "prompt_attend: null pointer");
+    ODMKV_CHECK_ARG(d->dtype == ODMKV_F16 || d->dtype == ODMKV_BF16, "prompt_attend: bad dtype %d", d->dtype);
+    ODMKV_CHECK_ARG(d->rows > 0 && d->L >= 0 && d->T >= 0 && d->L <= (1 << 26) && d->T <= (1 << 26) && d->rows <= (1 << 20), "prompt_attend: bad shape");
+    ODMKV_CHECK_ARG(d->Hkv > 0 && d->Hq > 0 && d->Hq % d->Hkv == 0 && d->Hq <= 65535, "prompt_attend: %d query heads over %d kv-heads", d->Hq, d->Hkv);
+    ODMKV_CHECK_ARG(d->window >= 0 && (d->window == 0 || d->causal), "prompt_attend: bad window");
+    ODMKV_CHECK_ARG(d->cap == 0.0f || (d->cap >= 0x1p-100f && d->cap < INFINITY), "prompt_attend: bad cap");
+    ODMKV_CHECK_ARG(!d->key_offsets || d->offsets, "prompt_attend: the keys' offsets without the queries'");
+    if (d->L == 0) return 0;
+    ODMKV_CHECK_ARG(d->q && d->out && ((d->k && d->v) || d->T == 0), "prompt_attend: null pointer");
+    ODMKV_CHECK_ARG((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->out) & 15) == 0 &&
+                    ((d->q_stride_b | d->q_stride_h | d->q_stride_t | d->k_stride_b | d->k_stride_h | d->k_stride_t | d->v_stride_b | d->v_stride_h | d->v_stride_t) & 7) == 0,
+                    "prompt_attend: rows must be 16-byte aligned");
+    const int G = d->Hq / d->Hkv;
+    const PromptCut cut = cut_of(d->offsets != nullptr, d->rows, G, d->Hkv, d->L, d->T);
+    const long long all = d->offsets ? d->L : (long long)d->rows * d->L, groups = cut.tiles * d->Hkv * cut.splits;
+    ODMKV_CHECK_ARG((long long)G * d->L < 0x7fff0000LL && groups * PROMPT_WAVES * 64 < 0x100000000LL && all * d->Hq < 0x100000000LL, "prompt_attend: too many queries");
+    const size_t need = odmkv_prompt_attend_workspace_bytes(d->offsets != nullptr, d->rows, d->Hq, d->Hkv, d->L, d->T);
+    if (need > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)) {
+        odmkv_set_error("prompt_attend: workspace too small");
+        return ODMKV_ENOSPACE;
+    }
+    float* const parts = (float*)d->workspace;
+    const PromptArgs a = {(const uint16_t*)d->q, (const uint16_t*)d->k, (const uint16_t*)d->v, d->q_stride_b, d->q_stride_h, d->q_stride_t, d->k_stride_b, d->k_stride_h,
+                          d->k_stride_t, d->v_stride_b, d->v_stride_h, d->v_stride_t, (uint16_t*)d->out, d->lse, d->offsets, d->key_offsets, d->starts, d->rows, d->L, d->T,
+                          d->Hq, d->Hkv, G, d->causal != 0, d->window, d->scaling, d->cap, cut.splits, parts, parts + (size_t)cut.splits * all * d->Hq * HD};
+    const int mode = d->cap > 0.0f ? (d->cap <= CAP_BY_EXP ? 1 : 2) : d->scaling > 0.0f ? 0 : 2;
+    const hipStream_t st = (hipStream_t)stream;
+    const auto run = [&](auto dt, auto mode_) {
+        const auto kernel = prompt_kernel<dt.value, mode_.value, PROMPT_WAVES>;
+        ODMKV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PROMPT_LDS));
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(PROMPT_WAVES * 64), PROMPT_LDS, st, a);
+        ODMKV_CHECK_LAUNCH("prompt_kernel");
+        if (cut.splits > 1) {
+            hipLaunchKernelGGL(prompt_merge_kernel<dt.value>, dim3((unsigned)((all * d->Hq + 3) / 4)), dim3(256), 0, st, a);
+            ODMKV_CHECK_LAUNCH("prompt_merge_kernel");
+        }
+        return 0;
+    };
+    const auto of_mode = [&](auto dt) { return mode == 0 ? run(dt, Int<0>()) : mode == 1 ? run(dt, Int<1>()) : run(dt, Int<2>()); };
+    return d->dtype == ODMKV_F16 ? of_mode(Int<ODMKV_F16>()) : of_mode(Int<ODMKV_BF16>());
+}

@@ -18,6 +18,7 @@ _LAZY = {
     "PackedCacheLayer": "kvquant.hf_cache",          # not in the reference: a cache layer without a dense copy
     "PagedCache": "kvquant.hf_cache",                # not in the reference: a model's cache over the next
     "PagedKVCache": "kvquant.paged_cache",           # not in the reference: 8 bits a value, rows that share pages
+    "prompt_attention": "kvquant.prompt",            # not in the reference: whole prompts in 16 bits, packed or padded
 }
 
 

@@ -105,6 +105,13 @@ class Rotate(C.Structure):
                 + [(n, C.c_int32) for n in ("layer", "T", "tokens", "Hq", "turned", "interleaved", "table")])
 
 
+class PromptAttend(C.Structure):
+    """struct odmkv_prompt_attend of include/odmkv.h."""
+    _fields_ = ([f for n in "qkv" for f in ((n, C.c_void_p), *((f"{n}_stride_{d}", C.c_int64) for d in "bht"))]
+                + [(n, C.c_void_p) for n in ("out", "lse", "offsets", "key_offsets", "starts", "workspace")] + [("workspace_bytes", C.c_size_t)]
+                + [(n, C.c_int32) for n in ("dtype", "rows", "L", "T", "Hq", "Hkv", "causal", "window")] + [("scaling", C.c_float), ("cap", C.c_float)])
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -198,6 +205,8 @@ def _load() -> C.CDLL:
         "odmkv_pages_compact": (C.c_int, [C.POINTER(Pages), C.POINTER(Pages), vp, sz, vp]),
         "odmkv_pages_attend_workspace_bytes": (sz, [C.POINTER(Pages), i32, i32, i32]),
         "odmkv_pages_attend": (C.c_int, [C.POINTER(Attend), vp]),
+        "odmkv_prompt_attend_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+        "odmkv_prompt_attend": (C.c_int, [C.POINTER(PromptAttend), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -221,7 +230,7 @@ EXPORTS = ("odmkv_version", "odmkv_last_error", "odmkv_score_workspace_bytes", "
            "odmkv_worklist_cut", "odmkv_decode_workspace_bytes", "odmkv_rotation_operands", "odmkv_decode_attn", "odmkv_decode_attn_static",
            "odmkv_decode_step", "odmkv_decode_block_workspace_bytes", "odmkv_decode_block", "odmkv_block_merge", "odmkv_exact_tail", "odmkv_flush_score", "odmkv_flush_rank",
            "odmkv_pages_init", "odmkv_pages_extend", "odmkv_pages_write", "odmkv_pages_write_rotated", "odmkv_pages_read", "odmkv_pages_reorder_workspace_bytes", "odmkv_pages_reorder", "odmkv_pages_select",
-           "odmkv_pages_truncate", "odmkv_pages_compact_workspace_bytes", "odmkv_pages_compact", "odmkv_pages_attend_workspace_bytes", "odmkv_pages_attend")
+           "odmkv_pages_truncate", "odmkv_pages_compact_workspace_bytes", "odmkv_pages_compact", "odmkv_pages_attend_workspace_bytes", "odmkv_pages_attend", "odmkv_prompt_attend_workspace_bytes", "odmkv_prompt_attend")
 
 
 def check(rc: int) -> None:

@@ -30,3 +30,39 @@ def test_bad_turns_are_refused():
         assert _rotate(**change) == -1 and says in _error(), (change, _error())
     assert _rotate(T=0) == 0 and _rotate(offsets=4096, tokens=0) == 0                   # nothing to store
     assert lib.odmkv_pages_write_rotated(None, None) == -1 and "null" in _error()
+
+
+def _prompt(**change):
+    from kvquant._lib import PromptAttend, lib
+    a = PromptAttend(*[4096, 1024, 128, 1024] * 3, 4096, 4096, 0, 0, 0, 0, 0, 0, 2, 1000, 1000, 8, 4, 1, 0, 0.1, 0.0)
+    for name, value in change.items():
+        setattr(a, name, value)
+    return lib.odmkv_prompt_attend(C.byref(a), None)
+
+
+def test_bad_prompts_are_refused():
+    from kvquant._lib import lib
+    nan, inf = float("nan"), float("inf")
+    for change, says in ((dict(dtype=2), "dtype"), (dict(rows=0), "shape"), (dict(L=-1), "shape"), (dict(T=-1), "shape"), (dict(L=(1 << 26) + 1), "shape"), (dict(Hkv=0), "heads"),
+                         (dict(Hq=7), "heads"), (dict(Hq=0), "heads"), (dict(window=-1), "window"), (dict(window=5, causal=0), "window"), (dict(cap=-1.0), "cap"), (dict(cap=nan), "cap"),
+                         (dict(cap=inf), "cap"), (dict(cap=1e-38), "cap"), (dict(key_offsets=4096), "offsets"), (dict(q=0), "null"), (dict(k=0), "null"), (dict(v=0), "null"),
+                         (dict(out=0), "null"), (dict(q=4100), "aligned"), (dict(out=4104), "aligned"), (dict(k_stride_t=100), "aligned"),
+                         (dict(rows=1 << 20, L=1 << 26), "too many"), (dict(Hq=65532, L=1 << 26), "too many")):
+        assert _prompt(**change) == -1 and says in _error(), (change, _error())
+    assert _prompt(L=0) == 0                                                             # nobody asks
+    assert lib.odmkv_prompt_attend(None, None) == -1 and "null" in _error()
+    # few queries over many keys: their blocks are shared out, and the shares need room
+    few = dict(rows=1, L=2, T=50000)
+    need = lib.odmkv_prompt_attend_workspace_bytes(0, 1, 8, 4, 2, 50000)
+    assert need > 0 and _prompt(**few) == -2 and _prompt(**few, workspace=4096, workspace_bytes=need - 1) == -2 and _prompt(**few, workspace=4100, workspace_bytes=need) == -2
+    assert lib.odmkv_prompt_attend_workspace_bytes(0, 0, 8, 4, 2, 50000) == 0 and lib.odmkv_prompt_attend_workspace_bytes(0, 1, 7, 4, 2, 50000) == 0
+
+
+def test_python_refuses_prompts_without_a_gpu():
+    import torch
+    from kvquant import prompt_attention
+    q = torch.zeros(1, 4, 5, 128, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        prompt_attention(q, q, q)
+    with pytest.raises(ValueError, match="queries must be"):
+        prompt_attention(None, q, q)

@@ -695,6 +695,11 @@ int odmkv_pages_truncate(const odmkv_pages_t* p, const int32_t* lengths, const i
 size_t odmkv_pages_compact_workspace_bytes(int pages);
 int odmkv_pages_compact(const odmkv_pages_t* p, const odmkv_pages_t* to, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Which rows have their first blocks in common: plan (device int32, odmkv_pages_plan_bytes) is what odmkv_pages_attend takes.  It goes on being right while rows grow
+ * (extend), and has to be made again when they are reordered, truncated or made anew. */
+size_t odmkv_pages_plan_bytes(int rows);
+int odmkv_pages_plan(const odmkv_pages_t* p, int32_t* plan, size_t plan_bytes, void* stream);
+
 /* Attention of the newest tokens' queries over the cache: query l of row b's n (counts[b], or L) stands at position
  * i = length - n + l and sees the tokens lo <= j < hi,
  *   lo = max(0, start of l, i - window + 1 if window > 0),  hi = min(max(i + 1, prefix), length);
@@ -716,7 +721,11 @@ typedef struct odmkv_attend {
     int32_t layer, L, Hq, window;
     int32_t max_length;                          /* about how long the longest row is: how the work is cut, not what is seen */
     float scaling, cap;                          /* cap 0: none; 2^-100 at least otherwise */
+    const int32_t* plan;                         /* odmkv_pages_plan's, of the tables as they are, or NULL */
 } odmkv_attend_t;
+/* With a plan, blocks that rows have in common are read once for all of them (up to 16 queries of a kv-head, heads of a group times L; more go the ordinary way); the workspace is the
+ * second function's then. */
+size_t odmkv_pages_attend_shared_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length);
 size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length);
 int odmkv_pages_attend(const odmkv_attend_t* a, void* stream);
 

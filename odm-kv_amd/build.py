@@ -25,7 +25,8 @@ LIB = os.path.join(LIBDIR, "libodmkv.so")
 BENCH_LIB = os.path.join(LIBDIR, "libodmkv_bench.so")
 SOURCES = ["error.hip", "score.hip", "window.hip", "allocate.hip", "pack.hip", "rows.hip", "decode.hip", "flush.hip", "codebook.hip",
            "levels.hip", "query_stats.hip", "store_edit.hip", "pages.hip", "rotate.hip", "attend.hip", "attend_narrow_f16.hip", "attend_narrow_bf16.hip",
-           "attend_wide_f16.hip", "attend_wide_bf16.hip", "prompt.hip", "worklist.cpp"]
+           "attend_wide_f16.hip", "attend_wide_bf16.hip", "attend_shared_f16.hip", "attend_shared_bf16.hip",
+           "prompt.hip", "worklist.cpp"]
 BENCH_SOURCES = ["bench_hooks.hip"]
 NATIVE = os.path.join(HERE, "kvquant", "_native.so")          # the CPython extension of csrc/torch_step.cpp (host code only)
 FLAGS = [
@@ -56,7 +57,7 @@ def _build_native(verbose: bool) -> None:
 
 def build(force: bool = False, verbose: bool = True) -> str:
     srcs = [os.path.join(CSRC, s) for s in SOURCES + BENCH_SOURCES]
-    deps = srcs + [os.path.join(CSRC, "torch_step.cpp")] + [os.path.join(CSRC, h) for h in ("common.h", "quant.h", "decode.h", "pages.h", "pages_write.h", "attend.h", "attend_narrow.h", "attend_wide.h", "exports.map")] + [
+    deps = srcs + [os.path.join(CSRC, "torch_step.cpp")] + [os.path.join(CSRC, h) for h in ("common.h", "quant.h", "decode.h", "pages.h", "pages_write.h", "attend.h", "attend_narrow.h", "attend_wide.h", "attend_shared.h", "exports.map")] + [
         os.path.join(HERE, "..", "include", "odmkv.h"), os.path.join(HERE, "..", "include", "odmkv_bench.h"), __file__]
     if (not force and os.path.exists(LIB) and os.path.exists(BENCH_LIB) and os.path.exists(NATIVE)
             and min(map(os.path.getmtime, (LIB, BENCH_LIB, NATIVE))) >= _newest(deps)):

@@ -28,6 +28,12 @@ struct AttendArgs {
     int splits;          // workgroups of a kv-head (narrow), or that share a row and kv-head's blocks (wide)
     float* part_out;     // narrow [Hkv, splits, G L, 128], wide [rows, Hkv, splits, G L, 128]
     float* part_lse;     // the same without the 128, base 2
+    // rows that have their first blocks in common (attend_shared.h)
+    const int32_t* plan;
+    int spare;           // workgroups of a kv-head beyond one for each 128 of a group's queries
+    float* common_out;   // partial results of what is in common: a kv-head's `common_parts`, each of 128
+    float* common_lse;
+    long long common_parts;
 };
 
 #define LOG2E 1.4426950408889634f
@@ -251,7 +257,7 @@ __device__ static inline int wave_scan(int v) {                 // inclusive
     }
     return v;
 }
-template <bool BY_ROW>
+template <bool BY_ROW, bool SHARED = false>
 __device__ static inline Share share_of(const AttendArgs& a, int at) {
     const odmkv_pages_t& p = a.p;
     const int lane = threadIdx.x & 63;
@@ -259,7 +265,7 @@ __device__ static inline Share share_of(const AttendArgs& a, int at) {
     if (a.splits == p.rows) return {at, at, 1};
     const auto blocks = [&](int row) {
         if (row >= p.rows) return 0;
-        const int len = p.length[row];
+        const int len = p.length[row] - (SHARED ? a.plan[1 + row] * BLOCK_TOKENS : 0);
         return (a.window > 0 ? min(len, min(a.window, 1 << 29) + a.L) : len) / BLOCK_TOKENS + 1;
     };
     long long total = 0;
@@ -269,10 +275,14 @@ __device__ static inline Share share_of(const AttendArgs& a, int at) {
         total += __builtin_amdgcn_readlane(wave_scan(mine), 63);
     }
     const int spare = a.splits - p.rows;
+    const auto share = [&](int blocks) {                        // (SHARED: what is not in common is short as a rule, and a share of less than a block a wavefront is none)
+        const int n = 1 + (int)((long long)blocks * spare / total);
+        return SHARED ? min(n, max(blocks / 4, 1)) : n;
+    };
     int before = 0;
     for (int r0 = 0; r0 < p.rows; r0 += 64) {
         if (p.rows > 64) mine = blocks(r0 + lane);
-        const int count = r0 + lane < p.rows ? 1 + (int)((long long)mine * spare / total) : 0;
+        const int count = r0 + lane < p.rows ? share(mine) : 0;
         const int upto = before + wave_scan(count);
         if (BY_ROW) {
             if (at < r0 + 64) return {at, __builtin_amdgcn_readlane(upto - count, at - r0), __builtin_amdgcn_readlane(count, at - r0)};
@@ -288,6 +298,51 @@ __device__ static inline Share share_of(const AttendArgs& a, int at) {
     return {-1, 0, 0};
 }
 
+// The plan of common blocks (pages.hip): groups of rows that have their first blocks in common.
+struct Plan {
+    const int32_t* at;
+    int rows;
+    __device__ inline Plan(const AttendArgs& a) : at(a.plan), rows(a.p.rows) {}
+    __device__ inline int groups() const { return at[0]; }
+    __device__ inline int common(int row) const { return at[1 + row]; }                     // blocks; 0: the row is in no group
+    __device__ inline int group(int row) const { return at[1 + rows + row]; }
+    __device__ inline int member(int row) const { return at[1 + 2 * rows + row]; }          // its place in the group
+    __device__ inline int order(int i) const { return at[1 + 3 * rows + i]; }               // rows, a group's behind one another
+    __device__ inline int begin(int g) const { return at[1 + 4 * rows + 3 * g]; }
+    __device__ inline int members(int g) const { return at[2 + 4 * rows + 3 * g]; }
+    __device__ inline int blocks(int g) const { return at[3 + 4 * rows + 3 * g]; }
+};
+
+#define SHARED_COLS 128      // queries of a kv-head that a workgroup takes over what is in common
+// The workgroups of a kv-head that take what is in common: one for each tile of a group, the `spare` others in proportion to the tiles' blocks, several blocks each at least:
+// a share costs its partial results.  Given a workgroup: its tile and share; given a group: how its tiles are shared; and where the group's partial results begin.
+struct CommonShare { int group, tile, split, splits, parts; };
+template <bool BY_GROUP = false>
+__device__ static inline CommonShare common_share_of(const AttendArgs& a, int at) {
+    const Plan plan(a);
+    const int lane = threadIdx.x & 63, R = a.G * a.L, groups = plan.groups();
+    const auto tiles_of = [&](int g) { return g < groups ? (plan.members(g) * R + SHARED_COLS - 1) / SHARED_COLS : 0; };
+    long long total = 0;
+    for (int g0 = 0; g0 < groups; g0 += 64) {
+        const int weight = tiles_of(g0 + lane) * (g0 + lane < groups ? plan.blocks(g0 + lane) : 0);
+        total += __builtin_amdgcn_readlane(wave_scan(weight), 63);
+    }
+    int before = 0, parts = 0;
+    for (int g0 = 0; g0 < groups; g0 += 64) {
+        const int g = g0 + lane, tiles = tiles_of(g), cols = g < groups ? plan.members(g) * R : 0, blocks = g < groups ? plan.blocks(g) : 0;
+        const int splits = min(1 + (int)((long long)blocks * a.spare / max(total, 1LL)), max(blocks / (cols > 64 ? 8 : 4), 1));
+        const int upto = before + wave_scan(tiles * splits), parts_upto = parts + wave_scan(splits * cols);
+        const unsigned long long here = BY_GROUP ? (at < g0 + 64 ? 1ULL << (at - g0) : 0) : __ballot(upto > at);
+        if (here) {
+            const int l = __builtin_ctzll(here), n = __builtin_amdgcn_readlane(splits, l), first = __builtin_amdgcn_readlane(upto - tiles * splits, l);
+            return {g0 + l, (at - first) / n, (at - first) % n, n, __builtin_amdgcn_readlane(parts_upto - splits * cols, l)};
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+        parts = __builtin_amdgcn_readlane(parts_upto, 63);
+    }
+    return {-1, 0, 0, 0, 0};
+}
+
 #define NARROW 16            // queries of a kv-head that the narrow kernel takes
 #define WIDE_WAVES 8
 
@@ -297,9 +352,14 @@ struct Cut {
     int groups;              // wide: 32s of queries of a workgroup; two for four wavefronts: two take the first half of every block, two the second
     bool wide, stream;       // stream: pages pass by the caches
     size_t parts;            // partial results
+    bool shared;             // rows have blocks in common: workgroups of a kv-head for those, of which `spare` beyond a tile's one, and their partial results
+    int workgroups, spare;
+    long long common_parts;
 };
 int launch_attend_narrow_f16(const AttendArgs& a, const Cut& cut, hipStream_t st);
 int launch_attend_narrow_bf16(const AttendArgs& a, const Cut& cut, hipStream_t st);
+int launch_attend_shared_f16(const AttendArgs& a, int workgroups, hipStream_t st);
+int launch_attend_shared_bf16(const AttendArgs& a, int workgroups, hipStream_t st);
 int launch_attend_wide_f16(const AttendArgs& a, const Cut& cut, hipStream_t st);
 int launch_attend_wide_bf16(const AttendArgs& a, const Cut& cut, hipStream_t st);
 

@@ -6,7 +6,8 @@
 // (32 queries, 64 shares each), 7.2 for 928 queries of 64 shares (31 MB).
 #define MERGE_AHEAD 8
 
-template <int DT, bool NARROW_PARTS>
+// SHARED: those of what the row has in common with others come first, its own behind them.
+template <int DT, bool NARROW_PARTS, bool SHARED>
 __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
     const odmkv_pages_t& p = a.p;
     const int R = a.G * a.L, r = blockIdx.x, h = blockIdx.y, row = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -15,10 +16,22 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
     __shared__ float part[4][HD], top_of[4], sum_of[4];
     int splits = a.splits;
     size_t at = ((size_t)row * p.Hkv + h) * a.splits * R + r;
+    int in_common = 0, cols = 0;
+    size_t common_at = 0;
+    if (SHARED) {
+        const Plan plan(a);
+        if (plan.common(row) > 0) {
+            const int g = plan.group(row);
+            const CommonShare share = common_share_of<true>(a, g);
+            in_common = share.splits;
+            cols = plan.members(g) * R;
+            common_at = (size_t)h * a.common_parts + share.parts + (size_t)plan.member(row) * R + r;
+        }
+    }
     if (NARROW_PARTS) {
-        const Share own = share_of<true>(a, row);
-        if (own.count == 1) return;                             // that workgroup has written the result
-        splits = own.count;
+        const Share own = share_of<true, SHARED>(a, row);
+        if (own.count == 1 && in_common == 0) return;           // that workgroup has written the result
+        splits = own.count + in_common;
         at = ((size_t)h * a.splits + own.first) * R + r;
     }
     // (each wavefront by its own largest: the partial results need not wait for the largest of all)
@@ -28,9 +41,11 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
         float2 v[MERGE_AHEAD];
 #pragma unroll
         for (int k = 0; k < MERGE_AHEAD; ++k) {
-            const size_t from = at + (size_t)min(i0 + 4 * k, splits - 1) * R;
-            lse[k] = a.part_lse[from];
-            v[k] = *reinterpret_cast<const float2*>(a.part_out + from * HD + 2 * lane);
+            const int i = min(i0 + 4 * k, splits - 1);
+            const bool common = SHARED && i < in_common;
+            const size_t from = common ? common_at + (size_t)i * cols : at + (size_t)(i - in_common) * R;
+            lse[k] = (common ? a.common_lse : a.part_lse)[from];
+            v[k] = *reinterpret_cast<const float2*>((common ? a.common_out : a.part_out) + from * HD + 2 * lane);
         }
         float to = top;
 #pragma unroll
@@ -79,11 +94,13 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
 static int launch_attend_merge(const AttendArgs& a, const Cut& cut, hipStream_t st) {
     const dim3 grid(a.G * a.L, a.p.Hkv, a.p.rows);
     if (a.p.dtype == ODMKV_F16) {
-        if (cut.wide) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_F16, false>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((attend_merge_kernel<ODMKV_F16, true>), grid, dim3(256), 0, st, a);
+        if (cut.shared) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_F16, true, true>), grid, dim3(256), 0, st, a);
+        else if (cut.wide) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_F16, false, false>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((attend_merge_kernel<ODMKV_F16, true, false>), grid, dim3(256), 0, st, a);
     } else {
-        if (cut.wide) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_BF16, false>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((attend_merge_kernel<ODMKV_BF16, true>), grid, dim3(256), 0, st, a);
+        if (cut.shared) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_BF16, true, true>), grid, dim3(256), 0, st, a);
+        else if (cut.wide) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_BF16, false, false>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((attend_merge_kernel<ODMKV_BF16, true, false>), grid, dim3(256), 0, st, a);
     }
     ODMKV_CHECK_LAUNCH("attend_merge_kernel");
     return 0;
@@ -93,7 +110,7 @@ static int launch_attend_merge(const AttendArgs& a, const Cut& cut, hipStream_t 
 // one of eight.  (A share more than that costs its partial results: with two of eight, 2048 queries over 4096 tokens took 330 us for 273, four of 777 145 for 51.)
 static Cut cut_of(const odmkv_pages_t& p, int R, int max_length) {
     const int blocks = max_length / BLOCK_TOKENS + 1, units = compute_units();
-    Cut c = {4, 1, 4, R > NARROW, false, 0};
+    Cut c = {4, 1, 4, R > NARROW, false, 0, false, 0, 0, 0};
     if (c.wide) {
         c.waves = R > 128 ? WIDE_WAVES : 4;
         c.groups = R <= 64 ? 2 : c.waves;
@@ -114,6 +131,28 @@ static Cut cut_of(const odmkv_pages_t& p, int R, int max_length) {
         c.parts = c.splits > p.rows ? (size_t)p.Hkv * c.splits * R : 0;
     }
     return c;
+}
+
+// Rows with blocks in common: how many workgroups what is in common gets is known on the device alone, which has one for each of a group's tiles and shares out the others.
+static Cut cut_shared(const odmkv_pages_t& p, int R, int max_length) {
+    Cut c = cut_of(p, R, max_length);
+    if (R > NARROW || p.rows < 2) return c;
+    const int blocks = max_length / BLOCK_TOKENS + 1, units = compute_units();
+    c.shared = true;
+    c.waves = 4;
+    c.stream = false;
+    c.splits = (int)std::max((long long)p.rows, std::min(2LL * units / p.Hkv, (long long)p.rows * std::max(1, blocks / 4)));
+    c.parts = (size_t)p.Hkv * c.splits * R;
+    c.spare = std::max(1, 2 * units / p.Hkv);
+    c.workgroups = (int)(((long long)p.rows * R + SHARED_COLS - 1) / SHARED_COLS) + p.rows / 2 + c.spare;
+    c.common_parts = (long long)p.rows * R + (long long)SHARED_COLS * c.spare;
+    return c;
+}
+
+extern "C" size_t odmkv_pages_attend_shared_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length) {
+    if (!p || p->Hkv <= 0 || p->rows <= 0 || Hq <= 0 || L <= 0 || max_length < 0) return 0;
+    const Cut c = cut_shared(*p, Hq / p->Hkv * L, max_length);
+    return align_up((c.parts + (size_t)p->Hkv * c.common_parts) * (HD + 1) * sizeof(float), 256);
 }
 
 extern "C" size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length) {
@@ -138,19 +177,24 @@ extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
                     "pages_attend: rows must be 16-byte aligned");
     AttendArgs a = {p, (const uint16_t*)d->q, d->q_stride_b, d->q_stride_h, d->q_stride_l, (uint16_t*)d->out, d->lse, d->counts, d->slopes,
                     d->prefix, d->starts, d->start_stride_b, d->start_stride_l, d->layer, d->L, d->Hq, d->Hq / p.Hkv, d->window, d->scaling, d->cap,
-                    1, nullptr, nullptr};
-    const size_t need = odmkv_pages_attend_workspace_bytes(&p, d->Hq, d->L, d->max_length);
+                    1, nullptr, nullptr, d->plan, 0, nullptr, nullptr, 0};
+    const size_t need = (d->plan ? odmkv_pages_attend_shared_workspace_bytes : odmkv_pages_attend_workspace_bytes)(&p, d->Hq, d->L, d->max_length);
     if (need > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)) {
         odmkv_set_error("pages_attend: workspace too small");
         return ODMKV_ENOSPACE;
     }
-    const Cut cut = cut_of(p, a.G * a.L, d->max_length);
+    const Cut cut = (d->plan ? cut_shared : cut_of)(p, a.G * a.L, d->max_length);
     a.splits = cut.splits;
     a.part_out = (float*)d->workspace;
     a.part_lse = a.part_out + cut.parts * HD;
     hipStream_t st = (hipStream_t)stream;
     const bool f16 = p.dtype == ODMKV_F16;
-    const int rc = cut.wide ? (f16 ? launch_attend_wide_f16(a, cut, st) : launch_attend_wide_bf16(a, cut, st))
+    a.spare = cut.spare;
+    a.common_out = a.part_lse + cut.parts;
+    a.common_parts = cut.common_parts;
+    a.common_lse = a.common_out + (size_t)p.Hkv * cut.common_parts * HD;
+    const int rc = cut.shared ? (f16 ? launch_attend_shared_f16(a, cut.workgroups, st) : launch_attend_shared_bf16(a, cut.workgroups, st))
+                 : cut.wide ? (f16 ? launch_attend_wide_f16(a, cut, st) : launch_attend_wide_bf16(a, cut, st))
                             : (f16 ? launch_attend_narrow_f16(a, cut, st) : launch_attend_narrow_bf16(a, cut, st));
     if (rc) return rc;
     return cut.parts ? launch_attend_merge(a, cut, st) : 0;

@@ -20,16 +20,16 @@
 
 #define NARROW_LDS(waves) ((waves) * NARROW * (HD + 4 + 2) * 4)
 
-template <int DT, int KIND, bool PLAIN, int WAVES, bool STREAM>
-__global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs a) {
+// SHARED: what rows have in common is read elsewhere (attend_shared.h), theirs begins behind it.
+template <int DT, int KIND, bool PLAIN, int WAVES, bool STREAM, bool SHARED>
+__device__ static inline void attend_rows(const AttendArgs& a, unsigned workgroup, float* narrow_lds) {
     const odmkv_pages_t& p = a.p;
-    extern __shared__ __align__(16) float narrow_lds[];
     float (*acc_of)[NARROW][HD + 4] = reinterpret_cast<float (*)[NARROW][HD + 4]>(narrow_lds);      // [WAVES]
     float (*ref_of)[NARROW] = reinterpret_cast<float (*)[NARROW]>(narrow_lds + WAVES * NARROW * (HD + 4));
     float (*sum_of)[NARROW] = ref_of + WAVES;
     // heads vary fastest: every head's longest row first, all heads alike
-    const int h = blockIdx.x % p.Hkv, group = blockIdx.x / p.Hkv;
-    const Share own = share_of<false>(a, group);
+    const int h = workgroup % p.Hkv, group = workgroup / p.Hkv;
+    const Share own = share_of<false, SHARED>(a, group);
     const int row = __builtin_amdgcn_readfirstlane(own.row), splits = __builtin_amdgcn_readfirstlane(own.count);
     if (row < 0) return;
     const int split = group - __builtin_amdgcn_readfirstlane(own.first);
@@ -39,6 +39,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
     const bool valid = n < R && l < count;
     Sight s = {0, 0, 0};
     if (valid) s = sight_of(a, row, len, count, l);
+    const int in_common = SHARED ? a.plan[1 + row] : 0;
+    if (SHARED) s.lo = max(s.lo, in_common * BLOCK_TOKENS);
     const bool sees = valid && s.lo < s.hi;
     const int first = wave_min_int(sees ? s.lo : 0x7fffffff) / BLOCK_TOKENS;
     const int last = (-wave_min_int(sees ? -s.hi : 0) + BLOCK_TOKENS - 1) / BLOCK_TOKENS;        // one past the last block that is seen
@@ -308,7 +310,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = total == 0.0f ? 0.0f : o[e] * inv;
     const float lse2 = total == 0.0f ? -INFINITY : to + __builtin_amdgcn_logf(total);
-    if (splits > 1) {
+    if (splits > 1 || in_common > 0) {
         const size_t unit_at = ((size_t)h * a.splits + group) * R + r;
         f32x4* dst = reinterpret_cast<f32x4*>(a.part_out + unit_at * HD + d);
         dst[0] = f32x4{o[0], o[1], o[2], o[3]};
@@ -321,6 +323,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs
     for (int e = 0; e < 4; ++e) b[e] = (uint32_t)to_16<DT>(o[2 * e]) | (uint32_t)to_16<DT>(o[2 * e + 1]) << 16;
     *reinterpret_cast<uint4*>(a.out + (((size_t)row * a.L + rl) * a.Hq + rh) * HD + d) = make_uint4(b[0], b[1], b[2], b[3]);
     if (a.lse && d == 0) a.lse[((size_t)row * a.Hq + rh) * a.L + rl] = lse2 * LN2;
+}
+
+template <int DT, int KIND, bool PLAIN, int WAVES, bool STREAM>
+__global__ __launch_bounds__(WAVES * 64, 2) void attend_narrow_kernel(AttendArgs a) {
+    extern __shared__ __align__(16) float narrow_lds[];
+    attend_rows<DT, KIND, PLAIN, WAVES, STREAM, false>(a, blockIdx.x, narrow_lds);
 }
 
 template <int DT>

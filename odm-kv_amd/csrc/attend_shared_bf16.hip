@@ -1,0 +1,4 @@
+// The bf16 kernels of attend_shared.h, in a file of their own: the compiler takes them beside the others.
+#include "attend_shared.h"
+
+int launch_attend_shared_bf16(const AttendArgs& a, int workgroups, hipStream_t st) { return launch_shared_of<ODMKV_BF16>(a, workgroups, st); }

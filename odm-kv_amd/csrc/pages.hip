@@ -509,6 +509,87 @@ extern "C" int odmkv_pages_truncate(const odmkv_pages_t* p, const int32_t* lengt
     return 0;
 }
 
+// ---- what rows have in common ---------------------------------------------------------------------
+// Rows whose first page is the same are a group; two rows have blocks in common up to the first whose pages differ (a page that two rows hold at the same block came there by
+// a copy of everything before it), a group what each of its rows has in common with its first one.  One workgroup, a thread a row; the first different block is looked for
+// in eight places at a time.
+__global__ __launch_bounds__(BOOK_THREADS) void pages_plan_common_kernel(odmkv_pages_t p, int32_t* plan) {
+    __shared__ int part[BOOK_THREADS / 64], page0[MAX_ROWS], full[MAX_ROWS], slots[MAX_ROWS], leaders[MAX_ROWS], least[MAX_ROWS], count[MAX_ROWS], begin[MAX_ROWS], number[MAX_ROWS];
+    const int tid = threadIdx.x, rows = p.rows;
+    const bool mine = tid < rows;
+    if (mine) {
+        slots[tid] = p.slot[tid];
+        full[tid] = p.length[tid] / BLOCK_TOKENS;
+        page0[tid] = full[tid] > 0 ? p.table[(size_t)slots[tid] * p.blocks] : -1 - tid;
+        least[tid] = full[tid];
+        count[tid] = 0;
+    }
+    __syncthreads();
+    int leader = tid, rank = 0;
+    if (mine) {
+        for (int j = tid - 1; j >= 0; --j) {
+            if (page0[j] != page0[tid]) continue;
+            leader = j;
+            rank += 1;
+        }
+        leaders[tid] = leader;
+        int same = min(full[tid], full[leader]);
+        if (leader != tid) {
+            const int32_t* a = p.table + (size_t)slots[tid] * p.blocks;
+            const int32_t* b = p.table + (size_t)slots[leader] * p.blocks;
+            int lo = 1, hi = same;                             // as many blocks are the same, and no more than that
+            while (lo < hi) {
+                const int step = (hi - lo + 7) / 8;
+                int equal = 0;
+#pragma unroll
+                for (int k = 1; k <= 8; ++k) {
+                    const int at = min(lo + k * step, hi) - 1;
+                    equal += a[at] == b[at] ? 1 : 0;
+                }
+                if (equal < 8) hi = min(lo + (equal + 1) * step, hi + 1) - 1;
+                lo = min(lo + equal * step, hi);
+            }
+            same = lo;
+        }
+        atomicMin(&least[leader], same);
+        atomicAdd(&count[leader], 1);
+    }
+    __syncthreads();
+    const bool is_group = mine && leader == tid && count[tid] > 1;
+    int n, total;
+    const int g = book_scan(is_group ? 1 : 0, part, n) - 1, end = book_scan(is_group ? count[tid] : 0, part, total);
+    if (is_group) {
+        number[tid] = g;
+        begin[tid] = end - count[tid];
+        int32_t* const to = plan + 1 + 4 * rows + 3 * g;
+        to[0] = begin[tid];
+        to[1] = count[tid];
+        to[2] = least[tid];
+    }
+    if (tid == 0) plan[0] = n;
+    __syncthreads();
+    if (!mine) return;
+    const bool grouped = count[leader] > 1;
+    plan[1 + tid] = grouped ? least[leader] : 0;
+    plan[1 + rows + tid] = grouped ? number[leader] : -1;
+    plan[1 + 2 * rows + tid] = rank;
+    if (grouped) plan[1 + 3 * rows + begin[leader] + rank] = tid;
+}
+
+extern "C" size_t odmkv_pages_plan_bytes(int rows) { return rows > 0 ? align_up(plan_words(rows) * sizeof(int32_t), 256) : 0; }
+
+extern "C" int odmkv_pages_plan(const odmkv_pages_t* p, int32_t* plan, size_t plan_bytes, void* stream) {
+    if (int rc = check_pages("pages_plan", p)) return rc;
+    ODMKV_CHECK_ARG(plan != nullptr && ((uintptr_t)plan & 15) == 0, "pages_plan: null or unaligned pointer");
+    if (plan_bytes < odmkv_pages_plan_bytes(p->rows)) {
+        odmkv_set_error("pages_plan: plan too small");
+        return ODMKV_ENOSPACE;
+    }
+    hipLaunchKernelGGL(pages_plan_common_kernel, dim3(1), dim3(BOOK_THREADS), 0, (hipStream_t)stream, *p, plan);
+    ODMKV_CHECK_LAUNCH("pages_plan_common_kernel");
+    return 0;
+}
+
 // ---- compaction -----------------------------------------------------------------------------------
 // One workgroup: where every page goes (its rank among those in use, -1: free), and the new pool's counts.
 __global__ __launch_bounds__(BOOK_THREADS) void pages_rank_kernel(odmkv_pages_t p, odmkv_pages_t to, int32_t* where) {

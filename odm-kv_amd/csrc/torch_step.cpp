@@ -257,11 +257,11 @@ PyObject* native_paged_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // paged_attend(attend entry, workspace entry, pages, device, layer, query, scaling, cap, window, max_length, want_lse, counts, slopes, prefix, starts,
-// stream): out, or (out, lse), or None.  counts, slopes, prefix, starts: None, or tensors of the right type and shape, contiguous.
+// stream, plan): out, or (out, lse), or None.  counts, slopes, prefix, starts: None, or tensors of the right type and shape, contiguous.
 PyObject* native_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    if (n != 16 || !THPVariable_Check(a[5])) {
+    if (n != 17 || !THPVariable_Check(a[5])) {
         PyErr_SetString(PyExc_TypeError, "paged_attend(attend, bytes, pages, device, layer, query, scaling, cap, window, max_length, want_lse, counts, "
-                                         "slopes, prefix, starts, stream)");
+                                         "slopes, prefix, starts, stream, plan)");
         return nullptr;
     }
     const attend_fn fn = (attend_fn)(uintptr_t)PyLong_AsUnsignedLongLong(a[0]);
@@ -275,6 +275,7 @@ PyObject* native_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const long long longest = PyLong_AsLongLong(a[9]);
     const int want_lse = PyObject_IsTrue(a[10]);
     const unsigned long long stream = PyLong_AsUnsignedLongLong(a[15]);
+    const unsigned long long plan = PyLong_AsUnsignedLongLong(a[16]);
     if (PyErr_Occurred()) return nullptr;
     GUARDED(
         const at::Tensor& q = THPVariable_Unpack(a[5]);
@@ -316,7 +317,7 @@ PyObject* native_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         d.workspace = bytes ? ws.data_ptr() : nullptr; d.workspace_bytes = bytes;
         d.layer = (int)layer; d.L = (int)L; d.Hq = (int)Hq; d.window = (int)window; d.max_length = (int)longest;
-        d.scaling = (float)scaling; d.cap = (float)cap;
+        d.scaling = (float)scaling; d.cap = (float)cap; d.plan = (const int32_t*)(uintptr_t)plan;
         const int rc = fn(&d, (void*)(uintptr_t)stream);
         if (rc) return raise_odmkv(rc, "attention over the paged cache");
         if (!want_lse) return THPVariable_Wrap(std::move(out));

@@ -94,7 +94,8 @@ class Attend(C.Structure):
     _fields_ = ([("pages", C.POINTER(Pages)), ("q", C.c_void_p)] + [(n, C.c_int64) for n in ("q_stride_b", "q_stride_h", "q_stride_l")]
                 + [(n, C.c_void_p) for n in ("out", "lse", "counts", "slopes", "prefix", "starts")]
                 + [("start_stride_b", C.c_int64), ("start_stride_l", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
-                + [(n, C.c_int32) for n in ("layer", "L", "Hq", "window", "max_length")] + [("scaling", C.c_float), ("cap", C.c_float)])
+                + [(n, C.c_int32) for n in ("layer", "L", "Hq", "window", "max_length")] + [("scaling", C.c_float), ("cap", C.c_float)]
+                + [("plan", C.c_void_p)])
 
 
 class Rotate(C.Structure):
@@ -203,6 +204,9 @@ def _load() -> C.CDLL:
         "odmkv_pages_truncate": (C.c_int, [C.POINTER(Pages), vp, vp, i32, vp, vp]),
         "odmkv_pages_compact_workspace_bytes": (sz, [i32]),
         "odmkv_pages_compact": (C.c_int, [C.POINTER(Pages), C.POINTER(Pages), vp, sz, vp]),
+        "odmkv_pages_plan_bytes": (sz, [i32]),
+        "odmkv_pages_plan": (C.c_int, [C.POINTER(Pages), vp, sz, vp]),
+        "odmkv_pages_attend_shared_workspace_bytes": (sz, [C.POINTER(Pages), i32, i32, i32]),
         "odmkv_pages_attend_workspace_bytes": (sz, [C.POINTER(Pages), i32, i32, i32]),
         "odmkv_pages_attend": (C.c_int, [C.POINTER(Attend), vp]),
         "odmkv_prompt_attend_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
@@ -217,7 +221,8 @@ def _load() -> C.CDLL:
 
 lib = _load()
 STEP_ENTRY = C.cast(lib.odmkv_decode_step, C.c_void_p).value      # what _native.Step calls
-PAGES_ENTRIES = tuple(C.cast(f, C.c_void_p).value for f in (lib.odmkv_pages_write, lib.odmkv_pages_attend, lib.odmkv_pages_attend_workspace_bytes))
+PAGES_ENTRIES = tuple(C.cast(f, C.c_void_p).value for f in (lib.odmkv_pages_write, lib.odmkv_pages_attend, lib.odmkv_pages_attend_workspace_bytes,
+                                                                   lib.odmkv_pages_attend_shared_workspace_bytes))
 EXPORTS = ("odmkv_version", "odmkv_last_error", "odmkv_score_workspace_bytes", "odmkv_score", "odmkv_score_model_dtype", "odmkv_score_expected", "odmkv_token_mean_workspace_bytes", "odmkv_token_mean", "odmkv_average_rope",
            "odmkv_project_rows", "odmkv_prompt_scores_workspace_bytes", "odmkv_prompt_scores", "odmkv_query_covariance_workspace_bytes", "odmkv_query_covariance", "odmkv_rotate_queries",
            "odmkv_normalize_workspace_bytes", "odmkv_normalize_scores",
@@ -230,7 +235,8 @@ EXPORTS = ("odmkv_version", "odmkv_last_error", "odmkv_score_workspace_bytes", "
            "odmkv_worklist_cut", "odmkv_decode_workspace_bytes", "odmkv_rotation_operands", "odmkv_decode_attn", "odmkv_decode_attn_static",
            "odmkv_decode_step", "odmkv_decode_block_workspace_bytes", "odmkv_decode_block", "odmkv_block_merge", "odmkv_exact_tail", "odmkv_flush_score", "odmkv_flush_rank",
            "odmkv_pages_init", "odmkv_pages_extend", "odmkv_pages_write", "odmkv_pages_write_rotated", "odmkv_pages_read", "odmkv_pages_reorder_workspace_bytes", "odmkv_pages_reorder", "odmkv_pages_select",
-           "odmkv_pages_truncate", "odmkv_pages_compact_workspace_bytes", "odmkv_pages_compact", "odmkv_pages_attend_workspace_bytes", "odmkv_pages_attend", "odmkv_prompt_attend_workspace_bytes", "odmkv_prompt_attend")
+           "odmkv_pages_truncate", "odmkv_pages_compact_workspace_bytes", "odmkv_pages_compact", "odmkv_pages_plan_bytes", "odmkv_pages_plan", "odmkv_pages_attend_shared_workspace_bytes",
+           "odmkv_pages_attend_workspace_bytes", "odmkv_pages_attend", "odmkv_prompt_attend_workspace_bytes", "odmkv_prompt_attend")
 
 
 def check(rc: int) -> None:

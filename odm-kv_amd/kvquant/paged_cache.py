@@ -36,7 +36,7 @@ KINDS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 _SCALING = HEAD_DIM ** -0.5
 _FAR = 2 ** 30                                # a window past everything
 _LEAST_CAP = 2.0 ** -100                      # (what 32 bits make 0 of would be no cap)
-_WRITE, _ATTEND, _ATTEND_BYTES = _lib.PAGES_ENTRIES
+_WRITE, _ATTEND, _ATTEND_BYTES, _SHARED_BYTES = _lib.PAGES_ENTRIES
 _native = _lib._native
 _device = torch.cuda.current_device
 _capturing = torch.cuda.is_current_stream_capturing
@@ -401,7 +401,7 @@ class PagedKVCache:
     def attend(self, layer: int, query: torch.Tensor, *, scaling: Optional[float] = None, softcap: Optional[float] = None,
                slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, prefix: Optional[torch.Tensor] = None,
                starts: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, return_lse: bool = False,
-               longest: Optional[int] = None):
+               longest: Optional[int] = None, shared: bool = False):
         """Attention of the newest tokens' queries, query [B, Hq, L, 128], over one layer, which holds those tokens already -> [B, L, Hq, 128] of
         the same type, and on request lse fp32 [B, Hq, L].
 
@@ -412,6 +412,10 @@ class PagedKVCache:
         (default 128 ** -0.5), then softcap * tanh(x / softcap), then less slope * |i - j| (`slopes`, fp32 [Hq]).  Queries that see nothing
         get 0, and -inf for lse.
 
+        `shared`: blocks that rows have in common (the pages that ``reorder`` and ``select`` let them share) are read once for all of them; for batches whose rows share most of what
+        they hold, samples or beams of long prompts.  The result is the same but for the order of sums.  Up to 16 queries of a kv-head (its query heads times L); more take the ordinary way.  Which
+        blocks those are is worked out on the device by the first such call (make it before a graph is captured), and again whenever rows are moved or cut.
+
         `longest`: about how long the longest row is, which decides how the work is cut and nothing else (default: the host's bound, and while a graph is captured
         max_tokens, since the rows may be that long at a replay)."""
         self._check_stored(layer)
@@ -420,11 +424,12 @@ class PagedKVCache:
         elif longest < 0:
             raise ValueError(f"longest must not be negative, got {longest}")
         longest = min(longest, self.max_tokens)
+        plan = self._plan_of_common() if shared else 0
         if _device() == self.device.index and isinstance(query, torch.Tensor) and (softcap is None or _LEAST_CAP <= softcap < math.inf) and (window is None or window >= 1):
             # (everything as the kernels take it: one native call)
-            done = _native.paged_attend(_ATTEND, _ATTEND_BYTES, self._at, self.device.index, layer, query, _SCALING if scaling is None else scaling,
+            done = _native.paged_attend(_ATTEND, _SHARED_BYTES if plan else _ATTEND_BYTES, self._at, self.device.index, layer, query, _SCALING if scaling is None else scaling,
                                         0.0 if softcap is None else softcap, 0 if window is None else min(window, _FAR), longest, return_lse,
-                                        counts, slopes, prefix, starts, _lib.stream_ptr(self.device))
+                                        counts, slopes, prefix, starts, _lib.stream_ptr(self.device), plan)
             if done is not None:
                 return done
         self._check_layer(layer)
@@ -448,15 +453,39 @@ class PagedKVCache:
         out = make(B, L, Hq, HEAD_DIM, dtype=query.dtype, device=self.device)
         lse = make(B, Hq, L, dtype=torch.float32, device=self.device) if return_lse else None
         if L:
-            nbytes = lib.odmkv_pages_attend_workspace_bytes(C.byref(self._p), Hq, L, longest)
+            nbytes = (lib.odmkv_pages_attend_shared_workspace_bytes if plan else lib.odmkv_pages_attend_workspace_bytes)(C.byref(self._p), Hq, L, longest)
             # (of its own for every call: two graphs that share one would race, and a graph's is the graph's)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
             a = _lib.Attend(C.pointer(self._p), query.data_ptr(), *query.stride()[:3], out.data_ptr(), _lib.ptr(lse), _lib.ptr(counts), _lib.ptr(slopes),
                             _lib.ptr(prefix), _lib.ptr(starts), 0 if starts is None else starts.stride(0),
                             0 if starts is None or starts.dim() == 1 else starts.stride(1), _lib.ptr(ws), nbytes, layer, L, Hq, min(window or 0, _FAR), longest,
-                            scaling, 0.0 if softcap is None else float(softcap))
+                            scaling, 0.0 if softcap is None else float(softcap), plan)
             self._call(lib.odmkv_pages_attend, C.byref(a))
         return (out, lse) if return_lse else out
+
+    # the plan of common blocks: made by the first call that asks for it, made again by whatever moves or cuts rows, so that replays of captured calls keep it right as well
+    _plan: Optional[torch.Tensor] = None
+    _unplanned = False                                       # rows may be moved by replays of calls that were captured while there was no plan
+
+    def _plan_of_common(self) -> int:
+        """The plan's address; it is of the tables as they are, or will be where the current call runs."""
+        if self._plan is None:
+            if _capturing():
+                raise RuntimeError("which blocks rows have in common is worked out by the first call with shared=True: make one before a graph is captured")
+            self._plan = torch.empty(lib.odmkv_pages_plan_bytes(self.batch) // 4, dtype=torch.int32, device=self.device)
+            self._make_plan()
+        elif self._unplanned:
+            self._make_plan()
+        return self._plan.data_ptr()
+
+    def _make_plan(self) -> None:
+        self._call(lib.odmkv_pages_plan, C.byref(self._p), self._plan.data_ptr(), self._plan.numel() * 4)
+
+    def _rows_moved(self) -> None:
+        if self._plan is not None:
+            self._make_plan()
+        elif _capturing():
+            self._unplanned = True
 
     def _small(self, t, what: str, dtype: torch.dtype, shapes):
         """A small operand on the cache's device, of its type and contiguous."""
@@ -486,6 +515,7 @@ class PagedKVCache:
         nbytes = lib.odmkv_pages_reorder_workspace_bytes(self.batch)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self._call(lib.odmkv_pages_reorder, C.byref(self._p), _lib.ptr(on_device), host, ws.data_ptr(), nbytes)
+        self._rows_moved()
 
     def select(self, parents) -> "PagedKVCache":
         """A batch of its own over the same pages, whose row b is a copy of this one's row parents[b]; this one's rows stay (``release`` it where it is
@@ -538,6 +568,7 @@ class PagedKVCache:
         if known is not None and min(known) < 0:
             raise ValueError(f"a length must not be negative, got {min(known)}")
         self._call(lib.odmkv_pages_truncate, C.byref(self._p), _lib.ptr(on_device), host, min(lengths, self.max_tokens) if isinstance(lengths, int) else 0, mask)
+        self._rows_moved()
         self._nothing_to_write()
         if known is not None:
             for b in meant:

@@ -66,3 +66,28 @@ def test_python_refuses_prompts_without_a_gpu():
         prompt_attention(q, q, q)
     with pytest.raises(ValueError, match="queries must be"):
         prompt_attention(None, q, q)
+
+
+@pytest.mark.parametrize("change,says", BAD, ids=[next(iter(c)) + "=" + str(next(iter(c.values()))) for c, _ in BAD])
+def test_a_plan_of_a_bad_cache_is_refused(change, says):
+    from kvquant._lib import lib
+    assert lib.odmkv_pages_plan(C.byref(_pages(**change)), 4096, 1 << 20, None) == -1 and says in _error(), _error()
+
+
+def test_bad_plans_are_refused():
+    from kvquant._lib import Attend, lib
+    pages = _pages()
+    p = C.byref(pages)
+    need = lib.odmkv_pages_plan_bytes(3)
+    assert need >= 4 * (1 + 4 * 3 + 3) and lib.odmkv_pages_plan_bytes(0) == 0
+    assert lib.odmkv_pages_plan(p, 0, need, None) == -1 and lib.odmkv_pages_plan(p, 4100, need, None) == -1 and "aligned" in _error()
+    assert lib.odmkv_pages_plan(p, 4096, need - 1, None) == -2 and "too small" in _error()
+    a = Attend(C.pointer(pages), 4096, 1024, 128, 1024, 4096, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 8, 0, 100, 0.1, 0.0, 4096)
+    need = lib.odmkv_pages_attend_shared_workspace_bytes(p, 8, 1, 100)
+    assert need > lib.odmkv_pages_attend_workspace_bytes(p, 8, 1, 100)
+    assert lib.odmkv_pages_attend(C.byref(a), None) == -2 and "workspace" in _error()
+    a.workspace, a.workspace_bytes = 4096, need - 1
+    assert lib.odmkv_pages_attend(C.byref(a), None) == -2
+    assert lib.odmkv_pages_attend_shared_workspace_bytes(None, 8, 1, 100) == 0
+    # what takes the ordinary way takes its workspace
+    assert lib.odmkv_pages_attend_shared_workspace_bytes(p, 8, 40, 9000) == lib.odmkv_pages_attend_workspace_bytes(p, 8, 40, 9000)

@@ -738,7 +738,8 @@ int odmkv_pages_attend(const odmkv_attend_t* a, void* stream);
  *   x_j = scaling * q . k_j;  cap > 0: x_j = cap * tanh(x_j / cap);  out = sum_j softmax(x)_j v_j,  lse = log sum_j exp(x_j);
  * a query that sees nothing: 0 and -inf.  What a query does not see has no part in its result, infinities and NaN
  * included (0 times them would be NaN).
- * q [rows, Hq, L, 128], k, v [rows, Hkv, T, 128] of dtype (fp16, bf16) with element strides (multiples of 8, 16-byte aligned); out [rows, L, Hq, 128], lse fp32 [rows, Hq, L] contiguous.
+ * q [rows, Hq, L, 128], k, v [rows, Hkv, T, 128] of dtype (fp16, bf16) with element strides (multiples of 8, 16-byte aligned, of a
+ * token below 2^24); out [rows, L, Hq, 128], lse fp32 [rows, Hq, L] contiguous.
  * Packed, with offsets (device int32 [rows + 1], ascending): q [Hq, L, 128], L the queries of all rows, row b's from offsets[b] to before offsets[b + 1]; k, v
  * [Hkv, T, 128] by key_offsets, or by offsets where that is NULL; out [L, Hq, 128], lse [Hq, L], 0 and -inf for queries that no row has; strides of a row are not looked at.  Nothing outside
  * the tensors is read or written, whatever offsets and starts say. */

@@ -120,3 +120,7 @@ __device__ static inline float wave_max(float v) { return wave_fold(v, [](float 
 __device__ static inline void request_to_lds(const uint16_t* from, uint32_t to) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(to) : "memory");      // (m0 is the place in LDS)
 }
+// the same from `bytes` behind a place that is one for the wavefront
+__device__ static inline void request_to_lds(const uint16_t* from, uint32_t bytes, uint32_t to) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(bytes), "s"(from), "{m0}"(to) : "memory");
+}

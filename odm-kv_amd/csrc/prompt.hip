@@ -109,8 +109,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
         hi = a.causal ? max(pos + 1, 0) : tile.m;
     }
     const bool sees = lo < hi;
-    const int wave_lo = wave_min_int(sees ? lo : 0x7fffffff), wave_hi = -wave_min_int(sees ? -hi : 0);          // what some query of the wavefront sees
-    const int open_from = -wave_min_int(valid ? -(sees ? lo : 0x7fffffff) : 0), open_to = wave_min_int(valid ? hi : 0x7fffffff);    // what all of them see
+    const auto least = [](int x) { return __builtin_amdgcn_readfirstlane(wave_min_int(x)); };
+    const int wave_lo = least(sees ? lo : 0x7fffffff), wave_hi = -least(sees ? -hi : 0);                        // what some query of the wavefront sees
+    const int open_from = -least(valid ? -(sees ? lo : 0x7fffffff) : 0), open_to = least(valid ? hi : 0x7fffffff);      // what all of them see
     if (lane == 0) {
         range[0][wave] = wave_lo;
         range[1][wave] = wave_hi;
@@ -130,24 +131,42 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     const uint16_t* const K = a.k + (a.offsets ? tile.k0 * a.kt : row * a.kb) + h * a.kh;
     const uint16_t* const V = a.v + (a.offsets ? tile.k0 * a.vt : row * a.vb) + h * a.vh;
     const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    uint32_t key_from[PIECES], value_from[PIECES];              // bytes from a block's first token
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+        const int e = tid + WAVES * 64 * c, t = e >> 4, p = e & 15;
+        key_from[c] = 2 * (t * (int)a.kt + 8 * (p ^ (t & 15)));
+        value_from[c] = 2 * (t * (int)a.vt + 8 * (p ^ ((t & 7) << 1)));
+    }
     const auto request = [&](int i) {
+        const int t0 = (b0 + i) * BLOCK_TOKENS, behind = tile.m - 1 - t0;
+        const uint16_t* const keys = K + t0 * a.kt;
+        const uint16_t* const values = V + t0 * a.vt;
 #pragma unroll
         for (int c = 0; c < PIECES; ++c) {
-            const int e = tid + WAVES * 64 * c, t = e >> 4, p = e & 15;
-            const int64_t at = min((b0 + i) * BLOCK_TOKENS + t, tile.m - 1);
             const uint32_t to = lds0 + (i & 1) * 2 * PROMPT_TILE + (WAVES * 64 * c + 64 * wave) * 16;
-            request_to_lds(K + at * a.kt + 8 * (p ^ (t & 15)), to);
-            request_to_lds(V + at * a.vt + 8 * (p ^ ((t & 7) << 1)), to + PROMPT_TILE);
+            uint32_t of_key = key_from[c], of_value = value_from[c];
+            if (behind < BLOCK_TOKENS - 1) {
+                const int over = max(((tid + WAVES * 64 * c) >> 4) - behind, 0);
+                of_key -= 2 * over * (int)a.kt;
+                of_value -= 2 * over * (int)a.vt;
+            }
+            request_to_lds(keys, of_key, to);
+            request_to_lds(values, of_value, to + PROMPT_TILE);
         }
     };
     if (mine > 0) request(0);
 
-    uint4 q[8];                                                 // dims 16 st + 8 half + e
+    uint4 q[8];                                                 // dims 16 st + 8 half + e; of the last query where there is none
     {
-        const uint16_t* src = a.q + (a.offsets ? (int64_t)(tile.q0 + l) * a.qt : row * a.qb + l * a.qt) + hq * a.qh + 8 * half;
+        const int at = min(l, tile.n - 1);
+        const uint16_t* src = a.q + (a.offsets ? (int64_t)(tile.q0 + at) * a.qt : row * a.qb + at * a.qt) + hq * a.qh + 8 * half;
 #pragma unroll
-        for (int st = 0; st < 8; ++st) q[st] = valid ? *reinterpret_cast<const uint4*>(src + 16 * st) : make_uint4(0, 0, 0, 0);
+        for (int st = 0; st < 8; ++st) q[st] = *reinterpret_cast<const uint4*>(src + 16 * st);
     }
+    // (they have come when the loop begins: waited for in the loop, they would be waited for in every turn, and the next block with them)
+#pragma unroll
+    for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(q[st].x), "+v"(q[st].y), "+v"(q[st].z), "+v"(q[st].w));
     const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
     const bool by_exp = MODE == 1 || (!PLAIN && a.cap > 0.0f && a.cap <= CAP_BY_EXP);
     const Cap cap = {a.cap * LOG2E, 2.0f * LOG2E * a.cap, 2.0f * LOG2E * inv_cap};
@@ -163,70 +182,36 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[db][e] = 0.0f;
 
-    const int key_at = col * 256 + ((half ^ (col & 15)) << 4);                                      // piece 2 st + half of token col
-    const int value_token = 4 * half + ((lane & 15) >> 2);                                          // a lane reads four dims of a token, and gets four tokens of a dim
-    const int value_at = value_token * 256 + (((lane >> 4 & 1) ^ value_token) << 5) + ((lane & 3) << 3);
-#pragma unroll 1
-    for (int i = 0; i < mine; ++i) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // this block has come, and nobody reads the one before any more
-        if (i + 1 < mine) request(i + 1);
-        const int t0 = (b0 + i) * BLOCK_TOKENS;
-        if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;                  // (of the wavefront's own queries none sees the block)
-        const uint8_t* const keys = smem + (i & 1) * 2 * PROMPT_TILE;
-        const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
+    // where a lane's operands lie in LDS, of the first buffer: of token `col` its pieces 2 st + half; of values four dims of a token, of which the lane gets four tokens of a dim
+    uint32_t key_at[8], value_at[4];
+    const int value_token = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+    for (int st = 0; st < 8; ++st) key_at[st] = lds0 + col * 256 + (((2 * st + half) ^ (col & 15)) << 4);
+#pragma unroll
+    for (int db = 0; db < 4; ++db) value_at[db] = lds0 + PROMPT_TILE + value_token * 256 + (((2 * db + (lane >> 4 & 1)) ^ value_token) << 5) + ((lane & 3) << 3);
+
+    const auto block = [&](uint32_t buffer, int t0) {
         f32x16 dot[2];
         uint4 w[4];
         const auto multiply_keys = [&](int tb) {
+            typedef const __attribute__((address_space(3))) u32x4* place;
 #pragma unroll
             for (int e = 0; e < 16; ++e) dot[tb][e] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < 8; ++st)
-                dot[tb] = multiply<DT>(*reinterpret_cast<const uint4*>(keys + 32 * 256 * tb + (key_at ^ (st << 5))), q[st], dot[tb]);
+            for (int st = 0; st < 8; ++st) {
+                const u32x4 x = *(place)(size_t)(key_at[st] + buffer + 32 * 256 * tb);
+                dot[tb] = multiply<DT>(make_uint4(x[0], x[1], x[2], x[3]), q[st], dot[tb]);
+            }
         };
         const auto multiply_values = [&](int st) {
+            typedef __attribute__((address_space(3))) s16x4* place;
 #pragma unroll
             for (int db = 0; db < 4; ++db) {
-                typedef __attribute__((address_space(3))) s16x4* place;
-                const uint32_t at = lds0 + (i & 1) * 2 * PROMPT_TILE + PROMPT_TILE + 16 * 256 * st + (value_at ^ (db << 6));
+                const uint32_t at = value_at[db] + buffer + 16 * 256 * st;
                 const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(size_t)at), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(size_t)(at + 8 * 256));
                 const uint2 u = __builtin_bit_cast(uint2, x), v = __builtin_bit_cast(uint2, y);
                 acc[db] = multiply<DT>(make_uint4(u.x, u.y, v.x, v.y), w[st], acc[db]);
             }
-        };
-        // products of half a block to scores (PLAIN: they stay products); the largest score
-        const auto to_scores = [&](int tb) {
-            f32x16& x = dot[tb];
-            if constexpr (!PLAIN) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = score(x[e]);
-            }
-            if (cut) {
-                const int tl = t0 + 32 * tb + 4 * half;         // token of score e: tl + 8 (e / 4) + e % 4
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int t = tl + 8 * (e >> 2) + (e & 3);
-                    x[e] = t >= lo && t < hi ? x[e] : -INFINITY;
-                }
-            }
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-            return PLAIN && top > -INFINITY ? top * c : top;    // (c is positive: the largest product is the largest score)
-        };
-        // the reference where a score is to move it, each query by itself; what the sums are to be multiplied by
-        const auto move_sums = [&](float top, float& old) {
-            if (!__any(top > ref + Weights<DT>::RISE_BY)) return false;
-            const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-            const float to = most > ref + Weights<DT>::RISE_BY ? most : ref;
-            old = ref > -INFINITY ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
-            sum *= old;
-            ref = to;
-            return true;
-        };
-        const auto multiply_sums = [&](float old) {
-#pragma unroll
-            for (int db = 0; db < 4; ++db) acc[db] *= old;
         };
         const auto weigh = [&](int tb) {
             const float shift = LIFT - (ref > -INFINITY ? ref : 0.0f);
@@ -244,19 +229,62 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
             w[2 * tb + 1] = make_uint4(word[4], word[5], word[6], word[7]);
             sum += z0 + z1;
         };
-        // the two halves' vector work stands beside the other half's matrix work
-        float old;
+        const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
+        // products of half a block to scores (PLAIN: they stay products); the reference where a score is to move it, each query's by itself
+        const auto look = [&](int tb) {
+            f32x16& x = dot[tb];
+            if constexpr (!PLAIN) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = score(x[e]);
+            }
+            if (cut) {
+                const int tl = t0 + 32 * tb + 4 * half;         // token of score e: tl + 8 (e / 4) + e % 4
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int t = tl + 8 * (e >> 2) + (e & 3);
+                    x[e] = t >= lo && t < hi ? x[e] : -INFINITY;
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+            if (PLAIN) top = top > -INFINITY ? top * c : top;   // (c is positive: the largest product is the largest score)
+            if (!__any(top > ref + Weights<DT>::RISE_BY)) return;
+            const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+            const float to = most > ref + Weights<DT>::RISE_BY ? most : ref;
+            const float old = ref > -INFINITY ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
+            sum *= old;
+            ref = to;
+#pragma unroll
+            for (int db = 0; db < 4; ++db) acc[db] *= old;
+        };
         multiply_keys(0);
-        if (move_sums(to_scores(0), old)) multiply_sums(old);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        look(0);
         multiply_keys(1);
         weigh(0);
-        const bool moved = move_sums(to_scores(1), old);
+        look(1);
         multiply_values(0);
         multiply_values(1);
         weigh(1);
-        if (moved) multiply_sums(old);
         multiply_values(2);
         multiply_values(3);
+    };
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // this block has come, and nobody reads the one before any more
+        if (i + 1 < mine) request(i + 1);
+        const int t0 = (b0 + i) * BLOCK_TOKENS;
+        const uint32_t buffer = (i & 1) * 2 * PROMPT_TILE;
+        if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;                  // (of the wavefront's own queries none sees the block)
+        block(buffer, t0);
     }
 
     const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
@@ -394,6 +422,7 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
     ODMKV_CHECK_ARG((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->out) & 15) == 0 &&
                     ((d->q_stride_b | d->q_stride_h | d->q_stride_t | d->k_stride_b | d->k_stride_h | d->k_stride_t | d->v_stride_b | d->v_stride_h | d->v_stride_t) & 7) == 0,
                     "prompt_attend: rows must be 16-byte aligned");
+    ODMKV_CHECK_ARG(d->k_stride_t >= 0 && d->k_stride_t < (1 << 24) && d->v_stride_t >= 0 && d->v_stride_t < (1 << 24), "prompt_attend: a token's stride must be below 2^24");
     const int G = d->Hq / d->Hkv;
     const PromptCut cut = cut_of(d->offsets != nullptr, d->rows, G, d->Hkv, d->L, d->T);
     const long long all = d->offsets ? d->L : (long long)d->rows * d->L, groups = cut.tiles * d->Hkv * cut.splits;

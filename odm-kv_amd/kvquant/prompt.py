@@ -73,6 +73,7 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
 
     offsets, key_offsets, starts = small(offsets, rows + 1, "offsets"), small(key_offsets, rows + 1, "key_offsets"), small(starts, rows, "starts")
     query, keys, values = (PagedKVCache._rows_ok(t) for t in (query, keys, values))
+    keys, values = (t.contiguous() if t.stride(2) >= 1 << 24 else t for t in (keys, values))
     out = torch.empty(B, L, Hq, HEAD_DIM, dtype=query.dtype, device=device)
     lse = torch.empty(B, Hq, L, dtype=torch.float32, device=device) if return_lse else None
     if L:

@@ -87,6 +87,8 @@ template <int DT> struct Weights {
     static constexpr float LIFT = DT == ODMKV_F16 ? 8.0f : 0.0f, RISE_BY = DT == ODMKV_F16 ? 7.0f : 8.0f;
 };
 
+__device__ static inline int value_turn(int t) { return (t & 3) << 1 | (t >> 2 & 1); }
+
 template <int DT, int MODE, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     constexpr bool PLAIN = MODE == 0;                           // 1: a cap by the exponential; 2: any
@@ -126,7 +128,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     const int first = from / BLOCK_TOKENS, blocks = max((upto + BLOCK_TOKENS - 1) / BLOCK_TOKENS - first, 0), share = (blocks + a.splits - 1) / a.splits;
     const int b0 = __builtin_amdgcn_readfirstlane(first + split * share), mine = __builtin_amdgcn_readfirstlane(min(share, blocks - split * share));
 
-    // 16-byte piece p of token t lies at p ^ (t % 16) of the token's place; of values 32-byte pieces at p ^ (t % 8): what a wavefront reads at a time falls on distinct banks.
+    // 16-byte piece p of token t lies at p ^ (t % 16) of the token's place; of values 32-byte pieces at p ^ value_turn(t): what half a wavefront reads at a time, 32 bytes of
+    // two pieces of four tokens, falls on distinct banks.
     // Tokens behind the row's end repeat its last one and are masked.
     const uint16_t* const K = a.k + (a.offsets ? tile.k0 * a.kt : row * a.kb) + h * a.kh;
     const uint16_t* const V = a.v + (a.offsets ? tile.k0 * a.vt : row * a.vb) + h * a.vh;
@@ -136,7 +139,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     for (int c = 0; c < PIECES; ++c) {
         const int e = tid + WAVES * 64 * c, t = e >> 4, p = e & 15;
         key_from[c] = 2 * (t * (int)a.kt + 8 * (p ^ (t & 15)));
-        value_from[c] = 2 * (t * (int)a.vt + 8 * (p ^ ((t & 7) << 1)));
+        value_from[c] = 2 * (t * (int)a.vt + 8 * (p ^ (value_turn(t) << 1)));
     }
     const auto request = [&](int i) {
         const int t0 = (b0 + i) * BLOCK_TOKENS, behind = tile.m - 1 - t0;
@@ -188,7 +191,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
 #pragma unroll
     for (int st = 0; st < 8; ++st) key_at[st] = lds0 + col * 256 + (((2 * st + half) ^ (col & 15)) << 4);
 #pragma unroll
-    for (int db = 0; db < 4; ++db) value_at[db] = lds0 + PROMPT_TILE + value_token * 256 + (((2 * db + (lane >> 4 & 1)) ^ value_token) << 5) + ((lane & 3) << 3);
+    for (int db = 0; db < 4; ++db) value_at[db] = lds0 + PROMPT_TILE + value_token * 256 + (((2 * db + (lane >> 4 & 1)) ^ value_turn(value_token)) << 5) + ((lane & 3) << 3);
 
     const auto block = [&](uint32_t buffer, int t0) {
         f32x16 dot[2];
@@ -230,8 +233,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
             sum += z0 + z1;
         };
         const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
-        // products of half a block to scores (PLAIN: they stay products); the reference where a score is to move it, each query's by itself
-        const auto look = [&](int tb) {
+        // products of half a block to scores (PLAIN: they stay products); the reference where a score is to move it, each query's by itself, and what the sums are to be
+        // multiplied by
+        const auto look = [&](int tb, float& old) {
             f32x16& x = dot[tb];
             if constexpr (!PLAIN) {
 #pragma unroll
@@ -249,16 +253,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
 #pragma unroll
             for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
             if (PLAIN) top = top > -INFINITY ? top * c : top;   // (c is positive: the largest product is the largest score)
-            if (!__any(top > ref + Weights<DT>::RISE_BY)) return;
+            if (!__any(top > ref + Weights<DT>::RISE_BY)) return false;
             const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
             const float to = most > ref + Weights<DT>::RISE_BY ? most : ref;
-            const float old = ref > -INFINITY ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
+            old = ref > -INFINITY ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
             sum *= old;
             ref = to;
+            return true;
+        };
+        const auto multiply_sums = [&](float old) {
 #pragma unroll
             for (int db = 0; db < 4; ++db) acc[db] *= old;
         };
+        float old;
         multiply_keys(0);
         __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
@@ -267,13 +275,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-        look(0);
+        if (look(0, old)) multiply_sums(old);
+        // one half's vector work stands beside the other's products
         multiply_keys(1);
         weigh(0);
-        look(1);
-        multiply_values(0);
+        const bool moved = look(1, old);
+        multiply_values(0);                                     // (weights of the reference before)
         multiply_values(1);
         weigh(1);
+        if (moved) multiply_sums(old);
         multiply_values(2);
         multiply_values(3);
     };

@@ -13,7 +13,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-#define PROMPT_WAVES 8
 #define PROMPT_COLS(waves) (32 * (waves))
 #define PROMPT_TILE (BLOCK_TOKENS * HD * 2)                      // bytes of a block of keys, or of values
 #define PROMPT_LDS (4 * PROMPT_TILE)
@@ -81,10 +80,10 @@ __device__ static inline uint32_t pair_16(float x, float y) {
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector((__attribute__((ext_vector_type(2))) float){x, y}, __attribute__((ext_vector_type(2))) __bf16));
 }
 
-// Weights go to 16 bits relative to a reference that follows the largest score of the query's own: it moves where a score passes it by more than RISE (base 2).  fp16: the
-// reference's weight is 2^8 and may grow to 2^15, so that a weight below fp16's normal numbers is off by 2^-33 of the largest at the most; bf16 has the range of 32 bits.
+// Weights go to 16 bits relative to a reference, a score of the query's own: its weight is 2^LIFT, and where the sum of sixteen weights passes LIMIT the reference moves to the
+// largest score.  fp16: so no weight passes the type's end, and one below its normal numbers is off by 2^-25, 2^-33 of the largest at the most; bf16 has the range of 32 bits.
 template <int DT> struct Weights {
-    static constexpr float LIFT = DT == ODMKV_F16 ? 8.0f : 0.0f, RISE_BY = DT == ODMKV_F16 ? 7.0f : 8.0f;
+    static constexpr float LIFT = DT == ODMKV_F16 ? 8.0f : 0.0f, LIMIT = 32768.0f;
 };
 
 __device__ static inline int value_turn(int t) { return (t & 3) << 1 | (t >> 2 & 1); }
@@ -193,7 +192,60 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
 #pragma unroll
     for (int db = 0; db < 4; ++db) value_at[db] = lds0 + PROMPT_TILE + value_token * 256 + (((2 * db + (lane >> 4 & 1)) ^ value_turn(value_token)) << 5) + ((lane & 3) << 3);
 
-    const auto block = [&](uint32_t buffer, int t0) {
+    float shift = INFINITY;                                     // LIFT - ref; what a score is to have added on its way into the exponential
+    // Half a block's products to weights, and their sum.  Vector work is what there is too much of beside the products, so that the largest score is not looked for: where the
+    // sum says that a weight may have grown too large, or nothing has been seen yet (the sum is infinite then, or not a number), they are made once more.
+    const auto weigh = [&](const f32x16& x, uint4* w) {
+        float z0 = 0.0f, z1 = 0.0f;
+        uint32_t word[8];
+        const auto weight = [&](float y) {
+            if constexpr (PLAIN) return __builtin_amdgcn_exp2f(__fmaf_rn(y, c, shift));
+            else if constexpr (MODE == 1) return __builtin_amdgcn_exp2f(__fmaf_rn(-cap.twice, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * (c * cap.plain))), cap.by + shift));
+            else return __builtin_amdgcn_exp2f(score(y) + shift);
+        };
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            const float p0 = weight(x[e]), p1 = weight(x[e + 1]);
+            z0 += p0;
+            z1 += p1;
+            word[e >> 1] = pair_16<DT>(p0, p1);
+        }
+        w[0] = make_uint4(word[0], word[1], word[2], word[3]);
+        w[1] = make_uint4(word[4], word[5], word[6], word[7]);
+        return z0 + z1;
+    };
+    // Once more: what is not seen is left out, the reference moves to the largest score where that is above it, each query's by itself, and the sums with it.
+    const auto weigh_again = [&](const f32x16& x, uint4* w, int tl, bool cut) {
+        float y[16], top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int t = tl + 8 * (e >> 2) + (e & 3);
+            y[e] = !cut || (t >= lo && t < hi) ? score(x[e]) : -INFINITY;
+            top = fmaxf(top, y[e]);
+        }
+        const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1])), to = most > ref + 2.0f ? most : ref;
+        const float old = ref > -INFINITY ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
+        sum *= old;
+#pragma unroll
+        for (int db = 0; db < 4; ++db) acc[db] *= old;
+        ref = to;
+        shift = to > -INFINITY ? LIFT - to : INFINITY;
+        float z = 0.0f;
+        uint32_t word[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(y[e] + (to > -INFINITY ? shift : 0.0f)), p1 = __builtin_amdgcn_exp2f(y[e + 1] + (to > -INFINITY ? shift : 0.0f));
+            z += p0 + p1;
+            word[e >> 1] = pair_16<DT>(p0, p1);
+        }
+        w[0] = make_uint4(word[0], word[1], word[2], word[3]);
+        w[1] = make_uint4(word[4], word[5], word[6], word[7]);
+        return z;
+    };
+    const auto block = [&](auto buffer_, int t0) {
+        constexpr uint32_t buffer = buffer_.value * 2 * PROMPT_TILE;
+        const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
         f32x16 dot[2];
         uint4 w[4];
         const auto multiply_keys = [&](int tb) {
@@ -202,7 +254,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
             for (int e = 0; e < 16; ++e) dot[tb][e] = 0.0f;
 #pragma unroll
             for (int st = 0; st < 8; ++st) {
-                const u32x4 x = *(place)(size_t)(key_at[st] + buffer + 32 * 256 * tb);
+                const u32x4 x = *(place)(size_t)(key_at[st] + (buffer + 32 * 256 * tb));
                 dot[tb] = multiply<DT>(make_uint4(x[0], x[1], x[2], x[3]), q[st], dot[tb]);
             }
         };
@@ -210,91 +262,37 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
             typedef __attribute__((address_space(3))) s16x4* place;
 #pragma unroll
             for (int db = 0; db < 4; ++db) {
-                const uint32_t at = value_at[db] + buffer + 16 * 256 * st;
+                const uint32_t at = value_at[db] + (buffer + 16 * 256 * st);
                 const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(size_t)at), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(size_t)(at + 8 * 256));
                 const uint2 u = __builtin_bit_cast(uint2, x), v = __builtin_bit_cast(uint2, y);
                 acc[db] = multiply<DT>(make_uint4(u.x, u.y, v.x, v.y), w[st], acc[db]);
             }
         };
-        const auto weigh = [&](int tb) {
-            const float shift = LIFT - (ref > -INFINITY ? ref : 0.0f);
-            float z0 = 0.0f, z1 = 0.0f;
-            uint32_t word[8];
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e], c, shift) : dot[tb][e] + shift);
-                const float p1 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e + 1], c, shift) : dot[tb][e + 1] + shift);
-                z0 += p0;
-                z1 += p1;
-                word[e >> 1] = pair_16<DT>(p0, p1);
-            }
-            w[2 * tb] = make_uint4(word[0], word[1], word[2], word[3]);
-            w[2 * tb + 1] = make_uint4(word[4], word[5], word[6], word[7]);
-            sum += z0 + z1;
-        };
-        const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
-        // products of half a block to scores (PLAIN: they stay products); the reference where a score is to move it, each query's by itself, and what the sums are to be
-        // multiplied by
-        const auto look = [&](int tb, float& old) {
-            f32x16& x = dot[tb];
-            if constexpr (!PLAIN) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = score(x[e]);
-            }
-            if (cut) {
-                const int tl = t0 + 32 * tb + 4 * half;         // token of score e: tl + 8 (e / 4) + e % 4
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int t = tl + 8 * (e >> 2) + (e & 3);
-                    x[e] = t >= lo && t < hi ? x[e] : -INFINITY;
-                }
-            }
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-            if (PLAIN) top = top > -INFINITY ? top * c : top;   // (c is positive: the largest product is the largest score)
-            if (!__any(top > ref + Weights<DT>::RISE_BY)) return false;
-            const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-            const float to = most > ref + Weights<DT>::RISE_BY ? most : ref;
-            old = ref > -INFINITY ? __builtin_amdgcn_exp2f(ref - to) : 1.0f;
-            sum *= old;
-            ref = to;
-            return true;
-        };
-        const auto multiply_sums = [&](float old) {
-#pragma unroll
-            for (int db = 0; db < 4; ++db) acc[db] *= old;
-        };
-        float old;
+        const int tl = t0 + 4 * half;                           // token of score e: tl + 8 (e / 4) + e % 4
         multiply_keys(0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-        if (look(0, old)) multiply_sums(old);
         // one half's vector work stands beside the other's products
         multiply_keys(1);
-        weigh(0);
-        const bool moved = look(1, old);
-        multiply_values(0);                                     // (weights of the reference before)
+        float z = weigh(dot[0], w);
+        if (cut || __any(!(z <= Weights<DT>::LIMIT))) z = weigh_again(dot[0], w, tl, cut);
+        sum += z;
+        multiply_values(0);
         multiply_values(1);
-        weigh(1);
-        if (moved) multiply_sums(old);
+        z = weigh(dot[1], w + 2);
+        if (cut || __any(!(z <= Weights<DT>::LIMIT))) z = weigh_again(dot[1], w + 2, tl + 32, cut);
+        sum += z;
         multiply_values(2);
         multiply_values(3);
     };
-#pragma unroll 1
-    for (int i = 0; i < mine; ++i) {
+    const auto turn = [&](int i, auto buffer) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // this block has come, and nobody reads the one before any more
         if (i + 1 < mine) request(i + 1);
         const int t0 = (b0 + i) * BLOCK_TOKENS;
-        const uint32_t buffer = (i & 1) * 2 * PROMPT_TILE;
-        if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;                  // (of the wavefront's own queries none sees the block)
-        block(buffer, t0);
+        if (t0 < wave_hi && t0 + BLOCK_TOKENS > wave_lo) block(buffer, t0);           // (of the wavefront's own queries some see the block)
+    };
+#pragma unroll 1
+    for (int i = 0; i < mine; i += 2) {
+        turn(i, Int<0>());
+        if (i + 1 < mine) turn(i + 1, Int<1>());
     }
 
     const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
@@ -402,20 +400,35 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
     }
 }
 
-// How a call is cut: tiles of queries at the most, and workgroups that share a tile's blocks where there are too few tiles for the compute units.
-struct PromptCut { long long tiles; int splits; };
-static PromptCut cut_of(bool packed, int rows, int G, int Hkv, int L, int T) {
-    const long long cols = PROMPT_COLS(PROMPT_WAVES);
+// How a call is cut: wavefronts of a workgroup, tiles of queries at the most, and workgroups that share a tile's blocks.
+//
+// Eight wavefronts share a block among twice as many queries; two workgroups of four, which do not wait for one another, leave more of the vector work beside the products, and a cap is
+// that above all: 12001 tokens in a window of 4096 with a cap 480 us for 429, but 16384 without 2063 for 2150 (packed prompts of up to 2999: 460 for 454).
+//
+// Shares: what they are to gain is compute units that would have no tile, or none in the last round; what they cost is their partial results.
+struct PromptCut { int waves; long long tiles; int splits; };
+static PromptCut cut_of(bool packed, int rows, int G, int Hkv, int L, int T, bool capped) {
     PromptCut c;
+    c.waves = capped ? 4 : 8;
+    const long long cols = PROMPT_COLS(c.waves), slots = compute_units() * (8 / c.waves);
     c.tiles = packed ? ((long long)G * L + cols - 1) / cols + rows + 2 : (long long)rows * (((long long)G * L + cols - 1) / cols);
-    const long long blocks = (packed ? T / rows : T) / BLOCK_TOKENS + 1;
-    c.splits = (int)std::max(1LL, std::min(compute_units() / std::max(1LL, c.tiles * Hkv), blocks / 4));
+    const long long blocks = (packed ? T / rows : T) / BLOCK_TOKENS + 1, groups = c.tiles * Hkv;
+    // in units of a block's time, about a microsecond: a workgroup's fixed part is some four of them, the merge a launch and its reading
+    const double partial = (double)(packed ? 1 : rows) * L * G * Hkv * (HD + 1) * 4 * 2 / 5e6;
+    double least = 0.0;
+    c.splits = 1;
+    for (int s = 1; s <= 128 && (s == 1 || s * 4LL <= blocks) && (s == 1 || groups * s <= 4 * slots); ++s) {
+        const double cost = (double)((groups * s + slots - 1) / slots) * ((double)blocks / s + 4.0) + (s > 1 ? 4.0 + s * partial : 0.0);
+        if (s > 1 && cost >= least) continue;
+        least = cost;
+        c.splits = s;
+    }
     return c;
 }
 
-extern "C" size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T) {
+extern "C" size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T, float cap) {
     if (rows <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || L <= 0 || T < 0) return 0;
-    const PromptCut c = cut_of(packed != 0, rows, Hq / Hkv, Hkv, L, T);
+    const PromptCut c = cut_of(packed != 0, rows, Hq / Hkv, Hkv, L, T, cap > 0.0f);
     return c.splits > 1 ? align_up((size_t)c.splits * (packed ? 1 : rows) * L * Hq * (HD + 1) * sizeof(float), 256) : 0;
 }
 
@@ -434,10 +447,10 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
                     "prompt_attend: rows must be 16-byte aligned");
     ODMKV_CHECK_ARG(d->k_stride_t >= 0 && d->k_stride_t < (1 << 24) && d->v_stride_t >= 0 && d->v_stride_t < (1 << 24), "prompt_attend: a token's stride must be below 2^24");
     const int G = d->Hq / d->Hkv;
-    const PromptCut cut = cut_of(d->offsets != nullptr, d->rows, G, d->Hkv, d->L, d->T);
+    const PromptCut cut = cut_of(d->offsets != nullptr, d->rows, G, d->Hkv, d->L, d->T, d->cap > 0.0f);
     const long long all = d->offsets ? d->L : (long long)d->rows * d->L, groups = cut.tiles * d->Hkv * cut.splits;
-    ODMKV_CHECK_ARG((long long)G * d->L < 0x7fff0000LL && groups * PROMPT_WAVES * 64 < 0x100000000LL && all * d->Hq < 0x100000000LL, "prompt_attend: too many queries");
-    const size_t need = odmkv_prompt_attend_workspace_bytes(d->offsets != nullptr, d->rows, d->Hq, d->Hkv, d->L, d->T);
+    ODMKV_CHECK_ARG((long long)G * d->L < 0x7fff0000LL && groups * cut.waves * 64 < 0x100000000LL && all * d->Hq < 0x100000000LL, "prompt_attend: too many queries");
+    const size_t need = odmkv_prompt_attend_workspace_bytes(d->offsets != nullptr, d->rows, d->Hq, d->Hkv, d->L, d->T, d->cap);
     if (need > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)) {
         odmkv_set_error("prompt_attend: workspace too small");
         return ODMKV_ENOSPACE;
@@ -446,12 +459,12 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
     const PromptArgs a = {(const uint16_t*)d->q, (const uint16_t*)d->k, (const uint16_t*)d->v, d->q_stride_b, d->q_stride_h, d->q_stride_t, d->k_stride_b, d->k_stride_h,
                           d->k_stride_t, d->v_stride_b, d->v_stride_h, d->v_stride_t, (uint16_t*)d->out, d->lse, d->offsets, d->key_offsets, d->starts, d->rows, d->L, d->T,
                           d->Hq, d->Hkv, G, d->causal != 0, d->window, d->scaling, d->cap, cut.splits, parts, parts + (size_t)cut.splits * all * d->Hq * HD};
-    const int mode = d->cap > 0.0f ? (d->cap <= CAP_BY_EXP ? 1 : 2) : d->scaling > 0.0f ? 0 : 2;
+    const int mode = d->cap > 0.0f ? (d->cap <= CAP_BY_EXP ? 1 : 2) : d->scaling > 0x1p-100f ? 0 : 2;
     const hipStream_t st = (hipStream_t)stream;
-    const auto run = [&](auto dt, auto mode_) {
-        const auto kernel = prompt_kernel<dt.value, mode_.value, PROMPT_WAVES>;
+    const auto run = [&](auto dt, auto mode_, auto waves) {
+        const auto kernel = prompt_kernel<dt.value, mode_.value, waves.value>;
         ODMKV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PROMPT_LDS));
-        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(PROMPT_WAVES * 64), PROMPT_LDS, st, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(waves.value * 64), PROMPT_LDS, st, a);
         ODMKV_CHECK_LAUNCH("prompt_kernel");
         if (cut.splits > 1) {
             hipLaunchKernelGGL(prompt_merge_kernel<dt.value>, dim3((unsigned)((all * d->Hq + 3) / 4)), dim3(256), 0, st, a);
@@ -459,6 +472,7 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
         }
         return 0;
     };
-    const auto of_mode = [&](auto dt) { return mode == 0 ? run(dt, Int<0>()) : mode == 1 ? run(dt, Int<1>()) : run(dt, Int<2>()); };
+    const auto of_waves = [&](auto dt, auto mode_) { return cut.waves == 8 ? run(dt, mode_, Int<8>()) : run(dt, mode_, Int<4>()); };
+    const auto of_mode = [&](auto dt) { return mode == 0 ? run(dt, Int<0>(), Int<8>()) : mode == 1 ? run(dt, Int<1>(), Int<4>()) : of_waves(dt, Int<2>()); };
     return d->dtype == ODMKV_F16 ? of_mode(Int<ODMKV_F16>()) : of_mode(Int<ODMKV_BF16>());
 }

@@ -8,6 +8,7 @@
 #include <stdlib.h>
 #include <string.h>
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/odmkv.h"
@@ -330,7 +331,158 @@ PyObject* native_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     )
 }
 
+typedef int (*rotate_fn)(const odmkv_rotate_t*, void*);
+typedef int (*prompt_fn)(const odmkv_prompt_attend_t*, void*);
+typedef size_t (*prompt_bytes_fn)(int, int, int, int, int, int, float);
+
+// [B, heads, T, 128] in 16 bits with rows that start on 16 bytes, and nothing to record
+bool heads_fit(const at::Tensor& t, at::ScalarType type, int device) {
+    if (t.dim() != 4 || !t.is_cuda() || t.get_device() != device || t.scalar_type() != type || (t.requires_grad() && at::GradMode::is_enabled())) return false;
+    const auto r = t.strides();
+    return t.size(3) == ODMKV_HEAD_DIM && r[3] == 1 && ((r[0] | r[1] | r[2]) & 7) == 0 && ((uintptr_t)t.data_ptr() & 15) == 0 && t.size(2) <= (1 << 26);
+}
+// None, or int32 [n] on the device; false: something else
+bool ints_fit(PyObject* o, int64_t n, int device, const int32_t*& at) {
+    at = nullptr;
+    if (o == Py_None) return true;
+    if (!THPVariable_Check(o)) return false;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.get_device() != device || t.scalar_type() != at::kInt || t.dim() != 1 || t.size(0) != n || !t.is_contiguous()) return false;
+    at = (const int32_t*)t.data_ptr();
+    return true;
+}
+PyObject* pair_of(at::Tensor a, at::Tensor b) {
+    PyObject* both = PyTuple_New(2);
+    if (both) {
+        PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(a)));
+        PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(b)));
+    }
+    return both;
+}
+
+// paged_write_rotated(entry, pages, device, layer, query, keys, values, cosine, sine, offsets, starts, interleaved, return_keys, grown, stream): query turned, or (query, keys), or
+// None
+PyObject* native_paged_write_rotated(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 15) {
+        PyErr_SetString(PyExc_TypeError, "paged_write_rotated(entry, pages, device, layer, query, keys, values, cosine, sine, offsets, starts, interleaved, return_keys, grown, stream)");
+        return nullptr;
+    }
+    for (int i = 4; i < 9; ++i)
+        if (!THPVariable_Check(a[i])) Py_RETURN_NONE;
+    const rotate_fn fn = (rotate_fn)(uintptr_t)PyLong_AsUnsignedLongLong(a[0]);
+    const odmkv_pages_t* p = (const odmkv_pages_t*)(uintptr_t)PyLong_AsUnsignedLongLong(a[1]);
+    const int device = (int)PyLong_AsLong(a[2]);
+    const long layer = PyLong_AsLong(a[3]);
+    const int interleaved = PyObject_IsTrue(a[11]);
+    const int want_keys = PyObject_IsTrue(a[12]);
+    const long long grown = PyLong_AsLongLong(a[13]);
+    const unsigned long long stream = PyLong_AsUnsignedLongLong(a[14]);
+    if (PyErr_Occurred()) return nullptr;
+    GUARDED(
+        const at::Tensor& q = THPVariable_Unpack(a[4]);
+        const at::Tensor& k = THPVariable_Unpack(a[5]);
+        const at::Tensor& v = THPVariable_Unpack(a[6]);
+        const at::Tensor& c = THPVariable_Unpack(a[7]);
+        const at::Tensor& s = THPVariable_Unpack(a[8]);
+        const at::ScalarType type = scalar_of(p->dtype);
+        const bool packed = a[9] != Py_None;
+        const int64_t B = packed ? 1 : p->rows;
+        if (layer < 0 || layer >= p->layers || !heads_fit(q, type, device) || !heads_fit(k, type, device) || !heads_fit(v, type, device)) Py_RETURN_NONE;
+        const int64_t T = k.size(2);
+        const int64_t Hq = q.size(1);
+        if (q.size(0) != B || k.size(0) != B || v.sizes() != k.sizes() || k.size(1) != p->Hkv || q.size(2) != T || Hq < 1 || Hq > 65535 || T < 1 || T < grown) Py_RETURN_NONE;
+        for (const at::Tensor* t : {&c, &s})
+            if (t->dim() != 2 || !t->is_cuda() || t->get_device() != device || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->sizes() != c.sizes()) Py_RETURN_NONE;
+        const int64_t half = c.size(1);
+        if (half < 8 || half > ODMKV_HEAD_DIM / 2 || half % 8 || c.size(0) < 1 || c.size(0) > INT32_MAX) Py_RETURN_NONE;
+        odmkv_rotate_t d;
+        memset(&d, 0, sizeof d);
+        if (!ints_fit(a[9], (int64_t)p->rows + 1, device, d.offsets) || !ints_fit(a[10], p->rows, device, d.starts)) Py_RETURN_NONE;
+        at::Tensor turned = at::empty({B, T, Hq, ODMKV_HEAD_DIM}, q.options());
+        at::Tensor keys;
+        if (want_keys) keys = at::empty({B, T, (int64_t)p->Hkv, ODMKV_HEAD_DIM}, q.options());
+        d.pages = p;
+        d.q = q.data_ptr(); d.q_stride_b = q.stride(0); d.q_stride_h = q.stride(1); d.q_stride_t = q.stride(2);
+        d.k = k.data_ptr(); d.k_stride_b = k.stride(0); d.k_stride_h = k.stride(1); d.k_stride_t = k.stride(2);
+        d.v = v.data_ptr(); d.v_stride_b = v.stride(0); d.v_stride_h = v.stride(1); d.v_stride_t = v.stride(2);
+        d.q_out = turned.data_ptr(); d.k_out = want_keys ? keys.data_ptr() : nullptr;
+        d.cosine = (const float*)c.data_ptr(); d.sine = (const float*)s.data_ptr();
+        d.layer = (int)layer; d.T = (int)(packed ? (grown > 1 ? grown : 1) : T); d.tokens = (int)T; d.Hq = (int)Hq;
+        d.turned = (int)(2 * half); d.interleaved = interleaved; d.table = (int)c.size(0);
+        const int rc = fn(&d, (void*)(uintptr_t)stream);
+        if (rc) return raise_odmkv(rc, "storing turned tokens");
+        turned = turned.transpose(1, 2);
+        if (!want_keys) return THPVariable_Wrap(std::move(turned));
+        return pair_of(std::move(turned), keys.transpose(1, 2));
+    )
+}
+
+// prompt_attend(entry, workspace entry, device, query, keys, values, offsets, key_offsets, starts, causal, window, scaling, cap, want_lse, stream): out, or (out, lse), or None
+PyObject* native_prompt_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 15) {
+        PyErr_SetString(PyExc_TypeError, "prompt_attend(entry, bytes, device, query, keys, values, offsets, key_offsets, starts, causal, window, scaling, cap, want_lse, stream)");
+        return nullptr;
+    }
+    for (int i = 3; i < 6; ++i)
+        if (!THPVariable_Check(a[i])) Py_RETURN_NONE;
+    const prompt_fn fn = (prompt_fn)(uintptr_t)PyLong_AsUnsignedLongLong(a[0]);
+    const prompt_bytes_fn bytes_of = (prompt_bytes_fn)(uintptr_t)PyLong_AsUnsignedLongLong(a[1]);
+    const int device = (int)PyLong_AsLong(a[2]);
+    const int causal = PyObject_IsTrue(a[9]);
+    const long long window = PyLong_AsLongLong(a[10]);
+    const double scaling = PyFloat_AsDouble(a[11]);
+    const double cap = PyFloat_AsDouble(a[12]);
+    const int want_lse = PyObject_IsTrue(a[13]);
+    const unsigned long long stream = PyLong_AsUnsignedLongLong(a[14]);
+    if (PyErr_Occurred()) return nullptr;
+    GUARDED(
+        const at::Tensor& q = THPVariable_Unpack(a[3]);
+        const at::Tensor& k = THPVariable_Unpack(a[4]);
+        const at::Tensor& v = THPVariable_Unpack(a[5]);
+        const at::ScalarType type = q.scalar_type();
+        if ((type != at::kHalf && type != at::kBFloat16) || !heads_fit(q, type, device) || !heads_fit(k, type, device) || !heads_fit(v, type, device)) Py_RETURN_NONE;
+        const int64_t B = q.size(0);
+        const int64_t Hq = q.size(1);
+        const int64_t L = q.size(2);
+        const int64_t Hkv = k.size(1);
+        const int64_t T = k.size(2);
+        const bool packed = a[6] != Py_None;
+        if (k.sizes() != v.sizes() || k.size(0) != B || B < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq > 65535 || L < 1 || k.stride(2) >= (1 << 24) || v.stride(2) >= (1 << 24)) Py_RETURN_NONE;
+        int64_t rows = B;
+        if (packed) {
+            if (B != 1 || !THPVariable_Check(a[6]) || (a[7] == Py_None && L != T)) Py_RETURN_NONE;
+            const at::Tensor& t = THPVariable_Unpack(a[6]);
+            if (t.dim() != 1 || t.size(0) < 2) Py_RETURN_NONE;
+            rows = t.size(0) - 1;
+        } else if (a[7] != Py_None) Py_RETURN_NONE;
+        if (rows > (1 << 20)) Py_RETURN_NONE;
+        odmkv_prompt_attend_t d;
+        memset(&d, 0, sizeof d);
+        if (!ints_fit(a[6], rows + 1, device, d.offsets) || !ints_fit(a[7], rows + 1, device, d.key_offsets) || !ints_fit(a[8], rows, device, d.starts)) Py_RETURN_NONE;
+        at::Tensor out = at::empty({B, L, Hq, ODMKV_HEAD_DIM}, q.options());
+        at::Tensor lse;
+        if (want_lse) lse = at::empty({B, Hq, L}, q.options().dtype(at::kFloat));
+        const size_t bytes = bytes_of(packed, (int)rows, (int)Hq, (int)Hkv, (int)L, (int)T, (float)cap);
+        at::Tensor ws;
+        if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));      // (of its own for every call: a graph's is the graph's)
+        d.q = q.data_ptr(); d.q_stride_b = q.stride(0); d.q_stride_h = q.stride(1); d.q_stride_t = q.stride(2);
+        d.k = k.data_ptr(); d.k_stride_b = k.stride(0); d.k_stride_h = k.stride(1); d.k_stride_t = k.stride(2);
+        d.v = v.data_ptr(); d.v_stride_b = v.stride(0); d.v_stride_h = v.stride(1); d.v_stride_t = v.stride(2);
+        d.out = out.data_ptr(); d.lse = want_lse ? (float*)lse.data_ptr() : nullptr;
+        d.workspace = bytes ? ws.data_ptr() : nullptr; d.workspace_bytes = bytes;
+        d.dtype = type == at::kHalf ? ODMKV_F16 : ODMKV_BF16;
+        d.rows = (int)rows; d.L = (int)L; d.T = (int)T; d.Hq = (int)Hq; d.Hkv = (int)Hkv; d.causal = causal; d.window = (int)window;
+        d.scaling = (float)scaling; d.cap = (float)cap;
+        const int rc = fn(&d, (void*)(uintptr_t)stream);
+        if (rc) return raise_odmkv(rc, "attention of a prompt");
+        if (!want_lse) return THPVariable_Wrap(std::move(out));
+        return pair_of(std::move(out), std::move(lse));
+    )
+}
+
 PyMethodDef module_methods[] = {
+    {"paged_write_rotated", (PyCFunction)(void*)native_paged_write_rotated, METH_FASTCALL, nullptr},
+    {"prompt_attend", (PyCFunction)(void*)native_prompt_attend, METH_FASTCALL, nullptr},
     {"paged_write", (PyCFunction)(void*)native_paged_write, METH_FASTCALL, nullptr},
     {"paged_attend", (PyCFunction)(void*)native_paged_attend, METH_FASTCALL, nullptr},
     {"alias", (PyCFunction)(void*)native_alias, METH_FASTCALL, nullptr},

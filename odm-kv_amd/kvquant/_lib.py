@@ -222,7 +222,8 @@ def _load() -> C.CDLL:
 lib = _load()
 STEP_ENTRY = C.cast(lib.odmkv_decode_step, C.c_void_p).value      # what _native.Step calls
 PAGES_ENTRIES = tuple(C.cast(f, C.c_void_p).value for f in (lib.odmkv_pages_write, lib.odmkv_pages_attend, lib.odmkv_pages_attend_workspace_bytes,
-                                                                   lib.odmkv_pages_attend_shared_workspace_bytes))
+                                                                   lib.odmkv_pages_attend_shared_workspace_bytes, lib.odmkv_pages_write_rotated))
+PROMPT_ENTRIES = tuple(C.cast(f, C.c_void_p).value for f in (lib.odmkv_prompt_attend, lib.odmkv_prompt_attend_workspace_bytes))
 EXPORTS = ("odmkv_version", "odmkv_last_error", "odmkv_score_workspace_bytes", "odmkv_score", "odmkv_score_model_dtype", "odmkv_score_expected", "odmkv_token_mean_workspace_bytes", "odmkv_token_mean", "odmkv_average_rope",
            "odmkv_project_rows", "odmkv_prompt_scores_workspace_bytes", "odmkv_prompt_scores", "odmkv_query_covariance_workspace_bytes", "odmkv_query_covariance", "odmkv_rotate_queries",
            "odmkv_normalize_workspace_bytes", "odmkv_normalize_scores",

@@ -36,7 +36,7 @@ KINDS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 _SCALING = HEAD_DIM ** -0.5
 _FAR = 2 ** 30                                # a window past everything
 _LEAST_CAP = 2.0 ** -100                      # (what 32 bits make 0 of would be no cap)
-_WRITE, _ATTEND, _ATTEND_BYTES, _SHARED_BYTES = _lib.PAGES_ENTRIES
+_WRITE, _ATTEND, _ATTEND_BYTES, _SHARED_BYTES, _WRITE_ROTATED = _lib.PAGES_ENTRIES
 _native = _lib._native
 _device = torch.cuda.current_device
 _capturing = torch.cuda.is_current_stream_capturing
@@ -298,6 +298,16 @@ class PagedKVCache:
         its nearest, offsets that do not fit, whose rows are not stored) is raised by ``refresh``."""
         if layer in self._written:                           # (the new tail would be taken for the old one)
             raise ValueError(f"layer {layer} has no tokens to store: it has stored those of the last extend already, or rows have been moved or cut since")
+        if not self._replayed and _capturing():
+            self._replayed = True
+        if (positions is None and isinstance(cosine, torch.Tensor) and cosine.dim() == 2 and _device() == self.device.index
+                and (self.max_tokens if _capturing() else max(self._bounds)) <= cosine.shape[0]):
+            # (everything as the kernel takes it: one native call)
+            done = _native.paged_write_rotated(_WRITE_ROTATED, self._at, self.device.index, layer, query, keys, values, cosine, sine, offsets, starts, interleaved, return_keys,
+                                               self._grown, _lib.stream_ptr(self.device))
+            if done is not None:
+                self._written.add(layer)
+                return done
         self._check_layer(layer)
         B = self.batch if offsets is None else 1
         rows = f"[{B}, heads, {'T' if offsets is None else 'N'}, {HEAD_DIM}]"
@@ -330,8 +340,6 @@ class PagedKVCache:
                 longest = max(self.refresh())
             if longest > cosine.shape[0]:
                 raise ValueError(f"a table of {cosine.shape[0]} positions for rows of up to {longest} tokens")
-        if not self._replayed and _capturing():
-            self._replayed = True
         offsets = self._small(offsets, "offsets", torch.int32, ((self.batch + 1,),))
         positions = self._small(positions, "positions", torch.int32, ((B, T),))
         starts = self._small(starts, "starts", torch.int32, ((self.batch,),))

@@ -13,7 +13,10 @@ import torch
 
 from . import _lib
 from ._lib import HEAD_DIM, lib
-from .paged_cache import _FAR, _LEAST_CAP, _SCALING, _as, PagedKVCache
+from .paged_cache import _device, _FAR, _LEAST_CAP, _SCALING, _as, PagedKVCache
+
+_ATTEND, _ATTEND_BYTES = _lib.PROMPT_ENTRIES
+_native = _lib._native
 
 
 def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, *, offsets: Optional[torch.Tensor] = None,
@@ -30,6 +33,14 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     M, 128] by `key_offsets`, or by the same offsets; `starts` is [S] then.  Queries that no sequence has get 0 and -inf.  Nothing is read back.
 
     Grouped heads: Hq a multiple of Hkv.  For inference: tensors that require gradients are refused while gradients are recorded."""
+    if isinstance(query, torch.Tensor) and query.is_cuda and query.device.index == _device() and (softcap is None or _LEAST_CAP <= softcap < math.inf) and (
+            window is None or (window >= 1 and causal)):
+        # (everything as the kernel takes it: one native call)
+        done = _native.prompt_attend(_ATTEND, _ATTEND_BYTES, query.device.index, query, keys, values, offsets, key_offsets, starts, causal,
+                                     0 if window is None else min(window, _FAR), _SCALING if scaling is None else scaling, 0.0 if softcap is None else softcap,
+                                     return_lse, _lib.stream_ptr(query.device))
+        if done is not None:
+            return done
     for t, what in ((query, "queries"), (keys, "keys"), (values, "values")):
         if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.shape[3] != HEAD_DIM:
             raise ValueError(f"{what} must be [B, heads, tokens, {HEAD_DIM}], got {tuple(getattr(t, 'shape', ())) or type(t).__name__}")

@@ -308,39 +308,50 @@ struct Plan {
     __device__ inline int group(int row) const { return at[1 + rows + row]; }
     __device__ inline int member(int row) const { return at[1 + 2 * rows + row]; }          // its place in the group
     __device__ inline int order(int i) const { return at[1 + 3 * rows + i]; }               // rows, a group's behind one another
-    __device__ inline int begin(int g) const { return at[1 + 4 * rows + 3 * g]; }
-    __device__ inline int members(int g) const { return at[2 + 4 * rows + 3 * g]; }
-    __device__ inline int blocks(int g) const { return at[3 + 4 * rows + 3 * g]; }
+    __device__ inline int begin(int g) const { return at[1 + 4 * rows + 4 * g]; }
+    __device__ inline int members(int g) const { return at[2 + 4 * rows + 4 * g]; }
+    __device__ inline int blocks(int g) const { return at[3 + 4 * rows + 4 * g]; }
+    __device__ inline int slot(int g) const { return at[4 + 4 * rows + 4 * g]; }            // where its first row's table lies
 };
 
 #define SHARED_COLS 128      // queries of a kv-head that a workgroup takes over what is in common
 // The workgroups of a kv-head that take what is in common: one for each tile of a group, the `spare` others in proportion to the tiles' blocks, several blocks each at least:
 // a share costs its partial results.  Given a workgroup: its tile and share; given a group: how its tiles are shared; and where the group's partial results begin.
-struct CommonShare { int group, tile, split, splits, parts; };
+struct CommonShare { int group, tile, split, splits, parts, begin, cols, blocks, slot; };
 template <bool BY_GROUP = false>
 __device__ static inline CommonShare common_share_of(const AttendArgs& a, int at) {
     const Plan plan(a);
-    const int lane = threadIdx.x & 63, R = a.G * a.L, groups = plan.groups();
-    const auto tiles_of = [&](int g) { return g < groups ? (plan.members(g) * R + SHARED_COLS - 1) / SHARED_COLS : 0; };
-    long long total = 0;
-    for (int g0 = 0; g0 < groups; g0 += 64) {
-        const int weight = tiles_of(g0 + lane) * (g0 + lane < groups ? plan.blocks(g0 + lane) : 0);
-        total += __builtin_amdgcn_readlane(wave_scan(weight), 63);
+    const int lane = threadIdx.x & 63, R = a.G * a.L, most = a.p.rows / 2 - 1;
+    // (asked for beside the number of groups, not behind it)
+    struct Group { int begin, cols, blocks, slot; };
+    const auto group_of = [&](int g) {
+        const int at = min(g, most), begin = plan.begin(at), members = plan.members(at), blocks = plan.blocks(at), slot = plan.slot(at);
+        return g < plan.groups() ? Group{begin, members * R, blocks, slot} : Group{0, 0, 0, 0};
+    };
+    const auto tiles_of = [](const Group& g) { return (g.cols + SHARED_COLS - 1) / SHARED_COLS; };
+    Group mine = group_of(lane);
+    const int groups = plan.groups();
+    long long total = __builtin_amdgcn_readlane(wave_scan(tiles_of(mine) * mine.blocks), 63);
+    for (int g0 = 64; g0 < groups; g0 += 64) {
+        const Group next = group_of(g0 + lane);
+        total += __builtin_amdgcn_readlane(wave_scan(tiles_of(next) * next.blocks), 63);
     }
     int before = 0, parts = 0;
     for (int g0 = 0; g0 < groups; g0 += 64) {
-        const int g = g0 + lane, tiles = tiles_of(g), cols = g < groups ? plan.members(g) * R : 0, blocks = g < groups ? plan.blocks(g) : 0;
-        const int splits = min(1 + (int)((long long)blocks * a.spare / max(total, 1LL)), max(blocks / (cols > 64 ? 8 : 4), 1));
-        const int upto = before + wave_scan(tiles * splits), parts_upto = parts + wave_scan(splits * cols);
+        if (g0 > 0) mine = group_of(g0 + lane);
+        const int tiles = tiles_of(mine);
+        const int splits = min(1 + (int)((long long)mine.blocks * a.spare / max(total, 1LL)), max(mine.blocks / (mine.cols > 64 ? 8 : 4), 1));
+        const int upto = before + wave_scan(tiles * splits), parts_upto = parts + wave_scan(splits * mine.cols);
         const unsigned long long here = BY_GROUP ? (at < g0 + 64 ? 1ULL << (at - g0) : 0) : __ballot(upto > at);
         if (here) {
             const int l = __builtin_ctzll(here), n = __builtin_amdgcn_readlane(splits, l), first = __builtin_amdgcn_readlane(upto - tiles * splits, l);
-            return {g0 + l, (at - first) / n, (at - first) % n, n, __builtin_amdgcn_readlane(parts_upto - splits * cols, l)};
+            return {g0 + l, (at - first) / n, (at - first) % n, n, __builtin_amdgcn_readlane(parts_upto - splits * mine.cols, l),
+                    __builtin_amdgcn_readlane(mine.begin, l), __builtin_amdgcn_readlane(mine.cols, l), __builtin_amdgcn_readlane(mine.blocks, l), __builtin_amdgcn_readlane(mine.slot, l)};
         }
         before = __builtin_amdgcn_readlane(upto, 63);
         parts = __builtin_amdgcn_readlane(parts_upto, 63);
     }
-    return {-1, 0, 0, 0, 0};
+    return {-1, 0, 0, 0, 0, 0, 0, 0, 0};
 }
 
 #define NARROW 16            // queries of a kv-head that the narrow kernel takes

@@ -18,15 +18,13 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
     size_t at = ((size_t)row * p.Hkv + h) * a.splits * R + r;
     int in_common = 0, cols = 0;
     size_t common_at = 0;
-    if (SHARED) {
+    if (SHARED) {                                               // (nothing here waits for anything else here)
         const Plan plan(a);
-        if (plan.common(row) > 0) {
-            const int g = plan.group(row);
-            const CommonShare share = common_share_of<true>(a, g);
-            in_common = share.splits;
-            cols = plan.members(g) * R;
-            common_at = (size_t)h * a.common_parts + share.parts + (size_t)plan.member(row) * R + r;
-        }
+        const int common = plan.common(row), g = max(plan.group(row), 0), member = plan.member(row);
+        const CommonShare share = common_share_of<true>(a, g);
+        in_common = common > 0 ? share.splits : 0;
+        cols = share.cols;
+        common_at = (size_t)h * a.common_parts + share.parts + (size_t)member * R + r;
     }
     if (NARROW_PARTS) {
         const Share own = share_of<true, SHARED>(a, row);

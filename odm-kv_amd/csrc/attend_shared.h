@@ -21,36 +21,20 @@ __device__ static inline void attend_common(const AttendArgs& a, unsigned workgr
     const CommonShare own = common_share_of(a, workgroup / p.Hkv);
     if (own.group < 0) return;
     const Plan plan(a);
-    const int begin = __builtin_amdgcn_readfirstlane(plan.begin(own.group)), cols = __builtin_amdgcn_readfirstlane(plan.members(own.group)) * R;
-    const int in_common = __builtin_amdgcn_readfirstlane(plan.blocks(own.group)), split = __builtin_amdgcn_readfirstlane(own.split), splits = __builtin_amdgcn_readfirstlane(own.splits);
-    const int col0 = __builtin_amdgcn_readfirstlane(own.tile) * SHARED_COLS, slot = __builtin_amdgcn_readfirstlane(p.slot[plan.order(begin)]);
+    const int begin = own.begin, cols = own.cols, in_common = own.blocks, split = own.split, splits = own.splits, col0 = own.tile * SHARED_COLS, slot = own.slot;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const bool halves = cols - col0 <= 64;                      // two wavefronts a 32 of queries
     const int group = halves ? wave & 1 : wave, part = halves ? wave >> 1 : 0;
-    const int c0 = col0 + 32 * group + col, member = c0 / R, r = c0 - member * R, l = r / a.G, hq = h * a.G + r - l * a.G;
-    const bool in = c0 < cols;
-    const int row = in ? plan.order(begin + member) : 0, len = p.length[row], count = a.counts ? min(max(a.counts[row], 0), a.L) : a.L;
+    const int c0 = col0 + 32 * group + col, at = min(c0, cols - 1), member = at / R, r = at - member * R, l = r / a.G, hq = h * a.G + r - l * a.G;
+    const bool in = c0 < cols;                                  // (where there is no query the last one stands, and is left out at the end)
+    const int row = plan.order(begin + member), len = p.length[row], count = a.counts ? min(max(a.counts[row], 0), a.L) : a.L;
     const bool valid = in && l < count;
-    Sight s = {0, 0, 0};
-    if (valid) s = sight_of(a, row, len, count, l);
-    s.hi = min(s.hi, in_common * BLOCK_TOKENS);
-    const bool sees = valid && s.lo < s.hi;
-    const int wave_lo = wave_min_int(sees ? s.lo : 0x7fffffff), wave_hi = -wave_min_int(sees ? -s.hi : 0);       // what some query of the wavefront sees
-    const int open_from = -wave_min_int(valid ? -(sees ? s.lo : 0x7fffffff) : 0), open_to = wave_min_int(valid ? s.hi : 0x7fffffff);    // what all of them see
-    if (lane == 0) {
-        range[0][wave] = wave_lo;
-        range[1][wave] = wave_hi;
-    }
-    __syncthreads();
-    const int lo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3])), hi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
-    const int first = lo / BLOCK_TOKENS, blocks = max((hi + BLOCK_TOKENS - 1) / BLOCK_TOKENS - first, 0), share = (blocks + splits - 1) / splits;
-    const int b0 = __builtin_amdgcn_readfirstlane(first + split * share), mine = __builtin_amdgcn_readfirstlane(min(share, blocks - split * share));
-
     // ---- a block on its way: pieces of 16 codes, a token's 16 dims or a dim's 16 tokens
     constexpr int PIECES = PAGE_BYTES / 16 / THREADS;
     uint4 kc[PIECES], vc[PIECES];
     int page_of = 0;
+    int b0 = split * ((in_common + splits - 1) / splits), mine = min(in_common - b0, (in_common + splits - 1) / splits);
     const auto look_up = [&](int i) { return i + lane < mine ? p.table[(size_t)slot * p.blocks + b0 + i + lane] : 0; };
     const auto request = [&](int i) {                           // block b0 + i
         if ((i & 63) == 0) page_of = look_up(i);
@@ -73,7 +57,26 @@ __device__ static inline void attend_common(const AttendArgs& a, unsigned workgr
             *reinterpret_cast<f16x8*>(value_piece(buf, i >> 2, 2 * (i & 3) + 1)) = codes_f16<KIND>(vc[c].y, vc[c].w);
         }
     };
+    // (asked for as if all of what is in common were seen: what each query sees is known a few reads later)
     if (mine > 0) request(0);
+    Sight s = {0, 0, 0};
+    if (valid) s = sight_of(a, row, len, count, l);
+    s.hi = min(s.hi, in_common * BLOCK_TOKENS);
+    const bool sees = valid && s.lo < s.hi;
+    const int wave_lo = wave_min_int(sees ? s.lo : 0x7fffffff), wave_hi = -wave_min_int(sees ? -s.hi : 0);       // what some query of the wavefront sees
+    const int open_from = -wave_min_int(valid ? -(sees ? s.lo : 0x7fffffff) : 0), open_to = wave_min_int(valid ? s.hi : 0x7fffffff);    // what all of them see
+    if (lane == 0) {
+        range[0][wave] = wave_lo;
+        range[1][wave] = wave_hi;
+    }
+    __syncthreads();
+    const int lo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3])), hi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
+    const int first = lo / BLOCK_TOKENS, blocks = max((hi + BLOCK_TOKENS - 1) / BLOCK_TOKENS - first, 0), share = (blocks + splits - 1) / splits;
+    if (first + split * share != b0 || min(share, blocks - split * share) != mine) {
+        b0 = __builtin_amdgcn_readfirstlane(first + split * share);
+        mine = __builtin_amdgcn_readfirstlane(min(share, blocks - split * share));
+        if (mine > 0) request(0);
+    }
 
     f16x8 q[8];                                                 // dims 16 st + 8 half + e
     float qdown = 1.0f;
@@ -81,7 +84,7 @@ __device__ static inline void attend_common(const AttendArgs& a, unsigned workgr
         uint4 raw[8];
         const uint16_t* src = a.q + row * a.qb + hq * a.qh + l * a.ql + 8 * half;
 #pragma unroll
-        for (int st = 0; st < 8; ++st) raw[st] = valid ? *reinterpret_cast<const uint4*>(src + 16 * st) : make_uint4(0, 0, 0, 0);
+        for (int st = 0; st < 8; ++st) raw[st] = *reinterpret_cast<const uint4*>(src + 16 * st);
         if constexpr (DT == ODMKV_BF16) {
             uint32_t top = 0;
 #pragma unroll
@@ -130,26 +133,16 @@ __device__ static inline void attend_common(const AttendArgs& a, unsigned workgr
         if (t0 >= wave_hi || t0 + BLOCK_TOKENS <= wave_lo) continue;      // (of the wavefront's own queries none sees the block)
         const float c = scale_of(ks, qs);
         const bool cut = t0 < open_from || t0 + BLOCK_TOKENS > open_to;
-        f32x16 dot[2];
-        f16x8 w[4];
         Terms z = terms_of(sums, u);
-        const auto multiply_keys = [&](int tb, int place) {
-            f32x16& x = dot[tb];
+#pragma unroll 1
+        for (int place = part; place < (halves ? part + 1 : 2); ++place) {
+            f32x16 x;
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = 0.0f;
 #pragma unroll
             for (int st = 0; st < 8; ++st) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(*key_piece(buf, 32 * place + col, 2 * st + half), q[st], x, 0, 0, 0);
-        };
-        const auto multiply_values = [&](int st, int place) {
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(value_piece(buf, 32 * db + col, 2 * place + half)), w[st], acc[db], 0, 0, 0);
-        };
-        // products of half a block to scores (PLAIN: they stay products); the largest score
-        const auto to_scores = [&](int tb, int place) {
-            f32x16& x = dot[tb];
             const int tl = t0 + 32 * place + 4 * half;             // token of score e: tl + 8 (e / 4) + e % 4
-            if constexpr (!PLAIN) {
+            if constexpr (!PLAIN) {                                // (PLAIN: they stay products)
                 if (by_exp) {
                     const float k = c * cap.plain;
 #pragma unroll
@@ -177,54 +170,33 @@ __device__ static inline void attend_common(const AttendArgs& a, unsigned workgr
             float top = x[0];
 #pragma unroll
             for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-            return PLAIN && top > -INFINITY ? top * c : top;         // (c is not negative: the largest product is the largest score)
-        };
-        // the sums' references where a score is to move them: what the values' sums are to be multiplied by
-        const auto move_sums = [&](float top, float& old) {
-            if (!__any(top > z.limit)) return false;
-            const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-            old = raise(sums, most, most, u.lift);
-            z = terms_of(sums, u);
-            return true;
-        };
-        const auto multiply_sums = [&](float old) {
+            if (PLAIN) top = top > -INFINITY ? top * c : top;      // (c is not negative: the largest product is the largest score)
+            if (__any(top > z.limit)) {
+                const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                const float most = fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1])), old = raise(sums, most, most, u.lift);
+                z = terms_of(sums, u);
 #pragma unroll
-            for (int db = 0; db < 4; ++db) acc[db] *= old;
-        };
-        // the factor comes out of the exponential itself, the block's sum is freed of it
-        const auto weigh = [&](int tb) {
+                for (int db = 0; db < 4; ++db) acc[db] *= old;
+            }
+            // the factor comes out of the exponential itself, the sum is freed of it
+            f16x8 w[2];
             float z0 = 0.0f, z1 = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e], c, z.shift) : dot[tb][e] + z.shift);
-                const float p1 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(dot[tb][e + 1], c, z.shift) : dot[tb][e + 1] + z.shift);
+                const float p0 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(x[e], c, z.shift) : x[e] + z.shift);
+                const float p1 = __builtin_amdgcn_exp2f(PLAIN ? __fmaf_rn(x[e + 1], c, z.shift) : x[e + 1] + z.shift);
                 z0 += p0;
                 z1 += p1;
-                w[2 * tb + (e >> 3)][e & 7] = (_Float16)p0;
-                w[2 * tb + (e >> 3)][(e & 7) + 1] = (_Float16)p1;
+                w[e >> 3][e & 7] = (_Float16)p0;
+                w[e >> 3][(e & 7) + 1] = (_Float16)p1;
             }
             sums.sum = __fmaf_rn(z0 + z1, __builtin_amdgcn_exp2f(-z.factor), sums.sum);
-        };
-        float old;
-        if (halves) {
-            multiply_keys(0, part);
-            if (move_sums(to_scores(0, part), old)) multiply_sums(old);
-            weigh(0);
-            multiply_values(0, 2 * part);
-            multiply_values(1, 2 * part + 1);
-        } else {                                                // one half's vector work beside the other's products
-            multiply_keys(0, 0);
-            if (move_sums(to_scores(0, 0), old)) multiply_sums(old);
-            multiply_keys(1, 1);
-            weigh(0);
-            const bool moved = move_sums(to_scores(1, 1), old);
-            multiply_values(0, 0);
-            multiply_values(1, 1);
-            weigh(1);
-            if (moved) multiply_sums(old);
-            multiply_values(2, 2);
-            multiply_values(3, 3);
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int db = 0; db < 4; ++db)
+                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8*>(value_piece(buf, 32 * db + col, 2 * (2 * place + st) + half)), w[st], acc[db],
+                                                                     0, 0, 0);
         }
     }
     if (halves) {                                               // the second half's sums join the first's, by way of LDS

@@ -25,8 +25,9 @@ __host__ __device__ static inline size_t tail_at(const odmkv_pages_t& p, int lay
 }
 
 // A plan of common blocks: how many groups; by row the blocks that its group has in common (0: it is in none), its group, its place there; the groups' rows one behind the
-// other; by group where it begins among those, its rows, its blocks
-__host__ __device__ static inline size_t plan_words(int rows) { return 1 + 4 * (size_t)rows + 3 * (size_t)(rows / 2); }
+// other; by group where it begins among those, its rows, its blocks, the slot of its
+// first row
+__host__ __device__ static inline size_t plan_words(int rows) { return 1 + 4 * (size_t)rows + 4 * (size_t)(rows / 2); }
 
 // what is not finite is stored as 0, two 16-bit values at a time
 template <int DT>

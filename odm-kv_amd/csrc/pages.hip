@@ -561,10 +561,11 @@ __global__ __launch_bounds__(BOOK_THREADS) void pages_plan_common_kernel(odmkv_p
     if (is_group) {
         number[tid] = g;
         begin[tid] = end - count[tid];
-        int32_t* const to = plan + 1 + 4 * rows + 3 * g;
+        int32_t* const to = plan + 1 + 4 * rows + 4 * g;
         to[0] = begin[tid];
         to[1] = count[tid];
         to[2] = least[tid];
+        to[3] = slots[tid];
     }
     if (tid == 0) plan[0] = n;
     __syncthreads();

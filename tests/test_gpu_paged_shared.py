@@ -36,8 +36,9 @@ def _plan(c):
     common, group, member, order = (plan[1 + i * B:1 + (i + 1) * B] for i in range(4))
     groups = []
     for g in range(plan[0]):
-        begin, members, blocks = plan[1 + 4 * B + 3 * g:4 + 4 * B + 3 * g]
+        begin, members, blocks, slot = plan[1 + 4 * B + 4 * g:5 + 4 * B + 4 * g]
         rows = order[begin:begin + members]
+        assert slot == int(c.slot[rows[0]])
         for i, b in enumerate(rows):
             assert group[b] == g and member[b] == i and common[b] == blocks
         groups.append((rows, blocks))

@@ -6,6 +6,7 @@
 // same bits as those three operations one by one), then once to 16 bits, as a model that turns its keys itself hands them over.  Keys are stored as pages_write stores them:
 // what the cache holds hangs on the turned keys in 16 bits alone, not on how they arrive.
 #include <algorithm>
+#include <type_traits>
 #include "pages_write.h"
 
 struct RotateArgs {
@@ -119,7 +120,12 @@ __device__ static inline bool row_fits(const RotateArgs& a, int row, int start, 
 
 // The first workgroups store a block of a row and kv-head each, the others turn the queries of 32 tokens: eight threads a token, which keep its eight pairs' angles for
 // `heads` heads one behind the other.
-template <int DT, int KIND>
+//
+// STREAM: queries pass by the caches, both ways.  Those of a prompt that the last-level cache (256 MB) would not keep until they are read again cost the codes their places there, and the
+// loads themselves are faster: 32768 tokens of 32 heads (268 MB) 171 us for 158, and the cache's rows read back behind it 51 for 40.  Queries that come out of that cache (130 MB) take 38
+// us, and 55 past it.
+#define QUERIES_AHEAD 2
+template <int DT, int KIND, bool STREAM>
 __global__ __launch_bounds__(256) void pages_rotate_kernel(RotateArgs a) {
     const odmkv_pages_t& p = a.w.p;
     const int tid = threadIdx.x;
@@ -181,11 +187,27 @@ __global__ __launch_bounds__(256) void pages_rotate_kernel(RotateArgs a) {
     }
     Angles z = {};
     if (x < a.turned / 16) z = angles_at(a, position, x);
-    for (int h = h0; h < h1; ++h) {
-        uint4 q0 = *reinterpret_cast<const uint4*>(src + h * a.qh + d0), q1 = *reinterpret_cast<const uint4*>(src + h * a.qh + d1);
-        if (x < a.turned / 16) turn<DT, false>(q0, q1, z, a.interleaved);
-        *reinterpret_cast<uint4*>(dst + h * HD + d0) = q0;
-        *reinterpret_cast<uint4*>(dst + h * HD + d1) = q1;
+    for (int h = h0; h < h1; h += QUERIES_AHEAD) {
+        uint4 q0[QUERIES_AHEAD], q1[QUERIES_AHEAD];
+#pragma unroll
+        for (int i = 0; i < QUERIES_AHEAD; ++i) {
+            const uint16_t* const from = src + min(h + i, h1 - 1) * a.qh;
+            q0[i] = STREAM ? load_once(from + d0) : *reinterpret_cast<const uint4*>(from + d0);
+            q1[i] = STREAM ? load_once(from + d1) : *reinterpret_cast<const uint4*>(from + d1);
+        }
+#pragma unroll
+        for (int i = 0; i < QUERIES_AHEAD; ++i) {
+            if (h + i >= h1) break;
+            if (x < a.turned / 16) turn<DT, false>(q0[i], q1[i], z, a.interleaved);
+            uint16_t* const to = dst + (h + i) * HD;
+            if (STREAM) {
+                store_once(to + d0, q0[i]);
+                store_once(to + d1, q1[i]);
+            } else {
+                *reinterpret_cast<uint4*>(to + d0) = q0[i];
+                *reinterpret_cast<uint4*>(to + d1) = q1[i];
+            }
+        }
     }
 }
 
@@ -227,13 +249,22 @@ extern "C" int odmkv_pages_write_rotated(const odmkv_rotate_t* d, void* stream) 
     const long long kv_groups = (long long)((d->T + BLOCK_TOKENS - 2) / BLOCK_TOKENS + 1) * p.Hkv * p.rows;
     const long long tiles = d->Hq == 0 && !d->k_out ? 0 : ((d->offsets ? (long long)d->tokens : (long long)p.rows * d->T) + 31) / 32;
     a.heads = 1;
-    while (a.heads < 8 && tiles * ((d->Hq + 2 * a.heads - 1) / (2 * a.heads)) >= 4LL * compute_units()) a.heads *= 2;
+    while (a.heads < 4 && tiles * ((d->Hq + 2 * a.heads - 1) / (2 * a.heads)) >= 4LL * compute_units()) a.heads *= 2;
     a.head_groups = std::max(1, (d->Hq + a.heads - 1) / a.heads);
     a.kv_groups = (int)kv_groups;
     const long long groups = kv_groups + tiles * a.head_groups;
     ODMKV_CHECK_ARG(groups * 256 < 0x100000000LL, "pages_write_rotated: too many tokens");
-    const dim3 grid((unsigned)groups);
-    PAGES_DISPATCH(pages_rotate_kernel, &p, grid, dim3(256), 0, (hipStream_t)stream, a);
+    const auto run = [&](auto dt, auto kind) {
+        const bool past = (long long)(d->offsets ? 1 : p.rows) * a.tokens * d->Hq * HD * 2 > (192LL << 20);
+        if (past) hipLaunchKernelGGL((pages_rotate_kernel<dt.value, kind.value, true>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL((pages_rotate_kernel<dt.value, kind.value, false>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a);
+    };
+    const auto of_kind = [&](auto dt) {
+        if (p.kind == ODMKV_INT8) run(dt, std::integral_constant<int, ODMKV_INT8>());
+        else run(dt, std::integral_constant<int, ODMKV_E4M3>());
+    };
+    if (p.dtype == ODMKV_F16) of_kind(std::integral_constant<int, ODMKV_F16>());
+    else of_kind(std::integral_constant<int, ODMKV_BF16>());
     ODMKV_CHECK_LAUNCH("pages_rotate_kernel");
     return 0;
 }

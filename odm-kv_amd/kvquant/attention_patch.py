@@ -10,7 +10,7 @@ Stands where the reference's kvquant/attention_patch.py:13-62 stands.  Three beh
   press appends them in its forward hook, afterwards).  Evicted tokens are absent from the store, so
   no fake keys are needed.
 * new tokens of a `PagedCache` (kvquant/hf_cache.py) attend over its pages (``PagedKVCache.attend``), and so does its prompt where
-  scores are capped;
+  scores are capped; built with ``native_prompt`` it has its prompts attended by ``prompt_attention``;
 * everything else goes to the wrapped attention function as in the reference, with evicted keys
   replaced by a fake key whose weight underflows to zero (``search_hyperplane``).
 """
@@ -34,7 +34,7 @@ _NATIVE_PAIRS = 3 << 20
 _PATCH_ATTR = "_kvtoken_quant_attention_patched"
 # how many decode calls took the fused kernel / the wrapped attention function (diagnostics)
 call_counts = {"fused": 0, "dense": 0}
-paged_counts = {"paged": 0}                              # and the paged cache's kernels
+paged_counts = {"paged": 0, "prompt": 0}                 # and the paged cache's kernels, those of prompts by themselves
 
 
 def search_hyperplane(x: torch.Tensor, max_iter: int = 1000) -> torch.Tensor:
@@ -226,8 +226,9 @@ def _paged_refuses(module, L, attention_mask, dropout, kwargs) -> bool:
     return False
 
 
-def _paged_attention(paged, module, query, attention_mask, dropout, kwargs):
-    """Attention output [B, L, Hq, D] over a `PagedCache`, whose pages and tails hold the new tokens already."""
+def _paged_attention(paged, module, query, attention_mask, dropout, kwargs, rows=None):
+    """Attention output [B, L, Hq, D] over a `PagedCache`, whose pages and tails hold the new tokens already; over `rows` (a prompt's keys and values in 16 bits) where
+    they are given."""
     pool, index, k_len = paged
     window = kwargs.get("sliding_window")
     starts = None
@@ -237,7 +238,15 @@ def _paged_attention(paged, module, query, attention_mask, dropout, kwargs):
     if starts is False or _paged_refuses(module, query.shape[2], attention_mask, dropout, kwargs):
         raise RuntimeError("this call cannot be answered from the paged cache: it takes causal attention, with padding in front, a sliding window or a soft cap, "
                            "but no dropout, position bias, attention sinks as parameters or other masks")
-    out = pool.attend(index, query, scaling=kwargs.get("scaling"), softcap=kwargs.get("softcap"), window=window, starts=starts)
+    how = dict(scaling=kwargs.get("scaling"), softcap=kwargs.get("softcap"), window=window, starts=starts)
+    if rows is not None:
+        from kvquant.prompt import prompt_attention
+        out = prompt_attention(query, *rows, **how)
+        paged_counts["prompt"] += 1
+        return out
+    if getattr(pool, "shares", False):
+        how["shared"] = True
+    out = pool.attend(index, query, **how)
     paged_counts["paged"] += 1
     return out
 
@@ -252,7 +261,7 @@ def _attention_patch(func):
         if paged is None and kwargs.get("softcap") is not None:
             paged = getattr(key, "_odmkv_prompt", None)  # a prompt that such a cache holds: "sdpa" would leave the cap out
         if paged is not None:
-            return _paged_attention(paged, module, query, attention_mask, dropout, kwargs), None
+            return _paged_attention(paged, module, query, attention_mask, dropout, kwargs, getattr(key, "_odmkv_prompt_rows", None)), None
         # a decode step like the layer's last one: the native block checks the call, stores the token and attends
         state = module.__dict__.get("_odmkv_state")
         fast = None if state is None else getattr(state, "_fast", None)

@@ -155,7 +155,8 @@ class PagedCacheLayer(CacheLayerMixin):
         self.is_initialized = True
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
-        """Stores the new tokens.  The first ones of a row (the prompt) go back as they are, for the model's own attention in full precision, unless that caps scores, which
+        """Stores the new tokens.  With `native_prompt` the first ones of a row (the prompt) go back as `PagedTokens` that carry themselves, for the attention patch to hand to
+        `prompt_attention`.  Otherwise they go back as they are, for the model's own attention in full precision, unless that caps scores, which
         the registered functions that a model would use here leave out in silence (a call with `softcap` finds its way by the mark); these and all later ones go
         back as `PagedTokens`, for the attention patch, which reads everything from the pages."""
         owner, T = self.owner, key_states.shape[-2]
@@ -165,6 +166,10 @@ class PagedCacheLayer(CacheLayerMixin):
         owner.pool.write(self.index, key_states, value_states)
         before, self.length = self.length, self.length + T
         paged = (owner.pool, self.index, self.length)
+        if before == 0 and owner.native_prompt:
+            tokens = paged_tokens(key_states, value_states, paged)
+            tokens[0]._odmkv_prompt_rows = (key_states, value_states)
+            return tokens
         if before == 0 and not owner.capped:
             key_states._odmkv_prompt = paged
             return key_states, value_states
@@ -202,9 +207,13 @@ class PagedCache(Cache):
     windows included.  Where scores are capped, the prompt attends over the pages as well: one cap from the first token on.  Beams and samples share the pages of what they have in common: ``reorder_cache``, ``batch_repeat_interleave`` and
     ``batch_select_indices`` copy 16-bit tails and count holders.  The pool starts at the prompt's size and is grown as rows do.
 
-    `config`: the model's; its attention must be one of the registered functions (not "eager", which cannot be told to read the pages)."""
+    `config`: the model's; its attention must be one of the registered functions (not "eager", which cannot be told to read the pages).
 
-    def __init__(self, config, max_tokens: Optional[int] = None, kind: str = "int8"):
+    `shared`: steps read the pages that rows have in common once for all of them (``PagedKVCache.attend(shared=True)``): for beams and samples of long prompts.
+    `native_prompt`: the prompt is attended by ``kvquant.prompt_attention``, padding in front, windows and soft caps included, in the model's own precision where scores
+    are capped too; the model's own attention is not called then."""
+
+    def __init__(self, config, max_tokens: Optional[int] = None, kind: str = "int8", *, shared: bool = False, native_prompt: bool = False):
         text = config.get_text_config(decoder=True)
         head_dim = getattr(text, "head_dim", None) or text.hidden_size // text.num_attention_heads
         kinds = set(getattr(text, "layer_types", None) or ()) - {"full_attention", "sliding_attention"}
@@ -221,6 +230,7 @@ class PagedCache(Cache):
         self.capped = getattr(text, "attn_logit_softcapping", None) is not None
         self.max_tokens = int(text.max_position_embeddings if max_tokens is None else max_tokens)
         self.kind, self.pool, self._extended = kind, None, 0
+        self.shared, self.native_prompt = bool(shared), bool(native_prompt)
         super().__init__(layers=[PagedCacheLayer(self, i) for i in range(text.num_hidden_layers)])
 
     def _make(self, keys: torch.Tensor) -> None:
@@ -228,6 +238,7 @@ class PagedCache(Cache):
         if self.pool is None or (self._extended == 0 and self.pool.batch != B):
             self.pool = PagedKVCache(B, H, self.max_tokens, layers=len(self.layers), pages=B * (T // 64 + 4), kind=self.kind, dtype=keys.dtype,
                                      device=keys.device, head_dim=keys.shape[-1])
+            self.pool.shares = self.shared
 
     def _room(self, length: int) -> None:
         """The rows hold `length` tokens from here on: the first layer that comes by with new ones sees to it for all."""

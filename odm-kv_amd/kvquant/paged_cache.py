@@ -91,6 +91,8 @@ class PagedKVCache:
         with torch.cuda.device(device):
             _lib.check(lib.odmkv_pages_init(C.byref(self._p), _lib.stream_ptr(device)))
 
+    shares = False                                           # how a model's steps ask for `attend` (kvquant/attention_patch.py): with shared=True
+
     # ------------------------------------------------------------------ memory
     def _make_pool(self, pages: int) -> None:
         codes, empty = KINDS[self.kind][1], dict(device=self.device)
@@ -134,7 +136,7 @@ class PagedKVCache:
         new = object.__new__(PagedKVCache)
         for name in ("device", "dtype", "kind", "layers", "kv_heads", "max_tokens"):
             setattr(new, name, getattr(self, name))
-        new.batch = batch
+        new.batch, new.shares = batch, self.shares
         return new
 
     def _call(self, fn, *args) -> None:

@@ -15,7 +15,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 #define PROMPT_COLS(waves) (32 * (waves))
 #define PROMPT_TILE (BLOCK_TOKENS * HD * 2)                      // bytes of a block of keys, or of values
-#define PROMPT_LDS (4 * PROMPT_TILE)
+#define PROMPT_LDS(waves) (2 * PROMPT_TILE + max(2 * PROMPT_TILE, (waves) * 32 * HD * 2))
 
 struct PromptArgs {
     const uint16_t* q;
@@ -159,16 +159,25 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     };
     if (mine > 0) request(0);
 
-    uint4 q[8];                                                 // dims 16 st + 8 half + e; of the last query where there is none
+    // The queries come the same way, four rows a request, behind the first block's place.
+    const uint32_t queries_at = lds0 + 2 * PROMPT_TILE + wave * 32 * HD * 2;
     {
         const int at = min(l, tile.n - 1);
-        const uint16_t* src = a.q + (a.offsets ? (int64_t)(tile.q0 + at) * a.qt : row * a.qb + at * a.qt) + hq * a.qh + 8 * half;
+        const uint64_t src = (uint64_t)(a.q + (a.offsets ? (int64_t)(tile.q0 + at) * a.qt : row * a.qb + at * a.qt) + hq * a.qh);
 #pragma unroll
-        for (int st = 0; st < 8; ++st) q[st] = *reinterpret_cast<const uint4*>(src + 16 * st);
+        for (int j = 0; j < 8; ++j) {
+            const int of = 4 * j + (lane >> 4);
+            const uint64_t from = (uint64_t)(uint32_t)__shfl((int)(src >> 32), of) << 32 | (uint32_t)__shfl((int)src, of);
+            request_to_lds((const uint16_t*)from + (((lane ^ of) & 15) << 3), queries_at + 1024 * j);
+        }
     }
-    // (they have come when the loop begins: waited for in the loop, they would be waited for in every turn, and the next block with them)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    uint4 q[8];                                                 // dims 16 st + 8 half + e; of the last query where there is none
 #pragma unroll
-    for (int st = 0; st < 8; ++st) asm volatile("" : "+v"(q[st].x), "+v"(q[st].y), "+v"(q[st].z), "+v"(q[st].w));
+    for (int st = 0; st < 8; ++st) {
+        const u32x4 x = *(const __attribute__((address_space(3))) u32x4*)(size_t)(queries_at + col * 256 + (((2 * st + half) ^ (col & 15)) << 4));
+        q[st] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
     const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
     const bool by_exp = MODE == 1 || (!PLAIN && a.cap > 0.0f && a.cap <= CAP_BY_EXP);
     const Cap cap = {a.cap * LOG2E, 2.0f * LOG2E * a.cap, 2.0f * LOG2E * inv_cap};
@@ -272,12 +281,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
         multiply_keys(0);
         // one half's vector work stands beside the other's products
         multiply_keys(1);
-        float z = weigh(dot[0], w);
+        float z = INFINITY;
+        if (PLAIN || !cut) z = weigh(dot[0], w);                // (under a cap it is work that counts; without, products of the other half stand beside it)
         if (cut || __any(!(z <= Weights<DT>::LIMIT))) z = weigh_again(dot[0], w, tl, cut);
         sum += z;
         multiply_values(0);
         multiply_values(1);
-        z = weigh(dot[1], w + 2);
+        if (PLAIN || !cut) z = weigh(dot[1], w + 2);
         if (cut || __any(!(z <= Weights<DT>::LIMIT))) z = weigh_again(dot[1], w + 2, tl + 32, cut);
         sum += z;
         multiply_values(2);
@@ -345,10 +355,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
         }
         by = 1.0f;
     }
-    if (!valid) return;
     const auto result = [&](int db, int e) { return none ? 0.0f : acc[db][e] * by; };
     const int64_t nth = (a.offsets ? 0 : (int64_t)row * a.L) + tile.q0 + l;                         // of all queries
     if (a.splits > 1) {
+        if (!valid) return;
         const int64_t all = a.offsets ? a.L : (int64_t)a.rows * a.L, to = (split * all + nth) * a.Hq + hq;
         float* dst = a.part_out + to * HD + 4 * half;
 #pragma unroll
@@ -363,7 +373,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
         if (half == 0) a.part_lse[to] = lse2;
         return;
     }
-    uint16_t* dst = a.out + (nth * a.Hq + hq) * HD + 4 * half;
+    __syncthreads();
+    // Through the wavefront's own part of LDS, which nobody reads any more, so that a store writes four whole rows; 8 bytes of a row each, as the lanes hold them, took 4 % longer
+    // for packed prompts of up to 2999 tokens (454 us for 436, the queries' way among it), 25 % for queries over 64 keys.
+    uint8_t* const rows_at = smem + wave * 32 * HD * 2;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -371,9 +384,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
             uint32_t x[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) x[e] = pair_16<DT>(result(db, 4 * g + 2 * e), result(db, 4 * g + 2 * e + 1));
-            *reinterpret_cast<uint2*>(dst + 32 * db + 8 * g) = make_uint2(x[0], x[1]);
+            *reinterpret_cast<uint2*>(rows_at + col * 256 + (((4 * db + g) ^ (col & 15)) << 4) + 8 * half) = make_uint2(x[0], x[1]);
         }
-    if (a.lse && half == 0) a.lse[((a.offsets ? 0 : (int64_t)row * a.Hq) + hq) * a.L + tile.q0 + l] = lse2 * LN2;
+    __builtin_amdgcn_wave_barrier();
+    const uint32_t to = valid ? (uint32_t)(nth * a.Hq + hq) : 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int of = 4 * j + (lane >> 4);
+        const uint4 x = *reinterpret_cast<const uint4*>(rows_at + of * 256 + (((lane ^ of) & 15) << 4));
+        const uint32_t at = (uint32_t)__shfl((int)to, of);
+        if (at != 0xffffffffu) *reinterpret_cast<uint4*>(a.out + (int64_t)at * HD + 8 * (lane & 15)) = x;
+    }
+    if (valid && a.lse && half == 0) a.lse[((a.offsets ? 0 : (int64_t)row * a.Hq) + hq) * a.L + tile.q0 + l] = lse2 * LN2;
 }
 
 // The shares of a query's blocks, put together: a wavefront a query, a lane two dims.
@@ -463,8 +485,8 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
     const hipStream_t st = (hipStream_t)stream;
     const auto run = [&](auto dt, auto mode_, auto waves) {
         const auto kernel = prompt_kernel<dt.value, mode_.value, waves.value>;
-        ODMKV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PROMPT_LDS));
-        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(waves.value * 64), PROMPT_LDS, st, a);
+        ODMKV_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PROMPT_LDS(waves.value)));
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(waves.value * 64), PROMPT_LDS(waves.value), st, a);
         ODMKV_CHECK_LAUNCH("prompt_kernel");
         if (cut.splits > 1) {
             hipLaunchKernelGGL(prompt_merge_kernel<dt.value>, dim3((unsigned)((all * d->Hq + 3) / 4)), dim3(256), 0, st, a);

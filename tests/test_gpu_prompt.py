@@ -85,6 +85,34 @@ def test_many_sequences():
         plain.check(out[0, a:e], lse[0, :, a:e], *plain.attend(q[0, :, a:e], k[0, :, a:e], v[0, :, a:e]))
 
 
+@pytest.mark.parametrize("scaling", [None, -0.02], ids=["plain", "negative"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_tiles_than_workgroups_take_at_once(dtype, scaling):
+    """Sequences of many lengths, empty ones among them, chunks that see nothing, infinite values behind what is seen; the same bits twice."""
+    lengths = [700, 0, 333, 1, 0, 900, 64, 63, 257, 500, 128, 2, 31, 640, 0, 411]
+    keys = [700, 5, 333, 1, 0, 950, 64, 0, 100, 900, 128, 2, 31, 640, 64, 411]
+    ends, key_ends = torch.tensor([7, *lengths]).cumsum(0), torch.tensor([3, *keys]).cumsum(0)
+    N, M = int(ends[-1]) + 11, int(key_ends[-1]) + 2
+    q, k, v = _inputs(12, 1, 32, 8, N, M, dtype)
+    v[0, :, 3 + 650] = float("inf")                                     # of the first sequence, whose first queries do not see it
+    call = dict(offsets=ends.to(torch.int32).to(DEV), key_offsets=key_ends.to(torch.int32).to(DEV), scaling=scaling)
+    out, lse = _call(q, k, v, **call)
+    for a, e, x, y in zip(ends.tolist(), ends.tolist()[1:], key_ends.tolist(), key_ends.tolist()[1:]):
+        plain.check(out[0, a:e], lse[0, :, a:e], *plain.attend(q[0, :, a:e], k[0, :, x:y], v[0, :, x:y], scaling=scaling))
+    for a, e in ((0, 7), (N - 11, N)):
+        assert not out[0, a:e].any() and bool((lse[0, :, a:e] == -torch.inf).all())
+    for _ in range(3):
+        again, lse_again = _call(q, k, v, **call)
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16)) and torch.equal(lse.view(torch.int32), lse_again.view(torch.int32))
+
+
+def test_more_tiles_in_rows():
+    _check(*_inputs(13, 2, 32, 8, 1500, 1500, torch.bfloat16), starts=[0, 333])
+    _check(*_inputs(14, 17, 24, 8, 260, 400, torch.float16), window=90)
+    q, k, v = _inputs(15, 1, 32, 8, 4200, 1, torch.float16)             # most see nothing
+    _check(q, k, v)
+
+
 @pytest.mark.parametrize("bad", [[0, 50, 40, 100], [-7, 30, 60, 100], [0, 30, 60, 500], [90, 50, 20, 0], [0, 2 ** 31 - 1, -2 ** 31, 100], [100, 100, 100, 100]], ids=str)
 def test_offsets_that_do_not_ascend_stay_within_the_tensors(bad):
     q, k, v = _inputs(10, 1, 4, 2, 100, 100, torch.float16)

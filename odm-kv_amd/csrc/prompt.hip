@@ -30,6 +30,7 @@ struct PromptArgs {
     int rows, L, T, Hq, Hkv, G, causal, window;
     float scaling, cap;
     int splits;                  // workgroups that share a tile's blocks
+    int larger;                  // 0: equal shares; or how many 1024ths of them the first of two has
     float* part_out;             // [splits, queries in all, Hq, 128]
     float* part_lse;             // the same without the 128, base 2
 };
@@ -96,8 +97,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];             // [2][keys 64 x 256 bytes, values 64 x 256 bytes]
     __shared__ int range[2][WAVES];
     // heads vary fastest: a die of the chip then keeps few heads' keys and values in its L2
-    const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % a.splits;
-    const Tile tile = tile_of<COLS>(a, rest / a.splits);
+    // (of unequal shares the larger ones come first, all of them)
+    const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, tiles = gridDim.x / a.Hkv / a.splits, split = a.larger ? rest / tiles : rest % a.splits;
+    const Tile tile = tile_of<COLS>(a, a.larger ? rest - split * tiles : rest / a.splits);
     if (tile.row < -1) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
     const int r = tile.nth * COLS + 32 * wave + col, l = r / a.G, hq = h * a.G + r - l * a.G;
@@ -124,8 +126,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
         from = min(from, range[0][w]);
         upto = max(upto, range[1][w]);
     }
-    const int first = from / BLOCK_TOKENS, blocks = max((upto + BLOCK_TOKENS - 1) / BLOCK_TOKENS - first, 0), share = (blocks + a.splits - 1) / a.splits;
-    const int b0 = __builtin_amdgcn_readfirstlane(first + split * share), mine = __builtin_amdgcn_readfirstlane(min(share, blocks - split * share));
+    const int first = from / BLOCK_TOKENS, blocks = max((upto + BLOCK_TOKENS - 1) / BLOCK_TOKENS - first, 0);
+    const int share = a.larger ? (int)(((int64_t)blocks * a.larger + 1023) / 1024) : (blocks + a.splits - 1) / a.splits;
+    const int b0 = __builtin_amdgcn_readfirstlane(first + split * share), mine = __builtin_amdgcn_readfirstlane(min(a.larger && split ? blocks : share, blocks - split * share));
 
     // 16-byte piece p of token t lies at p ^ (t % 16) of the token's place; of values 32-byte pieces at p ^ value_turn(t): what half a wavefront reads at a time, 32 bytes of
     // two pieces of four tokens, falls on distinct banks.
@@ -357,26 +360,40 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     }
     const auto result = [&](int db, int e) { return none ? 0.0f : acc[db][e] * by; };
     const int64_t nth = (a.offsets ? 0 : (int64_t)row * a.L) + tile.q0 + l;                         // of all queries
-    if (a.splits > 1) {
-        if (!valid) return;
-        const int64_t all = a.offsets ? a.L : (int64_t)a.rows * a.L, to = (split * all + nth) * a.Hq + hq;
-        float* dst = a.part_out + to * HD + 4 * half;
-#pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                f32x4 x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = result(db, 4 * g + e);
-                *reinterpret_cast<f32x4*>(dst + 32 * db + 8 * g) = x;
-            }
-        if (half == 0) a.part_lse[to] = lse2;
-        return;
-    }
-    __syncthreads();
     // Through the wavefront's own part of LDS, which nobody reads any more, so that a store writes four whole rows; 8 bytes of a row each, as the lanes hold them, took 4 % longer
     // for packed prompts of up to 2999 tokens (454 us for 436, the queries' way among it), 25 % for queries over 64 keys.
     uint8_t* const rows_at = smem + wave * 32 * HD * 2;
+    const uint32_t to = valid ? (uint32_t)(nth * a.Hq + hq) : 0xffffffffu;
+    const auto rows_of = [&](auto write) {                      // 256 bytes of each row: write(row's place in the outputs, its 16 bytes)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int of = 4 * j + (lane >> 4);
+            const uint4 x = *reinterpret_cast<const uint4*>(rows_at + of * 256 + (((lane ^ of) & 15) << 4));
+            const uint32_t at = (uint32_t)__shfl((int)to, of);
+            if (at != 0xffffffffu) write(at, x);
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+    __syncthreads();
+    if (a.splits > 1) {
+        const int64_t all = a.offsets ? a.L : (int64_t)a.rows * a.L, part = split * all * a.Hq;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+#pragma unroll
+            for (int db = 0; db < 2; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = result(2 * side + db, 4 * g + e);
+                    *reinterpret_cast<f32x4*>(rows_at + col * 256 + (((8 * db + 2 * g + half) ^ (col & 15)) << 4)) = x;
+                }
+            rows_of([&](uint32_t at, const uint4& x) { *reinterpret_cast<uint4*>(a.part_out + (part + at) * HD + 64 * side + 4 * (lane & 15)) = x; });
+        }
+        if (valid && half == 0) a.part_lse[part + to] = lse2;
+        return;
+    }
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -386,36 +403,30 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
             for (int e = 0; e < 2; ++e) x[e] = pair_16<DT>(result(db, 4 * g + 2 * e), result(db, 4 * g + 2 * e + 1));
             *reinterpret_cast<uint2*>(rows_at + col * 256 + (((4 * db + g) ^ (col & 15)) << 4) + 8 * half) = make_uint2(x[0], x[1]);
         }
-    __builtin_amdgcn_wave_barrier();
-    const uint32_t to = valid ? (uint32_t)(nth * a.Hq + hq) : 0xffffffffu;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int of = 4 * j + (lane >> 4);
-        const uint4 x = *reinterpret_cast<const uint4*>(rows_at + of * 256 + (((lane ^ of) & 15) << 4));
-        const uint32_t at = (uint32_t)__shfl((int)to, of);
-        if (at != 0xffffffffu) *reinterpret_cast<uint4*>(a.out + (int64_t)at * HD + 8 * (lane & 15)) = x;
-    }
+    rows_of([&](uint32_t at, const uint4& x) { *reinterpret_cast<uint4*>(a.out + (int64_t)at * HD + 8 * (lane & 15)) = x; });
     if (valid && a.lse && half == 0) a.lse[((a.offsets ? 0 : (int64_t)row * a.Hq) + hq) * a.L + tile.q0 + l] = lse2 * LN2;
 }
 
-// The shares of a query's blocks, put together: a wavefront a query, a lane two dims.
+// The shares of a query's blocks, put together: half a wavefront a query, a lane four dims.
 template <int DT>
 __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t all = a.offsets ? a.L : (int64_t)a.rows * a.L, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 31;
+    const int64_t all = a.offsets ? a.L : (int64_t)a.rows * a.L, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (at >= all * a.Hq) return;
-    float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    float top = -INFINITY, sum = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[s * all * a.Hq + at]);
     const float by = top > -INFINITY ? top : 0.0f;
+#pragma unroll 2
     for (int s = 0; s < a.splits; ++s) {
         const float w = __builtin_amdgcn_exp2f(a.part_lse[s * all * a.Hq + at] - by);
-        const float2 v = *reinterpret_cast<const float2*>(a.part_out + (s * all * a.Hq + at) * HD + 2 * lane);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_out + (s * all * a.Hq + at) * HD + 4 * lane);
         sum += w;
-        o0 = __fmaf_rn(w, v.x, o0);
-        o1 = __fmaf_rn(w, v.y, o1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __fmaf_rn(w, v[e], o[e]);
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<uint32_t*>(a.out + at * HD + 2 * lane) = pair_16<DT>(o0 * inv, o1 * inv);
+    *reinterpret_cast<uint2*>(a.out + at * HD + 4 * lane) = make_uint2(pair_16<DT>(o[0] * inv, o[1] * inv), pair_16<DT>(o[2] * inv, o[3] * inv));
     if (a.lse && lane == 0) {
         const int64_t nth = at / a.Hq, row = a.offsets ? 0 : nth / a.L;
         a.lse[(row * a.Hq + at % a.Hq) * a.L + nth - row * a.L] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
@@ -428,7 +439,7 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
 // that above all: 12001 tokens in a window of 4096 with a cap 480 us for 429, but 16384 without 2063 for 2150 (packed prompts of up to 2999: 460 for 454).
 //
 // Shares: what they are to gain is compute units that would have no tile, or none in the last round; what they cost is their partial results.
-struct PromptCut { int waves; long long tiles; int splits; };
+struct PromptCut { int waves; long long tiles; int splits, larger; };
 static PromptCut cut_of(bool packed, int rows, int G, int Hkv, int L, int T, bool capped) {
     PromptCut c;
     c.waves = capped ? 4 : 8;
@@ -439,11 +450,21 @@ static PromptCut cut_of(bool packed, int rows, int G, int Hkv, int L, int T, boo
     const double partial = (double)(packed ? 1 : rows) * L * G * Hkv * (HD + 1) * 4 * 2 / 5e6;
     double least = 0.0;
     c.splits = 1;
+    c.larger = 0;
     for (int s = 1; s <= 128 && (s == 1 || s * 4LL <= blocks) && (s == 1 || groups * s <= 4 * slots); ++s) {
         const double cost = (double)((groups * s + slots - 1) / slots) * ((double)blocks / s + 4.0) + (s > 1 ? 4.0 + s * partial : 0.0);
         if (s > 1 && cost >= least) continue;
         least = cost;
         c.splits = s;
+    }
+    // Two unequal shares, where tiles leave compute units without one: those take the smaller shares, `turns` one after the other, in the time that a larger one takes.
+    // (2048 queries over 12800 keys, 24 heads over 8, 192 tiles: 386 us with whole tiles, 346 with shares of 76 and 24 %, of which 12 put them together.)
+    if (groups < slots) {
+        const double turns = (double)((groups + slots - groups - 1) / (slots - groups)), smaller = (blocks + 4.0 - 4.0 * turns) / (turns + 1.0), cost = blocks - smaller + 8.0 + 2 * partial;
+        if (smaller >= 4.0 && cost < least) {
+            c.splits = 2;
+            c.larger = 1024 - (int)(1024.0 * smaller / blocks);
+        }
     }
     return c;
 }
@@ -480,7 +501,7 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
     float* const parts = (float*)d->workspace;
     const PromptArgs a = {(const uint16_t*)d->q, (const uint16_t*)d->k, (const uint16_t*)d->v, d->q_stride_b, d->q_stride_h, d->q_stride_t, d->k_stride_b, d->k_stride_h,
                           d->k_stride_t, d->v_stride_b, d->v_stride_h, d->v_stride_t, (uint16_t*)d->out, d->lse, d->offsets, d->key_offsets, d->starts, d->rows, d->L, d->T,
-                          d->Hq, d->Hkv, G, d->causal != 0, d->window, d->scaling, d->cap, cut.splits, parts, parts + (size_t)cut.splits * all * d->Hq * HD};
+                          d->Hq, d->Hkv, G, d->causal != 0, d->window, d->scaling, d->cap, cut.splits, cut.larger, parts, parts + (size_t)cut.splits * all * d->Hq * HD};
     const int mode = d->cap > 0.0f ? (d->cap <= CAP_BY_EXP ? 1 : 2) : d->scaling > 0x1p-100f ? 0 : 2;
     const hipStream_t st = (hipStream_t)stream;
     const auto run = [&](auto dt, auto mode_, auto waves) {
@@ -489,7 +510,7 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
         hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(waves.value * 64), PROMPT_LDS(waves.value), st, a);
         ODMKV_CHECK_LAUNCH("prompt_kernel");
         if (cut.splits > 1) {
-            hipLaunchKernelGGL(prompt_merge_kernel<dt.value>, dim3((unsigned)((all * d->Hq + 3) / 4)), dim3(256), 0, st, a);
+            hipLaunchKernelGGL(prompt_merge_kernel<dt.value>, dim3((unsigned)((all * d->Hq + 7) / 8)), dim3(256), 0, st, a);
             ODMKV_CHECK_LAUNCH("prompt_merge_kernel");
         }
         return 0;

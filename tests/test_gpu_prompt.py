@@ -106,6 +106,13 @@ def test_more_tiles_than_workgroups_take_at_once(dtype, scaling):
         assert torch.equal(out.view(torch.int16), again.view(torch.int16)) and torch.equal(lse.view(torch.int32), lse_again.view(torch.int32))
 
 
+@pytest.mark.parametrize("change", [dict(), dict(starts=[4321]), dict(window=5000), dict(causal=False)], ids=str)
+def test_tiles_that_leave_units_without_one(change):
+    """Long chunks whose keys are shared out, two unequal shares among them."""
+    _check(*_inputs(16, 1, 24, 24, 2000, 9000, torch.float16), **change)
+    _check(*_inputs(17, 1, 32, 8, 1600, 6500, torch.bfloat16), **change)
+
+
 def test_more_tiles_in_rows():
     _check(*_inputs(13, 2, 32, 8, 1500, 1500, torch.bfloat16), starts=[0, 333])
     _check(*_inputs(14, 17, 24, 8, 260, 400, torch.float16), window=90)

@@ -392,7 +392,7 @@ PyObject* native_paged_write_rotated(PyObject*, PyObject* const* a, Py_ssize_t n
         const int64_t Hq = q.size(1);
         if (q.size(0) != B || k.size(0) != B || v.sizes() != k.sizes() || k.size(1) != p->Hkv || q.size(2) != T || Hq < 1 || Hq > 65535 || T < 1 || T < grown) Py_RETURN_NONE;
         for (const at::Tensor* t : {&c, &s})
-            if (t->dim() != 2 || !t->is_cuda() || t->get_device() != device || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->sizes() != c.sizes()) Py_RETURN_NONE;
+            if (t->dim() != 2 || !t->is_cuda() || t->get_device() != device || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->sizes() != c.sizes() || ((uintptr_t)t->data_ptr() & 15)) Py_RETURN_NONE;
         const int64_t half = c.size(1);
         if (half < 8 || half > ODMKV_HEAD_DIM / 2 || half % 8 || c.size(0) < 1 || c.size(0) > INT32_MAX) Py_RETURN_NONE;
         odmkv_rotate_t d;

@@ -346,7 +346,7 @@ class PagedKVCache:
         positions = self._small(positions, "positions", torch.int32, ((B, T),))
         starts = self._small(starts, "starts", torch.int32, ((self.batch,),))
         keys, values, query = (None if t is None else self._rows_ok(t) for t in (keys, values, query))
-        cosine, sine = cosine.contiguous(), sine.contiguous()
+        cosine, sine = (t.clone(memory_format=torch.contiguous_format) if not t.is_contiguous() or t.data_ptr() % 16 else t for t in (cosine, sine))
         turned, turned_keys = (torch.empty(B, T, heads, HEAD_DIM, dtype=self.dtype, device=self.device) if wanted else None
                                for heads, wanted in ((Hq, query is not None), (self.kv_heads, return_keys)))
         if T:

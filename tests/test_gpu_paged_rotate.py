@@ -291,3 +291,16 @@ def test_refusals():
         c.attend(1, q)
     c.write(1, k, v)                                                        # a layer without positions beside one with them
     assert c.refresh() == [T, T]
+
+
+def test_tables_that_lie_anywhere():
+    """Tables off 16 bytes, transposed, and as every other row of a larger one: the same bits."""
+    q, k, v = (_random(s, 2, h, 70, dtype=torch.float16).to(DEV) for s, h in ((31, 4), (32, 2), (33, 2)))
+    cos, sin = (t.to(DEV) for t in _tables(80, 64))
+    want = None
+    for lay in (lambda t: t, lambda t: torch.cat((t.new_zeros(1), t.flatten()))[1:].view(80, 32), lambda t: t.t().contiguous().t(), lambda t: t.repeat_interleave(2, dim=0)[::2]):
+        c = _cache(2, 2, 80)
+        c.extend(70)
+        got = (*c.write_rotated(0, q, k, v, lay(cos), lay(sin), return_keys=True), *c.read(0, 70))
+        want = got if want is None else want
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -756,7 +756,7 @@ typedef struct odmkv_prompt_attend {
     int32_t dtype, rows, L, T, Hq, Hkv, causal, window;
     float scaling, cap;                          /* cap 0: none; 2^-100 at least otherwise */
 } odmkv_prompt_attend_t;
-size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T, float cap);
+size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T, int causal, int window, float cap);
 int odmkv_prompt_attend(const odmkv_prompt_attend_t* a, void* stream);
 
 #ifdef __cplusplus

@@ -7,6 +7,7 @@
 // a workgroup's tokens lie together: a block of 64 keys and values serves all heads of the group, and few blocks lie across a query's end.  The rows of the first product are
 // tokens; what a lane holds of the weights is its operand of the second product as it is, whose other operand, values dim by dim, comes out of LDS by transposing reads.
 // Blocks go from memory into LDS without passing through registers, the next one on its way while this one is used: one barrier a block.
+#include <algorithm>
 #include "attend.h"
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -435,17 +436,20 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
 
 // How a call is cut: wavefronts of a workgroup, tiles of queries at the most, and workgroups that share a tile's blocks.
 //
-// Eight wavefronts share a block among twice as many queries; two workgroups of four, which do not wait for one another, leave more of the vector work beside the products, and a cap is
-// that above all: 12001 tokens in a window of 4096 with a cap 480 us for 429, but 16384 without 2063 for 2150 (packed prompts of up to 2999: 460 for 454).
+// Eight wavefronts share a block among twice as many queries; two workgroups of four, which do not wait for one another, leave more of the vector work beside the products, and what a
+// workgroup does before its first block and behind its last one beside the other's.  A cap is vector work above all: 12001 tokens in a window of 4096 with a cap 480 us for 429, but 16384
+// without 2049 for 2141.  Few keys: 300 packed prompts of 64 tokens 169 us for 129, 40 of 500 202 for 190, 16384 tokens in a window of 700 287 for 275; a prompt of 60 tokens 10.1 for 8.8;
+// the same at 16 prompts of 1500 on average (484), and at 512 keys for every query.
 //
 // Shares: what they are to gain is compute units that would have no tile, or none in the last round; what they cost is their partial results.
 struct PromptCut { int waves; long long tiles; int splits, larger; };
-static PromptCut cut_of(bool packed, int rows, int G, int Hkv, int L, int T, bool capped) {
+static PromptCut cut_of(bool packed, int rows, int G, int Hkv, int L, int T, bool causal, int window, bool capped) {
     PromptCut c;
-    c.waves = capped ? 4 : 8;
+    const int keys = packed ? T / rows : T, of_tile = causal && L == T ? keys / 2 : keys;          // what a tile sees, about
+    c.waves = capped || (window > 0 ? std::min(of_tile, window) : of_tile) <= 768 ? 4 : 8;
     const long long cols = PROMPT_COLS(c.waves), slots = compute_units() * (8 / c.waves);
     c.tiles = packed ? ((long long)G * L + cols - 1) / cols + rows + 2 : (long long)rows * (((long long)G * L + cols - 1) / cols);
-    const long long blocks = (packed ? T / rows : T) / BLOCK_TOKENS + 1, groups = c.tiles * Hkv;
+    const long long blocks = (window > 0 ? std::min((long long)keys, window + cols / G) : keys) / BLOCK_TOKENS + 1, groups = c.tiles * Hkv;
     // in units of a block's time, about a microsecond: a workgroup's fixed part is some four of them, the merge a launch and its reading
     const double partial = (double)(packed ? 1 : rows) * L * G * Hkv * (HD + 1) * 4 * 2 / 5e6;
     double least = 0.0;
@@ -469,9 +473,9 @@ static PromptCut cut_of(bool packed, int rows, int G, int Hkv, int L, int T, boo
     return c;
 }
 
-extern "C" size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T, float cap) {
+extern "C" size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T, int causal, int window, float cap) {
     if (rows <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || L <= 0 || T < 0) return 0;
-    const PromptCut c = cut_of(packed != 0, rows, Hq / Hkv, Hkv, L, T, cap > 0.0f);
+    const PromptCut c = cut_of(packed != 0, rows, Hq / Hkv, Hkv, L, T, causal != 0, window, cap > 0.0f);
     return c.splits > 1 ? align_up((size_t)c.splits * (packed ? 1 : rows) * L * Hq * (HD + 1) * sizeof(float), 256) : 0;
 }
 
@@ -490,10 +494,10 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
                     "prompt_attend: rows must be 16-byte aligned");
     ODMKV_CHECK_ARG(d->k_stride_t >= 0 && d->k_stride_t < (1 << 24) && d->v_stride_t >= 0 && d->v_stride_t < (1 << 24), "prompt_attend: a token's stride must be below 2^24");
     const int G = d->Hq / d->Hkv;
-    const PromptCut cut = cut_of(d->offsets != nullptr, d->rows, G, d->Hkv, d->L, d->T, d->cap > 0.0f);
+    const PromptCut cut = cut_of(d->offsets != nullptr, d->rows, G, d->Hkv, d->L, d->T, d->causal != 0, d->window, d->cap > 0.0f);
     const long long all = d->offsets ? d->L : (long long)d->rows * d->L, groups = cut.tiles * d->Hkv * cut.splits;
     ODMKV_CHECK_ARG((long long)G * d->L < 0x7fff0000LL && groups * cut.waves * 64 < 0x100000000LL && all * d->Hq < 0x100000000LL, "prompt_attend: too many queries");
-    const size_t need = odmkv_prompt_attend_workspace_bytes(d->offsets != nullptr, d->rows, d->Hq, d->Hkv, d->L, d->T, d->cap);
+    const size_t need = odmkv_prompt_attend_workspace_bytes(d->offsets != nullptr, d->rows, d->Hq, d->Hkv, d->L, d->T, d->causal, d->window, d->cap);
     if (need > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)) {
         odmkv_set_error("prompt_attend: workspace too small");
         return ODMKV_ENOSPACE;
@@ -516,6 +520,6 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
         return 0;
     };
     const auto of_waves = [&](auto dt, auto mode_) { return cut.waves == 8 ? run(dt, mode_, Int<8>()) : run(dt, mode_, Int<4>()); };
-    const auto of_mode = [&](auto dt) { return mode == 0 ? run(dt, Int<0>(), Int<8>()) : mode == 1 ? run(dt, Int<1>(), Int<4>()) : of_waves(dt, Int<2>()); };
+    const auto of_mode = [&](auto dt) { return mode == 0 ? of_waves(dt, Int<0>()) : mode == 1 ? run(dt, Int<1>(), Int<4>()) : of_waves(dt, Int<2>()); };
     return d->dtype == ODMKV_F16 ? of_mode(Int<ODMKV_F16>()) : of_mode(Int<ODMKV_BF16>());
 }

@@ -333,7 +333,7 @@ PyObject* native_paged_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 typedef int (*rotate_fn)(const odmkv_rotate_t*, void*);
 typedef int (*prompt_fn)(const odmkv_prompt_attend_t*, void*);
-typedef size_t (*prompt_bytes_fn)(int, int, int, int, int, int, float);
+typedef size_t (*prompt_bytes_fn)(int, int, int, int, int, int, int, int, float);
 
 // [B, heads, T, 128] in 16 bits with rows that start on 16 bytes, and nothing to record
 bool heads_fit(const at::Tensor& t, at::ScalarType type, int device) {
@@ -462,7 +462,7 @@ PyObject* native_prompt_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor out = at::empty({B, L, Hq, ODMKV_HEAD_DIM}, q.options());
         at::Tensor lse;
         if (want_lse) lse = at::empty({B, Hq, L}, q.options().dtype(at::kFloat));
-        const size_t bytes = bytes_of(packed, (int)rows, (int)Hq, (int)Hkv, (int)L, (int)T, (float)cap);
+        const size_t bytes = bytes_of(packed, (int)rows, (int)Hq, (int)Hkv, (int)L, (int)T, causal, (int)window, (float)cap);
         at::Tensor ws;
         if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));      // (of its own for every call: a graph's is the graph's)
         d.q = q.data_ptr(); d.q_stride_b = q.stride(0); d.q_stride_h = q.stride(1); d.q_stride_t = q.stride(2);

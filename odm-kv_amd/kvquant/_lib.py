@@ -209,7 +209,7 @@ def _load() -> C.CDLL:
         "odmkv_pages_attend_shared_workspace_bytes": (sz, [C.POINTER(Pages), i32, i32, i32]),
         "odmkv_pages_attend_workspace_bytes": (sz, [C.POINTER(Pages), i32, i32, i32]),
         "odmkv_pages_attend": (C.c_int, [C.POINTER(Attend), vp]),
-        "odmkv_prompt_attend_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, f32]),
+        "odmkv_prompt_attend_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32, i32, f32]),
         "odmkv_prompt_attend": (C.c_int, [C.POINTER(PromptAttend), vp]),
     }
     for name, (res, args) in sig.items():

@@ -88,7 +88,7 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     out = torch.empty(B, L, Hq, HEAD_DIM, dtype=query.dtype, device=device)
     lse = torch.empty(B, Hq, L, dtype=torch.float32, device=device) if return_lse else None
     if L:
-        nbytes = lib.odmkv_prompt_attend_workspace_bytes(offsets is not None, rows, Hq, Hkv, L, T, 0.0 if softcap is None else softcap)
+        nbytes = lib.odmkv_prompt_attend_workspace_bytes(offsets is not None, rows, Hq, Hkv, L, T, bool(causal), min(window or 0, _FAR), 0.0 if softcap is None else softcap)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None          # (of its own for every call: a graph's is the graph's)
         a = _lib.PromptAttend(*(x for t in (query, keys, values) for x in (t.data_ptr(), *t.stride()[:3])), out.data_ptr(), _lib.ptr(lse), _lib.ptr(offsets),
                               _lib.ptr(key_offsets), _lib.ptr(starts), _lib.ptr(ws), nbytes, _lib._DT[query.dtype], rows, L, T, Hq, Hkv, causal, min(window or 0, _FAR),

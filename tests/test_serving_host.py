@@ -53,9 +53,9 @@ def test_bad_prompts_are_refused():
     assert lib.odmkv_prompt_attend(None, None) == -1 and "null" in _error()
     # few queries over many keys: their blocks are shared out, and the shares need room
     few = dict(rows=1, L=2, T=50000)
-    need = lib.odmkv_prompt_attend_workspace_bytes(0, 1, 8, 4, 2, 50000, 0.0)
+    need = lib.odmkv_prompt_attend_workspace_bytes(0, 1, 8, 4, 2, 50000, 1, 0, 0.0)
     assert need > 0 and _prompt(**few) == -2 and _prompt(**few, workspace=4096, workspace_bytes=need - 1) == -2 and _prompt(**few, workspace=4100, workspace_bytes=need) == -2
-    assert lib.odmkv_prompt_attend_workspace_bytes(0, 0, 8, 4, 2, 50000, 0.0) == 0 and lib.odmkv_prompt_attend_workspace_bytes(0, 1, 7, 4, 2, 50000, 0.0) == 0
+    assert lib.odmkv_prompt_attend_workspace_bytes(0, 0, 8, 4, 2, 50000, 1, 0, 0.0) == 0 and lib.odmkv_prompt_attend_workspace_bytes(0, 1, 7, 4, 2, 50000, 1, 0, 0.0) == 0
 
 
 def test_python_refuses_prompts_without_a_gpu():

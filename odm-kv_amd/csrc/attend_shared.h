@@ -4,6 +4,11 @@
 // side), over a share of the group's blocks.  A wavefront holds 32 queries, the columns of v_mfma_f32_32x32x16_f16, as in the kernel for many queries (attend_wide.h): a block is turned into
 // fp16 once a workgroup; where a tile has 64 queries or fewer, two wavefronts share 32 of them and take a half of every block each.  The workgroups behind them take the rows' own
 // blocks (attend_narrow.h).  Both leave partial results, which a second launch puts together.  Codes, weights and sums are treated as in the other two kernels.
+//
+// What is left is fixed cost: 64 samples of 8192 tokens (8 heads, e4m3, 52 MB that have to be read) take 34.2 us here and 9.0 in the merge, where the ordinary way reads 1.1 GB.  Of it a
+// share of what is in common takes 1.25 us a block and 19 besides (launch, plan, first block and queries, 5.5 for its partial results), the rows' own blocks alone 18.5; the two
+// share the chip: half a block behind one another, so that one's loads stand beside the other's products.  Shares of 8 blocks (29.5 us) beat 16 (39) and 32 (62); finer ones
+// lose by their partial results (42 us in all for 40), which take no less when a store writes whole rows of them by way of LDS (8 samples 17.8 -> 19).
 #pragma once
 
 #include "attend_narrow.h"

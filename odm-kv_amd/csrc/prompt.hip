@@ -7,6 +7,12 @@
 // a workgroup's tokens lie together: a block of 64 keys and values serves all heads of the group, and few blocks lie across a query's end.  The rows of the first product are
 // tokens; what a lane holds of the weights is its operand of the second product as it is, whose other operand, values dim by dim, comes out of LDS by transposing reads.
 // Blocks go from memory into LDS without passing through registers, the next one on its way while this one is used: one barrier a block.
+//
+// Bound by the products and by the vector work that finds no place beside them: 16384 tokens, 32 heads over 8, in 2.02 ms, 1085 TFLOP/s (a library's product of 8192^3: 1219 to 1429;
+// this kernel without any vector work: 1245), matrix cores busy 52 % of the cycles, vector instructions 43 %.  A product of 32 cycles takes 18 ns, a 16-byte read of LDS beside it 6
+// more, its share of the vector work 5: so operands are read as rarely as 32 queries a wavefront allow (64 would not leave room for two wavefronts a SIMD), without bank conflicts,
+// and the largest score of a block is not looked for.  With a cap 34 % and 57 %: 12001 tokens in a window of 4096 in 419 us.  Prompts of 1500 tokens on average, 28 heads over 4, 455 us
+// (800 TFLOP/s): ten tiles a compute unit, each with a first block to wait for and a last one that few queries see whole.
 #include <algorithm>
 #include "attend.h"
 
@@ -88,6 +94,7 @@ template <int DT> struct Weights {
     static constexpr float LIFT = DT == ODMKV_F16 ? 8.0f : 0.0f, LIMIT = 32768.0f;
 };
 
+// (without conflicts: 1 % of the time of 16384 tokens)
 __device__ static inline int value_turn(int t) { return (t & 3) << 1 | (t >> 2 & 1); }
 
 template <int DT, int MODE, int WAVES>
@@ -408,7 +415,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     if (valid && a.lse && half == 0) a.lse[((a.offsets ? 0 : (int64_t)row * a.Hq) + hq) * a.L + tile.q0 + l] = lse2 * LN2;
 }
 
-// The shares of a query's blocks, put together: half a wavefront a query, a lane four dims.
+// The shares of a query's blocks, put together by their log-sum-exps: half a wavefront a query, a lane four dims.  Bound by memory: two shares of 2048 queries of 24 heads, 63 MB, in 13 us
+// (4.8 TB/s).
 template <int DT>
 __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
     const int lane = threadIdx.x & 31;

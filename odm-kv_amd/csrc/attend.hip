@@ -5,12 +5,17 @@
 // fourth share, eight shares of a wavefront on their way at a time, a lane two dims.  Bound by the latency of two dependent reads: 4.0 us behind a step over 32768 tokens
 // (32 queries, 64 shares each), 7.2 for 928 queries of 64 shares (31 MB).
 #define MERGE_AHEAD 8
+#define MERGE_MANY 1024
 
 // SHARED: those of what the row has in common with others come first, its own behind them.
-template <int DT, bool NARROW_PARTS, bool SHARED>
+// APART: a query's wavefronts, four of them, or one where there are many queries: finding out where a query's partial results lie is what takes the time then.
+template <int DT, bool NARROW_PARTS, bool SHARED, int APART>
 __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
     const odmkv_pages_t& p = a.p;
-    const int R = a.G * a.L, r = blockIdx.x, h = blockIdx.y, row = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int R = a.G * a.L, h = blockIdx.y, row = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
+    const int of_workgroup = APART == 4 ? tid >> 6 : __builtin_amdgcn_readfirstlane(tid >> 6), wave = APART == 4 ? of_workgroup : 0;
+    const int r = APART == 4 ? blockIdx.x : 4 * blockIdx.x + of_workgroup;
+    if (APART == 1 && r >= R) return;
     const int l = r / a.G, hq = h * a.G + r - l * a.G;
     if (l >= (a.counts ? min(max(a.counts[row], 0), a.L) : a.L)) return;
     __shared__ float part[4][HD], top_of[4], sum_of[4];
@@ -34,12 +39,12 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
     }
     // (each wavefront by its own largest: the partial results need not wait for the largest of all)
     float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int i0 = wave; i0 < splits; i0 += 4 * MERGE_AHEAD) {
+    for (int i0 = wave; i0 < splits; i0 += APART * MERGE_AHEAD) {
         float lse[MERGE_AHEAD];
         float2 v[MERGE_AHEAD];
 #pragma unroll
         for (int k = 0; k < MERGE_AHEAD; ++k) {
-            const int i = min(i0 + 4 * k, splits - 1);
+            const int i = min(i0 + APART * k, splits - 1);
             const bool common = SHARED && i < in_common;
             const size_t from = common ? common_at + (size_t)i * cols : at + (size_t)(i - in_common) * R;
             lse[k] = (common ? a.common_lse : a.part_lse)[from];
@@ -48,7 +53,7 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
         float to = top;
 #pragma unroll
         for (int k = 0; k < MERGE_AHEAD; ++k) {
-            if (i0 + 4 * k >= splits) lse[k] = -INFINITY;
+            if (i0 + APART * k >= splits) lse[k] = -INFINITY;
             to = fmaxf(to, lse[k]);
         }
         const float by = to > -INFINITY ? to : 0.0f, old = __builtin_amdgcn_exp2f(top - by);
@@ -64,23 +69,25 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
             o1 = __fmaf_rn(w, v[k].y, o1);
         }
     }
-    part[wave][2 * lane] = o0;
-    part[wave][2 * lane + 1] = o1;
-    if (lane == 0) {
-        sum_of[wave] = sum;
-        top_of[wave] = top;
-    }
-    __syncthreads();
-    if (tid >= 64) return;
-    top = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
-    const float by = top > -INFINITY ? top : 0.0f;
-    sum = o0 = o1 = 0.0f;
+    if constexpr (APART == 4) {
+        part[wave][2 * lane] = o0;
+        part[wave][2 * lane + 1] = o1;
+        if (lane == 0) {
+            sum_of[wave] = sum;
+            top_of[wave] = top;
+        }
+        __syncthreads();
+        if (tid >= 64) return;
+        top = fmaxf(fmaxf(top_of[0], top_of[1]), fmaxf(top_of[2], top_of[3]));
+        const float by = top > -INFINITY ? top : 0.0f;
+        sum = o0 = o1 = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float f = __builtin_amdgcn_exp2f(top_of[w] - by);
-        sum = __fmaf_rn(f, sum_of[w], sum);
-        o0 = __fmaf_rn(f, part[w][2 * lane], o0);
-        o1 = __fmaf_rn(f, part[w][2 * lane + 1], o1);
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(top_of[w] - by);
+            sum = __fmaf_rn(f, sum_of[w], sum);
+            o0 = __fmaf_rn(f, part[w][2 * lane], o0);
+            o1 = __fmaf_rn(f, part[w][2 * lane + 1], o1);
+        }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     o0 *= inv;
@@ -90,16 +97,18 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
 }
 
 static int launch_attend_merge(const AttendArgs& a, const Cut& cut, hipStream_t st) {
-    const dim3 grid(a.G * a.L, a.p.Hkv, a.p.rows);
-    if (a.p.dtype == ODMKV_F16) {
-        if (cut.shared) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_F16, true, true>), grid, dim3(256), 0, st, a);
-        else if (cut.wide) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_F16, false, false>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((attend_merge_kernel<ODMKV_F16, true, false>), grid, dim3(256), 0, st, a);
-    } else {
-        if (cut.shared) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_BF16, true, true>), grid, dim3(256), 0, st, a);
-        else if (cut.wide) hipLaunchKernelGGL((attend_merge_kernel<ODMKV_BF16, false, false>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((attend_merge_kernel<ODMKV_BF16, true, false>), grid, dim3(256), 0, st, a);
-    }
+    const int R = a.G * a.L;
+    const dim3 grid(R, a.p.Hkv, a.p.rows);
+    // (64 samples, 2048 queries: NN us for NN)
+    const bool many = (long long)R * a.p.Hkv * a.p.rows > MERGE_MANY;
+    const auto of_type = [&](auto dt) {
+        if (cut.shared && many) hipLaunchKernelGGL((attend_merge_kernel<dt.value, true, true, 1>), dim3((R + 3) / 4, a.p.Hkv, a.p.rows), dim3(256), 0, st, a);
+        else if (cut.shared) hipLaunchKernelGGL((attend_merge_kernel<dt.value, true, true, 4>), grid, dim3(256), 0, st, a);
+        else if (cut.wide) hipLaunchKernelGGL((attend_merge_kernel<dt.value, false, false, 4>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((attend_merge_kernel<dt.value, true, false, 4>), grid, dim3(256), 0, st, a);
+    };
+    if (a.p.dtype == ODMKV_F16) of_type(Int<ODMKV_F16>());
+    else of_type(Int<ODMKV_BF16>());
     ODMKV_CHECK_LAUNCH("attend_merge_kernel");
     return 0;
 }
@@ -141,7 +150,7 @@ static Cut cut_shared(const odmkv_pages_t& p, int R, int max_length) {
     c.stream = false;
     c.splits = (int)std::max((long long)p.rows, std::min(2LL * units / p.Hkv, (long long)p.rows * std::max(1, blocks / 4)));
     c.parts = (size_t)p.Hkv * c.splits * R;
-    c.spare = std::max(1, 2 * units / p.Hkv);
+    c.spare = std::max(1, units / p.Hkv);
     c.workgroups = (int)(((long long)p.rows * R + SHARED_COLS - 1) / SHARED_COLS) + p.rows / 2 + c.spare;
     c.common_parts = (long long)p.rows * R + (long long)SHARED_COLS * c.spare;
     return c;

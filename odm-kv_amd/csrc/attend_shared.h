@@ -5,10 +5,10 @@
 // fp16 once a workgroup; where a tile has 64 queries or fewer, two wavefronts share 32 of them and take a half of every block each.  The workgroups behind them take the rows' own
 // blocks (attend_narrow.h).  Both leave partial results, which a second launch puts together.  Codes, weights and sums are treated as in the other two kernels.
 //
-// What is left is fixed cost: 64 samples of 8192 tokens (8 heads, e4m3, 52 MB that have to be read) take 34.2 us here and 9.0 in the merge, where the ordinary way reads 1.1 GB.  Of it a
-// share of what is in common takes 1.25 us a block and 19 besides (launch, plan, first block and queries, 5.5 for its partial results), the rows' own blocks alone 18.5; the two
-// share the chip: half a block behind one another, so that one's loads stand beside the other's products.  Shares of 8 blocks (29.5 us) beat 16 (39) and 32 (62); finer ones
-// lose by their partial results (42 us in all for 40), which take no less when a store writes whole rows of them by way of LDS (8 samples 17.8 -> 19).
+// What is left is mostly fixed cost: 64 samples of 8192 tokens (8 heads, e4m3, 52 MB that have to be read) take 33.1 us here and 7.7 in the merge, where the ordinary way reads 1.1 GB.
+// 16 beams of 32768 tokens, 28 heads over 4, 31.7 and 8.4: 3 for the launch, 3 for the plan and what it leads to, 3.5 for the first of a share's 8 blocks, 15 for the others (2.1 each: one wavefront a SIMD, whose
+// reads, products and weights wait for one another), 7 for the partial results.  The rows' own blocks alone take 12 to 18 and stand beside that.  Shares of 16 blocks take 47, of 4 blocks the same 31.9; partial
+// results in whole rows by way of LDS no less (8 samples 17.8 -> 19); eight wavefronts, a half of a block each, leave no place for the rows' own workgroups beside them (31.7 -> 39.9).
 #pragma once
 
 #include "attend_narrow.h"

@@ -398,9 +398,13 @@ PyObject* native_paged_write_rotated(PyObject*, PyObject* const* a, Py_ssize_t n
         odmkv_rotate_t d;
         memset(&d, 0, sizeof d);
         if (!ints_fit(a[9], (int64_t)p->rows + 1, device, d.offsets) || !ints_fit(a[10], p->rows, device, d.starts)) Py_RETURN_NONE;
-        at::Tensor turned = at::empty({B, T, Hq, ODMKV_HEAD_DIM}, q.options());
+        // (token by token, looked at head by head)
+        const auto by_token = [&](int64_t heads) {
+            return at::empty_strided({B, heads, T, ODMKV_HEAD_DIM}, {T * heads * ODMKV_HEAD_DIM, ODMKV_HEAD_DIM, heads * ODMKV_HEAD_DIM, 1}, q.options());
+        };
+        at::Tensor turned = by_token(Hq);
         at::Tensor keys;
-        if (want_keys) keys = at::empty({B, T, (int64_t)p->Hkv, ODMKV_HEAD_DIM}, q.options());
+        if (want_keys) keys = by_token(p->Hkv);
         d.pages = p;
         d.q = q.data_ptr(); d.q_stride_b = q.stride(0); d.q_stride_h = q.stride(1); d.q_stride_t = q.stride(2);
         d.k = k.data_ptr(); d.k_stride_b = k.stride(0); d.k_stride_h = k.stride(1); d.k_stride_t = k.stride(2);
@@ -411,9 +415,8 @@ PyObject* native_paged_write_rotated(PyObject*, PyObject* const* a, Py_ssize_t n
         d.turned = (int)(2 * half); d.interleaved = interleaved; d.table = (int)c.size(0);
         const int rc = fn(&d, (void*)(uintptr_t)stream);
         if (rc) return raise_odmkv(rc, "storing turned tokens");
-        turned = turned.transpose(1, 2);
         if (!want_keys) return THPVariable_Wrap(std::move(turned));
-        return pair_of(std::move(turned), keys.transpose(1, 2));
+        return pair_of(std::move(turned), std::move(keys));
     )
 }
 

@@ -303,7 +303,7 @@ class PagedKVCache:
         if not self._replayed and _capturing():
             self._replayed = True
         if (positions is None and isinstance(cosine, torch.Tensor) and cosine.dim() == 2 and _device() == self.device.index
-                and (self.max_tokens if _capturing() else max(self._bounds)) <= cosine.shape[0]):
+                and (self.max_tokens <= cosine.shape[0] or (max(self._bounds) <= cosine.shape[0] and not _capturing()))):
             # (everything as the kernel takes it: one native call)
             done = _native.paged_write_rotated(_WRITE_ROTATED, self._at, self.device.index, layer, query, keys, values, cosine, sine, offsets, starts, interleaved, return_keys,
                                                self._grown, _lib.stream_ptr(self.device))

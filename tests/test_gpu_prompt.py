@@ -113,6 +113,13 @@ def test_tiles_that_leave_units_without_one(change):
     _check(*_inputs(17, 1, 32, 8, 1600, 6500, torch.bfloat16), **change)
 
 
+@pytest.mark.parametrize("change", [dict(window=1000), dict(window=130, cap=20.0), dict(window=3000, starts=[7500])], ids=str)
+def test_few_queries_over_a_window(change):
+    """A window's blocks shared out, fewer of them than the keys have."""
+    _check(*_inputs(18, 1, 32, 8, 100, 8000, torch.float16), **change)
+    _check(*_inputs(19, 1, 14, 2, 1, 8000, torch.bfloat16), **change)
+
+
 def test_more_tiles_in_rows():
     _check(*_inputs(13, 2, 32, 8, 1500, 1500, torch.bfloat16), starts=[0, 333])
     _check(*_inputs(14, 17, 24, 8, 260, 400, torch.float16), window=90)

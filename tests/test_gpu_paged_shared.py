@@ -229,3 +229,23 @@ def test_two_calls_give_the_same_bits():
     side.synchronize()
     for x, y in zip(first, second):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("n", [1, 64, 3000])
+def test_a_row_by_itself(n):
+    """A batch of one row, and rows of which only one holds anything: there is nothing in common, whatever is asked for."""
+    k, v = (x.to(DEV) for x in _rows(40, 1, 2, n, torch.bfloat16))
+    one = _cache(1, 2, n + 4, dtype=torch.bfloat16)
+    one.append(k, v)
+    q = _queries(41, 1, 8, 1, torch.bfloat16)
+    for a, b in zip(one.attend(0, q.to(DEV), return_lse=True), one.attend(0, q.to(DEV), shared=True, return_lse=True)):
+        assert torch.equal(a, b)
+    one.truncate(n)
+    one.reorder([0])
+    _check_attend(one, [(k[0].cpu(), v[0].cpu())], "int8", q)
+    three = one.select([0, 0, 0])
+    three.free([0, 2])
+    q = _queries(42, 3, 8, 1, torch.bfloat16).to(DEV)
+    want, got = (three.attend(0, q, **how) for how in (dict(), dict(shared=True)))
+    # (each is rounded to bf16 once, by 2^-8 of itself at most; what else differs is the order of sums in 32 bits and weights in fp16, less than a step of either)
+    assert not got[0].any() and not got[2].any() and (want[1].float() - got[1].float()).abs().max() <= 2 * 2.0 ** -8 * want[1].float().abs().max()

@@ -168,3 +168,40 @@ def test_capped_windowed_and_padded_prompts_of_a_model():
             attention(module, q.to(DEV), keys, values, None, dropout=0.1)
         with pytest.raises(RuntimeError, match="newest tokens alone"):
             keys + 1
+
+
+@torch.no_grad()
+def test_offsets_that_pass_32_bits():
+    """Tensors of more than 2^32 bytes and 2^31 elements: their last tokens, a prompt's and a step's."""
+    from kvquant import PagedKVCache, prompt_attention
+    N, Hq, dtype = 540001, 32, torch.bfloat16
+    q = torch.zeros(1, N, Hq, 128, dtype=dtype, device=DEV).transpose(1, 2)
+    k, v = (torch.zeros(1, N, 1, 128, dtype=dtype, device=DEV).transpose(1, 2) for _ in range(2))
+    g = torch.Generator().manual_seed(9)
+    ends = [torch.randn(1, h, 300, 128, generator=g).to(dtype) for h in (Hq, 1, 1)]
+    for t, x in zip((q, k, v), ends):
+        t[:, :, -300:] = x.to(DEV)
+    cos, sin = torch.zeros(N, 64), torch.zeros(N, 64)
+    angles = torch.arange(N - 300, N, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(64, dtype=torch.float64) / 64)
+    cos[-300:], sin[-300:] = angles.cos().float(), angles.sin().float()
+    cache = PagedKVCache(1, 1, N + 1, dtype=dtype)
+    cache.extend(N)
+    turned, keys = cache.write_rotated(0, q, k, v, cos.to(DEV), sin.to(DEV), offsets=torch.tensor([0, N], dtype=torch.int32, device=DEV), return_keys=True)
+    want_q, want_k = _turned(ends[0][0], cos[-300:], sin[-300:], False), _turned(ends[1][0], cos[-300:], sin[-300:], False, key=True)
+    assert torch.equal(turned[0, :, -300:].cpu(), want_q) and torch.equal(keys[0, :, -300:].cpu(), want_k)
+    out, lse = prompt_attention(turned, keys, v, window=64, return_lse=True)
+    prompt_rows.check(out[0, -200:].cpu(), lse[0, :, -200:].cpu(), *prompt_rows.attend(want_q[:, -200:], want_k, ends[2][0], window=64))
+    del q, k, v, turned, keys, out, lse, cache
+    # pages of the last of many layers
+    cache = PagedKVCache(1, 8, 700, layers=10, pages=9000, kind="int8", dtype=dtype)
+    assert cache.k_codes.numel() > 2 ** 32
+    k, v = (torch.randn(1, 8, 600, 128, generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(4, 16, 1, 128, generator=g).to(dtype)
+    cache.extend(600)
+    cache.write(9, k.to(DEV), v.to(DEV))
+    samples = cache.select([0, 0, 0, 0])
+    out = samples.attend(9, q.to(DEV), shared=True).cpu().double()
+    held = [plain.held(x[0], "int8") for x in (k, v)]
+    for b in range(4):
+        want, _, tol, _ = plain.attend(q[b], *held)
+        assert bool(((out[b] - want).abs() <= tol + torch.finfo(dtype).eps / 2 * (want.abs() + tol)).all())

@@ -15,6 +15,7 @@
 // (800 TFLOP/s): ten tiles a compute unit, each with a first block to wait for and a last one that few queries see whole.
 #include <algorithm>
 #include "attend.h"
+#include "spans.h"
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -56,20 +57,16 @@ __device__ static inline Tile tile_of(const PromptArgs& a, int at) {
     int before = 0;
     for (int s0 = -1; s0 <= a.rows; s0 += 64) {
         const int s = s0 + lane;
-        int begin = 0, end = 0;
-        if (s <= a.rows) {
-            begin = s < 0 ? 0 : min(max(a.offsets[s], 0), a.L);
-            end = s == a.rows ? a.L : max(min(a.offsets[s + 1], a.L), begin);
-        }
-        const int count = (int)(((int64_t)a.G * (end - begin) + COLS - 1) / COLS), upto = before + wave_scan(count);
+        const Span here = s <= a.rows ? span_of(s < 0 ? 0 : a.offsets[s], s == a.rows ? a.L : a.offsets[s + 1], a.L) : Span{0, 0};
+        const int count = (int)(((int64_t)a.G * here.n + COLS - 1) / COLS), upto = before + wave_scan(count);
         const unsigned long long behind = __ballot(upto > at);
         if (behind) {
             const int l = __builtin_ctzll(behind), row = s0 + l, nth = __builtin_amdgcn_readlane(upto, l) - 1 - at;
-            const int q0 = __builtin_amdgcn_readlane(begin, l), n = __builtin_amdgcn_readlane(end, l) - q0;
+            const int q0 = __builtin_amdgcn_readlane(here.begin, l), n = __builtin_amdgcn_readlane(here.n, l);
             if (row < 0 || row >= a.rows) return {-1, nth, q0, n, 0, 0};
             const int32_t* const of = a.key_offsets ? a.key_offsets : a.offsets;
-            const int k0 = min(max(of[row], 0), a.T), m = max(min(of[row + 1], a.T) - k0, 0);
-            return {row, nth, q0, n, k0, m};
+            const Span keys = span_of(of[row], of[row + 1], a.T);
+            return {row, nth, q0, n, keys.begin, keys.n};
         }
         before = __builtin_amdgcn_readlane(upto, 63);
     }

@@ -139,6 +139,30 @@ def test_offsets_that_do_not_ascend_stay_within_the_tensors(bad):
     assert bool((guard[0] == 7).all()) and bool((guard[2] == 7).all()) and bool(torch.isfinite(guard).all())
 
 
+SOUND = [0, 30, 70, 100]
+
+
+@pytest.mark.parametrize("bad", [[0, 100, -2 ** 31, 120], [0, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1], [150, -2 ** 31, 5, 60], [-2 ** 31, -2 ** 31, 200, 2 ** 31 - 1], [200, 0, 300, -1],
+                                 [2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1], [0, 50, 40, 150]], ids=str)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_key_offsets_that_do_not_ascend_beside_sound_ones(bad, dtype):
+    """Sound queries: each sequence sees what its two offsets say of the keys there are, and nothing of what lies in front of and behind them."""
+    q, inner_k, inner_v = _inputs(31, 1, 6, 2, 100, 150, dtype)
+    room = 70000                                                        # NaN on both sides: whoever reads them shows it
+    k, v = (torch.full((1, 2, room + 150 + room, 128), float("nan"), dtype=dtype, device=DEV) for _ in range(2))
+    for to, x in ((k, inner_k), (v, inner_v)):
+        to[:, :, room:room + 150] = x
+    k, v = k[:, :, room:room + 150], v[:, :, room:room + 150]
+    offsets, key_offsets = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (SOUND, bad))
+    for how in (dict(), dict(causal=False), dict(window=20, cap=30.0)):
+        out, lse = _call(q, k, v, offsets=offsets, key_offsets=key_offsets, causal=how.get("causal", True), window=how.get("window"), softcap=how.get("cap"))
+        for s in range(3):
+            a, e = SOUND[s:s + 2]
+            x = min(max(bad[s], 0), 150)
+            y = max(min(max(bad[s + 1], 0), 150), x)
+            plain.check(out[0, a:e], lse[0, :, a:e], *plain.attend(q[0, :, a:e], k[0, :, x:y], v[0, :, x:y], **how))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_infinities_and_nan_where_nobody_looks(dtype):
     """In padding, in other sequences, behind a query's end and in front of its window: a query's result is what it is without them; whoever sees them gets them."""

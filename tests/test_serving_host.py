@@ -91,3 +91,34 @@ def test_bad_plans_are_refused():
     assert lib.odmkv_pages_attend_shared_workspace_bytes(None, 8, 1, 100) == 0
     # what takes the ordinary way takes its workspace
     assert lib.odmkv_pages_attend_shared_workspace_bytes(p, 8, 40, 9000) == lib.odmkv_pages_attend_workspace_bytes(p, 8, 40, 9000)
+
+
+# ---- what offsets say, where nobody on the host has seen them (csrc/spans.h, as the kernel compiles it)
+@pytest.fixture(scope="module")
+def span_of(tmp_path_factory):
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    at = tmp_path_factory.mktemp("spans")
+    (at / "spans.cpp").write_text('#include "spans.h"\nextern "C" void span(int first, int last, int all, int* to) { const Span s = span_of(first, last, all); to[0] = s.begin; to[1] = s.n; }\n')
+    subprocess.run(["g++", "-O2", "-fwrapv", "-shared", "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(root, "odm-kv_amd", "csrc"),
+                    str(at / "spans.cpp"), "-o", str(at / "spans.so")], check=True)
+    f = C.CDLL(str(at / "spans.so")).span
+    f.argtypes, f.restype = [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int)], None
+
+    def call(first, last, all):
+        to = (C.c_int * 2)()
+        f(first, last, all, to)
+        return to[0], to[1]
+    return call
+
+
+def test_spans_of_any_offsets_stay_within_what_there_is(span_of):
+    """Offsets that ascend are taken as they are, within the tensors; what does not ascend is empty; both ends of 32 bits among them."""
+    some = [-2 ** 31, -2 ** 31 + 1, -2 ** 30, -1, 0, 1, 63, 64, 99, 100, 101, 2 ** 26, 2 ** 30, 2 ** 31 - 2, 2 ** 31 - 1]
+    for all in (0, 1, 100, 2 ** 26):
+        for first in some:
+            for last in some:
+                begin = min(max(first, 0), all)
+                want = begin, max(min(max(last, 0), all) - begin, 0)
+                assert span_of(first, last, all) == want, (first, last, all)

@@ -413,7 +413,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
 }
 
 // The shares of a query's blocks, put together by their log-sum-exps: half a wavefront a query, a lane four dims.  Bound by memory: two shares of 2048 queries of 24 heads, 63 MB, in 13 us
-// (4.8 TB/s).
+// (4.8 TB/s).  bf16: the weights, of one at most each, meet the values smaller by a power of two that takes their sum to a half or below: values at the type's end are as good as at 32 bits' own.
 template <int DT>
 __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
     const int lane = threadIdx.x & 31;
@@ -423,15 +423,17 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[s * all * a.Hq + at]);
     const float by = top > -INFINITY ? top : 0.0f;
+    const int less = DT == ODMKV_F16 ? 0 : 33 - __builtin_clz(a.splits);
+    const float down = __builtin_amdgcn_ldexpf(1.0f, -less);
 #pragma unroll 2
     for (int s = 0; s < a.splits; ++s) {
         const float w = __builtin_amdgcn_exp2f(a.part_lse[s * all * a.Hq + at] - by);
         const f32x4 v = *reinterpret_cast<const f32x4*>(a.part_out + (s * all * a.Hq + at) * HD + 4 * lane);
         sum += w;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __fmaf_rn(w, v[e], o[e]);
+        for (int e = 0; e < 4; ++e) o[e] = __fmaf_rn(w * down, v[e], o[e]);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(1.0f / sum, less);
     *reinterpret_cast<uint2*>(a.out + at * HD + 4 * lane) = make_uint2(pair_16<DT>(o[0] * inv, o[1] * inv), pair_16<DT>(o[2] * inv, o[3] * inv));
     if (a.lse && lane == 0) {
         const int64_t nth = at / a.Hq, row = a.offsets ? 0 : nth / a.L;

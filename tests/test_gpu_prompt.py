@@ -207,6 +207,31 @@ def test_values_at_the_type_s_end():
         _check(q, k, -v)
 
 
+SIGNS = ("all above", "all below", "halves", "blocks", "tokens")
+
+
+def _at_the_end(v, signs, by=1.0):
+    """Values of the type's largest magnitude and 0.98 of it, times `by`; their signs one for all, or another for each half of the tokens, each block of 64, each token."""
+    t = torch.arange(v.shape[2], device=v.device)
+    flip = {"all above": 0 * t, "all below": 0 * t + 1, "halves": (t >= v.shape[2] // 2).long(), "blocks": t // 64 % 2, "tokens": t % 2}[signs]
+    size = torch.where(v > 0, 1.0, 0.98).to(v.dtype) * (torch.finfo(v.dtype).max * by)
+    return torch.where(flip[None, None, :, None] > 0, -size, size)
+
+
+@pytest.mark.parametrize("signs", SIGNS)
+@pytest.mark.parametrize("shape", [(1, 8, 1, 1, 20000), (1, 4, 2, 3, 6000), (2, 6, 2, 5, 3000), (1, 24, 24, 2000, 9000)], ids=str)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_at_the_type_s_end_in_shares(dtype, shape, signs):
+    """Few queries over many keys: a tile's keys are shared out, and the shares' results, of values that 32 bits just hold, are put together."""
+    from kvquant import _lib
+    B, Hq, H, L, T = shape
+    assert _lib.lib.odmkv_prompt_attend_workspace_bytes(0, B, Hq, H, L, T, 1, 0, 0.0) >= 2 * B * L * Hq * 129 * 4
+    q, k, v = _inputs(32, *shape, dtype)
+    _check(q, k, _at_the_end(v, signs))
+    if dtype == torch.bfloat16 and L < 10:
+        _check(q, k, _at_the_end(v, signs, by=2.0 ** -6))               # (what 64 shares of one sign add up to)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scores_that_rise(dtype):
     """Every later key outscores the ones before by far, or falls behind: the reference moves many times, or never."""

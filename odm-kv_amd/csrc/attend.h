@@ -119,10 +119,10 @@ __device__ static inline float raise(Sums& s, float most, float valued, float li
     s = {to, s.sum * __builtin_amdgcn_exp2f(-rise), next};
     return __builtin_amdgcn_exp2f(at - next);
 }
-// 2^(unit - 8) x, all that it may be
-__device__ static inline float in_unit(const Sums& s, float x) {
+// 2^(unit - 8 - less) x, all that it may be
+__device__ static inline float in_unit(const Sums& s, float x, int less = 0) {
     const float power = fmaxf(s.unit - 8.0f, -500.0f), whole = floorf(power);
-    return __builtin_amdgcn_ldexpf(x * __builtin_amdgcn_exp2f(power - whole), (int)whole);
+    return __builtin_amdgcn_ldexpf(x * __builtin_amdgcn_exp2f(power - whole), (int)whole - less);
 }
 // Products to scores; never 0, so that a place that is not seen (-inf) stays that (a block whose keys are all 0 has products of 0 alone).
 __device__ static inline float scale_of(float ks, float qs) { return ks * qs != 0.0f ? ks * qs : 0x1p-120f; }

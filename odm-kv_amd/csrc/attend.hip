@@ -1,9 +1,13 @@
 // The entry of the attention over the paged 8-bit cache: its checks, how a call is cut into workgroups, the merge of partial results.
+#include <cfloat>
 #include "attend.h"
 
 // The shares of a row and kv-head's blocks, put together: out = sum_s w_s out_s / sum_s w_s, w_s = exp(lse_s - largest).  A workgroup a query, its four wavefronts every
 // fourth share, eight shares of a wavefront on their way at a time, a lane two dims.  Bound by the latency of two dependent reads: 4.0 us behind a step over 32768 tokens
 // (32 queries, 64 shares each), 7.2 for 928 queries of 64 shares (31 MB).
+//
+// bf16: values may lie at the type's end, and a result that stands for codes a little past 32 bits' own.  The latter are stopped there, and the weights, of one at most each, meet the values smaller
+// by a power of two that takes their sum to a half or below, so that nothing is infinite on its way to a mean that is not.  (A power of two: every other result keeps its bits.)
 #define MERGE_AHEAD 8
 #define MERGE_MANY 1024
 
@@ -37,6 +41,9 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
         splits = own.count + in_common;
         at = ((size_t)h * a.splits + own.first) * R + r;
     }
+    const int less = DT == ODMKV_F16 ? 0 : 33 - __builtin_clz(splits);
+    const float down = __builtin_amdgcn_ldexpf(1.0f, -less);
+    const auto held = [](float x) { return DT == ODMKV_F16 ? x : __builtin_amdgcn_fmed3f(x, -FLT_MAX, FLT_MAX); };      // (of a query that is not a number the weights are not)
     // (each wavefront by its own largest: the partial results need not wait for the largest of all)
     float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
     for (int i0 = wave; i0 < splits; i0 += APART * MERGE_AHEAD) {
@@ -65,8 +72,8 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
         for (int k = 0; k < MERGE_AHEAD; ++k) {
             const float w = __builtin_amdgcn_exp2f(lse[k] - by);
             sum += w;
-            o0 = __fmaf_rn(w, v[k].x, o0);
-            o1 = __fmaf_rn(w, v[k].y, o1);
+            o0 = __fmaf_rn(w * down, held(v[k].x), o0);
+            o1 = __fmaf_rn(w * down, held(v[k].y), o1);
         }
     }
     if constexpr (APART == 4) {
@@ -89,7 +96,7 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
             o1 = __fmaf_rn(f, part[w][2 * lane + 1], o1);
         }
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(1.0f / sum, less);
     o0 *= inv;
     o1 *= inv;
     *reinterpret_cast<uint32_t*>(a.out + (((size_t)row * a.L + l) * a.Hq + hq) * HD + 2 * lane) = (uint32_t)to_16<DT>(o0) | (uint32_t)to_16<DT>(o1) << 16;

@@ -277,13 +277,14 @@ __device__ static inline void attend_rows(const AttendArgs& a, unsigned workgrou
         }
     }
 
-    // every wavefront's result, of the sum of its own weights
+    // Every wavefront's result, of the sum of its own weights.  (bf16: a half of it, since codes may stand for a little more than 32 bits hold.)
+    constexpr int HALF = DT == ODMKV_BF16;
     sums.sum = column_sum(sums.sum);
     const float own_inv = sums.sum == 0.0f ? 0.0f : 1.0f / sums.sum;
 #pragma unroll
     for (int m = 0; m < 8; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc_of[wave][n][16 * m + 4 * j + e] = in_unit(sums, acc[m][e] * own_inv);
+        for (int e = 0; e < 4; ++e) acc_of[wave][n][16 * m + 4 * j + e] = in_unit(sums, acc[m][e] * own_inv, HALF);
     if (j == 0) {
         ref_of[wave][n] = sums.ref;
         sum_of[wave][n] = sums.sum;
@@ -292,21 +293,27 @@ __device__ static inline void attend_rows(const AttendArgs& a, unsigned workgrou
     // a thread takes eight dims of a query
     const int r = tid >> 4, d = (tid & 15) * 8, rl = r / a.G, rh = h * a.G + r - rl * a.G;
     if (r >= R || rl >= count) return;                          // (of eight wavefronts the last four have no query)
-    float to = ref_of[0][r], total = 0.0f, o[8];
+    float to = ref_of[0][r], total = 0.0f, f[WAVES], o[8];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) to = fmaxf(to, ref_of[w][r]);
     const float by = to > -INFINITY ? to : 0.0f;
 #pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        // (a query that is not a number has a sum that is not, and a reference that may be anything)
+        f[w] = sum_of[w][r] == 0.0f ? 0.0f : sum_of[w][r] * __builtin_amdgcn_exp2f(ref_of[w][r] - by);
+        total += f[w];
+    }
+    // (bf16: values may lie at the type's end, so the weights meet them smaller by the power of two that takes their sum below one; every other result keeps its bits)
+    const int less = DT == ODMKV_F16 ? 0 : __builtin_amdgcn_frexp_expf(total);
+#pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-        // (a query that is not a number has a sum that is not, and a reference that may be anything)
-        const float f = sum_of[w][r] == 0.0f ? 0.0f : sum_of[w][r] * __builtin_amdgcn_exp2f(ref_of[w][r] - by);
-        total += f;
+        const float part = __builtin_amdgcn_ldexpf(f[w], -less);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = __fmaf_rn(acc_of[w][r][d + e], f, o[e]);
+        for (int e = 0; e < 8; ++e) o[e] = __fmaf_rn(acc_of[w][r][d + e], part, o[e]);
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inv = total == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(1.0f / total, less + HALF);
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = total == 0.0f ? 0.0f : o[e] * inv;
     const float lse2 = total == 0.0f ? -INFINITY : to + __builtin_amdgcn_logf(total);

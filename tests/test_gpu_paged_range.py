@@ -183,3 +183,35 @@ def test_a_token_that_outweighs_the_others_is_rounded_once(at, L, kind):
     # half a step of fp16 at each value: 2^-11 of the power of two below it, 2^-25 for the smallest
     half = (2.0 ** (torch.frexp(want.abs()).exponent - 12).double()).clamp(min=2.0 ** -25)
     assert bool(sees.any()) and bool(((out - want).abs()[sees] <= (half + 2.0 ** -21 * want.abs())[sees]).all()), float(((out - want).abs() / half)[sees].max())
+
+
+def _at_the_end(v, signs, by):
+    """Values of bf16's largest magnitude and 0.97 of it, times `by`; their signs one for all, or another for each half of the tokens, each block of 64, each token."""
+    t = torch.arange(v.shape[2])
+    flip = {"all above": 0 * t, "all below": 0 * t + 1, "halves": (t >= v.shape[2] // 2).long(), "blocks": t // 64 % 2, "tokens": t % 2}[signs]
+    size = torch.where(v > 0, 1.0, 0.97).to(v.dtype) * (torch.finfo(v.dtype).max * by)
+    return torch.where(flip[None, None, :, None] > 0, -size, size)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("signs", ["all above", "all below", "halves", "blocks", "tokens"])
+@pytest.mark.parametrize("by", [1.0, 2.0 ** -5])
+def test_values_at_the_type_s_end(by, signs, kind):
+    """bf16 values whose weighted sum passes 32 bits though their mean does not: a row in shares and by itself, among few queries and many, and rows with most of it in common."""
+    dtype, n = torch.bfloat16, 3000
+    k, v = _rows(51, 1, 2, n, dtype)
+    v = _at_the_end(v, signs, by)
+    for L in (1, 4, 40):
+        q = _queries(52, 1, 8, L, dtype)
+        out, lse = _filled(k, v, [n], kind).attend(0, q.to(DEV), return_lse=True)
+        _check(out[0], lse[0], q[0], k[0], v[0], kind)
+        out, lse = _attend(k, v, q, kind)
+        _check(out, lse, q[0], k[0], v[0], kind)
+    one = _filled(k, v, [n], kind)
+    for rows in (3, 40):
+        c = one.select([0] * rows)
+        q = _queries(53, rows, 8, 2, dtype)
+        out, lse = c.attend(0, q.to(DEV), return_lse=True, shared=True)
+        for b in (0, rows - 1):
+            _check(out[b], lse[b], q[b], k[0], v[0], kind)
+        c.release()

@@ -85,6 +85,20 @@ __device__ static inline uint32_t pair_16(float x, float y) {
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector((__attribute__((ext_vector_type(2))) float){x, y}, __attribute__((ext_vector_type(2))) __bf16));
 }
 
+// Values' weights are rounded, those in the weights' sum are not: of fp16 values at the type's end a mean may come out 2^-11 past it, which would be infinite, and is stopped there
+// (two packed instructions behind the conversion; in 32 bits in front of it they took 2 %, and what was rounded once was rounded twice).  An infinity, and what is not a number, stay that where they are
+// said to be `odd`.  bf16 needs no stop: one weight is exactly one, and the others of values at the type's end are less than 2^-8 together, or their sum is past 32 bits and made once more.
+template <int DT>
+__device__ static inline uint32_t stopped_pair(uint32_t w, bool odd_low, bool odd_high) {
+    if constexpr (DT != ODMKV_F16) return w;
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+    const u16x2 below = {(uint16_t)(odd_low ? 0xffff : 0xfbff), (uint16_t)(odd_high ? 0xffff : 0xfbff)};      // (of numbers below 0 as they lie there the larger ones are the lower ones)
+    const i16x2 above = {(int16_t)(odd_low ? 0x7fff : 0x7bff), (int16_t)(odd_high ? 0x7fff : 0x7bff)};
+    const u16x2 x = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w), below);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(i16x2, x), above));
+}
+
 // Weights go to 16 bits relative to a reference, a score of the query's own: its weight is 2^LIFT, and where the sum of sixteen weights passes LIMIT the reference moves to the
 // largest score.  fp16: so no weight passes the type's end, and one below its normal numbers is off by 2^-25, 2^-33 of the largest at the most; bf16 has the range of 32 bits.
 template <int DT> struct Weights {
@@ -319,12 +333,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     float by = none ? 0.0f : 1.0f / sum;
     const float lse2 = none ? -INFINITY : ref - LIFT + __builtin_amdgcn_logf(sum);
     // A value that is not finite has spoilt the queries that do not see its token as well (0 times it is not 0), and bf16 values at the type's end may have passed 32 bits: their
-    // sums are made once more, token by token, of what is seen alone.
+    // sums are made once more, token by token, of what is seen alone, and of halves of the values.
     bool spoilt = false;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int e = 0; e < 16; ++e) spoilt |= !(fabsf(acc[db][e]) < INFINITY);
+    bool odd = spoilt;
     if (__any(spoilt && sum < INFINITY)) {
 #pragma unroll
         for (int db = 0; db < 4; ++db)
@@ -356,12 +371,19 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
                     const uint32_t vw[2] = {u.x, u.y};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float v = Elem<DT>::to_f32((uint16_t)(vw[e >> 1] >> (16 * (e & 1))));
+                        const float v = 0.5f * Elem<DT>::to_f32((uint16_t)(vw[e >> 1] >> (16 * (e & 1))));
                         acc[db][4 * g + e] = seen ? __fmaf_rn(p, v, acc[db][4 * g + e]) : acc[db][4 * g + e];
                     }
                 }
         }
-        by = 1.0f;
+        // (an infinite value that is seen stays one; what is finite ends where the type does)
+        constexpr float HALF_MOST = DT == ODMKV_F16 ? 32752.0f : 1.6947656946257677e38f;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[db][e] = fabsf(acc[db][e]) < INFINITY ? __builtin_amdgcn_fmed3f(acc[db][e], -HALF_MOST, HALF_MOST) : acc[db][e];
+        by = 2.0f;
+        odd = true;
     }
     const auto result = [&](int db, int e) { return none ? 0.0f : acc[db][e] * by; };
     const int64_t nth = (a.offsets ? 0 : (int64_t)row * a.L) + tile.q0 + l;                         // of all queries
@@ -405,7 +427,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
         for (int g = 0; g < 4; ++g) {
             uint32_t x[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) x[e] = pair_16<DT>(result(db, 4 * g + 2 * e), result(db, 4 * g + 2 * e + 1));
+            for (int e = 0; e < 2; ++e) x[e] = stopped_pair<DT>(pair_16<DT>(result(db, 4 * g + 2 * e), result(db, 4 * g + 2 * e + 1)), odd, odd);
             *reinterpret_cast<uint2*>(rows_at + col * 256 + (((4 * db + g) ^ (col & 15)) << 4) + 8 * half) = make_uint2(x[0], x[1]);
         }
     rows_of([&](uint32_t at, const uint4& x) { *reinterpret_cast<uint4*>(a.out + (int64_t)at * HD + 8 * (lane & 15)) = x; });
@@ -434,7 +456,9 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(PromptArgs a) {
         for (int e = 0; e < 4; ++e) o[e] = __fmaf_rn(w * down, v[e], o[e]);
     }
     const float inv = sum == 0.0f ? 0.0f : __builtin_amdgcn_ldexpf(1.0f / sum, less);
-    *reinterpret_cast<uint2*>(a.out + at * HD + 4 * lane) = make_uint2(pair_16<DT>(o[0] * inv, o[1] * inv), pair_16<DT>(o[2] * inv, o[3] * inv));
+    const auto odd = [&](int e) { return !(fabsf(o[e]) < INFINITY); };
+    *reinterpret_cast<uint2*>(a.out + at * HD + 4 * lane) = make_uint2(stopped_pair<DT>(pair_16<DT>(o[0] * inv, o[1] * inv), odd(0), odd(1)),
+                                                                       stopped_pair<DT>(pair_16<DT>(o[2] * inv, o[3] * inv), odd(2), odd(3)));
     if (a.lse && lane == 0) {
         const int64_t nth = at / a.Hq, row = a.offsets ? 0 : nth / a.L;
         a.lse[(row * a.Hq + at % a.Hq) * a.L + nth - row * a.L] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;

@@ -232,6 +232,33 @@ def test_values_at_the_type_s_end_in_shares(dtype, shape, signs):
         _check(q, k, _at_the_end(v, signs, by=2.0 ** -6))               # (what 64 shares of one sign add up to)
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("shape", [(1, 4, 2, 32, 32), (1, 2, 1, 1, 1000), (1, 8, 1, 3, 9000), (2, 4, 4, 200, 200), (1, 32, 8, 700, 700)], ids=str)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_mean_of_the_type_s_largest_is_that(dtype, shape, sign):
+    """All values are the type's largest (or its negative), and weights round upwards: their sum over the sum of what they were passes one, the result does not pass the type's end.
+    One key in 64 outweighs the others by nearly two: of a weight of 2^8 they have 128.069, in fp16 128.125, and of a weight of 1 just above a half and a step's half, in bf16 a half and a step."""
+    B, Hq, H, L, T = shape
+    q, k, v = (torch.zeros(B, h, n, 128, dtype=dtype, device=DEV) for h, n in ((Hq, L), (H, T), (H, T)))
+    q[..., 0], k[:, :, ::64, 0] = 1, 1
+    v[:] = sign * torch.finfo(dtype).max
+    out, _ = _check(q, k, v, scaling=0.69314718 * (0.99922 if dtype == torch.float16 else 0.99434))
+    none = max(0, L - T)
+    assert bool((out[:, none:] == sign * torch.finfo(dtype).max).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinite_values_beside_the_type_s_largest(dtype):
+    """Whoever sees an infinite value, or both infinities, or a NaN, gets what the definition says, in one share and in several; the others stay within the type's end."""
+    for shape in ((1, 4, 2, 150, 150), (1, 4, 2, 40, 7000)):
+        q, k, v = _inputs(33, *shape, dtype)
+        v = _at_the_end(v, "tokens")
+        last = shape[4]
+        v[0, 0, last - 30, 3], v[0, 0, last - 20, 3], v[0, 1, last - 25, 7], v[0, 1, 5, 9] = float("inf"), float("-inf"), float("nan"), float("-inf")
+        _check(q, k, v)
+        _check(q, k, v, window=12)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scores_that_rise(dtype):
     """Every later key outscores the ones before by far, or falls behind: the reference moves many times, or never."""

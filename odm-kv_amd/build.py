@@ -57,7 +57,7 @@ def _build_native(verbose: bool) -> None:
 
 def build(force: bool = False, verbose: bool = True) -> str:
     srcs = [os.path.join(CSRC, s) for s in SOURCES + BENCH_SOURCES]
-    deps = srcs + [os.path.join(CSRC, "torch_step.cpp")] + [os.path.join(CSRC, h) for h in ("common.h", "quant.h", "decode.h", "pages.h", "pages_write.h", "spans.h", "attend.h", "attend_narrow.h", "attend_wide.h", "attend_shared.h", "exports.map")] + [
+    deps = srcs + [os.path.join(CSRC, "torch_step.cpp")] + [os.path.join(CSRC, h) for h in ("common.h", "quant.h", "decode.h", "pages.h", "pages_write.h", "spans.h", "parts.h", "attend.h", "attend_narrow.h", "attend_wide.h", "attend_shared.h", "exports.map")] + [
         os.path.join(HERE, "..", "include", "odmkv.h"), os.path.join(HERE, "..", "include", "odmkv_bench.h"), __file__]
     if (not force and os.path.exists(LIB) and os.path.exists(BENCH_LIB) and os.path.exists(NATIVE)
             and min(map(os.path.getmtime, (LIB, BENCH_LIB, NATIVE))) >= _newest(deps)):

@@ -1,6 +1,7 @@
 // The entry of the attention over the paged 8-bit cache: its checks, how a call is cut into workgroups, the merge of partial results.
 #include <cfloat>
 #include "attend.h"
+#include "parts.h"
 
 // The shares of a row and kv-head's blocks, put together: out = sum_s w_s out_s / sum_s w_s, w_s = exp(lse_s - largest).  A workgroup a query, its four wavefronts every
 // fourth share, eight shares of a wavefront on their way at a time, a lane two dims.  Bound by the latency of two dependent reads: 4.0 us behind a step over 32768 tokens
@@ -167,12 +168,12 @@ static Cut cut_shared(const odmkv_pages_t& p, int R, int max_length) {
 extern "C" size_t odmkv_pages_attend_shared_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length) {
     if (!p || p->Hkv <= 0 || p->rows <= 0 || Hq <= 0 || L <= 0 || max_length < 0) return 0;
     const Cut c = cut_shared(*p, Hq / p->Hkv * L, max_length);
-    return align_up((c.parts + (size_t)p->Hkv * c.common_parts) * (HD + 1) * sizeof(float), 256);
+    return align_up(part_places(c.parts, (size_t)p->Hkv * c.common_parts).floats * sizeof(float), 256);
 }
 
 extern "C" size_t odmkv_pages_attend_workspace_bytes(const odmkv_pages_t* p, int Hq, int L, int max_length) {
     if (!p || p->Hkv <= 0 || p->rows <= 0 || Hq <= 0 || L <= 0 || max_length < 0) return 0;
-    return align_up(cut_of(*p, Hq / p->Hkv * L, max_length).parts * (HD + 1) * sizeof(float), 256);
+    return align_up(part_places(cut_of(*p, Hq / p->Hkv * L, max_length).parts, 0).floats * sizeof(float), 256);
 }
 
 extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
@@ -201,13 +202,14 @@ extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
     const Cut cut = (d->plan ? cut_shared : cut_of)(p, a.G * a.L, d->max_length);
     a.splits = cut.splits;
     a.part_out = (float*)d->workspace;
-    a.part_lse = a.part_out + cut.parts * HD;
+    const PartPlaces at = part_places(cut.parts, (size_t)p.Hkv * cut.common_parts);
+    a.part_lse = a.part_out + at.lse;
     hipStream_t st = (hipStream_t)stream;
     const bool f16 = p.dtype == ODMKV_F16;
     a.spare = cut.spare;
-    a.common_out = a.part_lse + cut.parts;
+    a.common_out = a.part_out + at.common_out;
     a.common_parts = cut.common_parts;
-    a.common_lse = a.common_out + (size_t)p.Hkv * cut.common_parts * HD;
+    a.common_lse = a.part_out + at.common_lse;
     const int rc = cut.shared ? (f16 ? launch_attend_shared_f16(a, cut.workgroups, st) : launch_attend_shared_bf16(a, cut.workgroups, st))
                  : cut.wide ? (f16 ? launch_attend_wide_f16(a, cut, st) : launch_attend_wide_bf16(a, cut, st))
                             : (f16 ? launch_attend_narrow_f16(a, cut, st) : launch_attend_narrow_bf16(a, cut, st));

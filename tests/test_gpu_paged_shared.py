@@ -76,6 +76,20 @@ def test_rows_in_common(prompts, parents, fresh, Hq, H, L, kind, dtype):
     assert _plan(c) == _plan_of_tables(c)
 
 
+ODD = [([200], [0] * 3, [1, 0, 5], 7, 1, 1), ([130], [0] * 5, [3, 64, 0, 1, 70], 5, 1, 1), ([300, 130], [0, 1, 0, 1, 1, 0, 0], [2, 3, 64, 9, 1, 0, 5], 3, 1, 3),
+       ([150], [0] * 151, [b % 70 for b in range(151)], 7, 1, 1), ([130], [0] * 201, [b % 3 for b in range(201)], 3, 1, 2), ([500], [0] * 79, [b % 66 for b in range(79)], 5, 1, 3),
+       ([70, 200], [b % 2 for b in range(111)], [b % 5 for b in range(111)], 10, 2, 1), ([64], [0] * 1023, [1] * 1023, 1, 1, 1), ([64], [0] * 1024, [1] * 1024, 3, 1, 1)]
+
+
+@pytest.mark.parametrize("prompts,parents,fresh,Hq,H,L", ODD, ids=[f"{c[0]}x{len(c[1])}-{c[3]}-{c[4]}-{c[5]}" for c in ODD])
+def test_odd_counts_of_queries(prompts, parents, fresh, Hq, H, L):
+    """One kv-head and odd numbers of rows and query heads: partial results whose number is no multiple of four, and more than 1024 queries, of which a workgroup puts four together."""
+    for dtype in (torch.float16, torch.bfloat16):
+        c, rows = _samples(len(parents), prompts, parents, fresh, H, dtype, "int8")
+        _check_attend(c, rows, "int8", _queries(7, len(parents), Hq, L, dtype))
+        assert _plan(c) == _plan_of_tables(c)
+
+
 MASKS = {"cap": dict(softcap=20.0), "large cap": dict(softcap=3000.0), "window inside": dict(window=30), "window across": dict(window=200), "bias": dict(slopes=0.25),
          "scaling": dict(scaling=-0.05), "prefix": dict(prefix=[130, 0, 500, 400, 1]), "starts": dict(starts=[70, 0, 256, 310, 10 ** 6]), "starts of each": dict(starts="each"),
          "counts": dict(counts=[2, 0, 1, 2, 0]), "all": dict(softcap=30.0, slopes=0.1, window=290, prefix=[100, 400, 3, 0, 290], starts=[5, 200, 0, 64, 0], counts=[1, 2, 2, 0, 2])}

@@ -93,17 +93,22 @@ def test_bad_plans_are_refused():
     assert lib.odmkv_pages_attend_shared_workspace_bytes(p, 8, 40, 9000) == lib.odmkv_pages_attend_workspace_bytes(p, 8, 40, 9000)
 
 
-# ---- what offsets say, where nobody on the host has seen them (csrc/spans.h, as the kernel compiles it)
-@pytest.fixture(scope="module")
-def span_of(tmp_path_factory):
+# ---- headers that the host compiles as the entry points and kernels do
+def _compiled(folder, name, source):
     import os
     import subprocess
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    at = tmp_path_factory.mktemp("spans")
-    (at / "spans.cpp").write_text('#include "spans.h"\nextern "C" void span(int first, int last, int all, int* to) { const Span s = span_of(first, last, all); to[0] = s.begin; to[1] = s.n; }\n')
+    (folder / f"{name}.cpp").write_text(f'#include "{name}.h"\n{source}\n')
     subprocess.run(["g++", "-O2", "-fwrapv", "-shared", "-fPIC", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(root, "odm-kv_amd", "csrc"),
-                    str(at / "spans.cpp"), "-o", str(at / "spans.so")], check=True)
-    f = C.CDLL(str(at / "spans.so")).span
+                    str(folder / f"{name}.cpp"), "-o", str(folder / f"{name}.so")], check=True)
+    return C.CDLL(str(folder / f"{name}.so"))
+
+
+@pytest.fixture(scope="module")
+def span_of(tmp_path_factory):
+    """What offsets say, where nobody on the host has seen them (csrc/spans.h)."""
+    f = _compiled(tmp_path_factory.mktemp("spans"), "spans",
+                  'extern "C" void span(int first, int last, int all, int* to) { const Span s = span_of(first, last, all); to[0] = s.begin; to[1] = s.n; }').span
     f.argtypes, f.restype = [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int)], None
 
     def call(first, last, all):
@@ -122,3 +127,18 @@ def test_spans_of_any_offsets_stay_within_what_there_is(span_of):
                 begin = min(max(first, 0), all)
                 want = begin, max(min(max(last, 0), all) - begin, 0)
                 assert span_of(first, last, all) == want, (first, last, all)
+
+
+def test_partial_results_lie_apart_and_on_16_bytes(tmp_path):
+    """Any number of results, odd ones among them: results begin on 16 bytes, nothing lies in another's place, and all of it within what is asked for."""
+    f = _compiled(tmp_path, "parts", 'extern "C" void places(size_t parts, size_t common, size_t* to) { const PartPlaces p = part_places(parts, common); to[0] = p.lse; '
+                  'to[1] = p.common_out; to[2] = p.common_lse; to[3] = p.floats; }').places
+    f.argtypes, f.restype = [C.c_size_t, C.c_size_t, C.POINTER(C.c_size_t)], None
+    for parts in (0, 1, 2, 3, 4, 5, 21, 63, 3 * 7 * 5, 2 ** 20 + 1, 2 ** 26 + 3):
+        for common in (0, 1, 2, 3, 128 * 5 + 21, 2 ** 25 + 1):
+            to = (C.c_size_t * 4)()
+            f(parts, common, to)
+            lse, out, common_lse, floats = to
+            assert lse % 4 == 0 and out % 4 == 0, (parts, common)
+            assert lse >= 128 * parts and out >= lse + parts and common_lse >= out + 128 * common and floats >= common_lse + common, (parts, common)
+            assert floats <= 129 * (parts + common) + 8

@@ -335,9 +335,11 @@ typedef int (*rotate_fn)(const odmkv_rotate_t*, void*);
 typedef int (*prompt_fn)(const odmkv_prompt_attend_t*, void*);
 typedef size_t (*prompt_bytes_fn)(int, int, int, int, int, int, int, int, float);
 
+// gradients that a call would have to record, or a tangent that it would have to carry on
+bool recorded(const at::Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
 // [B, heads, T, 128] in 16 bits with rows that start on 16 bytes, and nothing to record
 bool heads_fit(const at::Tensor& t, at::ScalarType type, int device) {
-    if (t.dim() != 4 || !t.is_cuda() || t.get_device() != device || t.scalar_type() != type || (t.requires_grad() && at::GradMode::is_enabled())) return false;
+    if (t.dim() != 4 || !t.is_cuda() || t.get_device() != device || t.scalar_type() != type || recorded(t)) return false;
     const auto r = t.strides();
     return t.size(3) == ODMKV_HEAD_DIM && r[3] == 1 && ((r[0] | r[1] | r[2]) & 7) == 0 && ((uintptr_t)t.data_ptr() & 15) == 0 && t.size(2) <= (1 << 26);
 }
@@ -392,7 +394,7 @@ PyObject* native_paged_write_rotated(PyObject*, PyObject* const* a, Py_ssize_t n
         const int64_t Hq = q.size(1);
         if (q.size(0) != B || k.size(0) != B || v.sizes() != k.sizes() || k.size(1) != p->Hkv || q.size(2) != T || Hq < 1 || Hq > 65535 || T < 1 || T < grown) Py_RETURN_NONE;
         for (const at::Tensor* t : {&c, &s})
-            if (t->dim() != 2 || !t->is_cuda() || t->get_device() != device || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->sizes() != c.sizes() || ((uintptr_t)t->data_ptr() & 15)) Py_RETURN_NONE;
+            if (t->dim() != 2 || !t->is_cuda() || t->get_device() != device || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->sizes() != c.sizes() || ((uintptr_t)t->data_ptr() & 15) || recorded(*t)) Py_RETURN_NONE;
         const int64_t half = c.size(1);
         if (half < 8 || half > ODMKV_HEAD_DIM / 2 || half % 8 || c.size(0) < 1 || c.size(0) > INT32_MAX) Py_RETURN_NONE;
         odmkv_rotate_t d;

@@ -57,6 +57,12 @@ def _as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return t.clamp(-2 ** 31, 2 ** 31 - 1).to(dtype) if dtype == torch.int32 and t.dtype == torch.int64 else t.to(dtype)
 
 
+def _recorded(*tensors) -> bool:
+    """Whether a call would have to record gradients for any of these, or to carry a tangent on (dual numbers do so without gradients as well)."""
+    unpack, recording = torch.autograd.forward_ad.unpack_dual, torch.is_grad_enabled()
+    return any(isinstance(t, torch.Tensor) and ((recording and t.requires_grad) or unpack(t).tangent is not None) for t in tensors)
+
+
 class PagedKVCache:
     """`batch` rows of at most `max_tokens` tokens, `layers` layers of `kv_heads` heads of 128; `pages`: full blocks that there is room for in each layer
     (default: every row's longest).  `kind`: "int8" or "e4m3".  The tensors are attributes, laid out as include/odmkv.h says (struct odmkv_pages)."""
@@ -297,7 +303,8 @@ class PagedKVCache:
         A row's new tokens stand where they lie in the row, less `starts` (int32 [B]: where the text behind padding begins; padding stands at 0), or at `positions` (int32
         [B, T]).  Packed: with `offsets` (int32 [B + 1]) keys, values and query are [1, heads, N, 128], row b's tokens those from offsets[b] to before offsets[b + 1], as many as the row has
         grown by, and positions [1, N].  The host checks the table against the rows' lengths; what only the device can see (positions that the table has no row for, which count as
-        its nearest, offsets that do not fit, whose rows are not stored) is raised by ``refresh``."""
+        its nearest, offsets that do not fit, whose rows are not stored) is raised by ``refresh``.  For inference: tensors and tables that require gradients are refused while those
+        are recorded, and so are dual numbers."""
         if layer in self._written:                           # (the new tail would be taken for the old one)
             raise ValueError(f"layer {layer} has no tokens to store: it has stored those of the last extend already, or rows have been moved or cut since")
         if not self._replayed and _capturing():
@@ -320,8 +327,8 @@ class PagedKVCache:
             self._check_tensor(t, what)
         if any(t.shape[2] != keys.shape[2] for t, _ in given):
             raise ValueError(f"{' and '.join(f'{t.shape[2]} {what}' for t, what in given)} a row")
-        if torch.is_grad_enabled() and any(t.requires_grad for t, _ in given):
-            raise RuntimeError("the cache records no gradients: turn and store under torch.no_grad()")
+        if _recorded(*(t for t, _ in given), cosine, sine):
+            raise RuntimeError("the cache records no gradients and carries no tangents: turn and store under torch.no_grad(), outside of dual numbers")
         T, Hq = keys.shape[2], 0 if query is None else query.shape[1]
         if T < self._grown:
             raise ValueError(f"{T} tokens{' a row' if offsets is None else ''}, but rows have grown by up to {self._grown}")

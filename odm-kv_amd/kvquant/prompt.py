@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import HEAD_DIM, lib
-from .paged_cache import _device, _FAR, _LEAST_CAP, _SCALING, _as, PagedKVCache
+from .paged_cache import _device, _FAR, _LEAST_CAP, _SCALING, _as, _recorded, PagedKVCache
 
 _ATTEND, _ATTEND_BYTES = _lib.PROMPT_ENTRIES
 _native = _lib._native
@@ -32,7 +32,7 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     Packed: with `offsets` (int32 [S + 1] on the device, ascending) query is [1, Hq, N, 128], sequence s's queries those from offsets[s] to before offsets[s + 1], its keys and values in [1, Hkv,
     M, 128] by `key_offsets`, or by the same offsets; `starts` is [S] then.  Queries that no sequence has get 0 and -inf.  Nothing is read back.
 
-    Grouped heads: Hq a multiple of Hkv.  For inference: tensors that require gradients are refused while gradients are recorded."""
+    Grouped heads: Hq a multiple of Hkv.  For inference: tensors that require gradients are refused while gradients are recorded, and so are dual numbers."""
     if isinstance(query, torch.Tensor) and query.is_cuda and query.device.index == _device() and (softcap is None or _LEAST_CAP <= softcap < math.inf) and (
             window is None or (window >= 1 and causal)):
         # (everything as the kernel takes it: one native call)
@@ -49,8 +49,8 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
             raise ValueError(f"{what} must be float16 or bfloat16, all of one type, got {t.dtype}")
         if t.device != query.device:
             raise ValueError(f"{what} lie on {t.device}, queries on {query.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (query, keys, values)):
-        raise RuntimeError("prompt_attention records no gradients: call it under torch.no_grad()")
+    if _recorded(query, keys, values):
+        raise RuntimeError("prompt_attention records no gradients and carries no tangents: call it under torch.no_grad(), outside of dual numbers")
     B, Hq, L, _ = query.shape
     Hkv, T = keys.shape[1], keys.shape[2]
     if keys.shape != values.shape:

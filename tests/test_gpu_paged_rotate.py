@@ -293,6 +293,30 @@ def test_refusals():
     assert c.refresh() == [T, T]
 
 
+def test_what_would_be_recorded_is_refused():
+    """Gradients while they are recorded, tangents with and without: of tokens and of tables, each by itself, by the native call and (with positions) by the other; nothing is stored then."""
+    from torch.autograd import forward_ad
+    H, T = 2, 10
+    given = [*(_random(s, 2, h, T, dtype=torch.float16).to(DEV) for s, h in ((1, 4), (2, H), (3, H))), *(t.to(DEV) for t in _tables(64, 128))]
+    c = _cache(2, H, 64)
+    c.extend(T)
+    where = torch.arange(T, dtype=torch.int32, device=DEV).expand(2, T).contiguous()
+    for how in (dict(), dict(positions=where)):
+        for i in range(5):
+            args = list(given)
+            args[i] = args[i].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="no gradients"):
+                c.write_rotated(0, *args, **how)
+            with forward_ad.dual_level(), torch.no_grad():
+                args[i] = forward_ad.make_dual(given[i].clone(), torch.ones_like(given[i]))
+                with pytest.raises(RuntimeError, match="no tangents"):
+                    c.write_rotated(0, *args, **how)
+    learned = [*given[:3], *(t.clone().requires_grad_() for t in given[3:])]
+    with torch.no_grad():                                                                    # learned tables, at inference
+        got = c.write_rotated(0, *learned)
+    assert torch.equal(got, _turned(given[0].cpu(), given[3][:T].cpu(), given[4][:T].cpu(), False).to(DEV))
+
+
 def test_tables_that_lie_anywhere():
     """Tables off 16 bytes, transposed, and as every other row of a larger one: the same bits."""
     q, k, v = (_random(s, 2, h, 70, dtype=torch.float16).to(DEV) for s, h in ((31, 4), (32, 2), (33, 2)))

@@ -330,6 +330,27 @@ def test_captured_and_on_another_stream():
         assert torch.equal(there[0], got[0])
 
 
+def test_what_would_be_recorded_is_refused():
+    """Gradients while they are recorded, tangents with and without: of each operand by itself, by the native call and by the other."""
+    from torch.autograd import forward_ad
+    from kvquant import prompt_attention
+    given = _inputs(41, 1, 4, 2, 10, 10, torch.float16)
+    odd = torch.zeros(1, 4, 10, 129, dtype=torch.float16, device=DEV)[..., 1:]              # (not by the native call)
+    want = prompt_attention(*given)
+    for first in (given[0], odd):
+        for i in range(3):
+            args = [first, *given[1:]]
+            args[i] = args[i].detach().requires_grad_()
+            with pytest.raises(RuntimeError, match="no gradients"):
+                prompt_attention(*args)
+            with forward_ad.dual_level(), torch.no_grad():
+                args[i] = forward_ad.make_dual(args[i].detach(), torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="no tangents"):
+                    prompt_attention(*args)
+    with forward_ad.dual_level():                                                            # (plain tensors among dual numbers)
+        assert torch.equal(prompt_attention(*given), want)
+
+
 def test_refusals():
     from kvquant import prompt_attention
     q, k, v = _inputs(21, 2, 4, 2, 10, 10, torch.float16)

@@ -142,3 +142,16 @@ def test_partial_results_lie_apart_and_on_16_bytes(tmp_path):
             assert lse % 4 == 0 and out % 4 == 0, (parts, common)
             assert lse >= 128 * parts and out >= lse + parts and common_lse >= out + 128 * common and floats >= common_lse + common, (parts, common)
             assert floats <= 129 * (parts + common) + 8
+
+
+def test_what_a_call_would_have_to_record():
+    import torch
+    from torch.autograd import forward_ad
+    from kvquant.paged_cache import _recorded
+    x = torch.ones(3)
+    y = x.clone().requires_grad_()
+    assert not _recorded(x, None, 5) and _recorded(x, y) and _recorded(2 * y)
+    with torch.no_grad():
+        assert not _recorded(x, y)
+    with forward_ad.dual_level(), torch.no_grad():
+        assert not _recorded(x, y) and _recorded(x, forward_ad.make_dual(x, torch.ones(3)))

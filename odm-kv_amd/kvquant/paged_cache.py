@@ -31,6 +31,7 @@ BLOCK = 64                                    # tokens of a page
 MAX_ROWS = 1024                               # the bookkeeping runs in one workgroup, a thread a row
 HOST_ROWS = 512                               # batches up to here have a row's number each travel in the launch's arguments
 MAX_GROUP = 8
+_NARROW = 16                                  # queries of a kv-head up to which blocks in common are read once (csrc/attend.h: NARROW)
 KINDS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 
 _SCALING = HEAD_DIM ** -0.5
@@ -430,8 +431,9 @@ class PagedKVCache:
         get 0, and -inf for lse.
 
         `shared`: blocks that rows have in common (the pages that ``reorder`` and ``select`` let them share) are read once for all of them; for batches whose rows share most of what
-        they hold, samples or beams of long prompts.  The result is the same but for the order of sums.  Up to 16 queries of a kv-head (its query heads times L); more take the ordinary way.  Which
-        blocks those are is worked out on the device by the first such call (make it before a graph is captured), and again whenever rows are moved or cut.
+        they hold, samples or beams of long prompts.  The result is the same but for the order of sums.  Up to 16 queries of a kv-head (its query heads times L); more, and a batch of
+        one row, take the ordinary way.  Which blocks those are is worked out on the device by the first call that reads them (make it before a graph is captured), and again whenever rows are
+        moved or cut.
 
         `longest`: about how long the longest row is, which decides how the work is cut and nothing else (default: the host's bound, and while a graph is captured
         max_tokens, since the rows may be that long at a replay)."""
@@ -441,7 +443,7 @@ class PagedKVCache:
         elif longest < 0:
             raise ValueError(f"longest must not be negative, got {longest}")
         longest = min(longest, self.max_tokens)
-        plan = self._plan_of_common() if shared else 0
+        plan = self._plan_of_common() if shared and self._reads_common(query) else 0
         if _device() == self.device.index and isinstance(query, torch.Tensor) and (softcap is None or _LEAST_CAP <= softcap < math.inf) and (window is None or window >= 1):
             # (everything as the kernels take it: one native call)
             done = _native.paged_attend(_ATTEND, _SHARED_BYTES if plan else _ATTEND_BYTES, self._at, self.device.index, layer, query, _SCALING if scaling is None else scaling,
@@ -483,6 +485,10 @@ class PagedKVCache:
     # the plan of common blocks: made by the first call that asks for it, made again by whatever moves or cuts rows, so that replays of captured calls keep it right as well
     _plan: Optional[torch.Tensor] = None
     _unplanned = False                                       # rows may be moved by replays of calls that were captured while there was no plan
+
+    def _reads_common(self, query) -> bool:
+        """Whether a call reads what rows have in common once for all of them: a plan that nobody reads would be made again at every move of rows."""
+        return self.batch > 1 and isinstance(query, torch.Tensor) and query.dim() == 4 and query.shape[1] * query.shape[2] <= _NARROW * self.kv_heads
 
     def _plan_of_common(self) -> int:
         """The plan's address; it is of the tables as they are, or will be where the current call runs."""

@@ -129,6 +129,29 @@ def test_more_queries_than_sixteen_take_the_ordinary_way():
     assert torch.equal(c.attend(0, odd, shared=True), c.attend(0, q[:, :, :1], shared=True))
 
 
+def test_no_plan_is_kept_that_nobody_reads():
+    """More queries than sixteen, and a batch of one row, take the ordinary way: no plan is made, and they can be captured without one."""
+    c, rows = _samples(6, [300], [0] * 3, [5, 6, 7], 2, torch.float16, "int8")
+    wide, one = _queries(5, 3, 8, 5, torch.float16), c.select([1])
+    for cache, q, held in ((c, wide, rows), (one, wide[:1, :, :1], rows[1:2])):
+        _check_attend(cache, held, "int8", q)
+        assert cache._plan is None
+        q = q.to(DEV)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = cache.attend(0, q, shared=True)
+        for _ in range(3):
+            graph.replay()
+            want = cache.attend(0, q, longest=cache.max_tokens)
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        cache.reorder(list(range(cache.batch)))
+        assert cache._plan is None
+    _check_attend(c, rows, "int8", _queries(5, 3, 8, 4, torch.float16))                    # sixteen
+    assert _plan(c) == _plan_of_tables(c) == [([0, 1, 2], 4)]
+    _check_attend(c, rows, "int8", wide)
+
+
 def test_the_plan_follows_the_rows():
     """Beams that are reordered, cut into what they share, freed, forked and compacted: the plan is what the tables say, the attention what the rows hold."""
     B, H, dtype = 6, 2, torch.bfloat16

@@ -110,7 +110,7 @@ __device__ static inline int value_turn(int t) { return (t & 3) << 1 | (t >> 2 &
 
 template <int DT, int MODE, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
-    constexpr bool PLAIN = MODE == 0;                           // 1: a cap by the exponential; 2: any
+    constexpr bool PLAIN = MODE == 0, by_exp = MODE == 1;       // 1: a cap by the exponential; 2: a larger one, or a scaling that is not above 2^-100
     constexpr int COLS = PROMPT_COLS(WAVES), PIECES = PROMPT_TILE / 16 / (WAVES * 64);
     constexpr float LIFT = Weights<DT>::LIFT;
     extern __shared__ __align__(16) uint8_t smem[];             // [2][keys 64 x 256 bytes, values 64 x 256 bytes]
@@ -201,7 +201,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
         q[st] = make_uint4(x[0], x[1], x[2], x[3]);
     }
     const float inv_cap = !PLAIN && a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
-    const bool by_exp = MODE == 1 || (!PLAIN && a.cap > 0.0f && a.cap <= CAP_BY_EXP);
     const Cap cap = {a.cap * LOG2E, 2.0f * LOG2E * a.cap, 2.0f * LOG2E * inv_cap};
     const float c = PLAIN ? a.scaling * LOG2E : a.scaling;
     const auto score = [&](float x) {                           // of a product, base 2

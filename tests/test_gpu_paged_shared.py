@@ -286,3 +286,23 @@ def test_a_row_by_itself(n):
     want, got = (three.attend(0, q, **how) for how in (dict(), dict(shared=True)))
     # (each is rounded to bf16 once, by 2^-8 of itself at most; what else differs is the order of sums in 32 bits and weights in fp16, less than a step of either)
     assert not got[0].any() and not got[2].any() and (want[1].float() - got[1].float()).abs().max() <= 2 * 2.0 ** -8 * want[1].float().abs().max()
+
+
+@pytest.mark.parametrize("n", [1, 64, 3000])
+def test_rows_of_which_one_holds_anything(n):
+    """A plan that there was when the others were freed, and one made behind that: every element and log-sum-exp is the definition's, empty rows give 0 and -inf."""
+    k, v = (x.to(DEV) for x in _rows(40, 1, 2, n, torch.bfloat16))
+    one = _cache(1, 2, n + 4, dtype=torch.bfloat16)
+    one.append(k, v)
+    q = _queries(42, 3, 8, 1, torch.bfloat16)
+    mine, empty = ((x[0].cpu() for x in (k, v)), (x[0, :, :0].cpu() for x in (k, v)))
+    mine, empty = tuple(mine), tuple(empty)
+    for before in (True, False):
+        three = one.select([0, 0, 0])
+        if before:
+            _check_attend(three, [mine] * 3, "int8", q)
+        three.free([0, 2])
+        _check_attend(three, [empty, mine, empty], "int8", q)
+        out, lse = three.attend(0, q.to(DEV), shared=True, return_lse=True)
+        assert not out[[0, 2]].any() and bool((lse[[0, 2]] == -torch.inf).all()) and _plan(three) == []
+        three.release()

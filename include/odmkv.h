@@ -720,7 +720,7 @@ typedef struct odmkv_attend {
     void* workspace; size_t workspace_bytes;
     int32_t layer, L, Hq, window;
     int32_t max_length;                          /* about how long the longest row is: how the work is cut, not what is seen */
-    float scaling, cap;                          /* cap 0: none; 2^-100 at least otherwise */
+    float scaling, cap;                          /* cap 0: none; 2^-100 at least otherwise; past 2^100: 2^100 */
     const int32_t* plan;                         /* odmkv_pages_plan's, of the tables as they are, or NULL */
 } odmkv_attend_t;
 /* With a plan, blocks that rows have in common are read once for all of them (up to 16 queries of a kv-head, heads of a group times L; more go the ordinary way); the workspace is the
@@ -754,7 +754,7 @@ typedef struct odmkv_prompt_attend {
     const int32_t* starts;                       /* device [rows], or NULL */
     void* workspace; size_t workspace_bytes;
     int32_t dtype, rows, L, T, Hq, Hkv, causal, window;
-    float scaling, cap;                          /* cap 0: none; 2^-100 at least otherwise */
+    float scaling, cap;                          /* cap 0: none; 2^-100 at least otherwise; past 2^100: 2^100 */
 } odmkv_prompt_attend_t;
 size_t odmkv_prompt_attend_workspace_bytes(int packed, int rows, int Hq, int Hkv, int L, int T, int causal, int window, float cap);
 int odmkv_prompt_attend(const odmkv_prompt_attend_t* a, void* stream);

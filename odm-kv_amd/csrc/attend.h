@@ -76,6 +76,8 @@ __device__ static inline uint4 piece16(const uint8_t* at) {
 // Scores in base 2 from raw products: cap tanh(c x / cap) log2(e) = C - 2 C / (1 + 2^(k x)).  The reciprocal is off by 2^-23 of at most 1, the score by
 // 2^-22 C: 1.1e-5 for the largest cap that goes this way, of weights that fp16 rounds by 2.4e-4.  Larger caps take tanh by itself.
 #define CAP_BY_EXP 64.0f
+// A larger one counts as this: times log2(e) it would pass 32 bits, and its reciprocal would lose digits.  It changes scores of up to 2^88 by less than they are rounded.
+#define LARGEST_CAP 0x1p100f
 struct Cap { float by, twice, plain; };                         // C, 2 C, and what makes k of c
 __device__ static inline float capped(float kx, const Cap& m) {
     return __fmaf_rn(-m.twice, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(kx)), m.by);

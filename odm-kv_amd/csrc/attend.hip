@@ -192,7 +192,7 @@ extern "C" int odmkv_pages_attend(const odmkv_attend_t* d, void* stream) {
     ODMKV_CHECK_ARG((((uintptr_t)d->q | (uintptr_t)d->out) & 15) == 0 && ((d->q_stride_b | d->q_stride_h | d->q_stride_l) & 7) == 0,
                     "pages_attend: rows must be 16-byte aligned");
     AttendArgs a = {p, (const uint16_t*)d->q, d->q_stride_b, d->q_stride_h, d->q_stride_l, (uint16_t*)d->out, d->lse, d->counts, d->slopes,
-                    d->prefix, d->starts, d->start_stride_b, d->start_stride_l, d->layer, d->L, d->Hq, d->Hq / p.Hkv, d->window, d->scaling, d->cap,
+                    d->prefix, d->starts, d->start_stride_b, d->start_stride_l, d->layer, d->L, d->Hq, d->Hq / p.Hkv, d->window, d->scaling, std::min(d->cap, LARGEST_CAP),
                     1, nullptr, nullptr, d->plan, 0, nullptr, nullptr, 0};
     const size_t need = (d->plan ? odmkv_pages_attend_shared_workspace_bytes : odmkv_pages_attend_workspace_bytes)(&p, d->Hq, d->L, d->max_length);
     if (need > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < need)) {

@@ -535,7 +535,7 @@ extern "C" int odmkv_prompt_attend(const odmkv_prompt_attend_t* d, void* stream)
     float* const parts = (float*)d->workspace;
     const PromptArgs a = {(const uint16_t*)d->q, (const uint16_t*)d->k, (const uint16_t*)d->v, d->q_stride_b, d->q_stride_h, d->q_stride_t, d->k_stride_b, d->k_stride_h,
                           d->k_stride_t, d->v_stride_b, d->v_stride_h, d->v_stride_t, (uint16_t*)d->out, d->lse, d->offsets, d->key_offsets, d->starts, d->rows, d->L, d->T,
-                          d->Hq, d->Hkv, G, d->causal != 0, d->window, d->scaling, d->cap, cut.splits, cut.larger, parts, parts + (size_t)cut.splits * all * d->Hq * HD};
+                          d->Hq, d->Hkv, G, d->causal != 0, d->window, d->scaling, std::min(d->cap, LARGEST_CAP), cut.splits, cut.larger, parts, parts + (size_t)cut.splits * all * d->Hq * HD};
     const int mode = d->cap > 0.0f ? (d->cap <= CAP_BY_EXP ? 1 : 2) : d->scaling > 0x1p-100f ? 0 : 2;
     const hipStream_t st = (hipStream_t)stream;
     const auto run = [&](auto dt, auto mode_, auto waves) {

@@ -26,7 +26,7 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
 
     Query l stands at position i = T - L + l (a prompt: L = T; a later chunk over all keys so far: L < T; where there are more queries than keys, the first ones see nothing) and sees keys
     lo <= j < hi: lo is its row's start (`starts`, int32 [B]: where the text behind padding begins; default 0), and not before i - window + 1; hi is i + 1, or T where
-    `causal` is False.  Scores are scaling * q.k (default 128 ** -0.5), then softcap * tanh(x / softcap).  Queries that see nothing get 0, and -inf for lse; what a query
+    `causal` is False.  Scores are scaling * q.k (default 128 ** -0.5), then softcap * tanh(x / softcap) (a softcap past 2 ** 100 counts as that).  Queries that see nothing get 0, and -inf for lse; what a query
     does not see has no part in its result, infinities and NaN included.
 
     Packed: with `offsets` (int32 [S + 1] on the device, ascending) query is [1, Hq, N, 128], sequence s's queries those from offsets[s] to before offsets[s + 1], its keys and values in [1, Hkv,

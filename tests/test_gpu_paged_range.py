@@ -215,3 +215,18 @@ def test_values_at_the_type_s_end(by, signs, kind):
         for b in (0, rows - 1):
             _check(out[b], lse[b], q[b], k[0], v[0], kind)
         c.release()
+
+
+@pytest.mark.parametrize("cap", [2.0 ** 40, 2.0 ** 100, 2.0 ** 125, 2.0 ** 127, 3.4e38])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_caps_that_cap_nothing(dtype, cap):
+    """A cap past all scores by 2^30 changes them by 2^-60: the results are the definition's without one, up to the largest cap that 32 bits hold; few queries, many, and what rows have in common."""
+    n = 700
+    k, v = _rows(54, 1, 2, n, dtype)
+    one = _filled(k, v, [n], "int8")
+    c = one.select([0] * 3)
+    for L, shared in ((1, False), (4, True), (40, False)):
+        q = _queries(55, 3, 8, L, dtype)
+        out, lse = c.attend(0, q.to(DEV), softcap=cap, shared=shared, return_lse=True)
+        for b in range(3):
+            _check(out[b], lse[b], q[b], k[0], v[0], "int8")

@@ -269,6 +269,16 @@ def test_scores_that_rise(dtype):
         _check(q, k, v, cap=50.0)
 
 
+@pytest.mark.parametrize("cap", [2.0 ** 40, 2.0 ** 100, 2.0 ** 125, 2.0 ** 127, 3.4e38])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_caps_that_cap_nothing(dtype, cap):
+    """A cap past all scores by 2^30 changes them by 2^-60: the results are the definition's without one, up to the largest cap that 32 bits hold."""
+    for shape in ((1, 6, 2, 150, 150), (1, 8, 1, 2, 5000)):
+        q, k, v = _inputs(20, *shape, dtype)
+        out, lse = _call(q, k, v, softcap=cap)
+        plain.check(out[0], lse[0], *plain.attend(q[0], k[0], v[0]))
+
+
 def test_strides_types_and_bits():
     """Slices of one projection, rows that do not start on 16 bytes, one row for all heads: the same bits as of copies; a call made twice gives the same bits."""
     g = torch.Generator().manual_seed(16)

@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(AttendArgs a) {
 static int launch_attend_merge(const AttendArgs& a, const Cut& cut, hipStream_t st) {
     const int R = a.G * a.L;
     const dim3 grid(R, a.p.Hkv, a.p.rows);
-    // (a wavefront a query: 2048 queries of 18 parts each 9.2 -> 7.7 us, 3072 of 8 13.6 -> 6.6, but 448 of 65 parts 8.4 -> 13.1)
+    // (a wavefront a query: 2048 queries of 18 parts each 9.2 -> 7.7 us, 48 rows of 64 queries of 8 parts 13.6 -> 6.6, but 448 of 65 parts 8.4 -> 13.1)
     const bool many = (long long)R * a.p.Hkv * a.p.rows > MERGE_MANY;
     const auto of_type = [&](auto dt) {
         if (cut.shared && many) hipLaunchKernelGGL((attend_merge_kernel<dt.value, true, true, 1>), dim3((R + 3) / 4, a.p.Hkv, a.p.rows), dim3(256), 0, st, a);

@@ -12,7 +12,11 @@
 // this kernel without any vector work: 1245), matrix cores busy 52 % of the cycles, vector instructions 43 %.  A product of 32 cycles takes 18 ns, a 16-byte read of LDS beside it 6
 // more, its share of the vector work 5: so operands are read as rarely as 32 queries a wavefront allow (64 would not leave room for two wavefronts a SIMD), without bank conflicts,
 // and the largest score of a block is not looked for.  With a cap 34 % and 57 %: 12001 tokens in a window of 4096 in 419 us.  Prompts of 1500 tokens on average, 28 heads over 4, 455 us
-// (800 TFLOP/s): ten tiles a compute unit, each with a first block to wait for and a last one that few queries see whole.
+// (800 TFLOP/s): some twenty tiles of four wavefronts a compute unit, each with a first block to wait for and a last one that few queries see whole.  One prompt of 1024, 2048, 3000 or 4096 tokens,
+// 32 heads over 8: 32, 62, 93 and 144 us (272, 556, 794 and 957 TFLOP/s): one round of tiles up to some 3000, as long as the last of them, which sees all keys.
+//
+// A query's bits hang on the 31 others of its wavefront: weights are made in one of two ways, and sums a second time, for all of them together.  Both ways are as far from the formula as they may be, and
+// the same call gives the same bits.
 #include <algorithm>
 #include "attend.h"
 #include "spans.h"

@@ -209,7 +209,8 @@ class PagedCache(Cache):
 
     `config`: the model's; its attention must be one of the registered functions (not "eager", which cannot be told to read the pages).
 
-    `shared`: steps read the pages that rows have in common once for all of them (``PagedKVCache.attend(shared=True)``): for beams and samples of long prompts.
+    `shared`: steps read the pages that rows have in common once for all of them (``PagedKVCache.attend(shared=True)``): for beams and samples of long prompts,
+    not for windows much shorter than those, nor for samples of several prompts behind one system prompt.
     `native_prompt`: the prompt is attended by ``kvquant.prompt_attention``, padding in front, windows and soft caps included, in the model's own precision where scores
     are capped too; the model's own attention is not called then."""
 

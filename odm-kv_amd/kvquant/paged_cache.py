@@ -431,7 +431,9 @@ class PagedKVCache:
         get 0, and -inf for lse.
 
         `shared`: blocks that rows have in common (the pages that ``reorder`` and ``select`` let them share) are read once for all of them; for batches whose rows share most of what
-        they hold, samples or beams of long prompts.  The result is the same but for the order of sums.  Up to 16 queries of a kv-head (its query heads times L); more, and a batch of
+        they see, samples or beams of long prompts.  Rows with the same first block are one group, and have in common what each of them shares with the first of them: prompts behind one
+        system prompt, with samples each, are a group with the system prompt in common, and gain nothing by their own.  Nor do windows much shorter than what is in common: both may be
+        slower than the ordinary way.  The result is the same but for the order of sums.  Up to 16 queries of a kv-head (its query heads times L); more, and a batch of
         one row, take the ordinary way.  Which blocks those are is worked out on the device by the first call that reads them (make it before a graph is captured), and again whenever rows are
         moved or cut.
 

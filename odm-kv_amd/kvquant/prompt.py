@@ -32,6 +32,8 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     Packed: with `offsets` (int32 [S + 1] on the device, ascending) query is [1, Hq, N, 128], sequence s's queries those from offsets[s] to before offsets[s + 1], its keys and values in [1, Hkv,
     M, 128] by `key_offsets`, or by the same offsets; `starts` is [S] then.  Queries that no sequence has get 0 and -inf.  Nothing is read back.
 
+    The same call gives the same bits; a query's last bits may differ where its neighbours do (32 queries make their weights together).
+
     Grouped heads: Hq a multiple of Hkv.  For inference: tensors that require gradients are refused while gradients are recorded, and so are dual numbers."""
     if isinstance(query, torch.Tensor) and query.is_cuda and query.device.index == _device() and (softcap is None or _LEAST_CAP <= softcap < math.inf) and (
             window is None or (window >= 1 and causal)):

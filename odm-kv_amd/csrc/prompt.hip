@@ -342,7 +342,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_kernel(PromptArgs a) {
     for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int e = 0; e < 16; ++e) spoilt |= !(fabsf(acc[db][e]) < INFINITY);
-    bool odd = spoilt;
+    bool odd = spoilt || !(sum < INFINITY);                     // (or will not be a number)
     if (__any(spoilt && sum < INFINITY)) {
 #pragma unroll
         for (int db = 0; db < 4; ++db)

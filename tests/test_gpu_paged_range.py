@@ -230,3 +230,23 @@ def test_caps_that_cap_nothing(dtype, cap):
         out, lse = c.attend(0, q.to(DEV), softcap=cap, shared=shared, return_lse=True)
         for b in range(3):
             _check(out[b], lse[b], q[b], k[0], v[0], "int8")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_that_are_not_numbers(dtype):
+    """They give what is not a number, from a row in shares, by itself and with most of it in common, among few queries and many; the others what the definition says."""
+    n = 3000
+    k, v = _rows(56, 1, 2, n, dtype)
+    one = _filled(k, v, [n], "int8")
+    c = one.select([0] * 3)
+    for cache, rows, L, shared in ((one, 1, 1, False), (one, 1, 40, False), (c, 3, 1, False), (c, 3, 4, True), (c, 3, 40, False)):
+        q = _queries(57, rows, 8, L, dtype)
+        want = cache.attend(0, q.to(DEV), shared=shared, return_lse=True)
+        bad = q.clone()
+        bad[rows - 1, 5, L - 1] = float("nan")
+        got = cache.attend(0, bad.to(DEV), shared=shared, return_lse=True)
+        for x, y, at in zip(got, want, ((rows - 1, L - 1, 5), (rows - 1, 5, L - 1))):
+            assert bool(torch.isnan(x[at]).all()), (rows, L, shared)
+            x[at] = y[at]
+        for b in range(rows):
+            _check(got[0][b], got[1][b], q[b], k[0], v[0], "int8")

@@ -259,6 +259,22 @@ def test_infinite_values_beside_the_type_s_largest(dtype):
         _check(q, k, v, window=12)
 
 
+@pytest.mark.parametrize("shape", [(1, 4, 2, 150, 150), (1, 4, 2, 3, 7000)], ids=str)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_that_are_not_numbers(dtype, shape):
+    """They give what is not a number, in one share and in several, and their neighbours what they gave without them."""
+    q, k, v = _inputs(34, *shape, dtype)
+    for bad in (float("nan"), float("inf")):
+        q[0, 1, 2, 5], k[..., 5] = bad, 0                               # (infinite times 0 is not a number)
+        out, lse = _call(q, k, v)
+        assert bool(torch.isnan(out[0, 2, 1]).all()) and bool(torch.isnan(lse[0, 1, 2]))
+        clean = q.clone()
+        clean[0, 1, 2, 5] = 0
+        want, want_lse, tol, lse_tol = plain.attend(clean[0], k[0], v[0])
+        out[0, 2, 1], lse[0, 1, 2] = want[2, 1].to(dtype), want_lse[1, 2].float()
+        plain.check(out[0], lse[0], want, want_lse, tol, lse_tol)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scores_that_rise(dtype):
     """Every later key outscores the ones before by far, or falls behind: the reference moves many times, or never."""
